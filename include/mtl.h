@@ -795,6 +795,46 @@ int mtl_decode_step_persist(const mtl_decode_step_args* args, const mtl_decode_l
                             const mtl_decode_layer* layers_dev, void* workspace, size_t workspace_bytes,
                             int32_t blocking, mtl_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Weights in 4-bit codes with group scales: w[n, k] = (code[n, k] -
+ * zeros[n, k / group]) scales[n, k / group], codes and zeros in 0..15 (8 where
+ * zeros is NULL), group 32, 64 or 128.  No counterpart in the reference,
+ * whose projections are nn.Linear (model.py:151-170).
+ *
+ * Layout, with NT = ceil(N / 16) and KB = ceil(K / 128):
+ *   codes   [NT, KB, 64, 16] bytes.  Of rows 16 t .. and columns 128 kb ..,
+ *           entry l = r + 16 j holds four little-endian 32-bit words; word i
+ *           the codes of row r, columns 32 i + 8 j + e (e = 0..7), code e in
+ *           bits 16 (e & 1) + 4 (e / 2) and up.
+ *   scales  [NT, KB, 16, 128 / group], float or bf16 (scale_dtype)
+ *   zeros   the same shape, bytes, or NULL
+ * Rows and columns past N and K have scale 0.  codes and scales 16-byte,
+ * zeros 4-byte aligned.  N <= 2^27, K <= 2^20.
+ *
+ * mtl_linear_w4: y [M, N] = x [M, K] W^T (+ bias [N]) for 0 <= M <= 64 rows;
+ *   x, bias and y of type dtype (MTL_F32 or MTL_BF16), rows ldx and ldy
+ *   elements apart.  Products and sums are as exact as fp32 ones.  y must
+ *   not overlap x.  No row of x changes another row's result.
+ * mtl_dequantize_w4: W [N, K] (rows ldw elements apart) of type dtype, each
+ *   value rounded once from fp32.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    const void* x;
+    const uint8_t* codes;
+    const void* scales;
+    const uint8_t* zeros;      /* or NULL */
+    const void* bias;          /* [N] or NULL */
+    void* y;
+    int64_t ldx, ldy;
+    int64_t M, N, K;
+    int32_t group, dtype, scale_dtype;
+    int32_t reserved;
+} mtl_linear_w4_args;
+
+int mtl_linear_w4(const mtl_linear_w4_args* args, mtl_stream_t stream);
+int mtl_dequantize_w4(const uint8_t* codes, const void* scales, const uint8_t* zeros, void* W, int64_t ldw, int64_t N,
+                      int64_t K, int32_t group, int32_t dtype, int32_t scale_dtype, mtl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,7 +15,7 @@ import os
 import torch  # noqa: F401  (must be loaded first, see module docstring)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmtl.so")
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 MTL_F32 = 0
 MTL_BF16 = 1
@@ -125,6 +125,15 @@ class DecodeStepBatchedArgs(ctypes.Structure):
     ]
 
 
+class LinearW4Args(ctypes.Structure):
+    """mirror of mtl_linear_w4_args"""
+    _fields_ = [
+        ("x", _vp), ("codes", _vp), ("scales", _vp), ("zeros", _vp), ("bias", _vp), ("y", _vp),
+        ("ldx", _i64), ("ldy", _i64), ("M", _i64), ("N", _i64), ("K", _i64),
+        ("group", _i32), ("dtype", _i32), ("scale_dtype", _i32), ("reserved", _i32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol of include/mtl.h
 SIGNATURES = {
     "mtl_last_error": (ctypes.c_char_p, []),
@@ -180,6 +189,8 @@ SIGNATURES = {
     "mtl_decode_norm_gemv": (ctypes.c_int, [_fp, _fp, ctypes.c_float, _fp, _fp, _fp, _i32, _i32, _i32, _vp]),
     "mtl_decode_ssm": (ctypes.c_int, [_fp, _i32, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _i32, _i32, _i32, _i32,
                                       _vp]),
+    "mtl_linear_w4": (ctypes.c_int, [ctypes.POINTER(LinearW4Args), _vp]),
+    "mtl_dequantize_w4": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp]),
 }
 
 _lib = None

@@ -1171,3 +1171,188 @@ def decode_ssm(xpart, xc, gz, W_dt, b_dt, A_log, Dv, ssm_state, y):
                                               _ptr(b_dt), _ptr(A_log), _ptr(Dv), _ptr(ssm_state), _ptr(y), b, D, N,
                                               R, _stream(xc)), "decode_ssm")
     return y
+
+
+# --------------------------------------------------------------------------- 4-bit weights
+W4_GROUPS = (32, 64, 128)
+W4_MAX_ROWS = 64          # rows of x that linear_w4 takes
+_W4_TILE, _W4_BLOCK = 16, 128
+
+
+class W4:
+    """A weight matrix [n, k] in 4-bit codes: w = (code - zero) * scale, one scale (and zero, or 8) for each run of
+    `group` columns of a row.  pack_w4 and quantize_w4 make it; the tensors are laid out as include/mtl.h says
+    (codes [n/16, k/128, 64, 16] uint8, scales and zeros [n/16, k/128, 16, 128/group], sizes rounded up)."""
+
+    __slots__ = ("codes", "scales", "zeros", "n", "k", "group")
+
+    def __init__(self, codes, scales, zeros, n, k, group):
+        if group not in W4_GROUPS:
+            raise ValueError(f"group must be one of {W4_GROUPS}, got {group}")
+        if not (1 <= n <= 1 << 27 and 1 <= k <= 1 << 20):
+            raise ValueError(f"a 4-bit matrix has 1..2^27 rows and 1..2^20 columns, got {n} x {k}")
+        nt, kb = -(-n // _W4_TILE), -(-k // _W4_BLOCK)
+        shape = (nt, kb, _W4_TILE, _W4_BLOCK // group)
+        if codes.dtype != torch.uint8 or tuple(codes.shape) != (nt, kb, 64, 16) or not codes.is_contiguous():
+            raise ValueError(f"codes must be contiguous uint8 {(nt, kb, 64, 16)}, got {tuple(codes.shape)} {codes.dtype}")
+        if scales.dtype not in _ACT_DTYPES or tuple(scales.shape) != shape or not scales.is_contiguous():
+            raise ValueError(f"scales must be contiguous float32 or bfloat16 {shape}, got {tuple(scales.shape)} "
+                             f"{scales.dtype}")
+        if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != shape
+                                  or not zeros.is_contiguous()):
+            raise ValueError(f"zeros must be contiguous uint8 {shape}, got {tuple(zeros.shape)} {zeros.dtype}")
+        if any(t is not None and t.device != codes.device for t in (scales, zeros)):
+            raise ValueError("codes, scales and zeros must be on one device")
+        self.codes, self.scales, self.zeros, self.n, self.k, self.group = codes, scales, zeros, n, k, group
+
+
+def _w4_tiles(t, n, k, per_row):
+    """[n, per-row entries] -> zero-padded [n/16, k/128, 16, per_row]."""
+    nt, kb = -(-n // _W4_TILE), -(-k // _W4_BLOCK)
+    full = torch.zeros(nt * _W4_TILE, kb * per_row, device=t.device, dtype=t.dtype)
+    full[:n, :t.shape[1]] = t
+    return full.view(nt, _W4_TILE, kb, per_row).transpose(1, 2).contiguous()
+
+
+def pack_w4(codes, scales, zeros=None, group=64):
+    """Lays out a 4-bit matrix once: codes [n, k] uint8 in 0..15, scales [n, ceil(k / group)] float32 or bfloat16, zeros
+    the same shape, uint8 in 0..15 (None: 8 everywhere).  Works on any device; one that holds values past 15 raises
+    (which waits for the device)."""
+    if codes.dim() != 2 or codes.dtype != torch.uint8:
+        raise ValueError(f"codes must be uint8 [n, k], got {tuple(codes.shape)} {codes.dtype}")
+    if group not in W4_GROUPS:
+        raise ValueError(f"group must be one of {W4_GROUPS}, got {group}")
+    n, k = codes.shape
+    if not (1 <= n <= 1 << 27 and 1 <= k <= 1 << 20):
+        raise ValueError(f"a 4-bit matrix has 1..2^27 rows and 1..2^20 columns, got {n} x {k}")
+    ng = -(-k // group)
+    if scales.dtype not in _ACT_DTYPES or tuple(scales.shape) != (n, ng):
+        raise ValueError(f"scales must be float32 or bfloat16 {(n, ng)}, got {tuple(scales.shape)} {scales.dtype}")
+    if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != (n, ng)):
+        raise ValueError(f"zeros must be uint8 {(n, ng)}, got {tuple(zeros.shape)} {zeros.dtype}")
+    if any(t is not None and t.device != codes.device for t in (scales, zeros)):
+        raise ValueError("codes, scales and zeros must be on one device")
+    if any(t is not None and int(t.max()) > 15 for t in (codes, zeros)):
+        raise ValueError("codes and zeros must be in 0..15")
+    scales = scales.detach()
+    c = _w4_tiles(codes, n, k, _W4_BLOCK)                                   # [nt, kb, 16 r, 128]
+    c = c.view(*c.shape[:3], 4, 4, 8).permute(0, 1, 4, 2, 3, 5)             # [nt, kb, 4 j, 16 r, 4 i, 8 e]
+    # nibbles of a word, low to high: codes 0 2 4 6 1 3 5 7
+    c = c[..., [0, 4, 1, 5]] | (c[..., [2, 6, 3, 7]] << 4)
+    c = c.reshape(c.shape[0], c.shape[1], 64, 16)
+    per = _W4_BLOCK // group
+    return W4(c.contiguous(), _w4_tiles(scales, n, k, per), None if zeros is None else _w4_tiles(zeros, n, k, per),
+              n, k, group)
+
+
+@torch.no_grad()
+def quantize_w4(W, group=64, zero_points=False, scale_dtype=torch.bfloat16):
+    """W [n, k] -> W4, each group of columns rounded to the nearest of its 16 values: scale = max |w| / 7 around code 8,
+    or with zero_points the range of the group (0 included) in 15 steps.  The scale is rounded to scale_dtype first and
+    the codes chosen for the rounded one.  Works on any device; W must be finite (checked, which waits for the
+    device)."""
+    if W.dim() != 2 or not W.dtype.is_floating_point:
+        raise ValueError(f"W must be a floating-point [n, k] matrix, got {tuple(W.shape)} {W.dtype}")
+    if group not in W4_GROUPS:
+        raise ValueError(f"group must be one of {W4_GROUPS}, got {group}")
+    if scale_dtype not in _ACT_DTYPES:
+        raise TypeError(f"scale_dtype must be float32 or bfloat16, got {scale_dtype}")
+    n, k = W.shape
+    if n == 0 or k == 0:
+        raise ValueError("W must not be empty")
+    if not bool(torch.isfinite(W).all()):
+        raise ValueError("W holds infinities or NaN")
+    w = W.float()
+    if k % group:
+        w = F.pad(w, (0, group - k % group))      # zeros widen no group's range past 0
+    w = w.view(n, -1, group)
+    if zero_points:
+        lo, hi = w.amin(-1).clamp_max(0.0), w.amax(-1).clamp_min(0.0)
+        # (halves: hi - lo may pass float32's largest)
+        scales = ((hi / 2 - lo / 2) / 7.5).to(scale_dtype)
+        s = scales.float()
+        inv = torch.where(s > 0, s, torch.inf)
+        zeros = (-lo / inv).round_().clamp_(0, 15)
+    else:
+        scales = (w.abs().amax(-1) / 7).to(scale_dtype)
+        s = scales.float()
+        inv = torch.where(s > 0, s, torch.inf)
+        zeros = torch.full_like(s, 8.0)
+    codes = (w / inv[..., None]).round_().add_(zeros[..., None]).clamp_(0, 15).to(torch.uint8).view(n, -1)[:, :k]
+    return pack_w4(codes, scales, zeros.to(torch.uint8) if zero_points else None, group)
+
+
+def _no_grad_recorded(name, *ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
+def _rows_of(t, cols):
+    """t [..., cols] as (2-D tensor with unit column stride and rows that do not overlap, row stride)."""
+    if t.dim() != 2 or (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.reshape(-1, cols).contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else cols)
+
+
+def _overlap(a, b) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    span = lambda t: sum((s - 1) * st for s, st in zip(t.shape, t.stride())) * t.element_size() + t.element_size()
+    if a.numel() == 0 or b.numel() == 0 or a.device != b.device:
+        return False
+    return a.data_ptr() < b.data_ptr() + span(b) and b.data_ptr() < a.data_ptr() + span(a)
+
+
+def linear_w4(x, w4, bias=None, out=None):
+    """x [..., k] W^T (+ bias [n]) for at most W4_MAX_ROWS rows of x, W [n, k] in 4-bit codes (mtl_linear_w4); float32
+    or bfloat16, summed in float32.  More rows: dequantize_w4 and a matrix product.  Returns [..., n]."""
+    if not isinstance(w4, W4):
+        raise TypeError(f"linear_w4: w4 must be a W4 (pack_w4, quantize_w4), got {type(w4).__name__}")
+    if x.dim() < 1 or x.shape[-1] != w4.k:
+        raise ValueError(f"x must be [..., {w4.k}], got {tuple(x.shape)}")
+    code = _act_code(x, bias, out)
+    _same_device(x, w4.codes, bias, out)
+    _no_grad_recorded("linear_w4", x, bias)
+    shape = (*x.shape[:-1], w4.n)
+    x2, ldx = _rows_of(x, w4.k)
+    M = x2.shape[0]
+    if M > W4_MAX_ROWS:
+        raise ValueError(f"linear_w4 takes at most {W4_MAX_ROWS} rows of x, got {M}")
+    if bias is not None and (tuple(bias.shape) != (w4.n,) or not bias.is_contiguous()):
+        raise ValueError(f"bias must be contiguous [{w4.n}], got {tuple(bias.shape)}")
+    if out is None:
+        out = torch.empty(shape, device=x.device, dtype=x.dtype)
+        ldy = w4.n
+    else:
+        if tuple(out.shape) != shape or not (out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1
+                                                                     and out.stride(0) >= w4.n)):
+            raise ValueError(f"out must be {shape} with contiguous rows, got {tuple(out.shape)} strides {out.stride()}")
+        if any(t is not None and _overlap(out, t) for t in (x2, bias, w4.codes, w4.scales, w4.zeros)):
+            raise ValueError("out must not overlap an operand")
+        ldy = out.stride(0) if out.dim() == 2 and M > 1 else w4.n
+    a = _lib.LinearW4Args(_ptr(x2), _ptr(w4.codes), _ptr(w4.scales), _ptr(w4.zeros), _ptr(bias), _ptr(out), ldx, ldy, M,
+                          w4.n, w4.k, w4.group, code, _ACT_DTYPES[w4.scales.dtype], 0)
+    with _dev_guard(x):
+        _lib.check(_lib.load().mtl_linear_w4(ctypes.byref(a), _stream(x)), "linear_w4")
+    return out
+
+
+def dequantize_w4(w4, dtype=torch.float32, out=None):
+    """The matrix [n, k] of a W4 in float32 or bfloat16 (mtl_dequantize_w4): what a prompt's product reads."""
+    if not isinstance(w4, W4):
+        raise TypeError(f"dequantize_w4: w4 must be a W4 (pack_w4, quantize_w4), got {type(w4).__name__}")
+    if dtype not in _ACT_DTYPES:
+        raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
+    if out is None:
+        out = torch.empty(w4.n, w4.k, device=w4.codes.device, dtype=dtype)
+    elif tuple(out.shape) != (w4.n, w4.k) or out.dtype != dtype or (w4.k > 1 and out.stride(1) != 1) or \
+            (w4.n > 1 and out.stride(0) < w4.k):
+        raise ValueError(f"out must be {dtype} {(w4.n, w4.k)} with contiguous rows, got {tuple(out.shape)} {out.dtype}")
+    _same_device(w4.codes, out)
+    if any(t is not None and _overlap(out, t) for t in (w4.codes, w4.scales, w4.zeros)):
+        raise ValueError("out must not overlap an operand")
+    ldw = out.stride(0) if w4.n > 1 else w4.k
+    with _dev_guard(out):
+        _lib.check(_lib.load().mtl_dequantize_w4(_ptr(w4.codes), _ptr(w4.scales), _ptr(w4.zeros), _ptr(out), ldw, w4.n,
+                                                 w4.k, w4.group, _ACT_DTYPES[dtype], _ACT_DTYPES[w4.scales.dtype],
+                                                 _stream(out)), "dequantize_w4")
+    return out

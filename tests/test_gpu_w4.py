@@ -1,0 +1,170 @@
+"""linear_w4 and dequantize_w4 against float64, at the ends of their ranges and where a tile, a block or a group is
+partial."""
+import math
+
+import pytest
+import torch
+
+from mamba_lite import _lib, ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _matrix(n, k, group, zeros, scale_dtype, seed):
+    """(W4, the same matrix in float64 by its definition)"""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    ng = -(-k // group)
+    codes = torch.randint(0, 16, (n, k), device="cuda", generator=g, dtype=torch.uint8)
+    scales = ((torch.rand(n, ng, device="cuda", generator=g) + 0.5) * 0.01).to(scale_dtype)
+    z = torch.randint(0, 16, (n, ng), device="cuda", generator=g, dtype=torch.uint8) if zeros else None
+    col = torch.arange(k, device="cuda") // group
+    w = (codes.double() - (8.0 if z is None else z.double()[:, col])) * scales.double()[:, col]
+    return ops.pack_w4(codes, scales, z, group), w
+
+
+def _x(m, k, dtype, seed):
+    return torch.randn(m, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).to(dtype)
+
+
+def _tol(k, group, dtype):
+    """Of the norm.  float32: a random walk of k rounded sums, 2^-24 sqrt(k); sums over a group may run over codes
+    16 + q, six times the size of q - z, before 16 + z of the sum of x is taken off; splits, scales and the bias a few
+    roundings more.  bfloat16: the output's rounding, 2^-8."""
+    return 2.0 ** -24 * (math.sqrt(k) + 6 * math.sqrt(min(k, group)) + 4) + (2.0 ** -8 if dtype == torch.bfloat16 else 0)
+
+
+def _check(y, ref, tol):
+    assert y.shape == ref.shape
+    e = float((y.double() - ref).norm() / ref.norm().clamp_min(1e-300))
+    assert e < tol, (e, tol)
+    # no value is far off either: 6 times the root mean square of what the norm allows, plus its own rounding
+    worst = float(((y.double() - ref).abs() - tol * ref.abs()).max() / ref.norm() * math.sqrt(ref.numel()))
+    assert worst < 6 * tol, (worst, tol)
+
+
+SIZES = [(1, 1, 1), (1, 16, 128), (2, 15, 31), (3, 17, 129), (5, 768, 1536), (6, 33, 700), (16, 1001, 777),
+         (17, 100, 2048), (33, 48, 96), (64, 257, 1300), (1, 8192, 2048), (4, 40, 9000), (48, 20, 8192)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group,zeros,scale_dtype", [(32, True, torch.float32), (64, False, torch.bfloat16),
+                                                     (128, True, torch.bfloat16), (128, False, torch.float32)])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_linear_matches_float64(m, n, k, group, zeros, scale_dtype, dtype):
+    w4, w = _matrix(n, k, group, zeros, scale_dtype, n + k)
+    x = _x(m, k, dtype, m)
+    bias = _x(1, n, dtype, 7)[0] if m % 2 else None
+    ref = x.double() @ w.t().contiguous() + (0 if bias is None else bias.double())
+    y = ops.linear_w4(x, w4, bias)
+    assert y.dtype == dtype
+    _check(y, ref, _tol(k, group, dtype))
+    assert torch.equal(y, ops.linear_w4(x, w4, bias))          # the same bits every time
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group,zeros,scale_dtype", [(32, False, torch.bfloat16), (64, True, torch.float32),
+                                                     (128, True, torch.bfloat16)])
+@pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (15, 31), (17, 129), (768, 1536), (1001, 777), (100, 130), (5, 5000)])
+def test_matrix_is_the_rounded_product(n, k, group, zeros, scale_dtype, dtype):
+    w4, w = _matrix(n, k, group, zeros, scale_dtype, n + k)
+    got = ops.dequantize_w4(w4, dtype)
+    assert got.shape == (n, k) and torch.equal(got, w.float().to(dtype))       # one rounding (a code times a scale
+    # fits 24 bits + 5: float32 rounds it once, and so does the float64 value taken to float32)
+
+
+def test_rows_with_strides_and_outputs_in_place():
+    w4, w = _matrix(100, 300, 64, True, torch.bfloat16, 0)
+    for dtype in (torch.float32, torch.bfloat16):
+        big = _x(9, 700, dtype, 1)
+        for x in (big[:, 3:303], big[::2, 5:305], big[:1, 1:301], big[:, ::2][:, :300], big[4:5].expand(3, 700)[:, :300],
+                  big[:, :600].reshape(9, 2, 300)):
+            ref = x.double() @ w.t().contiguous()
+            _check(ops.linear_w4(x, w4), ref, _tol(300, 64, dtype))
+        room = torch.full((6, 130), 3.0, device="cuda", dtype=dtype)
+        got = ops.linear_w4(big[:4, :300], w4, out=room[1:5, 7:107])
+        _check(got, big[:4, :300].double() @ w.t().contiguous(), _tol(300, 64, dtype))
+        room[1:5, 7:107] = 3.0
+        assert bool((room == 3.0).all())                       # nothing written beside the rows
+        wide = torch.full((102, 311), 5.0, device="cuda", dtype=dtype)
+        ops.dequantize_w4(w4, dtype, out=wide[1:101, 3:303])
+        assert torch.equal(wide[1:101, 3:303], w.float().to(dtype))
+        wide[1:101, 3:303] = 5.0
+        assert bool((wide == 5.0).all())
+    assert ops.linear_w4(torch.empty(0, 300, device="cuda"), w4).shape == (0, 100)
+    assert ops.linear_w4(_x(1, 300, torch.float32, 2)[0], w4).shape == (100,)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [1e-30, 1e20, 3e35])
+def test_large_and_small_values(dtype, scale):
+    w4, w = _matrix(64, 512, 64, True, torch.float32, 3)
+    x = (_x(3, 512, torch.float32, 4).clamp(-4, 4) * scale).to(dtype)
+    ref = x.double() @ w.t().contiguous()
+    assert bool(ref.abs().max() < 3e38)
+    _check(ops.linear_w4(x, w4) / scale, ref / scale, _tol(512, 64, dtype) + 2.0 ** -24)
+    # rows of very different size do not disturb each other
+    x = _x(3, 512, torch.float32, 5) * torch.tensor([1e-12, 1.0, 1e12], device="cuda")[:, None]
+    y, ref = ops.linear_w4(x.to(dtype), w4), x.to(dtype).double() @ w.t().contiguous()
+    for m in range(3):
+        _check(y[m:m + 1], ref[m:m + 1], _tol(512, 64, dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,at", [(1, 0), (7, 3), (40, 39)])
+def test_infinities_and_nan_stay_in_their_row(m, at, dtype):
+    w4, w = _matrix(70, 400, 32, True, torch.bfloat16, 6)
+    x = _x(m, 400, dtype, 8)
+    clean = x.double() @ w.t().contiguous()
+    for bad, where in ((float("inf"), 5), (float("-inf"), 399), (float("nan"), 130)):
+        xb = x.clone()
+        xb[at, where] = bad
+        y = ops.linear_w4(xb, w4)
+        ref = xb.double()[at] @ w.t().contiguous()             # inf * 0 is NaN, inf * w an infinity of its sign
+        assert torch.equal(torch.isnan(y[at]), torch.isnan(ref))
+        ok = ~torch.isnan(ref)
+        assert torch.equal(y[at][ok].double(), ref[ok])
+        rest = [i for i in range(m) if i != at]
+        if rest:
+            _check(y[rest], clean[rest], _tol(400, 32, dtype))
+
+
+def test_streams_and_graph_replays():
+    w4, w = _matrix(300, 1000, 128, False, torch.bfloat16, 9)
+    x = _x(5, 1000, torch.float32, 10)
+    want = ops.linear_w4(x, w4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.linear_w4(x, w4)
+        ops.linear_w4(x, w4), ops.dequantize_w4(w4)            # warm for the capture
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    sx = x.clone()
+    with torch.cuda.graph(graph):
+        y = ops.linear_w4(sx, w4)
+        wm = ops.dequantize_w4(w4)
+    for i in range(4):
+        sx.copy_(x * (i + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.linear_w4(x * (i + 1), w4)) and torch.equal(wm, w.float())
+
+
+def test_refusals_on_the_gpu():
+    w4, _ = _matrix(20, 200, 64, True, torch.bfloat16, 11)
+    x = _x(2, 200, torch.float32, 12)
+    with pytest.raises(ValueError, match="at most 64"):
+        ops.linear_w4(_x(65, 200, torch.float32, 0), w4)
+    with pytest.raises(RuntimeError, match="operands"):
+        ops.linear_w4(x.cpu(), w4)
+    with pytest.raises(RuntimeError, match="operands"):
+        ops.linear_w4(x, w4, out=torch.empty(2, 20))
+    with pytest.raises(RuntimeError, match="backward"):
+        ops.linear_w4(x.requires_grad_(), w4)
+    with torch.no_grad():
+        ops.linear_w4(x, w4)
+    half = ops.W4(w4.codes, w4.scales, w4.zeros, 20, 200, 64)
+    half.scales = torch.zeros(2000, device="cuda", dtype=torch.bfloat16)[1:1 + w4.scales.numel()].view_as(w4.scales)
+    with pytest.raises(_lib.MTLError, match="aligned"):
+        ops.linear_w4(_x(2, 200, torch.float32, 12), half)

@@ -1,0 +1,167 @@
+"""4-bit weights on the host: the layout word by word, the choice of codes, and what the entry points refuse."""
+import ctypes
+
+import pytest
+import torch
+
+from mamba_lite import _lib, ops
+
+
+def _random(n, k, group, zeros, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    ng = -(-k // group)
+    return (torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8), torch.rand(n, ng, generator=g) + 0.5,
+            torch.randint(0, 16, (n, ng), generator=g, dtype=torch.uint8) if zeros else None)
+
+
+@pytest.mark.parametrize("n,k,group,zeros", [(1, 1, 32, True), (16, 128, 128, False), (17, 129, 64, True),
+                                             (40, 300, 32, True), (33, 256, 128, True)])
+def test_layout_is_the_documented_one(n, k, group, zeros):
+    codes, scales, z = _random(n, k, group, zeros)
+    w4 = ops.pack_w4(codes, scales, z, group)
+    nt, kb = -(-n // 16), -(-k // 128)
+    assert tuple(w4.codes.shape) == (nt, kb, 64, 16)
+    words = w4.codes.view(torch.int32)                      # [nt, kb, 64, 4]
+    for t in range(nt):
+        for b in range(kb):
+            for l in range(64):
+                r, j = l % 16, l // 16
+                for i in range(4):
+                    for e in range(8):
+                        row, col = 16 * t + r, 128 * b + 32 * i + 8 * j + e
+                        got = (int(words[t, b, l, i]) >> (16 * (e & 1) + 4 * (e // 2))) & 15
+                        inside = row < n and col < k
+                        assert got == (int(codes[row, col]) if inside else 0)
+                        s = float(w4.scales[t, b, r, (col % 128) // group])
+                        # past N or in a group past K: scale 0; columns past K in K's last group carry code 0
+                        assert s == (float(scales[row, col // group]) if row < n and col // group < scales.shape[1]
+                                     else 0.0)
+                        if zeros and inside:
+                            assert int(w4.zeros[t, b, r, (col % 128) // group]) == int(z[row, col // group])
+
+
+@pytest.mark.parametrize("scale_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("zero_points", [False, True])
+@pytest.mark.parametrize("n,k,group", [(5, 64, 32), (3, 200, 128), (20, 77, 64)])
+def test_quantize_rounds_to_the_nearest_value(n, k, group, zero_points, scale_dtype):
+    g = torch.Generator().manual_seed(1)
+    W = torch.randn(n, k, generator=g) + (0.7 if zero_points else 0.0)
+    W[0, :group] = 0.0                                       # a group of zeros
+    W[1, 0] = 9.0                                            # an outlier
+    w4 = ops.quantize_w4(W, group, zero_points, scale_dtype)
+    assert w4.scales.dtype == scale_dtype and (w4.zeros is not None) == zero_points
+    per = 128 // group
+    scales = w4.scales.transpose(1, 2).reshape(-1, w4.codes.shape[1] * per)[:n].double()
+    words = w4.codes.view(torch.int32).view(w4.codes.shape[0], w4.codes.shape[1], 4, 16, 4)
+    codes = torch.stack([(words >> (16 * (e & 1) + 4 * (e // 2))) & 15 for e in range(8)], -1)   # [nt,kb,j,r,i,e]
+    codes = codes.permute(0, 3, 1, 4, 2, 5).reshape(w4.codes.shape[0] * 16, -1)[:n, :k].double()
+    col = torch.arange(k) // group
+    z = 8.0 if w4.zeros is None else \
+        w4.zeros.transpose(1, 2).reshape(-1, w4.codes.shape[1] * per)[:n].double()[:, col]
+    s = scales[:, col]
+    back = (codes - z) * s
+    # half a step, and what rounding a scale down (bf16: by 2^-8) cuts off the end of the range, at most 15 steps; with
+    # zero points the zero's own rounding may cut off another half step
+    step = s * (0.5 + (0.5 if zero_points else 0.0) + 15 * (2.0 ** -8 if scale_dtype == torch.bfloat16 else 2.0 ** -23))
+    assert bool(((back - W.double()).abs() <= step + 1e-12).all())
+    assert bool((back[0, :group] == 0).all())
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(codes=torch.zeros(4, 8)), "uint8"),
+    (dict(codes=torch.zeros(4, 8, 1, dtype=torch.uint8)), "uint8"),
+    (dict(codes=torch.full((4, 64), 16, dtype=torch.uint8)), "0..15"),
+    (dict(zeros=torch.full((4, 1), 16, dtype=torch.uint8)), "0..15"),
+    (dict(zeros=torch.zeros(4, 2, dtype=torch.uint8)), "zeros"),
+    (dict(scales=torch.ones(4, 2)), "scales"),
+    (dict(scales=torch.ones(4, 1, dtype=torch.float16)), "scales"),
+    (dict(group=48), "group"),
+    (dict(codes=torch.zeros(0, 64, dtype=torch.uint8)), "rows"),
+])
+def test_pack_refuses(change, error):
+    a = dict(codes=torch.zeros(4, 64, dtype=torch.uint8), scales=torch.ones(4, 1), zeros=None, group=64)
+    a.update(change)
+    with pytest.raises(ValueError, match=error):
+        ops.pack_w4(**a)
+
+
+def test_quantize_refuses():
+    for bad in (torch.zeros(3), torch.zeros(3, 4, dtype=torch.int32), torch.zeros(0, 4),
+                torch.tensor([[1.0, float("inf")]]), torch.tensor([[float("nan"), 1.0]])):
+        with pytest.raises(ValueError):
+            ops.quantize_w4(bad)
+    with pytest.raises(ValueError, match="group"):
+        ops.quantize_w4(torch.zeros(2, 64), group=16)
+    with pytest.raises(TypeError, match="scale_dtype"):
+        ops.quantize_w4(torch.zeros(2, 64), scale_dtype=torch.float16)
+
+
+def test_a_made_up_layout_is_refused():
+    w = ops.pack_w4(*_random(20, 200, 64, True), group=64)
+    ops.W4(w.codes, w.scales, w.zeros, 20, 200, 64)
+    for a in ((w.codes[:1], w.scales, w.zeros, 20, 200, 64), (w.codes, w.scales[:1], w.zeros, 20, 200, 64),
+              (w.codes, w.scales, w.zeros[:1], 20, 200, 64), (w.codes, w.scales, w.zeros, 40, 200, 64),
+              (w.codes, w.scales, w.zeros, 20, 300, 64), (w.codes, w.scales, w.zeros, 20, 200, 32),
+              (w.codes, w.scales, w.zeros, 0, 200, 64), (w.codes, w.scales.half(), None, 20, 200, 64)):
+        with pytest.raises(ValueError):
+            ops.W4(*a)
+
+
+def test_calls_are_refused_on_the_host():
+    w4 = ops.pack_w4(*_random(20, 200, 64, True), group=64)
+    x = torch.zeros(2, 200)
+    with pytest.raises(RuntimeError, match="GPU"):
+        ops.linear_w4(x, w4)
+    with pytest.raises(RuntimeError, match="GPU"):
+        ops.dequantize_w4(w4)
+    for bad in (dict(x=torch.zeros(2, 199)), dict(x=torch.zeros(65, 200)), dict(bias=torch.zeros(19)),
+                dict(out=torch.zeros(2, 19)), dict(out=torch.zeros(2, 40)[:, ::2])):
+        with pytest.raises(ValueError):
+            ops.linear_w4(**{**dict(x=x, w4=w4), **bad})
+    shared = torch.zeros(4000)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.linear_w4(shared[:400].view(2, 200), w4, out=shared[390:430].view(2, 20))
+    with pytest.raises(TypeError, match="W4"):
+        ops.linear_w4(x, torch.zeros(20, 200))
+    with pytest.raises(TypeError):
+        ops.linear_w4(x.half(), w4)
+    with pytest.raises(TypeError):
+        ops.linear_w4(x, w4, bias=torch.zeros(20, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError, match="backward"):
+        ops.linear_w4(torch.zeros(2, 200, requires_grad=True), w4)
+    with pytest.raises(TypeError):
+        ops.dequantize_w4(w4, torch.float16)
+    with pytest.raises(ValueError):
+        ops.dequantize_w4(w4, out=torch.zeros(20, 199))
+
+
+def _args(**change):
+    buf = 0x1000
+    a = dict(x=buf, codes=buf, scales=buf, zeros=None, bias=None, y=buf, ldx=200, ldy=20, M=2, N=20, K=200, group=64,
+             dtype=0, scale_dtype=0, reserved=0)
+    a.update(change)
+    return _lib.LinearW4Args(**a)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(group=16), b"group"), (dict(M=65), b"M must"), (dict(M=-1), b"M must"), (dict(N=0), b"N must"),
+    (dict(K=0), b"K in"), (dict(K=(1 << 20) + 1), b"K in"), (dict(dtype=2), b"dtype"), (dict(scale_dtype=2), b"dtype"),
+    (dict(x=None), b"null"), (dict(codes=None), b"null"), (dict(y=None), b"null"), (dict(codes=0x1004), b"aligned"),
+    (dict(scales=0x1008), b"aligned"), (dict(zeros=0x1001), b"aligned"), (dict(ldx=199), b"overlap"),
+    (dict(ldy=19), b"overlap"),
+])
+def test_the_library_refuses(change, error):
+    lib = _lib.load()
+    assert lib.mtl_linear_w4(ctypes.byref(_args(**change)), None) == 1
+    assert error in lib.mtl_last_error()
+
+
+def test_the_library_refuses_a_matrix():
+    lib = _lib.load()
+    p = 0x1000
+    assert lib.mtl_linear_w4(None, None) == 1
+    assert lib.mtl_linear_w4(ctypes.byref(_args(M=0)), None) == 0            # nothing to do, nothing launched
+    for bad in ((p, p, None, None, 200, 20, 200, 64, 0, 0), (p, p, None, p, 199, 20, 200, 64, 0, 0),
+                (p, p, p + 1, p, 200, 20, 200, 64, 0, 0), (p, p, None, p, 200, 20, 200, 65, 0, 0),
+                (p, p, None, p, 200, 0, 200, 64, 0, 0)):
+        assert lib.mtl_dequantize_w4(*bad, None) == 1
