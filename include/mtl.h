@@ -835,6 +835,36 @@ int mtl_linear_w4(const mtl_linear_w4_args* args, mtl_stream_t stream);
 int mtl_dequantize_w4(const uint8_t* codes, const void* scales, const uint8_t* zeros, void* W, int64_t ldw, int64_t N,
                       int64_t K, int32_t group, int32_t dtype, int32_t scale_dtype, mtl_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Log probabilities of given tokens, with entropy and the most probable
+ * tokens, of rows of logits (float or bf16, dtype); row i is logits +
+ * (i / inner) stride_outer + (i % inner) stride_inner, its vocab values
+ * contiguous.  The reference leaves the logits to the caller (model.py:326,
+ * 359).  For a row x with token c, Z = sum e^x:
+ *   logprob     [rows] float: ln(e^x_c / Z); 0 for a token below 0 (padding),
+ *               NaN for one past the vocabulary
+ *   entropy     [rows] float: - sum p ln p
+ *   top_logprob [rows, top] float, top_token [rows, top]: the ln p and ids of
+ *               the largest logits in order, equal ones by id; -inf is never
+ *               among them (missing places: -inf and -1)
+ * A row of nothing but -inf has logprob -inf, entropy 0 and no alternatives;
+ * one that holds a NaN or +inf has NaN everywhere and ids -1 (a padding
+ * token's logprob stays 0).
+ * Sums in fp32.  top <= min(64, vocab).  Outputs contiguous.  Deterministic.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    const void* logits;
+    const int64_t* tokens;     /* [outer * inner] */
+    float* logprob;
+    float* entropy;
+    float* top_logprob;        /* NULL with top 0 */
+    int64_t* top_token;        /* NULL with top 0 */
+    int64_t outer, inner, stride_outer, stride_inner, vocab;
+    int32_t top, dtype;
+} mtl_token_logprobs_args;
+
+int mtl_token_logprobs(const mtl_token_logprobs_args* args, mtl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

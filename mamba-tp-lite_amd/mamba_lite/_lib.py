@@ -134,6 +134,15 @@ class LinearW4Args(ctypes.Structure):
     ]
 
 
+class TokenLogprobsArgs(ctypes.Structure):
+    """mirror of mtl_token_logprobs_args"""
+    _fields_ = [
+        ("logits", _vp), ("tokens", _vp), ("logprob", _vp), ("entropy", _vp), ("top_logprob", _vp), ("top_token", _vp),
+        ("outer", _i64), ("inner", _i64), ("stride_outer", _i64), ("stride_inner", _i64), ("vocab", _i64),
+        ("top", _i32), ("dtype", _i32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol of include/mtl.h
 SIGNATURES = {
     "mtl_last_error": (ctypes.c_char_p, []),
@@ -191,6 +200,7 @@ SIGNATURES = {
                                       _vp]),
     "mtl_linear_w4": (ctypes.c_int, [ctypes.POINTER(LinearW4Args), _vp]),
     "mtl_dequantize_w4": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp]),
+    "mtl_token_logprobs": (ctypes.c_int, [ctypes.POINTER(TokenLogprobsArgs), _vp]),
 }
 
 _lib = None

@@ -15,6 +15,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import typing
 
 import torch
 import torch.nn.functional as F
@@ -1356,3 +1357,50 @@ def dequantize_w4(w4, dtype=torch.float32, out=None):
                                                  w4.k, w4.group, _ACT_DTYPES[dtype], _ACT_DTYPES[w4.scales.dtype],
                                                  _stream(out)), "dequantize_w4")
     return out
+
+
+# --------------------------------------------------------------------------- log probabilities
+TOP_MAX = 64              # alternatives per row of token_logprobs
+
+
+class TokenLogprobs(typing.NamedTuple):
+    """What token_logprobs returns, for logits [..., V]: logprob and entropy [...] float32, top_logprob [..., top]
+    float32 and top_token [..., top] int64."""
+
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_logprob: torch.Tensor
+    top_token: torch.Tensor
+
+
+def token_logprobs(logits, tokens, top=0):
+    """ln p of a given token for each row of logits, the row's entropy, and its `top` most probable tokens in order,
+    equal logits by id (mtl_token_logprobs).  logits [..., V] float32 or bfloat16, tokens [...] int64; a negative token
+    is padding (logprob 0), one past the vocabulary has logprob NaN.  -inf masks a token; a row of nothing else has
+    logprob -inf, entropy 0 and no alternatives.  Missing alternatives are -inf and -1; a row with a NaN or +inf is NaN
+    (ids -1)."""
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must be [..., V >= 1], got {tuple(logits.shape)}")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if tokens.dtype != torch.int64 or tokens.shape != lead:
+        raise ValueError(f"tokens must be int64 {tuple(lead)}, got {tuple(tokens.shape)} {tokens.dtype}")
+    if not 0 <= top <= min(TOP_MAX, V):
+        raise ValueError(f"top must be in [0, {min(TOP_MAX, V)}], got {top}")
+    code = _act_code(logits)
+    _same_device(logits, tokens)
+    _no_grad_recorded("token_logprobs", logits)
+    x = logits
+    if V > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    if x.dim() > 3:
+        x = x.reshape(-1, *x.shape[-2:])          # (a view where the strides allow it)
+    x = x.view(*(1,) * (3 - x.dim()), *x.shape) if x.dim() < 3 else x
+    tokens = tokens.contiguous()
+    f = dict(device=x.device, dtype=torch.float32)
+    r = TokenLogprobs(torch.empty(lead, **f), torch.empty(lead, **f), torch.empty(*lead, top, **f),
+                      torch.empty(*lead, top, device=x.device, dtype=torch.int64))
+    a = _lib.TokenLogprobsArgs(_ptr(x), _ptr(tokens), _ptr(r.logprob), _ptr(r.entropy), _ptr(r.top_logprob),
+                               _ptr(r.top_token), x.shape[0], x.shape[1], x.stride(0), x.stride(1), V, top, code)
+    with _dev_guard(x):
+        _lib.check(_lib.load().mtl_token_logprobs(ctypes.byref(a), _stream(x)), "token_logprobs")
+    return r
