@@ -34,40 +34,205 @@ template <typename S> __device__ __forceinline__ float scale_at(const void* p, i
     else return static_cast<const float*>(p)[i];
 }
 
-// One workgroup per 16 rows of W; wavefront w takes every 4th block of columns.  Each weight is made in fp32 as the
-// matrix form rounds it, so an infinity or NaN in x meets it as it would meet the matrix.
-template <typename T, typename S, int G, bool Z>
-__global__ void __launch_bounds__(256) linear_w4_kernel(const W4Args a) {
-    constexpr int NG = kBlockK / G;
-    __shared__ float s_part[4][kTileRows];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, j = lane >> 4;
-    const int64_t t = blockIdx.x;
-    for (int m = 0; m < a.M; ++m) {
-        const T* x = static_cast<const T*>(a.x) + m * a.ldx;
-        float acc = 0.f;
-        for (int kb = wave; kb < a.KB; kb += 4) {
-            const uint4 w = reinterpret_cast<const uint4*>(a.codes)[(t * a.KB + kb) * 64 + lane];
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+typedef __bf16 B8h __attribute__((ext_vector_type(8)));
+typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 8;                  // wavefronts of a workgroup
+constexpr int kLdsBytes = 79 << 10;        // of a workgroup: two fit a CU
+
+struct LinearW4 {
+    W4Args a;
+    int rows;                  // rows of x per workgroup (blockIdx.y takes the next ones)
+    int kblocks;               // 128-column blocks of x in LDS at a time
+    int wk;                    // wavefronts that share a tile of W, each on every wk-th block
+    int xvec;                  // rows of x start on 16-byte boundaries
+};
+
+template <typename S, int NG> struct alignas(sizeof(S) * NG) Scales {        // one row's scales of a block
+    S v[NG];
+    __device__ __forceinline__ float at(int g) const {
+        if constexpr (sizeof(S) == 2) return bf16_to_f32(v[g]);
+        else return v[g];
+    }
+};
+
+// Products on the bf16 matrix cores, exact: a code is the bf16 number 16 + q (its four bits under an exponent), x in
+// float32 the sum of three bf16 numbers of 8 significand bits each, as rows of their own.  A group's sums
+// sum x (16 + q) run in fp32 on v_mfma_f32_16x16x32_bf16, then
+//   acc += s (sum x (16 + q) - (16 + z) sum x),  sum x made once per workgroup and kept beside x in LDS.
+// 8 vector instructions unpack the 8 codes of a word; making q - z first, in fp32, would take three times that.
+//
+// A workgroup keeps x, as the operand's 16-byte runs, in LDS; each wavefront streams tiles of W into
+// registers, kAhead blocks before their use.  Where there are few tiles, wk wavefronts share one and add their sums in order.
+//
+// |x| >= 2^96, infinities and NaN would spoil the difference: a block of columns in which some row holds one takes
+// the products weight by weight instead, as the matrix form would round them.
+template <typename T, typename S, int G, bool Z, int TM>
+__global__ void __launch_bounds__(kWaves * 64, 4) linear_w4_kernel(const LinearW4 p) {
+    constexpr int NG = kBlockK / G, P = sizeof(T) == 4 ? 3 : 1, R16 = TM * 16, kAhead = 4;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const W4Args& a = p.a;
+    const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m0 = blockIdx.y * p.rows, M = min(p.rows, a.M - m0), R = P * M;
+    const int wn = wave / p.wk, wkid = wave - wn * p.wk, WN = kWaves / p.wk;
+    const T* x = static_cast<const T*>(a.x) + m0 * a.ldx;
+    const int pitch = p.kblocks * 16 + 1;                     // (+ 1: the 16 rows of an operand start in different banks)
+    U4* s_x = reinterpret_cast<U4*>(smem);                    // [R][k / 8]
+    float* s_sum = reinterpret_cast<float*>(s_x + P * p.rows * pitch);                         // [group][R16]
+    int at_x[TM];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t at = ((t * a.KB + kb) * kTileRows + r) * NG + 32 * i / G;
-                const float s = scale_at<S>(a.scales, at);
-                const float z = Z ? (float)a.zeros[at] : 8.f;
-                const int k0 = kb * kBlockK + 32 * i + 8 * j;
+    for (int q = 0; q < TM; ++q) at_x[q] = min(q * 16 + r, R - 1) * pitch + j;
+    float* s_red = s_sum + p.kblocks * NG * R16;                                               // [wave][R16][16]
+    __shared__ int s_wide;
+
+    auto stage = [&](int kb0, int nb) {
+        if (threadIdx.x == 0) s_wide = 0;
+        __syncthreads();
+        const int n8 = nb * 16;
+        for (int u = threadIdx.x; u < M * n8; u += kWaves * 64) {
+            const int m = u / n8, k8 = u - m * n8, k = kb0 * kBlockK + k8 * 8;
+            const T* src = x + m * a.ldx + k;
+            float v[8];
+            if (p.xvec && k + 8 <= a.K) {
+                const F4v lo = ld4(src), hi = ld4(src + 4);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (k0 + e < a.K) acc = fmaf(Act<T>::load(x + k0 + e), s * ((float)code_of(ws[i], e) - z), acc);
+                for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = k + e < a.K ? Act<T>::load(src + e) : 0.f;
+            }
+            bool wide = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) wide |= !(fabsf(v[e]) < 0x1p96f);
+            if (wide) s_wide = 1;
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+                U4 part;
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const uint32_t b0 = __float_as_uint(v[e]) & 0xffff0000u, b1 = __float_as_uint(v[e + 1]) & 0xffff0000u;
+                    part[e / 2] = b0 >> 16 | b1;
+                    sum += __uint_as_float(b0) + __uint_as_float(b1);
+                    v[e] -= __uint_as_float(b0);
+                    v[e + 1] -= __uint_as_float(b1);
+                }
+                s_x[(q * M + m) * pitch + k8] = part;
+                // a group's columns lie in neighbouring lanes (n8 is a multiple of 16)
+                sum += dpp_mov<kDppXor1>(sum);
+                sum += dpp_mov<kDppXor2>(sum);
+                if constexpr (G >= 64) sum += dpp_mov<kDppHalfMirror>(sum);
+                if constexpr (G >= 128) sum += dpp_mov<kDppRowMirror>(sum);
+                if (k8 % (G / 8) == 0) s_sum[k8 / (G / 8) * R16 + q * M + m] = sum;
             }
         }
-        acc += __shfl_xor(acc, 16);
-        acc += __shfl_xor(acc, 32);
-        if (lane < 16) s_part[wave][lane] = acc;
         __syncthreads();
-        const int n = (int)t * kTileRows + threadIdx.x;
-        if (threadIdx.x < kTileRows && n < a.N) {
-            float v = (s_part[0][threadIdx.x] + s_part[1][threadIdx.x]) + (s_part[2][threadIdx.x] + s_part[3][threadIdx.x]);
-            if (a.bias) v += Act<T>::load(static_cast<const T*>(a.bias) + n);
-            Act<T>::store(static_cast<T*>(a.y) + m * a.ldy + n, v);
+    };
+
+    const int tiles = (a.N + kTileRows - 1) / kTileRows;
+    const bool once = p.kblocks >= a.KB;
+    if (once) stage(0, a.KB);
+    for (int t0 = blockIdx.x * WN; t0 < tiles; t0 += gridDim.x * WN) {
+        const int64_t t = min(t0 + wn, tiles - 1);           // (past the last tile: computed again, not stored)
+        F4v acc[TM];
+#pragma unroll
+        for (int q = 0; q < TM; ++q) acc[q] = F4v{0.f, 0.f, 0.f, 0.f};
+        for (int kb0 = 0; kb0 < a.KB; kb0 += p.kblocks) {
+            const int kb1 = min(kb0 + p.kblocks, a.KB);
+            if (!once) {
+                __syncthreads();
+                stage(kb0, kb1 - kb0);
+            }
+            if (s_wide) {
+#pragma unroll 1
+                for (int m = 0; m < M; ++m) {
+                    float v = 0.f;
+#pragma unroll 1
+                    for (int kb = kb0 + wkid; kb < kb1; kb += p.wk) {
+#pragma unroll 1
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t w = reinterpret_cast<const uint32_t*>(a.codes)[((t * a.KB + kb) * 64 + lane) * 4 + i];
+                            const int64_t at = ((t * a.KB + kb) * kTileRows + r) * NG + 32 * i / G;
+                            const float s = scale_at<S>(a.scales, at), z = Z ? (float)a.zeros[at] : 8.f;
+                            const int k = kb * kBlockK + 32 * i + 8 * j;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (k + e < a.K) v = fmaf(Act<T>::load(x + m * a.ldx + k + e), s * ((float)code_of(w, e) - z), v);
+                        }
+                    }
+                    v += __shfl_xor(v, 16);
+                    v += __shfl_xor(v, 32);
+                    // into row m's accumulator: lanes 4 j .. + 3 of tile m / 16
+#pragma unroll
+                    for (int q = 0; q < TM * 4; ++q)
+                        if ((m >> 4) * 4 + (m & 3) == q && ((m >> 2) & 3) == j) acc[q >> 2][q & 3] += v;
+                }
+                continue;
+            }
+            for (int kb = kb0 + wkid; kb < kb1; kb += kAhead * p.wk) {
+                U4 w[kAhead];
+                Scales<S, NG> sc[kAhead];
+                Scales<uint8_t, NG> zr[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int64_t b = t * a.KB + min(kb + u * p.wk, kb1 - 1);
+                    w[u] = __builtin_nontemporal_load(reinterpret_cast<const U4*>(a.codes) + b * 64 + lane);
+                    sc[u] = static_cast<const Scales<S, NG>*>(a.scales)[b * kTileRows + r];
+                    if constexpr (Z) zr[u] = reinterpret_cast<const Scales<uint8_t, NG>*>(a.zeros)[b * kTileRows + r];
+                }
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int kc = kb + u * p.wk - kb0;
+                    if (kc >= kb1 - kb0) break;
+                    F4v part[TM];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (i % (G / 32) == 0) {
+#pragma unroll
+                            for (int q = 0; q < TM; ++q) part[q] = F4v{0.f, 0.f, 0.f, 0.f};
+                        }
+                        const uint32_t c = w[u][i];
+                        const U4 b = {(c << 3 & 0x00780078u) | 0x41804180u, (c >> 1 & 0x00780078u) | 0x41804180u,
+                                      (c >> 5 & 0x00780078u) | 0x41804180u, (c >> 9 & 0x00780078u) | 0x41804180u};
+#pragma unroll
+                        for (int q = 0; q < TM; ++q) {
+                            const U4 xa = s_x[at_x[q] + kc * 16 + i * 4];
+                            part[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(B8h, xa),
+                                                                              __builtin_bit_cast(B8h, b), part[q], 0, 0, 0);
+                        }
+                        if (i % (G / 32) == G / 32 - 1) {
+                            const int g = i / (G / 32);
+                            const float s = sc[u].at(g);
+                            float c16 = 24.f;
+                            if constexpr (Z) c16 = 16.f + (float)zr[u].v[g];
+#pragma unroll
+                            for (int q = 0; q < TM; ++q) {
+                                const F4v sx = *reinterpret_cast<const F4v*>(&s_sum[(kc * NG + g) * R16 + q * 16 + 4 * j]);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[q][e] = fmaf(s, fmaf(-c16, sx[e], part[q][e]), acc[q][e]);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        // D[i][j]: row 4 (lane / 16) + i of x, row lane % 16 of W
+#pragma unroll
+        for (int q = 0; q < TM; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s_red[(wave * R16 + q * 16 + 4 * j + e) * 16 + r] = acc[q][e];
+        __syncthreads();
+        for (int o = threadIdx.x; o < WN * M * 16; o += kWaves * 64) {
+            const int c = o & 15, mt = o >> 4, m = mt % M, tn = mt / M, n = (t0 + tn) * kTileRows + c;
+            if (n < a.N) {
+                float v = 0.f;
+#pragma unroll
+                for (int q = P - 1; q >= 0; --q)             // the small parts first
+                    for (int w = 0; w < p.wk; ++w) v += s_red[((tn * p.wk + w) * R16 + q * M + m) * 16 + c];
+                if (a.bias) v += Act<T>::load(static_cast<const T*>(a.bias) + n);
+                Act<T>::store(static_cast<T*>(a.y) + (m0 + m) * a.ldy + n, v);
+            }
         }
         __syncthreads();
     }
@@ -100,10 +265,14 @@ __global__ void __launch_bounds__(256) dequantize_w4_kernel(const W4Args a) {
 // (T, S, G, Z) of a call
 #define MTL_W4_G(KERNEL, T, S, Z, ...)                                             \
     switch (group) {                                                               \
-        case 32: hipLaunchKernelGGL((KERNEL<T, S, 32, Z>), __VA_ARGS__); break;    \
-        case 64: hipLaunchKernelGGL((KERNEL<T, S, 64, Z>), __VA_ARGS__); break;    \
-        default: hipLaunchKernelGGL((KERNEL<T, S, 128, Z>), __VA_ARGS__); break;   \
+        case 32: hipLaunchKernelGGL((KERNEL(T, S, 32, Z)), __VA_ARGS__); break;    \
+        case 64: hipLaunchKernelGGL((KERNEL(T, S, 64, Z)), __VA_ARGS__); break;    \
+        default: hipLaunchKernelGGL((KERNEL(T, S, 128, Z)), __VA_ARGS__); break;   \
     }
+#define MTL_LINEAR_1(T, S, G, Z) linear_w4_kernel<T, S, G, Z, 1>
+#define MTL_LINEAR_2(T, S, G, Z) linear_w4_kernel<T, S, G, Z, 2>
+#define MTL_LINEAR_3(T, S, G, Z) linear_w4_kernel<T, S, G, Z, 3>
+#define MTL_MATRIX(T, S, G, Z) dequantize_w4_kernel<T, S, G, Z>
 #define MTL_W4_Z(KERNEL, T, S, ...)                        \
     if (a.zeros) { MTL_W4_G(KERNEL, T, S, true, __VA_ARGS__) } else { MTL_W4_G(KERNEL, T, S, false, __VA_ARGS__) }
 #define MTL_W4(KERNEL, ...)                                                                                     \
@@ -147,8 +316,23 @@ extern "C" int mtl_linear_w4(const mtl_linear_w4_args* p, mtl_stream_t stream) {
     MTL_REQUIRE(reinterpret_cast<uintptr_t>(p->zeros) % 4 == 0, "zeros must be 4-byte aligned");
     const W4Args a{p->x, p->codes, p->scales, p->zeros, p->bias, p->y, p->ldx, p->ldy, (int)p->M, (int)p->N, (int)p->K,
                    (int)((p->K + kBlockK - 1) / kBlockK)};
-    const int tiles = (int)((p->N + kTileRows - 1) / kTileRows);
-    MTL_W4(linear_w4_kernel, dim3(tiles), dim3(256), 0, as_stream(stream), a)
+    const int es = dtype == MTL_F32 ? 4 : 2, parts = dtype == MTL_F32 ? 3 : 1, ng = kBlockK / group;
+    LinearW4 l{a, 0, 0, 1, reinterpret_cast<uintptr_t>(p->x) % 16 == 0 && p->ldx * es % 16 == 0};
+    const int chunks = (a.M * parts + 47) / 48;              // 48 operand rows a workgroup
+    l.rows = (a.M + chunks - 1) / chunks;
+    const int tm = (l.rows * parts + 15) / 16, tiles = (a.N + kTileRows - 1) / kTileRows;
+    const int per_block = kBlockK * 2 * parts * l.rows + ng * tm * 64;     // x and the groups' sums
+    l.kblocks = std::min(a.KB, (kLdsBytes - kWaves * tm * 1024 - 16 * parts * l.rows) / per_block);
+    // about 16 wavefronts for each of 256 CUs, on no less than a block each
+    while (l.wk < kWaves && tiles * l.wk < 4096 && l.wk * 2 <= l.kblocks) l.wk *= 2;
+    const int groups = (tiles + kWaves / l.wk - 1) / (kWaves / l.wk), passes = (groups + 511) / 512;
+    const dim3 grid((groups + passes - 1) / passes, chunks);
+    const size_t lds = (size_t)l.kblocks * per_block + 16 * parts * l.rows + kWaves * tm * 1024;
+    switch (tm) {
+        case 1: MTL_W4(MTL_LINEAR_1, grid, dim3(kWaves * 64), lds, as_stream(stream), l) break;
+        case 2: MTL_W4(MTL_LINEAR_2, grid, dim3(kWaves * 64), lds, as_stream(stream), l) break;
+        default: MTL_W4(MTL_LINEAR_3, grid, dim3(kWaves * 64), lds, as_stream(stream), l) break;
+    }
     return check_launch("linear_w4");
 }
 
@@ -165,6 +349,6 @@ extern "C" int mtl_dequantize_w4(const uint8_t* codes, const void* scales, const
                    (int)((K + kBlockK - 1) / kBlockK)};
     const int64_t tiles = (N + kTileRows - 1) / kTileRows;
     const dim3 grid((a.KB + 3) / 4, (unsigned)std::min<int64_t>(tiles, 65535), (unsigned)((tiles + 65534) / 65535));
-    MTL_W4(dequantize_w4_kernel, grid, dim3(256), 0, as_stream(stream), a)
+    MTL_W4(MTL_MATRIX, grid, dim3(256), 0, as_stream(stream), a)
     return check_launch("dequantize_w4");
 }
