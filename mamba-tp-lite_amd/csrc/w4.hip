@@ -37,8 +37,10 @@ template <typename S> __device__ __forceinline__ float scale_at(const void* p, i
 typedef __bf16 B8h __attribute__((ext_vector_type(8)));
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 8;                  // wavefronts of a workgroup
-constexpr int kLdsBytes = 79 << 10;        // of a workgroup: two fit a CU
+constexpr int kWaves = 16;                 // most wavefronts of a workgroup
+constexpr uint32_t kWide = 0x6f800000u;    // 2^96
+constexpr int kAhead = 4;                  // blocks of W that a wavefront has in flight
+constexpr int kLdsBytes = 158 << 10;
 
 struct LinearW4 {
     W4Args a;
@@ -57,94 +59,173 @@ template <typename S, int NG> struct alignas(sizeof(S) * NG) Scales {        // 
 };
 
 // Products on the bf16 matrix cores, exact: a code is the bf16 number 16 + q (its four bits under an exponent), x in
-// float32 the sum of three bf16 numbers of 8 significand bits each, as rows of their own.  A group's sums
-// sum x (16 + q) run in fp32 on v_mfma_f32_16x16x32_bf16, then
-//   acc += s (sum x (16 + q) - (16 + z) sum x),  sum x made once per workgroup and kept beside x in LDS.
-// 8 vector instructions unpack the 8 codes of a word; making q - z first, in fp32, would take three times that.
+// float32 the sum of three bf16 numbers of 8 significand bits each, as rows of their own.  A group's sums run in fp32 on
+// v_mfma_f32_16x16x32_bf16, whose second operand is once 16 + q and once -(16 + z), the same for the whole group:
+//   acc += s sum x ((16 + q) - (16 + z))
+// 8 vector instructions unpack the 8 codes of a word; making q - z first, in fp32, would take three times that, and the
+// matrix cores idle meanwhile.
 //
-// A workgroup keeps x, as the operand's 16-byte runs, in LDS; each wavefront streams tiles of W into
-// registers, kAhead blocks before their use.  Where there are few tiles, wk wavefronts share one and add their sums in order.
+// A workgroup keeps x, as the operand's 16-byte runs, in LDS; each wavefront streams tiles of W into registers, kAhead
+// blocks before their use.  Where there are few tiles, wk wavefronts share one and add their sums in order.
 //
-// |x| >= 2^96, infinities and NaN would spoil the difference: a block of columns in which some row holds one takes
-// the products weight by weight instead, as the matrix form would round them.
+// |x| >= 2^96, infinities and NaN would spoil the difference: a part of x in which some row holds one takes the products
+// weight by weight instead, as the matrix form would round them.
 template <typename T, typename S, int G, bool Z, int TM>
-__global__ void __launch_bounds__(kWaves * 64, 4) linear_w4_kernel(const LinearW4 p) {
-    constexpr int NG = kBlockK / G, P = sizeof(T) == 4 ? 3 : 1, R16 = TM * 16, kAhead = 4;
+__global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p) {
+    constexpr int NG = kBlockK / G, P = sizeof(T) == 4 ? 3 : 1, R16 = TM * 16;
     extern __shared__ __align__(16) uint8_t smem[];
     const W4Args& a = p.a;
     const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m0 = blockIdx.y * p.rows, M = min(p.rows, a.M - m0), R = P * M;
-    const int wn = wave / p.wk, wkid = wave - wn * p.wk, WN = kWaves / p.wk;
+    const int threads = blockDim.x, wn = wave / p.wk, wkid = wave - wn * p.wk, WN = threads / 64 / p.wk;
     const T* x = static_cast<const T*>(a.x) + m0 * a.ldx;
     const int pitch = p.kblocks * 16 + 1;                     // (+ 1: the 16 rows of an operand start in different banks)
     U4* s_x = reinterpret_cast<U4*>(smem);                    // [R][k / 8]
-    float* s_sum = reinterpret_cast<float*>(s_x + P * p.rows * pitch);                         // [group][R16]
     int at_x[TM];
 #pragma unroll
     for (int q = 0; q < TM; ++q) at_x[q] = min(q * 16 + r, R - 1) * pitch + j;
-    float* s_red = s_sum + p.kblocks * NG * R16;                                               // [wave][R16][16]
+    float* s_red = reinterpret_cast<float*>(s_x + P * p.rows * pitch);                         // [wave][R16][16]
     __shared__ int s_wide;
 
-    auto stage = [&](int kb0, int nb) {
-        if (threadIdx.x == 0) s_wide = 0;
-        __syncthreads();
+    // x to LDS: a thread takes 8 columns of a row at a time, kUnits of them in flight
+    constexpr int kRaw = 8 * (int)sizeof(T) / 16, kUnits = 4 / kRaw;
+    U4 raw[kUnits][kRaw];
+    auto fetch = [&](int kb0, int nb, int u0) __attribute__((always_inline)) {
         const int n8 = nb * 16;
-        for (int u = threadIdx.x; u < M * n8; u += kWaves * 64) {
-            const int m = u / n8, k8 = u - m * n8, k = kb0 * kBlockK + k8 * 8;
+#pragma unroll
+        for (int n = 0; n < kUnits; ++n) {
+            const int u = min(u0 + n * threads, M * n8 - 1), m = u / n8, k = kb0 * kBlockK + (u - m * n8) * 8;
             const T* src = x + m * a.ldx + k;
-            float v[8];
             if (p.xvec && k + 8 <= a.K) {
-                const F4v lo = ld4(src), hi = ld4(src + 4);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+                for (int q = 0; q < kRaw; ++q) raw[n][q] = reinterpret_cast<const U4*>(src)[q];
             } else {
+                T v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = k + e < a.K ? Act<T>::load(src + e) : 0.f;
+                for (int e = 0; e < 8; ++e) v[e] = k + e < a.K ? src[e] : T(0);
+                __builtin_memcpy(raw[n], v, sizeof(v));
             }
-            bool wide = false;
+        }
+    };
+    auto put = [&](int nb, int u0) __attribute__((always_inline)) {
+        const int n8 = nb * 16;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) wide |= !(fabsf(v[e]) < 0x1p96f);
-            if (wide) s_wide = 1;
+        for (int n = 0; n < kUnits; ++n) {
+            const int u = u0 + n * threads;
+            if (u >= M * n8) break;
+            const int m = u / n8, k8 = u - m * n8;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[e] = sizeof(T) == 4 ? __uint_as_float(raw[n][e / 4 % kRaw][e % 4])
+                                      : __uint_as_float(raw[n][0][e / 2] << (e % 2 ? 0 : 16) & 0xffff0000u);
+            uint32_t most = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = max(most, abs_bits(v[e]));
+            if (most >= kWide) s_wide = 1;
 #pragma unroll
             for (int q = 0; q < P; ++q) {
                 U4 part;
-                float sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
-                    const uint32_t b0 = __float_as_uint(v[e]) & 0xffff0000u, b1 = __float_as_uint(v[e + 1]) & 0xffff0000u;
-                    part[e / 2] = b0 >> 16 | b1;
-                    sum += __uint_as_float(b0) + __uint_as_float(b1);
-                    v[e] -= __uint_as_float(b0);
-                    v[e + 1] -= __uint_as_float(b1);
+                    part[e / 2] = __builtin_amdgcn_perm(__float_as_uint(v[e + 1]), __float_as_uint(v[e]), 0x07060302);
+                    v[e] -= __uint_as_float(__float_as_uint(v[e]) & 0xffff0000u);
+                    v[e + 1] -= __uint_as_float(__float_as_uint(v[e + 1]) & 0xffff0000u);
                 }
                 s_x[(q * M + m) * pitch + k8] = part;
-                // a group's columns lie in neighbouring lanes (n8 is a multiple of 16)
-                sum += dpp_mov<kDppXor1>(sum);
-                sum += dpp_mov<kDppXor2>(sum);
-                if constexpr (G >= 64) sum += dpp_mov<kDppHalfMirror>(sum);
-                if constexpr (G >= 128) sum += dpp_mov<kDppRowMirror>(sum);
-                if (k8 % (G / 8) == 0) s_sum[k8 / (G / 8) * R16 + q * M + m] = sum;
             }
         }
-        __syncthreads();
     };
 
     const int tiles = (a.N + kTileRows - 1) / kTileRows;
     const bool once = p.kblocks >= a.KB;
-    if (once) stage(0, a.KB);
-    for (int t0 = blockIdx.x * WN; t0 < tiles; t0 += gridDim.x * WN) {
-        const int64_t t = min(t0 + wn, tiles - 1);           // (past the last tile: computed again, not stored)
+
+    // kAhead blocks of W in registers; as one is used up, the block kAhead further on (of the next tile, after the
+    // last) is loaded in its place, so the stream never stops at the end of a tile
+    U4 w[kAhead];
+    Scales<S, NG> sc[kAhead];
+    Scales<uint8_t, NG> zr[kAhead];
+    auto load = [&](int u, int t, int kb) __attribute__((always_inline)) {
+        const int64_t b = (int64_t)min(t, tiles - 1) * a.KB + min(kb + u * p.wk, a.KB - 1);
+        w[u] = __builtin_nontemporal_load(reinterpret_cast<const U4*>(a.codes) + b * 64 + lane);
+        sc[u] = static_cast<const Scales<S, NG>*>(a.scales)[b * kTileRows + r];
+        if constexpr (Z) zr[u] = reinterpret_cast<const Scales<uint8_t, NG>*>(a.zeros)[b * kTileRows + r];
+    };
+    const int stride = gridDim.x * WN;
+    int t = blockIdx.x * WN + wn;
+    // (x before W: what waits for x then does not wait for W, whose loads return after it)
+    fetch(0, min(p.kblocks, a.KB), threadIdx.x);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) load(u, t, wkid);
+    __builtin_amdgcn_sched_barrier(0);
+    if (threadIdx.x == 0) s_wide = 0;
+    __syncthreads();
+    bool staged = false;
+    for (int t0 = blockIdx.x * WN; t0 < tiles; t0 += stride, t += stride) {
         F4v acc[TM];
 #pragma unroll
         for (int q = 0; q < TM; ++q) acc[q] = F4v{0.f, 0.f, 0.f, 0.f};
         for (int kb0 = 0; kb0 < a.KB; kb0 += p.kblocks) {
             const int kb1 = min(kb0 + p.kblocks, a.KB);
-            if (!once) {
+            if (!once || !staged) {
+                const int nb = kb1 - kb0;
+                if (staged) {
+                    __syncthreads();
+                    if (threadIdx.x == 0) s_wide = 0;
+                    fetch(kb0, nb, threadIdx.x);
+                    __syncthreads();
+                }
+                put(nb, threadIdx.x);
+                for (int u = threadIdx.x + kUnits * threads; u < M * nb * 16; u += kUnits * threads) {
+                    fetch(kb0, nb, u);
+                    put(nb, u);
+                }
+                staged = true;
                 __syncthreads();
-                stage(kb0, kb1 - kb0);
             }
-            if (s_wide) {
+            const bool wide = s_wide;
+            for (int kb = kb0 + wkid; kb < kb1; kb += kAhead * p.wk) {
+                const bool more = kb + kAhead * p.wk < a.KB;
+                const int tn = more ? t : t + stride, kbn = more ? kb + kAhead * p.wk : wkid;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int kc = kb + u * p.wk - kb0;
+                    if (kc < kb1 - kb0 && !wide) {
+                        F4v part[TM];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (i % (G / 32) == 0) {
+#pragma unroll
+                                for (int q = 0; q < TM; ++q) part[q] = F4v{0.f, 0.f, 0.f, 0.f};
+                            }
+                            const uint32_t c = w[u][i];
+                            const U4 b = {(c << 3 & 0x00780078u) | 0x41804180u, (c >> 1 & 0x00780078u) | 0x41804180u,
+                                          (c >> 5 & 0x00780078u) | 0x41804180u, (c >> 9 & 0x00780078u) | 0x41804180u};
+                            // - (16 + z) in bf16, for every column
+                            uint32_t z = 0xc1c0c1c0u;
+                            if constexpr (Z) z = __float_as_uint(-16.f - (float)zr[u].v[i / (G / 32)]) >> 16 | __float_as_uint(-16.f - (float)zr[u].v[i / (G / 32)]);
+#pragma unroll
+                            for (int q = 0; q < TM; ++q) {
+                                const B8h xa = __builtin_bit_cast(B8h, s_x[at_x[q] + kc * 16 + i * 4]);
+                                part[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa, __builtin_bit_cast(B8h, b), part[q], 0, 0, 0);
+                                part[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa, __builtin_bit_cast(B8h, U4{z, z, z, z}), part[q], 0, 0, 0);
+                            }
+                            if (i % (G / 32) == G / 32 - 1) {
+                                const float s = sc[u].at(i / (G / 32));
+#pragma unroll
+                                for (int q = 0; q < TM; ++q)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) acc[q][e] = fmaf(s, part[q][e], acc[q][e]);
+                            }
+                        }
+                    }
+                    load(u, tn, kbn);
+                }
+            }
+            if (wide) {
+                const int64_t tb = (int64_t)min(t, tiles - 1) * a.KB;
 #pragma unroll 1
                 for (int m = 0; m < M; ++m) {
                     float v = 0.f;
@@ -152,13 +233,13 @@ __global__ void __launch_bounds__(kWaves * 64, 4) linear_w4_kernel(const LinearW
                     for (int kb = kb0 + wkid; kb < kb1; kb += p.wk) {
 #pragma unroll 1
                         for (int i = 0; i < 4; ++i) {
-                            const uint32_t w = reinterpret_cast<const uint32_t*>(a.codes)[((t * a.KB + kb) * 64 + lane) * 4 + i];
-                            const int64_t at = ((t * a.KB + kb) * kTileRows + r) * NG + 32 * i / G;
+                            const uint32_t c = reinterpret_cast<const uint32_t*>(a.codes)[((tb + kb) * 64 + lane) * 4 + i];
+                            const int64_t at = ((tb + kb) * kTileRows + r) * NG + 32 * i / G;
                             const float s = scale_at<S>(a.scales, at), z = Z ? (float)a.zeros[at] : 8.f;
                             const int k = kb * kBlockK + 32 * i + 8 * j;
 #pragma unroll
                             for (int e = 0; e < 8; ++e)
-                                if (k + e < a.K) v = fmaf(Act<T>::load(x + m * a.ldx + k + e), s * ((float)code_of(w, e) - z), v);
+                                if (k + e < a.K) v = fmaf(Act<T>::load(x + m * a.ldx + k + e), s * ((float)code_of(c, e) - z), v);
                         }
                     }
                     v += __shfl_xor(v, 16);
@@ -168,53 +249,6 @@ __global__ void __launch_bounds__(kWaves * 64, 4) linear_w4_kernel(const LinearW
                     for (int q = 0; q < TM * 4; ++q)
                         if ((m >> 4) * 4 + (m & 3) == q && ((m >> 2) & 3) == j) acc[q >> 2][q & 3] += v;
                 }
-                continue;
-            }
-            for (int kb = kb0 + wkid; kb < kb1; kb += kAhead * p.wk) {
-                U4 w[kAhead];
-                Scales<S, NG> sc[kAhead];
-                Scales<uint8_t, NG> zr[kAhead];
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    const int64_t b = t * a.KB + min(kb + u * p.wk, kb1 - 1);
-                    w[u] = __builtin_nontemporal_load(reinterpret_cast<const U4*>(a.codes) + b * 64 + lane);
-                    sc[u] = static_cast<const Scales<S, NG>*>(a.scales)[b * kTileRows + r];
-                    if constexpr (Z) zr[u] = reinterpret_cast<const Scales<uint8_t, NG>*>(a.zeros)[b * kTileRows + r];
-                }
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    const int kc = kb + u * p.wk - kb0;
-                    if (kc >= kb1 - kb0) break;
-                    F4v part[TM];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (i % (G / 32) == 0) {
-#pragma unroll
-                            for (int q = 0; q < TM; ++q) part[q] = F4v{0.f, 0.f, 0.f, 0.f};
-                        }
-                        const uint32_t c = w[u][i];
-                        const U4 b = {(c << 3 & 0x00780078u) | 0x41804180u, (c >> 1 & 0x00780078u) | 0x41804180u,
-                                      (c >> 5 & 0x00780078u) | 0x41804180u, (c >> 9 & 0x00780078u) | 0x41804180u};
-#pragma unroll
-                        for (int q = 0; q < TM; ++q) {
-                            const U4 xa = s_x[at_x[q] + kc * 16 + i * 4];
-                            part[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(B8h, xa),
-                                                                              __builtin_bit_cast(B8h, b), part[q], 0, 0, 0);
-                        }
-                        if (i % (G / 32) == G / 32 - 1) {
-                            const int g = i / (G / 32);
-                            const float s = sc[u].at(g);
-                            float c16 = 24.f;
-                            if constexpr (Z) c16 = 16.f + (float)zr[u].v[g];
-#pragma unroll
-                            for (int q = 0; q < TM; ++q) {
-                                const F4v sx = *reinterpret_cast<const F4v*>(&s_sum[(kc * NG + g) * R16 + q * 16 + 4 * j]);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) acc[q][e] = fmaf(s, fmaf(-c16, sx[e], part[q][e]), acc[q][e]);
-                            }
-                        }
-                    }
-                }
             }
         }
         // D[i][j]: row 4 (lane / 16) + i of x, row lane % 16 of W
@@ -222,19 +256,29 @@ __global__ void __launch_bounds__(kWaves * 64, 4) linear_w4_kernel(const LinearW
         for (int q = 0; q < TM; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s_red[(wave * R16 + q * 16 + 4 * j + e) * 16 + r] = acc[q][e];
-        __syncthreads();
-        for (int o = threadIdx.x; o < WN * M * 16; o += kWaves * 64) {
-            const int c = o & 15, mt = o >> 4, m = mt % M, tn = mt / M, n = (t0 + tn) * kTileRows + c;
-            if (n < a.N) {
-                float v = 0.f;
+        auto store = [&](int tile, int first, int m, int c) __attribute__((always_inline)) {
+            const int n = tile * kTileRows + c;
+            if (n >= a.N) return;
+            float v = 0.f;
 #pragma unroll
-                for (int q = P - 1; q >= 0; --q)             // the small parts first
-                    for (int w = 0; w < p.wk; ++w) v += s_red[((tn * p.wk + w) * R16 + q * M + m) * 16 + c];
-                if (a.bias) v += Act<T>::load(static_cast<const T*>(a.bias) + n);
-                Act<T>::store(static_cast<T*>(a.y) + (m0 + m) * a.ldy + n, v);
+            for (int q = P - 1; q >= 0; --q)                 // the small parts first
+#pragma unroll 4
+                for (int k = 0; k < p.wk; ++k) v += s_red[((first + k) * R16 + q * M + m) * 16 + c];
+            if (a.bias) v += Act<T>::load(static_cast<const T*>(a.bias) + n);
+            Act<T>::store(static_cast<T*>(a.y) + (m0 + m) * a.ldy + n, v);
+        };
+        if (p.wk == 1) {                                     // a wavefront's own sums: no other waits for it
+            __builtin_amdgcn_wave_barrier();
+            for (int m = j; m < M; m += 4) store(t, wave, m, r);
+            __builtin_amdgcn_wave_barrier();
+        } else {
+            __syncthreads();
+            for (int o = threadIdx.x; o < WN * M * 16; o += threads) {
+                const int mt = o >> 4, ti = mt / M;
+                store(t0 + ti, ti * p.wk, mt - ti * M, o & 15);
             }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
@@ -316,22 +360,38 @@ extern "C" int mtl_linear_w4(const mtl_linear_w4_args* p, mtl_stream_t stream) {
     MTL_REQUIRE(reinterpret_cast<uintptr_t>(p->zeros) % 4 == 0, "zeros must be 4-byte aligned");
     const W4Args a{p->x, p->codes, p->scales, p->zeros, p->bias, p->y, p->ldx, p->ldy, (int)p->M, (int)p->N, (int)p->K,
                    (int)((p->K + kBlockK - 1) / kBlockK)};
-    const int es = dtype == MTL_F32 ? 4 : 2, parts = dtype == MTL_F32 ? 3 : 1, ng = kBlockK / group;
+    const int es = dtype == MTL_F32 ? 4 : 2, parts = dtype == MTL_F32 ? 3 : 1;
     LinearW4 l{a, 0, 0, 1, reinterpret_cast<uintptr_t>(p->x) % 16 == 0 && p->ldx * es % 16 == 0};
-    const int chunks = (a.M * parts + 47) / 48;              // 48 operand rows a workgroup
-    l.rows = (a.M + chunks - 1) / chunks;
-    const int tm = (l.rows * parts + 15) / 16, tiles = (a.N + kTileRows - 1) / kTileRows;
-    const int per_block = kBlockK * 2 * parts * l.rows + ng * tm * 64;     // x and the groups' sums
-    l.kblocks = std::min(a.KB, (kLdsBytes - kWaves * tm * 1024 - 16 * parts * l.rows) / per_block);
-    // about 16 wavefronts for each of 256 CUs, on no less than a block each
-    while (l.wk < kWaves && tiles * l.wk < 4096 && l.wk * 2 <= l.kblocks) l.wk *= 2;
-    const int groups = (tiles + kWaves / l.wk - 1) / (kWaves / l.wk), passes = (groups + 511) / 512;
+    const int tiles = (a.N + kTileRows - 1) / kTileRows;
+    // At most 48 operand rows a workgroup (16 of fp32 x), fewer where that leaves the GPU short of workgroups
+    int tm = 3, chunks, groups, wn;
+    size_t lds;
+    for (;; --tm) {
+        chunks = (a.M + tm * 16 / parts - 1) / (tm * 16 / parts);
+        l.rows = (a.M + chunks - 1) / chunks;
+        tm = (l.rows * parts + 15) / 16;
+        const int per_block = kBlockK * 2 * parts * l.rows;
+        // (at most 12 KiB, so at least 4 blocks fit)
+        l.kblocks = std::min(a.KB, (kLdsBytes - kWaves * tm * 1024 - 16 * parts * l.rows) / per_block);
+        // about 16 wavefronts for each of 256 CUs, on no less than a block each
+        l.wk = 1;
+        while (l.wk < kWaves && tiles * chunks * l.wk < 4096 && l.wk * 2 <= l.kblocks) l.wk *= 2;
+        if (l.kblocks < a.KB) {                              // whole batches of every wavefront in each part of x
+            while (l.wk > 1 && l.wk * kAhead > l.kblocks) l.wk /= 2;
+            l.kblocks -= l.kblocks % (l.wk * kAhead);
+        }
+        // tiles side by side in a workgroup share x: as many as leave a workgroup for every CU
+        wn = std::max(1, std::min(kWaves / l.wk, tiles * chunks / 256));
+        lds = (size_t)l.kblocks * per_block + 16 * parts * l.rows + wn * l.wk * tm * 1024;
+        groups = (tiles + wn - 1) / wn;
+        if (tm == 1 || groups * chunks >= 256) break;
+    }
+    const int passes = (groups * chunks + 255) / 256;
     const dim3 grid((groups + passes - 1) / passes, chunks);
-    const size_t lds = (size_t)l.kblocks * per_block + 16 * parts * l.rows + kWaves * tm * 1024;
     switch (tm) {
-        case 1: MTL_W4(MTL_LINEAR_1, grid, dim3(kWaves * 64), lds, as_stream(stream), l) break;
-        case 2: MTL_W4(MTL_LINEAR_2, grid, dim3(kWaves * 64), lds, as_stream(stream), l) break;
-        default: MTL_W4(MTL_LINEAR_3, grid, dim3(kWaves * 64), lds, as_stream(stream), l) break;
+        case 1: MTL_W4(MTL_LINEAR_1, grid, dim3(wn * l.wk * 64), lds, as_stream(stream), l) break;
+        case 2: MTL_W4(MTL_LINEAR_2, grid, dim3(wn * l.wk * 64), lds, as_stream(stream), l) break;
+        default: MTL_W4(MTL_LINEAR_3, grid, dim3(wn * l.wk * 64), lds, as_stream(stream), l) break;
     }
     return check_launch("linear_w4");
 }

@@ -1306,34 +1306,54 @@ def _overlap(a, b) -> bool:
 def linear_w4(x, w4, bias=None, out=None):
     """x [..., k] W^T (+ bias [n]) for at most W4_MAX_ROWS rows of x, W [n, k] in 4-bit codes (mtl_linear_w4); float32
     or bfloat16, summed in float32.  More rows: dequantize_w4 and a matrix product.  Returns [..., n]."""
-    if not isinstance(w4, W4):
+    # (a decode step is bound by the host: every check here is a plain comparison)
+    if type(w4) is not W4:
         raise TypeError(f"linear_w4: w4 must be a W4 (pack_w4, quantize_w4), got {type(w4).__name__}")
-    if x.dim() < 1 or x.shape[-1] != w4.k:
-        raise ValueError(f"x must be [..., {w4.k}], got {tuple(x.shape)}")
-    code = _act_code(x, bias, out)
-    _same_device(x, w4.codes, bias, out)
-    _no_grad_recorded("linear_w4", x, bias)
-    shape = (*x.shape[:-1], w4.n)
-    x2, ldx = _rows_of(x, w4.k)
-    M = x2.shape[0]
+    n, k, codes, scales = w4.n, w4.k, w4.codes, w4.scales
+    dt, shape = x.dtype, x.shape
+    code = _ACT_DTYPES.get(dt)
+    if code is None:
+        raise TypeError(f"x must be float32 or bfloat16, got {dt}")
+    if not shape or shape[-1] != k:
+        raise ValueError(f"x must be [..., {k}], got {tuple(shape)}")
+    if codes.get_device() != x.get_device():
+        raise RuntimeError(f"all operands must be on one device, got x on {x.device}, w4 on {codes.device}")
+    if torch.is_grad_enabled():
+        _no_grad_recorded("linear_w4", x, bias)
+    if x.is_contiguous():
+        M, ldx = x.numel() // k, k
+    else:
+        x, ldx = _rows_of(x, k)
+        M = x.shape[0]
     if M > W4_MAX_ROWS:
         raise ValueError(f"linear_w4 takes at most {W4_MAX_ROWS} rows of x, got {M}")
-    if bias is not None and (tuple(bias.shape) != (w4.n,) or not bias.is_contiguous()):
-        raise ValueError(f"bias must be contiguous [{w4.n}], got {tuple(bias.shape)}")
+    if bias is not None and (bias.dtype != dt or bias.shape != (n,) or not bias.is_contiguous()):
+        if bias.dtype != dt:
+            raise TypeError(f"bias must be {dt} like x, got {bias.dtype}")
+        raise ValueError(f"bias must be contiguous [{n}], got {tuple(bias.shape)}")
+    ldy = n
     if out is None:
-        out = torch.empty(shape, device=x.device, dtype=x.dtype)
-        ldy = w4.n
+        out = x.new_empty((*shape[:-1], n))
     else:
-        if tuple(out.shape) != shape or not (out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1
-                                                                     and out.stride(0) >= w4.n)):
-            raise ValueError(f"out must be {shape} with contiguous rows, got {tuple(out.shape)} strides {out.stride()}")
-        if any(t is not None and _overlap(out, t) for t in (x2, bias, w4.codes, w4.scales, w4.zeros)):
+        if out.dtype != dt:
+            raise TypeError(f"out must be {dt} like x, got {out.dtype}")
+        if tuple(out.shape) != (*shape[:-1], n) or not (out.is_contiguous() or (
+                out.dim() == 2 and out.stride(1) == 1 and out.stride(0) >= n)):
+            raise ValueError(f"out must be {(*shape[:-1], n)} with contiguous rows, got {tuple(out.shape)} strides "
+                             f"{out.stride()}")
+        if any(t is not None and _overlap(out, t) for t in (x, bias, codes, scales, w4.zeros)):
             raise ValueError("out must not overlap an operand")
-        ldy = out.stride(0) if out.dim() == 2 and M > 1 else w4.n
-    a = _lib.LinearW4Args(_ptr(x2), _ptr(w4.codes), _ptr(w4.scales), _ptr(w4.zeros), _ptr(bias), _ptr(out), ldx, ldy, M,
-                          w4.n, w4.k, w4.group, code, _ACT_DTYPES[w4.scales.dtype], 0)
+        if out.dim() == 2 and M > 1:
+            ldy = out.stride(0)
+    if bias is not None or w4.zeros is not None:
+        _same_device(x, bias, w4.zeros)
+    _same_device(x, out)
+    a = _lib.LinearW4Args(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(w4.zeros), _ptr(bias), out.data_ptr(),
+                          ldx, ldy, M, n, k, w4.group, code, _ACT_DTYPES[scales.dtype])
     with _dev_guard(x):
-        _lib.check(_lib.load().mtl_linear_w4(ctypes.byref(a), _stream(x)), "linear_w4")
+        rc = _lib.load().mtl_linear_w4(ctypes.byref(a), _stream(x))
+    if rc:
+        _lib.check(rc, "linear_w4")
     return out
 
 
@@ -1388,19 +1408,27 @@ def token_logprobs(logits, tokens, top=0):
         raise ValueError(f"top must be in [0, {min(TOP_MAX, V)}], got {top}")
     code = _act_code(logits)
     _same_device(logits, tokens)
-    _no_grad_recorded("token_logprobs", logits)
+    if torch.is_grad_enabled():
+        _no_grad_recorded("token_logprobs", logits)
     x = logits
     if V > 1 and x.stride(-1) != 1:
         x = x.contiguous()
     if x.dim() > 3:
         x = x.reshape(-1, *x.shape[-2:])          # (a view where the strides allow it)
-    x = x.view(*(1,) * (3 - x.dim()), *x.shape) if x.dim() < 3 else x
-    tokens = tokens.contiguous()
-    f = dict(device=x.device, dtype=torch.float32)
-    r = TokenLogprobs(torch.empty(lead, **f), torch.empty(lead, **f), torch.empty(*lead, top, **f),
-                      torch.empty(*lead, top, device=x.device, dtype=torch.int64))
-    a = _lib.TokenLogprobsArgs(_ptr(x), _ptr(tokens), _ptr(r.logprob), _ptr(r.entropy), _ptr(r.top_logprob),
-                               _ptr(r.top_token), x.shape[0], x.shape[1], x.stride(0), x.stride(1), V, top, code)
+    if x.dim() == 3:
+        (outer, inner, _), (so, si, _) = x.shape, x.stride()
+    elif x.dim() == 2:
+        outer, inner, so, si = 1, x.shape[0], 0, x.stride(0)
+    else:
+        outer = inner = 1
+        so = si = 0
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    lp = torch.empty_like(tokens, dtype=torch.float32)
+    top_token = tokens.new_empty((*lead, top))
+    r = TokenLogprobs(lp, torch.empty_like(lp), torch.empty_like(top_token, dtype=torch.float32), top_token)
+    a = _lib.TokenLogprobsArgs(x.data_ptr(), tokens.data_ptr(), r.logprob.data_ptr(), r.entropy.data_ptr(),
+                               r.top_logprob.data_ptr(), r.top_token.data_ptr(), outer, inner, so, si, V, top, code)
     with _dev_guard(x):
         _lib.check(_lib.load().mtl_token_logprobs(ctypes.byref(a), _stream(x)), "token_logprobs")
     return r
