@@ -29,11 +29,16 @@ struct Sums {
 
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-    const float m = fmaxf(a.m, b.m), base = base_of(m);
-    const float da = fmaxf(a.m - base, -1e30f), db = fmaxf(b.m - base, -1e30f);
-    const float ea = fast_exp(da), eb = fast_exp(db);
-    return {m, ea * a.s + eb * b.s, ea * fmaf(da, a.s, a.t) + eb * fmaf(db, b.s, b.t)};
+// a's sums relative to the maximum m >= a.m
+__device__ __forceinline__ void rescale(Sums& a, float m) {
+    const float d = fmaxf(a.m - base_of(m), -1e30f), e = fast_exp(d);
+    a = {m, e * a.s, e * fmaf(d, a.s, a.t)};
+}
+// the sums of 16 or 64 lanes
+template <int WIDTH>
+__device__ __forceinline__ Sums group_join(Sums a) {
+    rescale(a, group_max<WIDTH>(a.m));
+    return {a.m, group_sum<WIDTH>(a.s), group_sum<WIDTH>(a.t)};
 }
 
 // An order of (value, index): larger value first, then lower index.  0: no value (-inf never is an alternative).
@@ -51,55 +56,79 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 __device__ __forceinline__ uint64_t lane_read64(uint64_t v, int lane) {
     return uint64_t(lane_read_u(uint32_t(v >> 32), lane)) << 32 | lane_read_u(uint32_t(v), lane);
 }
-__device__ __forceinline__ uint64_t xor_read64(uint64_t v, int m) {
-    return uint64_t(uint32_t(__shfl_xor(int(v >> 32), m))) << 32 | uint32_t(__shfl_xor(int(v), m));
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_mov64(uint64_t v) {
+    return uint64_t(dpp_mov_u<CTRL>(uint32_t(v >> 32))) << 32 | dpp_mov_u<CTRL>(uint32_t(v));
+}
+// the value of lane ^ M
+template <int M>
+__device__ __forceinline__ uint64_t xor_read64(uint64_t v) {
+    constexpr int kQuadReverse = 0x1B, kRowRor8 = 0x128;
+    if constexpr (M == 1) return dpp_mov64<kDppXor1>(v);
+    else if constexpr (M == 2) return dpp_mov64<kDppXor2>(v);
+    else if constexpr (M == 4) return dpp_mov64<kQuadReverse>(dpp_mov64<kDppHalfMirror>(v));     // 7 ^ 3
+    else if constexpr (M == 8) return dpp_mov64<kRowRor8>(v);
+    else return uint64_t(uint32_t(__shfl_xor(int(v >> 32), M))) << 32 | uint32_t(__shfl_xor(int(v), M));
+}
+// steps of a bitonic sort of the lanes in falling order: within runs of SIZE lanes, from distance M down
+template <int SIZE, int M>
+__device__ __forceinline__ void bitonic_steps(uint64_t& key, int lane) {
+    const uint64_t other = xor_read64<M>(key);
+    if ((other > key) == (((lane & M) == 0) == ((lane & SIZE) == 0))) key = other;
+    if constexpr (M > 1) bitonic_steps<SIZE, M / 2>(key, lane);
+}
+template <int SIZE = 2>
+__device__ __forceinline__ void bitonic_sort(uint64_t& key, int lane) {
+    bitonic_steps<SIZE, SIZE / 2>(key, lane);
+    if constexpr (SIZE < 64) bitonic_sort<SIZE * 2>(key, lane);
+}
+__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
+    const uint32_t hi = group_umax<64>(uint32_t(v >> 32));
+    return uint64_t(hi) << 32 | group_umax<64>(uint32_t(v >> 32) == hi ? uint32_t(v) : 0u);
+}
+// the n-th largest of the lanes' keys (0: the largest); nonzero keys differ
+__device__ __forceinline__ uint64_t nth_largest(uint64_t key, int n, int lane) {
+    if (n >= 8) {
+        bitonic_sort(key, lane);
+        return lane_read64(key, n);
+    }
+    for (; n > 0; --n) key = key == wave_max64(key) ? 0 : key;
+    return wave_max64(key);
 }
 
-// The largest keys of what a wavefront has seen, one a lane in falling order; the first `top` lanes are right, the
-// others hold further keys of it.
-struct TopList {
-    uint64_t key = 0, floor = 0;       // floor: the key of lane top - 1 (0: fewer seen), uniform
+// Candidates of one wavefront for the row's `top` largest keys: those that reach the floor, a key that `top` keys of
+// the row are known to reach.  They wait in LDS (64 to a flush); a flush merges them into a sorted list of 64, one a
+// lane, whose last wanted key is a floor too.
+struct Candidates {
+    uint64_t* wait;                    // [128]
+    uint64_t list = 0, floor = 1;
     float floor_value = -FLT_MAX;      // (above -inf, which never enters)
+    int waiting = 0;
 
-    __device__ __forceinline__ void set_floor(int top) {
-        floor = lane_read64(key, top - 1);
-        floor_value = floor ? key_value(floor) : -FLT_MAX;
-    }
-    // one lane's key each -> in falling order (bitonic)
-    __device__ __forceinline__ void sort(uint64_t mine, int lane, int top) {
-        key = mine;
-#pragma unroll
-        for (int size = 2; size <= 64; size *= 2)
-#pragma unroll
-            for (int m = size / 2; m > 0; m /= 2) {
-                const uint64_t other = xor_read64(key, m);
-                if ((other > key) == (((lane & m) == 0) == ((lane & size) == 0))) key = other;
-            }
-        set_floor(top);
-    }
-    // with another list in falling order: the larger of each and the reversed other are the 64 largest, bitonic
-    __device__ __forceinline__ void merge(uint64_t other, int lane) {
-        other = uint64_t(uint32_t(__shfl(int(other >> 32), 63 - lane))) << 32 | uint32_t(__shfl(int(other), 63 - lane));
-        key = other > key ? other : key;
-#pragma unroll
-        for (int m = 32; m > 0; m /= 2) {
-            const uint64_t x = xor_read64(key, m);
-            if ((x > key) == ((lane & m) == 0)) key = x;
+    __device__ __forceinline__ void raise(uint64_t f) {
+        if (f > floor) {
+            floor = f;
+            floor_value = key_value(f);
         }
     }
-    // every lane's key above the floor, but `skip`
-    __device__ __forceinline__ void insert(uint64_t mine, uint64_t skip, int lane, int top) {
-        bool left = mine != skip;
-        for (uint64_t mask; (mask = __ballot(left && mine > floor)) != 0;) {
-            const int l = __builtin_ctzll(mask);
-            const uint64_t c = lane_read64(mine, l);
-            const int at = __builtin_popcountll(__ballot(key > c));
-            const uint64_t up = uint64_t(uint32_t(__builtin_amdgcn_update_dpp(0, int(key >> 32), kDppWaveShr1, 0xF, 0xF, false))) << 32 |
-                                uint32_t(__builtin_amdgcn_update_dpp(0, int(key), kDppWaveShr1, 0xF, 0xF, false));
-            key = lane < at ? key : lane == at ? c : up;
-            left = left && lane != l;
-            set_floor(top);
-        }
+    __device__ __forceinline__ void add(uint64_t key, int lane, int top) {
+        const bool hit = key >= floor;
+        const uint64_t mask = __ballot(hit);
+        if (hit) wait[waiting + __builtin_popcountll(mask & ((uint64_t(1) << lane) - 1))] = key;
+        waiting += __builtin_popcountll(mask);
+        if (waiting < 64) return;
+        __builtin_amdgcn_wave_barrier();
+        uint64_t k = wait[lane];
+        bitonic_sort(k, lane);
+        // the larger of each and the reversed other list are the 64 largest, in bitonic order
+        k = uint64_t(uint32_t(__shfl(int(k >> 32), 63 - lane))) << 32 | uint32_t(__shfl(int(k), 63 - lane));
+        list = k > list ? k : list;
+        bitonic_steps<64, 32>(list, lane);
+        k = wait[64 + lane];
+        waiting -= 64;
+        __builtin_amdgcn_wave_barrier();
+        if (lane < waiting) wait[lane] = k;
+        raise(lane_read64(list, top - 1));
     }
 };
 
@@ -113,7 +142,9 @@ template <typename T, bool TOP>
 __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
     constexpr int VEC = 16 / (int)sizeof(T);
     __shared__ Sums s_sums[16];
-    __shared__ uint64_t s_list[TOP ? 16 : 1][64];
+    __shared__ uint64_t s_floor[16], s_own[16];
+    __shared__ int s_keys;
+    extern __shared__ __align__(16) uint64_t s_key[];      // TOP: [waves][128] waiting, then 8 more; the same again
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + (row / a.inner) * a.so + (row % a.inner) * a.si;
@@ -143,8 +174,12 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
         }
     };
 
+    if (threadIdx.x == 0) s_keys = 0;
     Sums q = {-INFINITY, 0.f, 0.f};
-    TopList list;
+    Candidates c;
+    uint64_t best = 0;                              // a lane's largest key, where it has reached the floor
+    c.wait = s_key + wave * 128;
+    const int share = TOP ? (a.top - 1) / waves : 0;
     if (wave < tiles) load(wave);
     for (int tile = wave; tile < tiles; tile += waves) {
         float v[kChunks][VEC], most[kChunks];
@@ -164,8 +199,8 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
             m = fmaxf(m, most[u]);
         }
         // (fmaxf drops a NaN; e^NaN reaches s all the same)
-        const float base = base_of(m), d0 = fmaxf(q.m - base, -1e30f), e0 = fast_exp(d0);
-        q = {m, e0 * q.s, e0 * fmaf(d0, q.s, q.t)};
+        rescale(q, m);
+        const float base = base_of(m);
 #pragma unroll
         for (int u = 0; u < kChunks; ++u)
 #pragma unroll
@@ -176,59 +211,103 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
             }
         if constexpr (TOP) {
             const int i0 = (int)((int64_t)tile * kTile * VEC - off) + lane * VEC;
-            uint64_t mine = ~uint64_t(0);
-            if (tile == wave) {                    // the first tile: the lanes' largest make the list
-                mine = 0;
+            if (tile == wave) {
+                // The first tile: each wavefront has share + 1 lanes whose largest reach its f, together `top` or more,
+                // so nothing below the least f is wanted.
 #pragma unroll
                 for (int u = 0; u < kChunks; ++u)
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         const uint64_t k = key_of(v[u][e], i0 + u * 64 * VEC + e);
-                        mine = k > mine ? k : mine;
+                        best = k > best ? k : best;
                     }
-                list.sort(mine, lane, a.top);
+                const uint64_t mine = nth_largest(best, share, lane);
+                if (lane == 0) s_floor[wave] = mine;
+                __syncthreads();
+                uint64_t f = s_floor[min(lane, waves - 1)];
+                f = ~wave_max64(~f);
+                c.raise(f);
             }
+            float all = most[0];
 #pragma unroll
-            for (int u = 0; u < kChunks; ++u) {
-                if (!__any(most[u] >= list.floor_value)) continue;
+            for (int u = 1; u < kChunks; ++u) all = fmaxf(all, most[u]);
+            if (__any(all >= c.floor_value)) {
+                // which of a lane's logits reach the floor; they enter one a lane at a time
+                uint32_t which = 0;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    if (__any(v[u][e] >= list.floor_value))
-                        list.insert(key_of(v[u][e], i0 + u * 64 * VEC + e), mine, lane, a.top);
+                for (int u = 0; u < kChunks; ++u)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) which |= (v[u][e] >= c.floor_value ? 1u : 0u) << (u * VEC + e);
+                while (__any(which != 0)) {
+                    const int e = __builtin_ctz(which | 0x80000000u);
+                    float value = v[0][0];
+#pragma unroll
+                    for (int n = 1; n < kChunks * VEC; ++n) value = e == n ? v[n / VEC][n % VEC] : value;
+                    const uint64_t k = which ? key_of(value, i0 + e / VEC * 64 * VEC + e % VEC) : 0;
+                    best = k > best ? k : best;
+                    c.add(k, lane, a.top);
+                    which &= which - 1;
+                }
             }
         }
     }
 
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) q = join(q, {__shfl_xor(q.m, o), __shfl_xor(q.s, o), __shfl_xor(q.t, o)});
+    q = group_join<64>(q);
     if (lane == 0) s_sums[wave] = q;
-    if constexpr (TOP) s_list[wave][lane] = list.key;
-    __syncthreads();
     if constexpr (TOP) {
-        for (int h = 1; h < waves; h *= 2) {
-            if (wave % (2 * h) == 0) {
-                list.merge(s_list[wave + h][lane], lane);
-                s_list[wave][lane] = list.key;
-            }
-            __syncthreads();
-        }
+        const uint64_t mine = nth_largest(best, share, lane);
+        __syncthreads();                           // (s_floor was read)
+        if (lane == 0) s_floor[wave] = mine, s_own[wave] = c.floor;
     }
-    if (wave != 0) return;
-    for (int w = 1; w < waves; ++w) q = join(q, s_sums[w]);
+    __syncthreads();
+    q = (lane & 15) < waves ? s_sums[lane & 15] : Sums{-INFINITY, 0.f, 0.f};
+    q = group_join<16>(q);
+    // one lane's (a product fused into a sum of two lanes rounds differently in the two)
+    q = {lane_read(q.m, 0), lane_read(q.s, 0), lane_read(q.t, 0)};
     const float ls = logf(q.s);
     const bool empty = q.m == -INFINITY && q.s == 0.f, bad = !(fabsf(ls) < INFINITY) && !empty;
-    if (lane == 0) {
-        const int64_t c = a.tokens[row];
+    if (threadIdx.x == 0) {
+        const int64_t token = a.tokens[row];
         float lp = 0.f;
-        if (c >= 0) lp = c >= a.V || bad ? NAN : empty ? -INFINITY : (Act<T>::load(x + c) - q.m) - ls;
+        if (token >= 0) lp = token >= a.V || bad ? NAN : empty ? -INFINITY : (Act<T>::load(x + token) - q.m) - ls;
         a.logprob[row] = lp;
         a.entropy[row] = bad ? NAN : empty ? 0.f : ls - q.t / q.s;
     }
     if constexpr (TOP) {
-        if (lane < a.top) {
-            const uint64_t k = bad ? 0 : list.key;
-            a.top_token[row * a.top + lane] = k ? (int64_t)(uint32_t)~uint32_t(k) : -1;
-            a.top_logprob[row * a.top + lane] = bad ? NAN : k ? (key_value(k) - q.m) - ls : -INFINITY;
+        // What reaches the highest floor is little more than `top` keys.  They are put side by side in any order; a
+        // key's place in the answer is how many are larger.
+        const uint64_t f0 = ~wave_max64(~s_floor[min(lane, waves - 1)]), f1 = wave_max64(s_own[min(lane, waves - 1)]);
+        const uint64_t f = f0 > f1 ? f0 : f1;
+        uint64_t* keep = s_key + waves * 128 + 8;
+        const uint64_t k0 = lane < a.top ? c.list : 0, k1 = lane < c.waiting ? c.wait[lane] : 0;
+        const uint64_t mask0 = __ballot(k0 >= f && !bad), mask1 = __ballot(k1 >= f && !bad);
+        const int n0 = __builtin_popcountll(mask0), n1 = __builtin_popcountll(mask1);
+        int first = 0;
+        if (lane == 0 && n0 + n1) first = atomicAdd(&s_keys, n0 + n1);
+        first = __builtin_amdgcn_readfirstlane(first);
+        const uint64_t below = (uint64_t(1) << lane) - 1;
+        if (mask0 >> lane & 1) keep[first + __builtin_popcountll(mask0 & below)] = k0;
+        if (mask1 >> lane & 1) keep[first + n0 + __builtin_popcountll(mask1 & below)] = k1;
+        __syncthreads();
+        const int keys = s_keys;
+        for (int o = threadIdx.x; o < keys; o += blockDim.x) {
+            const uint64_t k = keep[o];
+            int place = 0;
+            for (int i = 0; i < keys; i += 8) {
+                uint64_t other[8];
+#pragma unroll
+                for (int n = 0; n < 8; ++n) other[n] = keep[i + n];
+#pragma unroll
+                for (int n = 0; n < 8; ++n) place += i + n < keys && other[n] > k;
+            }
+            if (place < a.top) {
+                a.top_token[row * a.top + place] = (int64_t)(uint32_t)~uint32_t(k);
+                a.top_logprob[row * a.top + place] = (key_value(k) - q.m) - ls;
+            }
+        }
+        if (wave == 0 && lane >= keys && lane < a.top) {         // fewer than `top` tokens are left
+            a.top_token[row * a.top + lane] = -1;
+            a.top_logprob[row * a.top + lane] = bad ? NAN : -INFINITY;
         }
     }
 }
@@ -236,10 +315,9 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
 template <typename T>
 int launch(const LpArgs& a, int64_t rows, hipStream_t st) {
     const int64_t tiles = (a.V + kTile * (16 / (int)sizeof(T)) - 1) / (kTile * (16 / (int)sizeof(T)));
-    const int most = rows >= 2048 ? 4 : rows >= 512 ? 8 : 16;
-    int waves = 1;
-    while (waves < most && waves < tiles) waves *= 2;
-    if (a.top) hipLaunchKernelGGL((logprob_kernel<T, true>), dim3((unsigned)rows), dim3(waves * 64), 0, st, a);
+    // every wavefront has a first tile (the kernel's barrier after it counts on that)
+    const int waves = (int)std::min<int64_t>(rows >= 2048 ? 4 : rows >= 512 ? 8 : 16, tiles);
+    if (a.top) hipLaunchKernelGGL((logprob_kernel<T, true>), dim3((unsigned)rows), dim3(waves * 64), 2 * (waves * 128 + 8) * sizeof(uint64_t), st, a);
     else hipLaunchKernelGGL((logprob_kernel<T, false>), dim3((unsigned)rows), dim3(waves * 64), 0, st, a);
     return check_launch("token_logprobs");
 }
