@@ -174,7 +174,13 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
         }
     };
 
-    if (threadIdx.x == 0) s_keys = 0;
+    int64_t token = 0;
+    float given = 0.f;                              // the token's logit
+    if (threadIdx.x == 0) {
+        s_keys = 0;
+        token = a.tokens[row];
+        if (token >= 0 && token < a.V) given = Act<T>::load(x + token);
+    }
     Sums q = {-INFINITY, 0.f, 0.f};
     Candidates c;
     uint64_t best = 0;                              // a lane's largest key, where it has reached the floor
@@ -211,16 +217,16 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
             }
         if constexpr (TOP) {
             const int i0 = (int)((int64_t)tile * kTile * VEC - off) + lane * VEC;
+            float all = most[0];
+#pragma unroll
+            for (int u = 1; u < kChunks; ++u) all = fmaxf(all, most[u]);
             if (tile == wave) {
                 // The first tile: each wavefront has share + 1 lanes whose largest reach its f, together `top` or more,
                 // so nothing below the least f is wanted.
+                int at = 0;                        // the lowest index of the lane's largest
 #pragma unroll
-                for (int u = 0; u < kChunks; ++u)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const uint64_t k = key_of(v[u][e], i0 + u * 64 * VEC + e);
-                        best = k > best ? k : best;
-                    }
+                for (int n = kChunks * VEC - 1; n > 0; --n) at = v[n / VEC][n % VEC] == all ? n / VEC * 64 * VEC + n % VEC : at;
+                best = key_of(all, i0 + (v[0][0] == all ? 0 : at));
                 const uint64_t mine = nth_largest(best, share, lane);
                 if (lane == 0) s_floor[wave] = mine;
                 __syncthreads();
@@ -228,25 +234,24 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
                 f = ~wave_max64(~f);
                 c.raise(f);
             }
-            float all = most[0];
-#pragma unroll
-            for (int u = 1; u < kChunks; ++u) all = fmaxf(all, most[u]);
             if (__any(all >= c.floor_value)) {
-                // which of a lane's logits reach the floor; they enter one a lane at a time
-                uint32_t which = 0;
 #pragma unroll
-                for (int u = 0; u < kChunks; ++u)
+                for (int u = 0; u < kChunks; ++u) {
+                    if (!__any(most[u] >= c.floor_value)) continue;
+                    // which of a lane's logits reach the floor; they enter one a lane at a time
+                    uint32_t which = 0;
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) which |= (v[u][e] >= c.floor_value ? 1u : 0u) << (u * VEC + e);
-                while (__any(which != 0)) {
-                    const int e = __builtin_ctz(which | 0x80000000u);
-                    float value = v[0][0];
+                    for (int e = 0; e < VEC; ++e) which |= (v[u][e] >= c.floor_value ? 1u : 0u) << e;
+                    while (__any(which != 0)) {
+                        const int e = __builtin_ctz(which | 1u << (VEC - 1));
+                        float value = v[u][0];
 #pragma unroll
-                    for (int n = 1; n < kChunks * VEC; ++n) value = e == n ? v[n / VEC][n % VEC] : value;
-                    const uint64_t k = which ? key_of(value, i0 + e / VEC * 64 * VEC + e % VEC) : 0;
-                    best = k > best ? k : best;
-                    c.add(k, lane, a.top);
-                    which &= which - 1;
+                        for (int n = 1; n < VEC; ++n) value = e == n ? v[u][n] : value;
+                        const uint64_t k = which ? key_of(value, i0 + u * 64 * VEC + e) : 0;
+                        best = k > best ? k : best;
+                        c.add(k, lane, a.top);
+                        which &= which - 1;
+                    }
                 }
             }
         }
@@ -267,9 +272,8 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
     const float ls = logf(q.s);
     const bool empty = q.m == -INFINITY && q.s == 0.f, bad = !(fabsf(ls) < INFINITY) && !empty;
     if (threadIdx.x == 0) {
-        const int64_t token = a.tokens[row];
         float lp = 0.f;
-        if (token >= 0) lp = token >= a.V || bad ? NAN : empty ? -INFINITY : (Act<T>::load(x + token) - q.m) - ls;
+        if (token >= 0) lp = token >= a.V || bad ? NAN : empty ? -INFINITY : (given - q.m) - ls;
         a.logprob[row] = lp;
         a.entropy[row] = bad ? NAN : empty ? 0.f : ls - q.t / q.s;
     }
@@ -315,8 +319,10 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
 template <typename T>
 int launch(const LpArgs& a, int64_t rows, hipStream_t st) {
     const int64_t tiles = (a.V + kTile * (16 / (int)sizeof(T)) - 1) / (kTile * (16 / (int)sizeof(T)));
-    // every wavefront has a first tile (the kernel's barrier after it counts on that)
-    const int waves = (int)std::min<int64_t>(rows >= 2048 ? 4 : rows >= 512 ? 8 : 16, tiles);
+    // Few rows: many wavefronts each; no more than share the tiles evenly, and every one has a first tile (the kernel's
+    // barrier after it counts on that).  1022 rows of 50280 bf16 with 5 alternatives: 4 wavefronts 33.7 us, 8 36.3, 16 55.
+    const int64_t most = std::clamp<int64_t>(4096 / rows, 4, 16), turns = (tiles + most - 1) / most;
+    const int waves = (int)((tiles + turns - 1) / turns);
     if (a.top) hipLaunchKernelGGL((logprob_kernel<T, true>), dim3((unsigned)rows), dim3(waves * 64), 2 * (waves * 128 + 8) * sizeof(uint64_t), st, a);
     else hipLaunchKernelGGL((logprob_kernel<T, false>), dim3((unsigned)rows), dim3(waves * 64), 0, st, a);
     return check_launch("token_logprobs");
