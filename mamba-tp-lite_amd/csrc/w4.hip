@@ -282,27 +282,58 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
     }
 }
 
-// One wavefront per tile of 16 rows x 128 columns.
-template <typename T, typename S, int G, bool Z>
+// One wavefront per tile of 16 rows x 128 columns.  Rows of W on 16-byte boundaries (VEC): a lane's 8 columns leave in
+// 16-byte stores as they are.  Others: through LDS, so that a store writes neighbouring columns of one row.
+template <typename T, typename S, int G, bool Z, bool VEC>
 __global__ void __launch_bounds__(256) dequantize_w4_kernel(const W4Args a) {
     constexpr int NG = kBlockK / G;
-    const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
-    const int64_t t = blockIdx.y + (int64_t)blockIdx.z * 65535;
-    const int kb = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t n = t * kTileRows + r;
-    if (kb >= a.KB || n >= a.N) return;
-    const uint4 w = reinterpret_cast<const uint4*>(a.codes)[(t * a.KB + kb) * 64 + lane];
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-    T* out = static_cast<T*>(a.y) + n * a.ldy;
+    __shared__ T s_row[VEC ? 1 : 4][VEC ? 1 : kTileRows][kBlockK + 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, j = lane >> 4;
+    const int64_t tile = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + wave, t = tile / a.KB;
+    const int kb = (int)(tile - t * a.KB);
+    const int64_t n0 = t * kTileRows;
+    if (n0 >= a.N) return;
+    const int64_t b = t * a.KB + kb;
+    const U4 w = __builtin_nontemporal_load(reinterpret_cast<const U4*>(a.codes) + b * 64 + lane);
+    const Scales<S, NG> sc = static_cast<const Scales<S, NG>*>(a.scales)[b * kTileRows + r];
+    Scales<uint8_t, NG> zr;
+    if constexpr (Z) zr = reinterpret_cast<const Scales<uint8_t, NG>*>(a.zeros)[b * kTileRows + r];
+    T* out = static_cast<T*>(a.y) + n0 * a.ldy;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t at = ((t * a.KB + kb) * kTileRows + r) * NG + 32 * i / G;
-        const float s = scale_at<S>(a.scales, at);
-        const float z = Z ? (float)a.zeros[at] : 8.f;
-        const int k0 = kb * kBlockK + 32 * i + 8 * j;
+        const float s = sc.at(i / (G / 32));
+        const int zero = Z ? zr.v[i / (G / 32)] : 8;
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (k0 + e < a.K) Act<T>::store(out + k0 + e, s * ((float)code_of(ws[i], e) - z));
+        for (int e = 0; e < 8; ++e) v[e] = s * (float)((int)code_of(w[i], e) - zero);
+        const int k = 32 * i + 8 * j, k0 = kb * kBlockK + k;
+        if constexpr (!VEC) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) Act<T>::store(&s_row[wave][r][k + e], v[e]);
+        } else if (n0 + r < a.N) {
+            T* to = out + r * a.ldy + k0;
+            if (k0 + 8 <= a.K) {
+                if constexpr (sizeof(T) == 4) {
+                    st4(to, F4v{v[0], v[1], v[2], v[3]});
+                    st4(to + 4, F4v{v[4], v[5], v[6], v[7]});
+                } else {
+                    *reinterpret_cast<U4*>(to) = U4{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]),
+                                                    f32x2_to_bf16x2(v[4], v[5]), f32x2_to_bf16x2(v[6], v[7])};
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (k0 + e < a.K) Act<T>::store(to + e, v[e]);
+            }
+        }
+    }
+    if constexpr (!VEC) {
+        __builtin_amdgcn_wave_barrier();           // (a wavefront reads what it wrote: LDS is in order within it)
+#pragma unroll 4
+        for (int o = lane; o < kTileRows * kBlockK; o += 64) {
+            const int row = o / kBlockK, k = o % kBlockK;
+            if (n0 + row < a.N && kb * kBlockK + k < a.K) out[row * a.ldy + kb * kBlockK + k] = s_row[wave][row][k];
+        }
     }
 }
 
@@ -316,7 +347,8 @@ __global__ void __launch_bounds__(256) dequantize_w4_kernel(const W4Args a) {
 #define MTL_LINEAR_1(T, S, G, Z) linear_w4_kernel<T, S, G, Z, 1>
 #define MTL_LINEAR_2(T, S, G, Z) linear_w4_kernel<T, S, G, Z, 2>
 #define MTL_LINEAR_3(T, S, G, Z) linear_w4_kernel<T, S, G, Z, 3>
-#define MTL_MATRIX(T, S, G, Z) dequantize_w4_kernel<T, S, G, Z>
+#define MTL_MATRIX(T, S, G, Z) dequantize_w4_kernel<T, S, G, Z, false>
+#define MTL_MATRIX_VEC(T, S, G, Z) dequantize_w4_kernel<T, S, G, Z, true>
 #define MTL_W4_Z(KERNEL, T, S, ...)                        \
     if (a.zeros) { MTL_W4_G(KERNEL, T, S, true, __VA_ARGS__) } else { MTL_W4_G(KERNEL, T, S, false, __VA_ARGS__) }
 #define MTL_W4(KERNEL, ...)                                                                                     \
@@ -407,8 +439,12 @@ extern "C" int mtl_dequantize_w4(const uint8_t* codes, const void* scales, const
     MTL_REQUIRE(reinterpret_cast<uintptr_t>(zeros) % 4 == 0, "zeros must be 4-byte aligned");
     const W4Args a{nullptr, codes, scales, zeros, nullptr, W, 0, ldw, 0, (int)N, (int)K,
                    (int)((K + kBlockK - 1) / kBlockK)};
-    const int64_t tiles = (N + kTileRows - 1) / kTileRows;
-    const dim3 grid((a.KB + 3) / 4, (unsigned)std::min<int64_t>(tiles, 65535), (unsigned)((tiles + 65534) / 65535));
-    MTL_W4(MTL_MATRIX, grid, dim3(256), 0, as_stream(stream), a)
+    const int64_t groups = ((N + kTileRows - 1) / kTileRows * a.KB + 3) / 4, gy = (groups + (1 << 22) - 1) >> 22;
+    const dim3 grid((unsigned)((groups + gy - 1) / gy), (unsigned)gy);
+    if (reinterpret_cast<uintptr_t>(W) % 16 == 0 && ldw * (dtype == MTL_F32 ? 4 : 2) % 16 == 0) {
+        MTL_W4(MTL_MATRIX_VEC, grid, dim3(256), 0, as_stream(stream), a)
+    } else {
+        MTL_W4(MTL_MATRIX, grid, dim3(256), 0, as_stream(stream), a)
+    }
     return check_launch("dequantize_w4");
 }
