@@ -169,6 +169,10 @@ __device__ __forceinline__ uint32_t group_umax(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// A workgroup's barrier for what it keeps in LDS: __syncthreads would also wait for every global load in flight and
+// every store on its way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // Fixed-count register blocking: kernels that hold RUNS values per lane are
 // instantiated for these counts; a size needing `need` runs uses the
 // smallest instantiated count >= need (the extra runs are masked).

@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
                 best = key_of(all, i0 + (v[0][0] == all ? 0 : at));
                 const uint64_t mine = nth_largest(best, share, lane);
                 if (lane == 0) s_floor[wave] = mine;
-                __syncthreads();
+                lds_barrier();
                 uint64_t f = s_floor[min(lane, waves - 1)];
                 f = ~wave_max64(~f);
                 c.raise(f);
@@ -261,10 +261,10 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
     if (lane == 0) s_sums[wave] = q;
     if constexpr (TOP) {
         const uint64_t mine = nth_largest(best, share, lane);
-        __syncthreads();                           // (s_floor was read)
+        lds_barrier();                           // (s_floor was read)
         if (lane == 0) s_floor[wave] = mine, s_own[wave] = c.floor;
     }
-    __syncthreads();
+    lds_barrier();
     q = (lane & 15) < waves ? s_sums[lane & 15] : Sums{-INFINITY, 0.f, 0.f};
     q = group_join<16>(q);
     // one lane's (a product fused into a sum of two lanes rounds differently in the two)
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
         const uint64_t below = (uint64_t(1) << lane) - 1;
         if (mask0 >> lane & 1) keep[first + __builtin_popcountll(mask0 & below)] = k0;
         if (mask1 >> lane & 1) keep[first + n0 + __builtin_popcountll(mask1 & below)] = k1;
-        __syncthreads();
+        lds_barrier();
         const int keys = s_keys;
         for (int o = threadIdx.x; o < keys; o += blockDim.x) {
             const uint64_t k = keep[o];

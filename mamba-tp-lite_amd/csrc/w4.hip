@@ -46,7 +46,7 @@ struct LinearW4 {
     W4Args a;
     int rows;                  // rows of x per workgroup (blockIdx.y takes the next ones)
     int kblocks;               // 128-column blocks of x in LDS at a time
-    int wk;                    // wavefronts that share a tile of W, each on every wk-th block
+    int wk, wk_log2;           // wavefronts that share a tile of W, each on every wk-th block
     int xvec;                  // rows of x start on 16-byte boundaries
 };
 
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
     const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m0 = blockIdx.y * p.rows, M = min(p.rows, a.M - m0), R = P * M;
-    const int threads = blockDim.x, wn = wave / p.wk, wkid = wave - wn * p.wk, WN = threads / 64 / p.wk;
+    const int threads = blockDim.x, wn = wave >> p.wk_log2, wkid = wave & (p.wk - 1), WN = threads / 64 >> p.wk_log2;
     const T* x = static_cast<const T*>(a.x) + m0 * a.ldx;
     const int pitch = p.kblocks * 16 + 1;                     // (+ 1: the 16 rows of an operand start in different banks)
     U4* s_x = reinterpret_cast<U4*>(smem);                    // [R][k / 8]
@@ -88,14 +88,18 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
     float* s_red = reinterpret_cast<float*>(s_x + P * p.rows * pitch);                         // [wave][R16][16]
     __shared__ int s_wide;
 
+    // u / n8 for the fewer than 2^19 runs of x and at most 48 rows: the product is off by less than half of 1 / n8
+    auto row_of = [&](int u, float inv) __attribute__((always_inline)) { return (int)((u + 0.5f) * inv); };
     // x to LDS: a thread takes 8 columns of a row at a time, kUnits of them in flight
     constexpr int kRaw = 8 * (int)sizeof(T) / 16, kUnits = 4 / kRaw;
     U4 raw[kUnits][kRaw];
     auto fetch = [&](int kb0, int nb, int u0) __attribute__((always_inline)) {
         const int n8 = nb * 16;
+        const float inv = 1.f / n8;
 #pragma unroll
         for (int n = 0; n < kUnits; ++n) {
-            const int u = min(u0 + n * threads, M * n8 - 1), m = u / n8, k = kb0 * kBlockK + (u - m * n8) * 8;
+            if (__builtin_amdgcn_readfirstlane(u0) + n * threads >= M * n8) break;
+            const int u = min(u0 + n * threads, M * n8 - 1), m = row_of(u, inv), k = kb0 * kBlockK + (u - m * n8) * 8;
             const T* src = x + m * a.ldx + k;
             if (p.xvec && k + 8 <= a.K) {
 #pragma unroll
@@ -103,18 +107,21 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
             } else {
                 T v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = k + e < a.K ? src[e] : T(0);
+                for (int e = 0; e < 8; ++e) v[e] = src[min(e, a.K - 1 - k)];      // past the row: its last value again
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = k + e < a.K ? v[e] : T(0);
                 __builtin_memcpy(raw[n], v, sizeof(v));
             }
         }
     };
     auto put = [&](int nb, int u0) __attribute__((always_inline)) {
         const int n8 = nb * 16;
+        const float inv = 1.f / n8;
 #pragma unroll
         for (int n = 0; n < kUnits; ++n) {
             const int u = u0 + n * threads;
             if (u >= M * n8) break;
-            const int m = u / n8, k8 = u - m * n8;
+            const int m = row_of(u, inv), k8 = u - m * n8;
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -142,15 +149,52 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
     const bool once = p.kblocks >= a.KB;
 
     // kAhead blocks of W in registers; as one is used up, the block kAhead further on (of the next tile, after the
-    // last) is loaded in its place, so the stream never stops at the end of a tile
+    // last) is loaded in its place, so the stream never stops at the end of a tile.  The loads stand in no branch: the
+    // wait before a block's use then counts the younger ones out.
     U4 w[kAhead];
     Scales<S, NG> sc[kAhead];
     Scales<uint8_t, NG> zr[kAhead];
-    auto load = [&](int u, int t, int kb) __attribute__((always_inline)) {
-        const int64_t b = (int64_t)min(t, tiles - 1) * a.KB + min(kb + u * p.wk, a.KB - 1);
+    auto load = [&](int u, int64_t b0, int last) __attribute__((always_inline)) {
+        const int64_t b = b0 + min(u, last) * p.wk;          // (a batch's last block again, past it)
         w[u] = __builtin_nontemporal_load(reinterpret_cast<const U4*>(a.codes) + b * 64 + lane);
         sc[u] = static_cast<const Scales<S, NG>*>(a.scales)[b * kTileRows + r];
         if constexpr (Z) zr[u] = reinterpret_cast<const Scales<uint8_t, NG>*>(a.zeros)[b * kTileRows + r];
+    };
+    F4v acc[TM];
+    uint32_t mask = 0x00780078u, sixteen = 0x41804180u;      // (in registers: an and-or takes no literals)
+    asm("" : "+v"(mask), "+v"(sixteen));
+    // acc += the block in slot u times columns 128 kc .. of the part of x in LDS
+    auto multiply = [&](int u, int kc) __attribute__((always_inline)) {
+        F4v part[TM];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i % (G / 32) == 0) {
+#pragma unroll
+                for (int q = 0; q < TM; ++q) part[q] = F4v{0.f, 0.f, 0.f, 0.f};
+            }
+            const uint32_t c = w[u][i];
+            const U4 b = {(c << 3 & mask) | sixteen, (c >> 1 & mask) | sixteen, (c >> 5 & mask) | sixteen,
+                          (c >> 9 & mask) | sixteen};
+            // - (16 + z) in bf16, for every column
+            uint32_t z = 0xc1c0c1c0u;
+            if constexpr (Z) {
+                z = __float_as_uint(-16.f - (float)zr[u].v[i / (G / 32)]);
+                z |= z >> 16;
+            }
+#pragma unroll
+            for (int q = 0; q < TM; ++q) {
+                const B8h xa = __builtin_bit_cast(B8h, s_x[at_x[q] + kc * 16 + i * 4]);
+                part[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa, __builtin_bit_cast(B8h, b), part[q], 0, 0, 0);
+                part[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa, __builtin_bit_cast(B8h, U4{z, z, z, z}), part[q], 0, 0, 0);
+            }
+            if (i % (G / 32) == G / 32 - 1) {
+                const float s = sc[u].at(i / (G / 32));
+#pragma unroll
+                for (int q = 0; q < TM; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[q][e] = fmaf(s, part[q][e], acc[q][e]);
+            }
+        }
     };
     const int stride = gridDim.x * WN;
     int t = blockIdx.x * WN + wn;
@@ -158,13 +202,12 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
     fetch(0, min(p.kblocks, a.KB), threadIdx.x);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) load(u, t, wkid);
+    for (int u = 0; u < kAhead; ++u) load(u, (int64_t)min(t, tiles - 1) * a.KB + wkid, (a.KB - 1 - wkid) >> p.wk_log2);
     __builtin_amdgcn_sched_barrier(0);
     if (threadIdx.x == 0) s_wide = 0;
-    __syncthreads();
+    lds_barrier();
     bool staged = false;
     for (int t0 = blockIdx.x * WN; t0 < tiles; t0 += stride, t += stride) {
-        F4v acc[TM];
 #pragma unroll
         for (int q = 0; q < TM; ++q) acc[q] = F4v{0.f, 0.f, 0.f, 0.f};
         for (int kb0 = 0; kb0 < a.KB; kb0 += p.kblocks) {
@@ -172,10 +215,10 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
             if (!once || !staged) {
                 const int nb = kb1 - kb0;
                 if (staged) {
-                    __syncthreads();
+                    lds_barrier();
                     if (threadIdx.x == 0) s_wide = 0;
                     fetch(kb0, nb, threadIdx.x);
-                    __syncthreads();
+                    lds_barrier();
                 }
                 put(nb, threadIdx.x);
                 for (int u = threadIdx.x + kUnits * threads; u < M * nb * 16; u += kUnits * threads) {
@@ -183,45 +226,25 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
                     put(nb, u);
                 }
                 staged = true;
-                __syncthreads();
+                lds_barrier();
             }
             const bool wide = s_wide;
             for (int kb = kb0 + wkid; kb < kb1; kb += kAhead * p.wk) {
                 const bool more = kb + kAhead * p.wk < a.KB;
                 const int tn = more ? t : t + stride, kbn = more ? kb + kAhead * p.wk : wkid;
+                const int blocks = wide ? 0 : ((kb1 - 1 - kb) >> p.wk_log2) + 1, kc = kb - kb0;
+                if (tn < tiles) {
+                    const int64_t b0 = (int64_t)tn * a.KB + kbn;
+                    const int last = (a.KB - 1 - kbn) >> p.wk_log2;
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    const int kc = kb + u * p.wk - kb0;
-                    if (kc < kb1 - kb0 && !wide) {
-                        F4v part[TM];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (i % (G / 32) == 0) {
-#pragma unroll
-                                for (int q = 0; q < TM; ++q) part[q] = F4v{0.f, 0.f, 0.f, 0.f};
-                            }
-                            const uint32_t c = w[u][i];
-                            const U4 b = {(c << 3 & 0x00780078u) | 0x41804180u, (c >> 1 & 0x00780078u) | 0x41804180u,
-                                          (c >> 5 & 0x00780078u) | 0x41804180u, (c >> 9 & 0x00780078u) | 0x41804180u};
-                            // - (16 + z) in bf16, for every column
-                            uint32_t z = 0xc1c0c1c0u;
-                            if constexpr (Z) z = __float_as_uint(-16.f - (float)zr[u].v[i / (G / 32)]) >> 16 | __float_as_uint(-16.f - (float)zr[u].v[i / (G / 32)]);
-#pragma unroll
-                            for (int q = 0; q < TM; ++q) {
-                                const B8h xa = __builtin_bit_cast(B8h, s_x[at_x[q] + kc * 16 + i * 4]);
-                                part[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa, __builtin_bit_cast(B8h, b), part[q], 0, 0, 0);
-                                part[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa, __builtin_bit_cast(B8h, U4{z, z, z, z}), part[q], 0, 0, 0);
-                            }
-                            if (i % (G / 32) == G / 32 - 1) {
-                                const float s = sc[u].at(i / (G / 32));
-#pragma unroll
-                                for (int q = 0; q < TM; ++q)
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) acc[q][e] = fmaf(s, part[q][e], acc[q][e]);
-                            }
-                        }
+                    for (int u = 0; u < kAhead; ++u) {
+                        if (u < blocks) multiply(u, kc + u * p.wk);
+                        load(u, b0, last);
                     }
-                    load(u, tn, kbn);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u)
+                        if (u < blocks) multiply(u, kc + u * p.wk);
                 }
             }
             if (wide) {
@@ -256,28 +279,36 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
         for (int q = 0; q < TM; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s_red[(wave * R16 + q * 16 + 4 * j + e) * 16 + r] = acc[q][e];
-        auto store = [&](int tile, int first, int m, int c) __attribute__((always_inline)) {
-            const int n = tile * kTileRows + c;
-            if (n >= a.N) return;
+        // a quarter of a wavefront to a row m of a tile; where a sum has many parts all four to one, a fourth each
+        const int parts = P * p.wk;
+        const bool spread = parts >= 8;
+        auto store = [&](int tile, int first, int m) __attribute__((always_inline)) {
             float v = 0.f;
-#pragma unroll
-            for (int q = P - 1; q >= 0; --q)                 // the small parts first
 #pragma unroll 4
-                for (int k = 0; k < p.wk; ++k) v += s_red[((first + k) * R16 + q * M + m) * 16 + c];
-            if (a.bias) v += Act<T>::load(static_cast<const T*>(a.bias) + n);
-            Act<T>::store(static_cast<T*>(a.y) + (m0 + m) * a.ldy + n, v);
+            for (int i = spread ? j : 0; i < parts; i += spread ? 4 : 1)
+                v += s_red[((first + (i & (p.wk - 1))) * R16 + (i >> p.wk_log2) * M + m) * 16 + r];
+            if (spread) {
+                v += __shfl_xor(v, 16);
+                v += __shfl_xor(v, 32);
+            }
+            const int n = tile * kTileRows + r;
+            if ((j == 0 || !spread) && n < a.N) {
+                if (a.bias) v += Act<T>::load(static_cast<const T*>(a.bias) + n);
+                Act<T>::store(static_cast<T*>(a.y) + (m0 + m) * a.ldy + n, v);
+            }
         };
         if (p.wk == 1) {                                     // a wavefront's own sums: no other waits for it
             __builtin_amdgcn_wave_barrier();
-            for (int m = j; m < M; m += 4) store(t, wave, m, r);
+            for (int m = j; m < M; m += 4) store(t, wave, m);
             __builtin_amdgcn_wave_barrier();
         } else {
-            __syncthreads();
-            for (int o = threadIdx.x; o < WN * M * 16; o += threads) {
-                const int mt = o >> 4, ti = mt / M;
-                store(t0 + ti, ti * p.wk, mt - ti * M, o & 15);
+            lds_barrier();
+            const int step = threads / (spread ? 64 : 16);
+            for (int mt = spread ? wave : (int)threadIdx.x >> 4; mt < WN * M; mt += step) {
+                const int ti = WN == 1 ? 0 : mt / M;
+                store(t0 + ti, ti * p.wk, mt - ti * M);
             }
-            __syncthreads();
+            lds_barrier();
         }
     }
 }
@@ -346,7 +377,6 @@ __global__ void __launch_bounds__(256) dequantize_w4_kernel(const W4Args a) {
     }
 #define MTL_LINEAR_1(T, S, G, Z) linear_w4_kernel<T, S, G, Z, 1>
 #define MTL_LINEAR_2(T, S, G, Z) linear_w4_kernel<T, S, G, Z, 2>
-#define MTL_LINEAR_3(T, S, G, Z) linear_w4_kernel<T, S, G, Z, 3>
 #define MTL_MATRIX(T, S, G, Z) dequantize_w4_kernel<T, S, G, Z, false>
 #define MTL_MATRIX_VEC(T, S, G, Z) dequantize_w4_kernel<T, S, G, Z, true>
 #define MTL_W4_Z(KERNEL, T, S, ...)                        \
@@ -393,37 +423,42 @@ extern "C" int mtl_linear_w4(const mtl_linear_w4_args* p, mtl_stream_t stream) {
     const W4Args a{p->x, p->codes, p->scales, p->zeros, p->bias, p->y, p->ldx, p->ldy, (int)p->M, (int)p->N, (int)p->K,
                    (int)((p->K + kBlockK - 1) / kBlockK)};
     const int es = dtype == MTL_F32 ? 4 : 2, parts = dtype == MTL_F32 ? 3 : 1;
-    LinearW4 l{a, 0, 0, 1, reinterpret_cast<uintptr_t>(p->x) % 16 == 0 && p->ldx * es % 16 == 0};
+    LinearW4 l{a, 0, 0, 1, 0, reinterpret_cast<uintptr_t>(p->x) % 16 == 0 && p->ldx * es % 16 == 0};
     const int tiles = (a.N + kTileRows - 1) / kTileRows;
-    // At most 48 operand rows a workgroup (16 of fp32 x), fewer where that leaves the GPU short of workgroups
-    int tm = 3, chunks, groups, wn;
-    size_t lds;
-    for (;; --tm) {
-        chunks = (a.M + tm * 16 / parts - 1) / (tm * 16 / parts);
-        l.rows = (a.M + chunks - 1) / chunks;
-        tm = (l.rows * parts + 15) / 16;
-        const int per_block = kBlockK * 2 * parts * l.rows;
-        // (at most 12 KiB, so at least 4 blocks fit)
-        l.kblocks = std::min(a.KB, (kLdsBytes - kWaves * tm * 1024 - 16 * parts * l.rows) / per_block);
-        // about 16 wavefronts for each of 256 CUs, on no less than a block each
-        l.wk = 1;
-        while (l.wk < kWaves && tiles * chunks * l.wk < 4096 && l.wk * 2 <= l.kblocks) l.wk *= 2;
-        if (l.kblocks < a.KB) {                              // whole batches of every wavefront in each part of x
-            while (l.wk > 1 && l.wk * kAhead > l.kblocks) l.wk /= 2;
-            l.kblocks -= l.kblocks % (l.wk * kAhead);
-        }
-        // tiles side by side in a workgroup share x: as many as leave a workgroup for every CU
-        wn = std::max(1, std::min(kWaves / l.wk, tiles * chunks / 256));
-        lds = (size_t)l.kblocks * per_block + 16 * parts * l.rows + wn * l.wk * tm * 1024;
-        groups = (tiles + wn - 1) / wn;
-        if (tm == 1 || groups * chunks >= 256) break;
+    // Rows of x to a workgroup: one operand tile's (16, of fp32 x 5) while that makes at most 2048 (tile of W, rows of x)
+    // pairs, two tiles' where there are more: W is then read half as often.  Wavefronts to a pair: so many that the pairs
+    // make about 2048; pairs to a workgroup: so many that it has 8 wavefronts, 16 where its LDS leaves room for one
+    // workgroup a CU.  Measured, GPU us (pairs; chosen, its neighbours): 768x1536 1 row bf16 (48) 3.8, 4 / 2 wavefronts
+    // 3.7 / 5.0; 8192x2048 16 rows bf16 (512) 7.2, 8 / 2 9.7 / 8.3; 8192x2048 8 rows fp32 (1024) 6.8, 4 / 1 8.3 / 8.7;
+    // 50280x2048 8 rows fp32 (6286) two tiles 21.4, one 27.7; 2048x4096 64 rows bf16 (512) 10.7, two tiles 22.
+    const auto chunks_of = [&](int tm) { return (a.M + tm * 16 / parts - 1) / (tm * 16 / parts); };
+    int tm = tiles * (int64_t)chunks_of(1) <= 2048 ? 1 : 2;
+    const int chunks = chunks_of(tm);
+    l.rows = (a.M + chunks - 1) / chunks;
+    tm = (l.rows * parts + 15) / 16;
+    const int pairs = (int)std::min<int64_t>(tiles * (int64_t)chunks, 1 << 20);
+    const int per_block = kBlockK * 2 * parts * l.rows, pad = 16 * parts * l.rows;
+    // (a block of x takes at most 8 KiB, so at least 8 fit)
+    const auto blocks_of = [&](int waves) { return std::min(a.KB, (kLdsBytes - waves * tm * 1024 - pad) / per_block); };
+    l.kblocks = blocks_of(8);
+    while (l.wk < 8 && l.wk * 2 * pairs <= 2048 && l.wk * 2 <= a.KB) l.wk *= 2;
+    int wn = std::min(8 / l.wk, std::max(2, pairs / 64));
+    const bool two = (size_t)l.kblocks * per_block + pad + 8 * tm * 1024 <= kLdsBytes / 2;
+    if (l.wk == 1 && !two) {
+        wn = 16;
+        l.kblocks = blocks_of(16);
     }
-    const int passes = (groups * chunks + 255) / 256;
-    const dim3 grid((groups + passes - 1) / passes, chunks);
+    if (l.kblocks < a.KB) {                                  // whole batches of every wavefront in each part of x
+        while (l.wk > 1 && l.wk * kAhead > l.kblocks) l.wk /= 2, wn *= 2;
+        l.kblocks -= l.kblocks % (l.wk * kAhead);
+    }
+    l.wk_log2 = __builtin_ctz(l.wk);
+    const size_t lds = (size_t)l.kblocks * per_block + pad + wn * l.wk * tm * 1024;
+    const int64_t groups = (tiles + wn - 1) / wn, most = two ? 512 : 256, passes = (groups * chunks + most - 1) / most;
+    const dim3 grid((unsigned)((groups + passes - 1) / passes), chunks);
     switch (tm) {
         case 1: MTL_W4(MTL_LINEAR_1, grid, dim3(wn * l.wk * 64), lds, as_stream(stream), l) break;
-        case 2: MTL_W4(MTL_LINEAR_2, grid, dim3(wn * l.wk * 64), lds, as_stream(stream), l) break;
-        default: MTL_W4(MTL_LINEAR_3, grid, dim3(wn * l.wk * 64), lds, as_stream(stream), l) break;
+        default: MTL_W4(MTL_LINEAR_2, grid, dim3(wn * l.wk * 64), lds, as_stream(stream), l) break;
     }
     return check_launch("linear_w4");
 }
