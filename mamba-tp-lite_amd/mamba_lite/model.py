@@ -4,6 +4,9 @@ Same public surface as mamba-tp-lite's mamba_lite/model.py:
   MambaConfig, LayerCache, MambaCache.allocate, RMSNorm, MambaMixer
   (.prefill / .step / .forward), MambaBlock, MambaLM (.prefill / .step /
   .generate / .from_pretrained), load_hf_state_dict.
+Beside it: LinearW4 and MambaLM.quantize_w4 (projections and lm_head from 4-bit
+codes), MambaLM.score and generate's return_logprobs (log probabilities,
+entropy and the most probable tokens).
 Parameter names and shapes match the reference, so its state dicts (and HF
 `state-spaces/mamba-*-hf` checkpoints through from_pretrained) load as is.
 
@@ -255,6 +258,39 @@ def _linear_mod(mod, x: torch.Tensor) -> torch.Tensor:
     return mod(x)
 
 
+class LinearW4(nn.Module):
+    """nn.Linear with its weight [out_features, in_features] in 4-bit codes and group scales (ops.W4); made from a
+    nn.Linear, or by MambaLM.quantize_w4.  A decode step's rows (up to ops.W4_MAX_ROWS) are multiplied from the codes; a
+    prompt's take the matrix made from them, as does a call whose gradient is recorded (with respect to x: the weight
+    has none)."""
+
+    def __init__(self, w4: ops.W4, bias: torch.Tensor | None = None):
+        super().__init__()
+        self.out_features, self.in_features, self.group = w4.n, w4.k, w4.group
+        par = lambda t: None if t is None else nn.Parameter(t.detach(), requires_grad=False)
+        self.weight, self.scales, self.zeros, self.bias = par(w4.codes), par(w4.scales), par(w4.zeros), par(bias)
+
+    @classmethod
+    def from_linear(cls, lin: nn.Linear, group: int = 64, zero_points: bool = False,
+                    scale_dtype=torch.bfloat16) -> "LinearW4":
+        if type(lin) is not nn.Linear:
+            raise TypeError(f"a plain nn.Linear expected, got {type(lin).__name__}")
+        return cls(ops.quantize_w4(lin.weight, group, zero_points, scale_dtype), lin.bias)
+
+    def w4(self) -> ops.W4:
+        return ops.W4(self.weight, self.scales, self.zeros, self.out_features, self.in_features, self.group)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, group={self.group}, " \
+               f"zero_points={self.zeros is not None}, bias={self.bias is not None}"
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        w4 = self.w4()
+        if x.numel() <= ops.W4_MAX_ROWS * w4.k and not (torch.is_grad_enabled() and x.requires_grad):
+            return ops.linear_w4(x, w4, self.bias)
+        return _linear(x, ops.dequantize_w4(w4, x.dtype), self.bias)
+
+
 def _skinny_split(K: int, most: int = 16) -> int:
     """The largest split of K into ranges of whole 128-column granules, at
     most `most` parts."""
@@ -381,7 +417,7 @@ class MambaMixer(nn.Module):
             if tuple(out.ssm_state.shape) != (b, Dm, N) or out.ssm_state.dtype != torch.float32 or \
                     not out.ssm_state.is_contiguous():
                 raise ValueError(f"out.ssm_state must be contiguous float32 {(b, Dm, N)}")
-        split = b * l >= SPLIT_PROJ_MIN_TOKENS
+        split = b * l >= SPLIT_PROJ_MIN_TOKENS and type(self.in_proj) is not LinearW4
         x2 = None if split else _skinny_rows(x, self.in_proj.weight, skinny, self.in_proj.bias)
         # in_proj with the causal conv as its epilogue (<= 64 tokens)
         fused_conv = x2 is not None and ops.in_proj_conv_prefill_ok(x2, self.in_proj.weight, K)
@@ -626,7 +662,30 @@ class MambaLM(nn.Module):
         tensors, and a copy or a reloaded model makes its own."""
         return {k: v for k, v in self.__dict__.items() if k not in _CALL_PLANS}
 
+    @torch.no_grad()
+    def quantize_w4(self, group: int = 64, zero_points: bool = False, scale_dtype=torch.bfloat16,
+                    lm_head: bool = True) -> "MambaLM":
+        """Puts every block's in_proj and out_proj, and with lm_head a copy of the tied embedding for the head, into
+        4-bit codes (LinearW4), in place; the embedding itself and the small projections stay as they are.  A model
+        at the mamba-1.4b width keeps about a sixth of its fp32 bytes.  Returns self."""
+        for blk in self.layers:
+            for name in ("in_proj", "out_proj"):
+                if type(getattr(blk.mixer, name)) is not nn.Linear:
+                    raise TypeError(f"quantize_w4: {name} must be a plain nn.Linear, got "
+                                    f"{type(getattr(blk.mixer, name)).__name__}")
+        for blk in self.layers:
+            for name in ("in_proj", "out_proj"):
+                setattr(blk.mixer, name, LinearW4.from_linear(getattr(blk.mixer, name), group, zero_points, scale_dtype))
+        if lm_head:
+            self.head_w4 = LinearW4(ops.quantize_w4(self.embedding.weight, group, zero_points, scale_dtype))
+        for name in _CALL_PLANS:                 # (they hold the replaced weights' addresses)
+            self.__dict__.pop(name, None)
+        return self
+
     def lm_head(self, x: torch.Tensor) -> torch.Tensor:
+        head = self._modules.get("head_w4")
+        if head is not None:
+            return head(x)
         w = self.embedding.weight
         return ops.lm_head(x, w) if ops.lm_head_ok(x, w) else _linear(x, w)
 
@@ -659,6 +718,11 @@ class MambaLM(nn.Module):
         GraphedStepper captured, or `cache` itself) the final states are
         written into its tensors in place and out_cache is returned, so a
         captured decode graph can serve the next prompt without re-capture."""
+        xf, new = self._prefill_hidden(input_ids, cache, out_cache)
+        return self.lm_head(xf), new
+
+    def _prefill_hidden(self, input_ids, cache=None, out_cache=None):
+        """prefill() up to the lm_head's input [b, l, d_model]."""
         if out_cache is not None and len(out_cache.layers) != len(self.layers):
             raise ValueError("out_cache has the wrong number of layers")
         native = self._prefill_native(input_ids, cache, out_cache)
@@ -674,8 +738,23 @@ class MambaLM(nn.Module):
             new_layers.append(LayerCache(conv_state=cs, ssm_state=hs))
             return y
 
-        xf = self._run(x, layer)
-        return self.lm_head(xf), (out_cache if out_cache is not None else MambaCache(new_layers))
+        return self._run(x, layer), (out_cache if out_cache is not None else MambaCache(new_layers))
+
+    # rows of logits that score() makes at a time: 2^28 values (1 GiB in fp32)
+    _SCORE_LOGITS = 1 << 28
+
+    @torch.no_grad()
+    def score(self, input_ids: torch.Tensor, top: int = 0) -> ops.TokenLogprobs:
+        """input_ids [b, l] -> ln p of each token but a row's first, given the ones before it (logprob, entropy
+        [b, l - 1]), with the `top` most probable tokens at each place (top_logprob, top_token [b, l - 1, top]).  The
+        logits are made a part at a time and not kept."""
+        xf, _ = self._prefill_hidden(input_ids)
+        b, l = input_ids.shape
+        xf, given = xf[:, :-1].reshape(b * (l - 1), xf.shape[-1]), input_ids[:, 1:].reshape(-1)
+        step = max(1, self._SCORE_LOGITS // self.embedding.weight.shape[0])
+        parts = [ops.token_logprobs(self.lm_head(xf[i:i + step]), given[i:i + step], top=top)
+                 for i in range(0, max(len(given), 1), step)]
+        return ops.TokenLogprobs(*(torch.cat(t).view(b, l - 1, *t[0].shape[1:]) for t in zip(*parts)))
 
     # ---- short prompt as one C call ----
     def _short_prefill_plan(self):
@@ -718,7 +797,7 @@ class MambaLM(nn.Module):
         return None
 
     def _prefill_native(self, input_ids, cache, out_cache):
-        """prefill() through mtl_prefill_short or mtl_prefill_long, or None
+        """_prefill_hidden() through mtl_prefill_short or mtl_prefill_long, or None
         where neither applies (a size or layer shape they do not take, a
         dtype other than float32, caches that are not contiguous float32)."""
         cfg = self.cfg
@@ -770,7 +849,7 @@ class MambaLM(nn.Module):
                                           skinny_rows=skinny)
             except torch.OutOfMemoryError:      # its workspace, before any launch: op by op takes less at a time
                 return None
-        return self.lm_head(normed), (out_cache if out_cache is not None else MambaCache(new_layers))
+        return normed, (out_cache if out_cache is not None else MambaCache(new_layers))
 
     def step(self, input_ids: torch.Tensor, cache: MambaCache):
         """input_ids [b, 1] -> logits [b, 1, vocab]; cache updated in place
@@ -1200,23 +1279,34 @@ class MambaLM(nn.Module):
         return logits.unsqueeze(1)
 
     @torch.no_grad()
-    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, greedy: bool = True):
+    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, greedy: bool = True, return_logprobs: bool = False,
+                 top: int = 0):
         """Prefill once, then greedy decode through the cache (reference
-        model.py:355-365).  Returns the full token sequence.  The reference
+        model.py:355-365).  Returns the full token sequence; with
+        return_logprobs, (tokens, ops.TokenLogprobs of the new tokens
+        [b, max_new_tokens], with `top` alternatives each).  The reference
         has no sampling path: with greedy=False it sets the first token to
         None (model.py:359) and its first step fails; here that is a clear
         error before any work."""
         if not greedy:
             raise NotImplementedError("generate: only greedy decoding exists (the reference's greedy=False "
                                       "path has no sampler)")
+        if top and not return_logprobs:
+            raise ValueError("generate: top alternatives come with return_logprobs=True")
         logits, cache = self.prefill(input_ids)
-        next_id = logits[:, -1:].argmax(dim=-1)
-        tokens = [input_ids, next_id]
-        for _ in range(max_new_tokens - 1):
-            logits = self.step(next_id, cache)
-            next_id = logits[:, -1, :].argmax(dim=-1, keepdim=True)
+        logits = logits[:, -1:]
+        tokens, scores = [input_ids], []
+        for i in range(max(max_new_tokens, 1)):
+            if i:
+                logits = self.step(next_id, cache)
+            next_id = logits.argmax(dim=-1)
             tokens.append(next_id)
-        return torch.cat(tokens, dim=1)
+            if return_logprobs:
+                scores.append(ops.token_logprobs(logits, next_id, top=top))
+        tokens = torch.cat(tokens, dim=1)
+        if not return_logprobs:
+            return tokens
+        return tokens, ops.TokenLogprobs(*(torch.cat(t, dim=1) for t in zip(*scores)))
 
     @classmethod
     def from_pretrained(cls, hf_path: str, dtype=torch.float32) -> "MambaLM":

@@ -1,0 +1,204 @@
+"""LinearW4, a model whose projections and lm_head are in 4-bit codes, and log probabilities through the model: each
+against the same computation on the matrices that the codes stand for."""
+import copy
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from mamba_lite import ops
+from mamba_lite.cuda_graph import GraphedPrefill, GraphedStepper
+from mamba_lite.model import LinearW4, MambaCache, MambaConfig, MambaLM
+
+pytestmark = pytest.mark.gpu
+
+# The two sides differ in how fp32 sums of at most 2048 products are ordered, 2^-24 sqrt(2048) of each product's norm, as
+# tests of the per-op and one-call paths against each other do (1e-5 there for two layers)
+TOL = 1e-5
+
+
+def _rel(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm())
+
+
+def _model(d_model=256, n_layer=2, dtype=torch.float32, **kw):
+    torch.manual_seed(d_model + n_layer)
+    m = MambaLM(MambaConfig(d_model=d_model, n_layer=n_layer, vocab_size=1003, **kw)).cuda().eval()
+    with torch.no_grad():
+        for blk in m.layers:                        # small steps, as a trained model takes them
+            blk.mixer.dt_proj.bias.uniform_(-4.0, -2.0)
+    return m.to(dtype)
+
+
+def _on_matrices(q):
+    """A model of plain projections that hold the quantized ones' matrices."""
+    m = copy.deepcopy(q)
+    for blk in m.layers:
+        for name in ("in_proj", "out_proj"):
+            w = getattr(blk.mixer, name)
+            lin = torch.nn.Linear(w.in_features, w.out_features, bias=w.bias is not None).cuda().to(q.embedding.weight.dtype)
+            with torch.no_grad():
+                lin.weight.copy_(ops.dequantize_w4(w.w4(), lin.weight.dtype))
+                if w.bias is not None:
+                    lin.bias.copy_(w.bias)
+            setattr(blk.mixer, name, lin)
+    m._modules.pop("head_w4", None)
+    return m
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("zero_points,bias", [(False, True), (True, False)])
+def test_linear_w4_module(zero_points, bias, dtype):
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(300, 200, bias=bias).cuda().to(dtype)
+    q = LinearW4.from_linear(lin, 32, zero_points)
+    w = ops.dequantize_w4(q.w4(), torch.float32).double()
+    step = q.scales.max().item() * (1.5 if zero_points else 1.0)       # half a step, and the end of the range
+    assert float((w - lin.weight.detach().double()).abs().max()) <= step
+    tol = TOL if dtype == torch.float32 else 2.0 ** -7                 # the output's and (many rows) the matrix's rounding
+    with torch.no_grad():
+        for shape in ((300,), (1, 300), (4, 5, 300), (64, 300), (65, 300), (3, 40, 300), (1500, 300)):
+            x = torch.randn(shape, device="cuda").to(dtype)
+            ref = x.double() @ w.t().contiguous() + (lin.bias.double() if bias else 0)
+            y = q(x)
+            assert y.dtype == dtype and y.shape == ref.shape and _rel(y, ref) < tol
+        again = copy.deepcopy(q)
+        again.load_state_dict(q.state_dict())
+        assert torch.equal(again(x[:3]), q(x[:3]))
+    x = torch.randn(5, 300, device="cuda", dtype=dtype, requires_grad=True)   # the matrix's product, with x's gradient
+    g = torch.randn(5, 200, device="cuda").to(dtype)
+    q(x).backward(g)
+    assert _rel(x.grad, g.double() @ w) < tol and q.weight.grad is None
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(zero_points=True, group=128, scale_dtype=torch.float32)])
+@pytest.mark.parametrize("b,l", [(1, 5), (3, 30), (2, 200)])
+def test_prefill_and_steps_are_those_of_the_matrices(b, l, kw):
+    q = _model(bias=True).quantize_w4(lm_head=False, **kw)
+    ref = _on_matrices(q)
+    ids = torch.randint(0, 1003, (b, l + 4), device="cuda")
+    with torch.no_grad():
+        got, cq = q.prefill(ids[:, :l])
+        want, cr = ref.prefill(ids[:, :l])
+        assert _rel(got, want) < TOL
+        for t in range(l, l + 4):
+            got, want = q.step(ids[:, t:t + 1], cq), ref.step(ids[:, t:t + 1], cr)
+            assert _rel(got, want) < TOL
+        for a, c in zip(cq.layers, cr.layers):
+            assert _rel(a.ssm_state, c.ssm_state) < TOL and _rel(a.conv_state, c.conv_state) < TOL
+
+
+def test_bf16_model():
+    q = _model(d_model=512, dtype=torch.bfloat16).quantize_w4()
+    ref = _on_matrices(q)
+    ids = torch.randint(0, 1003, (2, 20), device="cuda")
+    with torch.no_grad():
+        head = ops.dequantize_w4(q.head_w4.w4(), torch.bfloat16)
+        got, cq = q.prefill(ids[:, :19])
+        xf, cr = ref._prefill_hidden(ids[:, :19])
+        # activations rounded to bf16 between a dozen operations: 2^-8 each, a walk of them
+        assert _rel(got, F.linear(xf, head)) < 2.0 ** -8 * 6
+        assert q.step(ids[:, 19:], cq).shape == (2, 1, q.cfg.vocab_size)
+
+
+def test_the_head_and_the_one_call_plans():
+    m = _model()
+    ids = torch.randint(0, 1003, (2, 40), device="cuda")
+    with torch.no_grad():
+        before, cache = m.prefill(ids)                     # makes the plain model's call plans
+        m.step(ids[:, :1], cache)
+        plain = copy.deepcopy(m)
+        q = m.quantize_w4(group=32)
+        assert q is m
+        got, _ = q.prefill(ids)
+        ref = _on_matrices(q)
+        xf, _ = ref._prefill_hidden(ids)
+        w = ops.dequantize_w4(q.head_w4.w4())
+        assert _rel(got, F.linear(xf, w)) < TOL
+        # 16 values for 32 weights: a step of about a seventh of 2.2 sigma, an error of 0.09 sigma in each of the three
+        # products of a layer and in the head
+        assert _rel(got, before) < 0.5
+        assert _rel(plain.prefill(ids)[0], before) == 0.0
+    with pytest.raises(TypeError, match="plain nn.Linear"):
+        q.quantize_w4()
+    state = q.state_dict()
+    other = _model().quantize_w4(group=32)
+    with torch.no_grad():
+        for p in other.parameters():
+            p.zero_()
+    other.load_state_dict(state)
+    with torch.no_grad():
+        assert torch.equal(other.prefill(ids)[0], got)
+
+
+@pytest.mark.parametrize("b", [1, 3])
+def test_captured_prefill_and_steps(b):
+    q = _model().quantize_w4()
+    ids = torch.randint(0, 1003, (b, 24), device="cuda")
+    with torch.no_grad():
+        cache = MambaCache.allocate(q.cfg, b, "cuda", torch.float32)
+        pre = GraphedPrefill(q, cache, b, 16, "cuda")
+        pre.capture()
+        step = GraphedStepper(q, cache, b, "cuda")
+        step.capture()
+        for turn in range(2):
+            prompt = ids.roll(turn, 1)
+            logits = pre.replay(prompt[:, :16])
+            want, c2 = q.prefill(prompt[:, :16])
+            torch.cuda.synchronize()
+            assert torch.equal(logits, want)
+            for t in range(16, 20):
+                got, want = step.replay(prompt[:, t:t + 1]), q.step(prompt[:, t:t + 1], c2)
+                torch.cuda.synchronize()
+                assert torch.equal(got, want)
+
+
+def _reference(logits, given, top):
+    lnp = torch.log_softmax(logits.double(), -1)
+    a, i = torch.sort(lnp, dim=-1, descending=True, stable=True)
+    return (lnp.gather(-1, given[..., None])[..., 0], -(lnp.exp() * lnp).sum(-1), a[..., :top], i[..., :top])
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("b,l", [(1, 1), (1, 2), (3, 37), (2, 300)])
+def test_score(b, l, quantized):
+    m = _model()
+    if quantized:
+        m.quantize_w4()
+    ids = torch.randint(0, 1003, (b, l), device="cuda")
+    r = m.score(ids, top=3)
+    assert r.logprob.shape == r.entropy.shape == (b, l - 1) and r.top_token.shape == r.top_logprob.shape == (b, l - 1, 3)
+    if l == 1:
+        return
+    with torch.no_grad():
+        logits, _ = m.prefill(ids)
+    want = _reference(logits[:, :-1], ids[:, 1:], 3)
+    # the head's product runs over other rows here: TOL of a logit's size, and token_logprobs' own rounding
+    tol = 4 * TOL * float(logits.abs().max()) + 2.0 ** -24 * 120
+    assert all(float((g - w).abs().max()) < tol for g, w in zip(r[:3], want[:3]))
+    gap = (want[2][..., :-1] - want[2][..., 1:]).min(-1)[0] > tol      # where the order is not a matter of rounding
+    assert torch.equal(r.top_token[..., 0][gap], want[3][..., 0][gap])
+    whole = m._SCORE_LOGITS
+    try:
+        m._SCORE_LOGITS = 1008 * 7                                     # 7 rows at a time
+        parts = m.score(ids, top=3)
+    finally:
+        m._SCORE_LOGITS = whole
+    assert float((parts.logprob - r.logprob).abs().max()) < tol and parts.top_token.shape == r.top_token.shape
+
+
+@pytest.mark.parametrize("b", [1, 4])
+def test_generate_with_log_probabilities(b):
+    m = _model().quantize_w4()
+    ids = torch.randint(0, 1003, (b, 9), device="cuda")
+    tokens = m.generate(ids, 6)
+    again, r = m.generate(ids, 6, return_logprobs=True, top=4)
+    assert torch.equal(tokens, again) and tokens.shape == (b, 15)
+    assert r.logprob.shape == (b, 6) and r.top_token.shape == (b, 6, 4)
+    assert torch.equal(r.top_token[..., 0], tokens[:, 9:])             # greedy: the most probable one was taken
+    assert torch.equal(r.top_logprob[..., 0], r.logprob)
+    s = m.score(tokens, top=1)
+    tol = 64 * TOL                                                     # a prompt's logits against the steps'
+    assert float((s.logprob[:, 8:] - r.logprob).abs().max()) < tol
+    with pytest.raises(ValueError, match="return_logprobs"):
+        m.generate(ids, 2, top=3)
