@@ -828,12 +828,41 @@ typedef struct {
     int64_t ldx, ldy;
     int64_t M, N, K;
     int32_t group, dtype, scale_dtype;
-    int32_t reserved;
+    int32_t y_f32;             /* 1: y holds floats whatever dtype is */
 } mtl_linear_w4_args;
 
 int mtl_linear_w4(const mtl_linear_w4_args* args, mtl_stream_t stream);
 int mtl_dequantize_w4(const uint8_t* codes, const void* scales, const uint8_t* zeros, void* W, int64_t ldw, int64_t N,
                       int64_t K, int32_t group, int32_t dtype, int32_t scale_dtype, mtl_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * mtl_decode_step_w4: mtl_decode_step_batched for a stack whose in_proj and
+ * out_proj are 4-bit matrices: a decode step of 1..32 rows in one call, up to
+ * the lm_head's input (MambaLM.step, model.py:343-353 over 308-311 and
+ * 249-294).  Per layer: mtl_linear_w4 (in_proj), the conv step, x_proj's
+ * partial products and their ordered sum, the SSM update, mtl_linear_w4
+ * (out_proj, in floats), the residual add and the next RMSNorm.
+ *   matrices    [2 n_layers]: in_proj [2 d_inner, d_model] and out_proj
+ *               [d_model, d_inner] of each layer in the layout above
+ *   layers      mtl_decode_layer without W_in and W_out; MTL_F32 reads W_xT,
+ *               MTL_BF16 (every parameter, activation and conv history in
+ *               bf16 behind the same pointers) W_x, 16-byte aligned
+ *   args        as mtl_decode_step_batched without fold, but z [b, 2 d_inner],
+ *               parts [b, d_model] floats, xpart [ceil(d_inner / 32), b, J]
+ *               floats; xn, sq and counters are not read
+ * d_model, d_inner <= 65536, d_state <= 16, dt_rank <= 256 with J = dt_rank
+ * + 2 d_state <= 288, d_conv 2..4; MTL_BF16: d_inner a multiple of 64, at
+ * least 256, J a multiple of 4.  Everything is checked before the first launch.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    const uint8_t* codes;
+    const void* scales;
+    const uint8_t* zeros;      /* or NULL */
+    int32_t group, scale_dtype;
+} mtl_w4_matrix;
+
+int mtl_decode_step_w4(const mtl_decode_step_batched_args* args, const mtl_decode_layer* layers,
+                       const mtl_w4_matrix* matrices, int32_t dtype, mtl_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Log probabilities of given tokens, with entropy and the most probable

@@ -182,10 +182,10 @@ __global__ void conv_state_copy_kernel(const T* __restrict__ in, T* __restrict__
     if (i < n) out[i] = in ? in[i] : T(0);
 }
 
-template <typename T, int K>
+template <typename T, int K, typename P = float>
 __global__ void __launch_bounds__(256) conv_step_kernel(T* __restrict__ state, const T* __restrict__ x,
-                                                        int64_t x_sb, const float* __restrict__ w,
-                                                        const float* __restrict__ bias, T* __restrict__ out,
+                                                        int64_t x_sb, const P* __restrict__ w,
+                                                        const P* __restrict__ bias, T* __restrict__ out,
                                                         int64_t o_sb, int D, int silu) {
     const int c = blockIdx.x * blockDim.x + threadIdx.x;
     const int b = blockIdx.y;
@@ -197,8 +197,8 @@ __global__ void __launch_bounds__(256) conv_step_kernel(T* __restrict__ state, c
     win[K - 1] = Act<T>::load(x + b * x_sb + c);
     float acc = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) acc = fmaf(win[k], w[(int64_t)c * K + k], acc);
-    if (bias) acc += bias[c];
+    for (int k = 0; k < K; ++k) acc = fmaf(win[k], Act<P>::load(w + (int64_t)c * K + k), acc);
+    if (bias) acc += Act<P>::load(bias + c);
     // in-place history shift: conv_state <- conv_in[..., 1:]
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) Act<T>::store(s + k, win[k + 1]);
@@ -417,6 +417,24 @@ extern "C" int mtl_causal_conv1d_fwd(const mtl_conv_params* p, mtl_stream_t stre
     MTL_REQUIRE(!a.par_bf || reinterpret_cast<uintptr_t>(p->w) % 8 == 0, "bf16 weights must be 8-byte aligned");
     return p->dtype == MTL_F32 ? launch_conv<float>(a, p->batch, st) : launch_conv<uint16_t>(a, p->batch, st);
 }
+
+namespace mtl {
+int conv_step_bf16(uint16_t* conv_state, const uint16_t* x, int64_t x_sb, const uint16_t* w, const uint16_t* bias,
+                   uint16_t* out, int64_t out_sb, int64_t batch, int64_t dim, int32_t width, mtl_stream_t stream) {
+    MTL_REQUIRE(batch >= 1 && batch <= 65535 && dim >= 1 && dim < (int64_t(1) << 31), "size out of range");
+    MTL_REQUIRE(conv_state && x && w && out, "null required pointer");
+    const dim3 grid((unsigned)((dim + 255) / 256), (unsigned)batch);
+    switch (width) {
+#define MTL_STEP_CASE(KK)                                                                                           \
+    case KK: hipLaunchKernelGGL((conv_step_kernel<uint16_t, KK, uint16_t>), grid, dim3(256), 0, as_stream(stream),  \
+                                conv_state, x, x_sb, w, bias, out, out_sb, (int)dim, 1); break;
+        MTL_STEP_CASE(2) MTL_STEP_CASE(3) MTL_STEP_CASE(4)
+#undef MTL_STEP_CASE
+        default: set_error("conv_step_bf16: width must be 2, 3 or 4"); return MTL_EINVAL;
+    }
+    return check_launch("conv_step");
+}
+}  // namespace mtl
 
 extern "C" int mtl_conv_step(void* conv_state, const void* x, int64_t x_sb, const float* w, const float* bias,
                              void* out, int64_t out_sb, int64_t batch, int64_t dim, int32_t width,

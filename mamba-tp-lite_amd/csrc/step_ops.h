@@ -15,6 +15,10 @@ int in_proj_conv_xproj(const T* x, int64_t x_rs, const T* W_in, const T* b_in, T
                        float* xpart, int64_t batch, int64_t d_model, int64_t d_inner, int32_t channels_per_part,
                        const float* sq, int32_t sq_tiles, float eps, mtl_stream_t stream);
 
+// conv step + SiLU, parameters in bf16 (conv.hip)
+int conv_step_bf16(uint16_t* conv_state, const uint16_t* x, int64_t x_sb, const uint16_t* w, const uint16_t* bias,
+                   uint16_t* out, int64_t out_sb, int64_t batch, int64_t dim, int32_t width, mtl_stream_t stream);
+
 // ksplit partial products of y = x W^T (+ bias in part 0), fp32 (linear.hip)
 template <typename T>
 int linear_parts(const T* x, int64_t x_rs, const T* W, const T* bias, float* y, int64_t y_rs, int64_t y_ks, int64_t M,

@@ -24,6 +24,7 @@ struct W4Args {
     void* y;
     int64_t ldx, ldy;
     int M, N, K, KB;           // KB: 128-column blocks of a row
+    int y_f32;                 // y holds floats whatever x is
 };
 
 // the code of column 32 i + 8 j + e in word w
@@ -294,7 +295,9 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
             const int n = tile * kTileRows + r;
             if ((j == 0 || !spread) && n < a.N) {
                 if (a.bias) v += Act<T>::load(static_cast<const T*>(a.bias) + n);
-                Act<T>::store(static_cast<T*>(a.y) + (m0 + m) * a.ldy + n, v);
+                const int64_t at = (m0 + m) * a.ldy + n;
+                if (a.y_f32) static_cast<float*>(a.y)[at] = v;
+                else Act<T>::store(static_cast<T*>(a.y) + at, v);
             }
         };
         if (p.wk == 1) {                                     // a wavefront's own sums: no other waits for it
@@ -421,7 +424,7 @@ extern "C" int mtl_linear_w4(const mtl_linear_w4_args* p, mtl_stream_t stream) {
     MTL_REQUIRE(p->ldx >= p->K && p->ldy >= p->N, "rows of x and y must not overlap");
     MTL_REQUIRE(reinterpret_cast<uintptr_t>(p->zeros) % 4 == 0, "zeros must be 4-byte aligned");
     const W4Args a{p->x, p->codes, p->scales, p->zeros, p->bias, p->y, p->ldx, p->ldy, (int)p->M, (int)p->N, (int)p->K,
-                   (int)((p->K + kBlockK - 1) / kBlockK)};
+                   (int)((p->K + kBlockK - 1) / kBlockK), p->y_f32 != 0};
     const int es = dtype == MTL_F32 ? 4 : 2, parts = dtype == MTL_F32 ? 3 : 1;
     LinearW4 l{a, 0, 0, 1, 0, reinterpret_cast<uintptr_t>(p->x) % 16 == 0 && p->ldx * es % 16 == 0};
     const int tiles = (a.N + kTileRows - 1) / kTileRows;
@@ -473,7 +476,7 @@ extern "C" int mtl_dequantize_w4(const uint8_t* codes, const void* scales, const
     MTL_REQUIRE(ldw >= K, "rows of W must not overlap");
     MTL_REQUIRE(reinterpret_cast<uintptr_t>(zeros) % 4 == 0, "zeros must be 4-byte aligned");
     const W4Args a{nullptr, codes, scales, zeros, nullptr, W, 0, ldw, 0, (int)N, (int)K,
-                   (int)((K + kBlockK - 1) / kBlockK)};
+                   (int)((K + kBlockK - 1) / kBlockK), 0};
     const int64_t groups = ((N + kTileRows - 1) / kTileRows * a.KB + 3) / 4, gy = (groups + (1 << 22) - 1) >> 22;
     const dim3 grid((unsigned)((groups + gy - 1) / gy), (unsigned)gy);
     if (reinterpret_cast<uintptr_t>(W) % 16 == 0 && ldw * (dtype == MTL_F32 ? 4 : 2) % 16 == 0) {

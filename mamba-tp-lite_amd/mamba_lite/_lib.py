@@ -130,8 +130,13 @@ class LinearW4Args(ctypes.Structure):
     _fields_ = [
         ("x", _vp), ("codes", _vp), ("scales", _vp), ("zeros", _vp), ("bias", _vp), ("y", _vp),
         ("ldx", _i64), ("ldy", _i64), ("M", _i64), ("N", _i64), ("K", _i64),
-        ("group", _i32), ("dtype", _i32), ("scale_dtype", _i32), ("reserved", _i32),
+        ("group", _i32), ("dtype", _i32), ("scale_dtype", _i32), ("y_f32", _i32),
     ]
+
+
+class W4Matrix(ctypes.Structure):
+    """mirror of mtl_w4_matrix"""
+    _fields_ = [("codes", _vp), ("scales", _vp), ("zeros", _vp), ("group", _i32), ("scale_dtype", _i32)]
 
 
 class TokenLogprobsArgs(ctypes.Structure):
@@ -200,6 +205,8 @@ SIGNATURES = {
                                       _vp]),
     "mtl_linear_w4": (ctypes.c_int, [ctypes.POINTER(LinearW4Args), _vp]),
     "mtl_dequantize_w4": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp]),
+    "mtl_decode_step_w4": (ctypes.c_int, [ctypes.POINTER(DecodeStepBatchedArgs), ctypes.POINTER(DecodeLayer),
+                                          ctypes.POINTER(W4Matrix), _i32, _vp]),
     "mtl_token_logprobs": (ctypes.c_int, [ctypes.POINTER(TokenLogprobsArgs), _vp]),
 }
 

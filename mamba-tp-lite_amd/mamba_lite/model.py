@@ -267,8 +267,8 @@ class LinearW4(nn.Module):
     def __init__(self, w4: ops.W4, bias: torch.Tensor | None = None):
         super().__init__()
         self.out_features, self.in_features, self.group = w4.n, w4.k, w4.group
-        par = lambda t: None if t is None else nn.Parameter(t.detach(), requires_grad=False)
-        self.weight, self.scales, self.zeros, self.bias = par(w4.codes), par(w4.scales), par(w4.zeros), par(bias)
+        for name, t in (("weight", w4.codes), ("scales", w4.scales), ("zeros", w4.zeros), ("bias", bias)):
+            self.register_parameter(name, None if t is None else nn.Parameter(t.detach(), requires_grad=False))
 
     @classmethod
     def from_linear(cls, lin: nn.Linear, group: int = 64, zero_points: bool = False,
@@ -638,11 +638,12 @@ class MambaBlock(nn.Module):
         return x_t + self.mixer.step(self.norm(x_t), cache)
 
 
-_CALL_PLANS = frozenset(("_short_plan", "_batched_tmpl", "_plan", "_step_tmpl", "_fused_memo", "_persist_tab",
+_CALL_PLANS = frozenset(("_short_plan", "_batched_tmpl", "_w4_tmpl", "_plan", "_step_tmpl", "_fused_memo", "_persist_tab",
                          "_persist_ws"))
 
 # what a MambaLM's layers are made of, and nothing else of, where _plain_stack holds
 _STACK_MODULES = frozenset((nn.ModuleList, MambaBlock, MambaMixer, RMSNorm, nn.Linear, nn.Conv1d))
+_W4_STACK_MODULES = _STACK_MODULES | {LinearW4}
 
 
 class MambaLM(nn.Module):
@@ -858,10 +859,17 @@ class MambaLM(nn.Module):
         layer); others run the per-op path (the matrix-core skinny GEMMs or
         the library's, the conv-step and SSM-update kernels)."""
         lt = self._layer_tensors()
-        if self._fused_step_ok(input_ids, cache, lt=lt):
+        w4 = len(lt) > 0 and type(self.layers[0].mixer.in_proj) is LinearW4
+        if not w4 and self._fused_step_ok(input_ids, cache, lt=lt):
             return self._step_fused(input_ids, cache, lt=lt)
         x = self.embedding(input_ids).squeeze(1)
-        if BATCHED_STEP_NATIVE:
+        if w4 and BATCHED_STEP_NATIVE:
+            got = self._w4_step_layers(x, cache, lt)
+            if got is not None:
+                h = x if x.dtype == torch.float32 else x.float()
+                normed = ops.decode_step_w4(*got, h, self.norm_f.weight, self.norm_f.eps, self.cfg, dtype=x.dtype)
+                return self.lm_head(normed).unsqueeze(1)
+        if BATCHED_STEP_NATIVE and not w4:
             got = self._batched_step_layers(x, cache, lt)
             if got is not None:
                 arr, fold = got
@@ -1033,6 +1041,89 @@ class MambaLM(nn.Module):
                          ptr(ts[_LT_A_LOG]), ptr(ts[_LT_D]), ptr(ts[_LT_W_OUT]), ptr(ts[_LT_B_OUT]))
             L.eps = self.layers[i].norm.eps
         return tmpl
+
+    # ---- a 4-bit stack's step in one call ----
+    def _w4_step_layers(self, x, cache, lt):
+        """(ctypes arrays of mtl_decode_layer with this call's cache pointers and of mtl_w4_matrix) for
+        mtl_decode_step_w4, or None where it does not apply: sizes, a stack of more than plain modules and LinearW4, a
+        weight or cache tensor that is not a contiguous tensor of x's dtype (SSM states: float32) and its shape on x's
+        device.  The weights are checked when their addresses (or x_proj's version, which its transposed copy follows)
+        change; the cache tensors every call."""
+        cfg, act, dev = self.cfg, x.dtype, x.device
+        nl = len(lt)
+        D, N, K, R = cfg.d_inner, cfg.d_state, cfg.d_conv, cfg.dt_rank
+        J = R + 2 * N
+        if act not in (torch.float32, torch.bfloat16) or x.dim() != 2 or not x.is_cuda or len(cache.layers) != nl:
+            return None
+        b, dm = x.shape
+        if not (1 <= b <= ops.IN_CONV_MAX_ROWS and N <= 16 and R <= 256 and J <= 288 and 2 <= K <= 4) or \
+                max(dm, D) > 65536 or (act == torch.bfloat16 and (D % 64 or D < 256 or J % 4)):
+            return None
+        nf = self.norm_f.weight
+        if nf.dtype != act or nf.device != dev or not nf.is_contiguous() or tuple(nf.shape) != (dm,):
+            return None
+        if not (ops.plain_call() and _no_global_hooks() and _plain_modules(self.layers, _W4_STACK_MODULES)):
+            return None
+        if act == torch.float32 and any(ts[_LT_XPROJ].is_inference() for ts in lt):
+            return None                  # (no version that the transposed copy could follow)
+        proj = [p for blk in self.layers._modules.values() for p in
+                (blk._modules["mixer"]._modules["in_proj"], blk._modules["mixer"]._modules["out_proj"])]
+        if any(type(p) is not LinearW4 for p in proj):
+            return None
+        ptr = lambda t: 0 if t is None else t.data_ptr()
+        sig = (dev, dm, act, tuple(ptr(t) for ts in lt for t in ts),
+               tuple(ptr(p._parameters[n]) for p in proj for n in ("scales", "zeros")),
+               tuple(ts[_LT_XPROJ]._version for ts in lt) if act == torch.float32 else None, self._norm_eps())
+        cached = getattr(self, "_w4_tmpl", None)
+        if cached is None or cached[0] != sig:
+            cached = (sig, self._w4_template(lt, proj, dev, dm, act))
+            self._w4_tmpl = cached
+        if cached[1] is None:
+            return None
+        cs_shape, hs_shape = (b, D, K - 1), (b, D, N)
+        for lc in cache.layers:
+            cs, hs = lc.conv_state, lc.ssm_state
+            if cs.dtype != act or hs.dtype != torch.float32 or cs.shape != cs_shape or hs.shape != hs_shape or \
+                    not cs.is_contiguous() or not hs.is_contiguous() or cs.device != dev or hs.device != dev:
+                return None
+        tmpl, mats = cached[1]
+        arr = type(tmpl).from_buffer_copy(tmpl)   # per call: read by the library without the GIL
+        for L, lc in zip(arr, cache.layers):
+            L.conv_state, L.ssm_state = lc.conv_state.data_ptr(), lc.ssm_state.data_ptr()
+        return arr, mats
+
+    def _w4_template(self, lt, proj, dev, dm, act):
+        """The weight half of _w4_step_layers, or None when a weight is not a contiguous `act` tensor of its shape on
+        dev, or one the library loads in 16-byte runs (codes, scales, a bf16 x_proj) is not aligned."""
+        cfg = self.cfg
+        D, N, K, R = cfg.d_inner, cfg.d_state, cfg.d_conv, cfg.dt_rank
+        ok = lambda t, shape: t.device == dev and t.dtype == act and t.is_contiguous() and tuple(t.shape) == shape
+        opt = lambda t, shape: t is None or ok(t, shape)
+        tmpl, mats = (_lib.DecodeLayer * len(lt))(), (_lib.W4Matrix * (2 * len(lt)))()
+        for i, (ts, L) in enumerate(zip(lt, tmpl)):
+            for p, m, shape in ((proj[2 * i], mats[2 * i], (2 * D, dm)), (proj[2 * i + 1], mats[2 * i + 1], (dm, D))):
+                w = p.w4()
+                if (w.n, w.k) != shape or w.codes.device != dev or not ops.aligned16(w.codes, w.scales) or \
+                        (w.zeros is not None and w.zeros.data_ptr() % 4):
+                    return None
+                m.codes, m.scales = w.codes.data_ptr(), w.scales.data_ptr()
+                m.zeros = None if w.zeros is None else w.zeros.data_ptr()
+                m.group, m.scale_dtype = w.group, ops._ACT_DTYPES[w.scales.dtype]
+            if not (ok(ts[_LT_NORM], (dm,)) and opt(ts[_LT_B_IN], (2 * D,)) and ok(ts[_LT_CONV_W], (D, 1, K))
+                    and opt(ts[_LT_CONV_B], (D,)) and ok(ts[_LT_XPROJ], (R + 2 * N, D)) and ok(ts[_LT_W_DT], (D, R))
+                    and ok(ts[_LT_B_DT], (D,)) and ok(ts[_LT_A_LOG], (D, N)) and opt(ts[_LT_D], (D,))
+                    and opt(ts[_LT_B_OUT], (dm,))) or not (act == torch.float32 or ops.aligned16(ts[_LT_XPROJ])):
+                return None
+            ptr = lambda t: None if t is None else t.data_ptr()
+            (L.norm_w, L.b_in, L.conv_w, L.conv_b, L.W_dt, L.dt_bias, L.A_log, L.Dv, L.b_out) = map(ptr, (
+                ts[_LT_NORM], ts[_LT_B_IN], ts[_LT_CONV_W], ts[_LT_CONV_B], ts[_LT_W_DT], ts[_LT_B_DT], ts[_LT_A_LOG],
+                ts[_LT_D], ts[_LT_B_OUT]))
+            if act == torch.float32:
+                L.W_xT = self.layers[i].mixer._xproj_t().data_ptr()
+            else:
+                L.W_x = ts[_LT_XPROJ].data_ptr()
+            L.eps = self.layers[i].norm.eps
+        return tmpl, mats
 
     # ---- fused decode step ----
     def _fused_step_ok(self, input_ids, cache, lt=None) -> bool:

@@ -1357,6 +1357,42 @@ def linear_w4(x, w4, bias=None, out=None):
     return out
 
 
+def decode_step_w4(layers, matrices, h, norm_f, eps_f, cfg, dtype=torch.float32):
+    """mtl_decode_step_w4: a decode step of every layer of a 4-bit stack in one
+    call.  `layers` is a ctypes array of _lib.DecodeLayer (this call's cache
+    pointers in it), `matrices` one of _lib.W4Matrix (in_proj and out_proj of
+    each layer); h [b, d_model] float32 holds the step's embedding rows and is
+    left holding the final residual stream.  Returns norm_f of it [b, d_model]
+    in `dtype`, the weights', conv histories' and output's type."""
+    _f32c(h, "h")
+    if dtype not in _ACT_DTYPES or norm_f.dtype != dtype or not norm_f.is_contiguous():
+        raise ValueError(f"decode_step_w4: norm_f must be contiguous {dtype} (float32 or bfloat16)")
+    if h.dim() != 2 or h.shape[1] != cfg.d_model:
+        raise ValueError(f"decode_step_w4: h must be [b, {cfg.d_model}]")
+    b, M = h.shape
+    if norm_f.numel() != M or norm_f.device != h.device:
+        raise ValueError(f"decode_step_w4: norm_f must hold {M} values on {h.device}")
+    if len(matrices) != 2 * len(layers):
+        raise ValueError("decode_step_w4: two matrices for each layer expected")
+    D, J = cfg.d_inner, cfg.dt_rank + 2 * cfg.d_state
+    pad = lambda n: -(-n // 64) * 64                      # 256-byte aligned slices
+    sizes = {"normed_out": b * M, "inp": b * M, "xc": b * D, "z": 2 * b * D, "y": b * D,
+             "xpart": max(-(-D // 32), 16) * b * J, "x_dbl": b * J, "parts": b * M}
+    ws = torch.empty(sum(pad(n) for n in sizes.values()), device=h.device, dtype=torch.float32)
+    a = _lib.DecodeStepBatchedArgs()
+    off = 0
+    for name, n in sizes.items():
+        setattr(a, name, ws.data_ptr() + 4 * off)
+        off += pad(n)
+    a.h, a.norm_f = h.data_ptr(), norm_f.data_ptr()
+    a.eps_f, a.n_layers, a.batch = float(eps_f), len(layers), b
+    a.d_model, a.d_inner, a.d_state, a.dt_rank, a.d_conv = M, D, cfg.d_state, cfg.dt_rank, cfg.d_conv
+    with _dev_guard(h):
+        _lib.check(_lib.load().mtl_decode_step_w4(ctypes.byref(a), layers, matrices, _ACT_DTYPES[dtype], _stream(h)),
+                   "decode_step_w4")
+    return ws.view(dtype)[:b * M].view(b, M)     # normed_out: the workspace's first slice
+
+
 def dequantize_w4(w4, dtype=torch.float32, out=None):
     """The matrix [n, k] of a W4 in float32 or bfloat16 (mtl_dequantize_w4): what a prompt's product reads."""
     if not isinstance(w4, W4):

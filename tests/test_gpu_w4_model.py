@@ -202,3 +202,87 @@ def test_generate_with_log_probabilities(b):
     assert float((s.logprob[:, 8:] - r.logprob).abs().max()) < tol
     with pytest.raises(ValueError, match="return_logprobs"):
         m.generate(ids, 2, top=3)
+
+
+SHAPES = [(256, 2, 1, 4, dict()), (320, 2, 3, 2, dict(zero_points=True, group=32)), (512, 2, 17, 3, dict(group=128)),
+          (2048, 2, 32, 4, dict(scale_dtype=torch.float32)), (768, 2, 2, 4, dict(zero_points=True))]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dm,expand,b,d_conv,kw", SHAPES)
+def test_the_one_call_step(dm, expand, b, d_conv, kw, dtype, monkeypatch):
+    """mtl_decode_step_w4 against the steps op by op (fp32: the same launches, the same bits; bf16: as near to the fp32
+    step on the same weights), eager and captured."""
+    import mamba_lite.model as mm
+    q = _model(dm, 2, dtype, expand=expand, d_conv=d_conv, bias=dm == 320).quantize_w4(**kw)
+    cache = MambaCache.allocate(q.cfg, b, "cuda", dtype)
+    for lc in cache.layers:
+        lc.conv_state.normal_(0, 0.6)
+        lc.ssm_state.normal_(0, 0.1)
+    clone = lambda t=dtype: MambaCache([type(lc)(lc.conv_state.to(t, copy=True), lc.ssm_state.clone())
+                                        for lc in cache.layers])
+    ids = torch.randint(0, 1003, (b, 2), device="cuda")
+    calls = []
+    real = ops.decode_step_w4
+    monkeypatch.setattr(ops, "decode_step_w4", lambda *a, **k: (calls.append(1), real(*a, **k))[1])
+    run = lambda m, c: [m.step(ids[:, t:t + 1], c) for t in range(2)]
+    with torch.no_grad():
+        c1, c2 = clone(), clone()
+        one = run(q, c1)
+        assert len(calls) == 2
+        monkeypatch.setattr(mm, "BATCHED_STEP_NATIVE", False)
+        old = run(q, c2)
+        assert len(calls) == 2
+        if dtype == torch.float32:
+            assert all(torch.equal(x, y) for x, y in zip(one, old))
+            assert all(torch.equal(x.ssm_state, y.ssm_state) and torch.equal(x.conv_state, y.conv_state)
+                       for x, y in zip(c1.layers, c2.layers))
+        else:
+            wide = copy.deepcopy(q).float()                    # the same weights, activations in fp32
+            c3 = clone(torch.float32)
+            ref = run(wide, c3)
+            for x, y, r in zip(one, old, ref):
+                # a dozen roundings of 2^-8 in a walk; and no further off than op by op, where out_proj's sum is rounded once
+                # more.  Both norms hold the n logits' own roundings, independent ones: a root of a sum of n squares
+                # spreads by 1 / sqrt(n) of itself at most (uniform errors: 0.45 / sqrt(n)), six of those allowed
+                assert _rel(x, r) < 2.0 ** -8 * 6 and _rel(x, r) <= (1 + 6 / r.numel() ** 0.5) * _rel(y, r)
+            for x, r in zip(c1.layers, c3.layers):
+                assert _rel(x.ssm_state, r.ssm_state) < 2.0 ** -8 * 6
+        monkeypatch.setattr(mm, "BATCHED_STEP_NATIVE", True)
+        st = GraphedStepper(q, clone(), b, "cuda")
+        st.capture()
+        for t in range(2):
+            got = st.replay(ids[:, t:t + 1])
+            torch.cuda.synchronize()
+            assert torch.equal(got, one[t])
+
+
+def test_what_keeps_the_step_op_by_op():
+    q = _model(512).quantize_w4()
+    cache = MambaCache.allocate(q.cfg, 2, "cuda", torch.float32)
+    x = torch.zeros(2, 512, device="cuda")
+    with torch.no_grad():
+        took = lambda: q._w4_step_layers(x, cache, q._layer_tensors()) is not None
+        assert took()
+        handle = q.layers[1].mixer.in_proj.register_forward_hook(lambda *_: None)
+        assert not took()
+        handle.remove()
+        assert took() and q._w4_step_layers(torch.zeros(33, 512, device="cuda"), cache, q._layer_tensors()) is None
+        q.norm_f.double()
+        assert not took()
+        q.norm_f.float()
+        q.layers[1].mixer.out_proj = torch.nn.Linear(1024, 512, bias=False).cuda()
+        assert not took()
+        before = q.step(torch.zeros(2, 1, dtype=torch.long, device="cuda"), cache)
+        assert bool(torch.isfinite(before).all())
+    # weights changed after a step: the next one reads them
+    q = _model(512).quantize_w4()
+    ids = torch.randint(0, 1003, (2, 1), device="cuda")
+    fresh = lambda: MambaCache.allocate(q.cfg, 2, "cuda", torch.float32)
+    with torch.no_grad():
+        q.step(ids, fresh())
+        q.layers[0].mixer.x_proj.weight.mul_(-1.5)
+        q.layers[1].mixer.in_proj.scales.mul_(0.5)
+        got = q.step(ids, fresh())
+        want = copy.deepcopy(q).step(ids, fresh())
+        assert torch.equal(got, want)

@@ -138,7 +138,7 @@ def test_calls_are_refused_on_the_host():
 def _args(**change):
     buf = 0x1000
     a = dict(x=buf, codes=buf, scales=buf, zeros=None, bias=None, y=buf, ldx=200, ldy=20, M=2, N=20, K=200, group=64,
-             dtype=0, scale_dtype=0, reserved=0)
+             dtype=0, scale_dtype=0, y_f32=0)
     a.update(change)
     return _lib.LinearW4Args(**a)
 
@@ -165,3 +165,41 @@ def test_the_library_refuses_a_matrix():
                 (p, p, p + 1, p, 200, 20, 200, 64, 0, 0), (p, p, None, p, 200, 20, 200, 65, 0, 0),
                 (p, p, None, p, 200, 0, 200, 64, 0, 0)):
         assert lib.mtl_dequantize_w4(*bad, None) == 1
+
+
+def _step_args(**change):
+    p = 0x1000
+    a = _lib.DecodeStepBatchedArgs()
+    for n in ("h", "norm_f", "inp", "xc", "z", "y", "xpart", "x_dbl", "parts", "normed_out"):
+        setattr(a, n, p)
+    a.h, a.normed_out, a.n_layers, a.batch = 0x2000, 0x3000, 1, 2
+    a.d_model, a.d_inner, a.d_state, a.dt_rank, a.d_conv = 256, 512, 16, 16, 4
+    L = (_lib.DecodeLayer * 1)()
+    for n in ("norm_w", "conv_w", "W_xT", "W_x", "W_dt", "dt_bias", "A_log", "conv_state", "ssm_state"):
+        setattr(L[0], n, p)
+    m = (_lib.W4Matrix * 2)()
+    for x in m:
+        x.codes, x.scales, x.group = p, p, 64
+    dtype = change.pop("dtype", 0)
+    for n, v in change.items():
+        if n.startswith("L_"):
+            setattr(L[0], n[2:], v)
+        elif n.startswith("m_"):
+            setattr(m[1], n[2:], v)
+        else:
+            setattr(a, n, v)
+    return ctypes.byref(a), L, m, dtype, None
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(batch=33), b"batch"), (dict(batch=0), b"batch"), (dict(n_layers=0), b"n_layers"), (dict(d_model=0), b"d_model"),
+    (dict(d_state=17), b"d_state"), (dict(dt_rank=257), b"dt_rank"), (dict(d_conv=5), b"d_conv"), (dict(fold=1), b"folded"),
+    (dict(dtype=2), b"dtype"), (dict(dtype=1, d_inner=200), b"multiple of 64"), (dict(dtype=1, dt_rank=17), b"of 4"),
+    (dict(parts=None), b"null"), (dict(h=0x1000), b"alias"), (dict(L_W_xT=None), b"null"), (dict(L_ssm_state=None), b"null"),
+    (dict(dtype=1, L_W_x=0x1008), b"aligned"), (dict(m_codes=None), b"codes"), (dict(m_scales=0x1008), b"aligned"),
+    (dict(m_group=48), b"group"), (dict(m_scale_dtype=2), b"scale_dtype"), (dict(xc=0x1004), b"aligned"),
+])
+def test_the_library_refuses_a_step(change, error):
+    lib = _lib.load()
+    assert lib.mtl_decode_step_w4(*_step_args(**change)) == 1
+    assert error in lib.mtl_last_error()
