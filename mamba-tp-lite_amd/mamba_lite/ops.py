@@ -1395,18 +1395,20 @@ def decode_step_w4(layers, matrices, h, norm_f, eps_f, cfg, dtype=torch.float32)
 
 def dequantize_w4(w4, dtype=torch.float32, out=None):
     """The matrix [n, k] of a W4 in float32 or bfloat16 (mtl_dequantize_w4): what a prompt's product reads."""
-    if not isinstance(w4, W4):
+    if type(w4) is not W4:
         raise TypeError(f"dequantize_w4: w4 must be a W4 (pack_w4, quantize_w4), got {type(w4).__name__}")
     if dtype not in _ACT_DTYPES:
         raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
     if out is None:
-        out = torch.empty(w4.n, w4.k, device=w4.codes.device, dtype=dtype)
-    elif tuple(out.shape) != (w4.n, w4.k) or out.dtype != dtype or (w4.k > 1 and out.stride(1) != 1) or \
-            (w4.n > 1 and out.stride(0) < w4.k):
-        raise ValueError(f"out must be {dtype} {(w4.n, w4.k)} with contiguous rows, got {tuple(out.shape)} {out.dtype}")
-    _same_device(w4.codes, out)
-    if any(t is not None and _overlap(out, t) for t in (w4.codes, w4.scales, w4.zeros)):
-        raise ValueError("out must not overlap an operand")
+        out = w4.codes.new_empty((w4.n, w4.k), dtype=dtype)
+    else:
+        if tuple(out.shape) != (w4.n, w4.k) or out.dtype != dtype or (w4.k > 1 and out.stride(1) != 1) or \
+                (w4.n > 1 and out.stride(0) < w4.k):
+            raise ValueError(f"out must be {dtype} {(w4.n, w4.k)} with contiguous rows, got {tuple(out.shape)} "
+                             f"{out.dtype}")
+        _same_device(w4.codes, out)
+        if any(t is not None and _overlap(out, t) for t in (w4.codes, w4.scales, w4.zeros)):
+            raise ValueError("out must not overlap an operand")
     ldw = out.stride(0) if w4.n > 1 else w4.k
     with _dev_guard(out):
         _lib.check(_lib.load().mtl_dequantize_w4(_ptr(w4.codes), _ptr(w4.scales), _ptr(w4.zeros), _ptr(out), ldw, w4.n,
@@ -1435,36 +1437,44 @@ def token_logprobs(logits, tokens, top=0):
     is padding (logprob 0), one past the vocabulary has logprob NaN.  -inf masks a token; a row of nothing else has
     logprob -inf, entropy 0 and no alternatives.  Missing alternatives are -inf and -1; a row with a NaN or +inf is NaN
     (ids -1)."""
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"logits must be [..., V >= 1], got {tuple(logits.shape)}")
-    lead, V = logits.shape[:-1], logits.shape[-1]
+    shape = logits.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"logits must be [..., V >= 1], got {tuple(shape)}")
+    lead, V = shape[:-1], shape[-1]
     if tokens.dtype != torch.int64 or tokens.shape != lead:
         raise ValueError(f"tokens must be int64 {tuple(lead)}, got {tuple(tokens.shape)} {tokens.dtype}")
-    if not 0 <= top <= min(TOP_MAX, V):
+    if not 0 <= top <= TOP_MAX or top > V:
         raise ValueError(f"top must be in [0, {min(TOP_MAX, V)}], got {top}")
-    code = _act_code(logits)
-    _same_device(logits, tokens)
+    code = _ACT_DTYPES.get(logits.dtype)
+    if code is None:
+        raise TypeError(f"logits must be float32 or bfloat16, got {logits.dtype}")
+    if logits.get_device() != tokens.get_device():
+        raise RuntimeError(f"all operands must be on one device, got logits on {logits.device}, tokens on {tokens.device}")
     if torch.is_grad_enabled():
         _no_grad_recorded("token_logprobs", logits)
     x = logits
     if V > 1 and x.stride(-1) != 1:
         x = x.contiguous()
-    if x.dim() > 3:
-        x = x.reshape(-1, *x.shape[-2:])          # (a view where the strides allow it)
-    if x.dim() == 3:
+    dim = len(shape)
+    if dim > 3:
+        x = x.reshape(-1, *shape[-2:])            # (a view where the strides allow it)
+    if dim >= 3:
         (outer, inner, _), (so, si, _) = x.shape, x.stride()
-    elif x.dim() == 2:
-        outer, inner, so, si = 1, x.shape[0], 0, x.stride(0)
+    elif dim == 2:
+        outer, inner, so, si = 1, shape[0], 0, x.stride(0)
     else:
         outer = inner = 1
         so = si = 0
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     lp = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(lp)
     top_token = tokens.new_empty((*lead, top))
-    r = TokenLogprobs(lp, torch.empty_like(lp), torch.empty_like(top_token, dtype=torch.float32), top_token)
-    a = _lib.TokenLogprobsArgs(x.data_ptr(), tokens.data_ptr(), r.logprob.data_ptr(), r.entropy.data_ptr(),
-                               r.top_logprob.data_ptr(), r.top_token.data_ptr(), outer, inner, so, si, V, top, code)
+    top_lp = torch.empty_like(top_token, dtype=torch.float32)
+    a = _lib.TokenLogprobsArgs(x.data_ptr(), tokens.data_ptr(), lp.data_ptr(), entropy.data_ptr(), top_lp.data_ptr(),
+                               top_token.data_ptr(), outer, inner, so, si, V, top, code)
     with _dev_guard(x):
-        _lib.check(_lib.load().mtl_token_logprobs(ctypes.byref(a), _stream(x)), "token_logprobs")
-    return r
+        rc = _lib.load().mtl_token_logprobs(ctypes.byref(a), _stream(x))
+    if rc:
+        _lib.check(rc, "token_logprobs")
+    return TokenLogprobs(lp, entropy, top_lp, top_token)
