@@ -879,7 +879,8 @@ int mtl_decode_step_w4(const mtl_decode_step_batched_args* args, const mtl_decod
  * A row of nothing but -inf has logprob -inf, entropy 0 and no alternatives;
  * one that holds a NaN or +inf has NaN everywhere and ids -1 (a padding
  * token's logprob stays 0).
- * Sums in fp32.  top <= min(64, vocab).  Outputs contiguous.  Deterministic.
+ * Sums in fp32.  Fewer than 2^24 rows, vocab <= 2^30, top <= min(64, vocab).
+ * Outputs contiguous.  Deterministic.
  * ---------------------------------------------------------------------- */
 typedef struct {
     const void* logits;
