@@ -206,6 +206,9 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
         if (waves > 1 && a.top <= 8) return nth_largest(lane < waves * (share + 1) ? s_best[lane] : 0, a.top - 1, lane);
         return ~wave_max64(~s_best[min(lane, waves - 1) * (share + 1) + share]);
     };
+    // The first tiles' floor lets about top x tiles / wavefronts keys by where it has the right rank; the looser one a few
+    // times that, so it is set once more from all tiles before they are placed.
+    const bool again = waves > 1 && a.top > 8;
     if (wave < tiles) load(wave);
     for (int tile = wave; tile < tiles; tile += waves) {
         float v[kChunks][VEC], most[kChunks];
@@ -276,8 +279,10 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
     q = group_join<64>(q);
     if (lane == 0) s_sums[wave] = q;
     if constexpr (TOP) {
-        lds_barrier();                             // (s_best was read)
-        show();
+        if (again) {
+            lds_barrier();                         // (s_best was read)
+            show();
+        }
         if (lane == 0) s_own[wave] = c.floor;
     }
     lds_barrier();
@@ -296,7 +301,7 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
     if constexpr (TOP) {
         // What reaches the highest floor is little more than `top` keys.  They are put side by side in any order; a
         // key's place in the answer is how many are larger.
-        const uint64_t f0 = row_floor(), f1 = wave_max64(s_own[min(lane, waves - 1)]);
+        const uint64_t f0 = again ? row_floor() : 0, f1 = wave_max64(s_own[min(lane, waves - 1)]);
         const uint64_t f = f0 > f1 ? f0 : f1;
         uint64_t* keep = s_key + waves * 128 + 8;
         const uint64_t k0 = lane < a.top ? c.list : 0, k1 = lane < c.waiting ? c.wait[lane] : 0;
