@@ -36,6 +36,7 @@ template <typename S> __device__ __forceinline__ float scale_at(const void* p, i
 }
 
 typedef __bf16 B8h __attribute__((ext_vector_type(8)));
+typedef uint16_t H2 __attribute__((ext_vector_type(2)));
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 16;                 // most wavefronts of a workgroup
@@ -123,25 +124,33 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
             const int u = u0 + n * threads;
             if (u >= M * n8) break;
             const int m = row_of(u, inv), k8 = u - m * n8;
-            float v[8];
+            if constexpr (P == 1) {                // bf16 as it is; its largest magnitude two values at a time
+                H2 most = {0, 0};
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                v[e] = sizeof(T) == 4 ? __uint_as_float(raw[n][e / 4 % kRaw][e % 4])
-                                      : __uint_as_float(raw[n][0][e / 2] << (e % 2 ? 0 : 16) & 0xffff0000u);
-            uint32_t most = 0;
+                for (int q = 0; q < 4; ++q)
+                    most = __builtin_elementwise_max(most, __builtin_bit_cast(H2, raw[n][0][q] & 0x7fff7fffu));
+                if (max(most[0], most[1]) >= (kWide >> 16)) s_wide = 1;
+                s_x[m * pitch + k8] = raw[n][0];
+            } else {
+                float v[8];
+                uint32_t most = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = max(most, abs_bits(v[e]));
-            if (most >= kWide) s_wide = 1;
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                U4 part;
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    part[e / 2] = __builtin_amdgcn_perm(__float_as_uint(v[e + 1]), __float_as_uint(v[e]), 0x07060302);
-                    v[e] -= __uint_as_float(__float_as_uint(v[e]) & 0xffff0000u);
-                    v[e + 1] -= __uint_as_float(__float_as_uint(v[e + 1]) & 0xffff0000u);
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = __uint_as_float(raw[n][e / 4 % kRaw][e % 4]);
+                    most = max(most, abs_bits(v[e]));
                 }
-                s_x[(q * M + m) * pitch + k8] = part;
+                if (most >= kWide) s_wide = 1;
+#pragma unroll
+                for (int q = 0; q < P; ++q) {      // the upper 8 significand bits of what is left, three times
+                    U4 part;
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        part[e / 2] = __builtin_amdgcn_perm(__float_as_uint(v[e + 1]), __float_as_uint(v[e]), 0x07060302);
+                        v[e] -= __uint_as_float(__float_as_uint(v[e]) & 0xffff0000u);
+                        v[e + 1] -= __uint_as_float(__float_as_uint(v[e + 1]) & 0xffff0000u);
+                    }
+                    s_x[(q * M + m) * pitch + k8] = part;
+                }
             }
         }
     };
