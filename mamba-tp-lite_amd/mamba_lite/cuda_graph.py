@@ -27,6 +27,16 @@ def _clone_cache(cache):
                        for l in cache.layers])
 
 
+def _weight_set(model) -> int:
+    """How often the model's weights have been replaced by others (MambaLM.quantize_w4): a graph reads the old ones."""
+    return getattr(model, "weight_set", 0)
+
+
+def _check_weight_set(graphed):
+    if _weight_set(graphed.model) != graphed._weight_set:
+        raise RuntimeError("model weights changed after capture(); capture again before replaying")
+
+
 class GraphedStepper:
     """Captures `model.step(static_ids, cache)` once, then replays it.
 
@@ -79,10 +89,12 @@ class GraphedStepper:
         self._derived_key = key_fn() if key_fn is not None else None
         held_fn = getattr(self.model, "_derived_tensors", None)
         self._held = held_fn() if held_fn is not None else None
+        self._weight_set = _weight_set(self.model)
 
     def replay(self, next_id: torch.Tensor) -> torch.Tensor:
         if self.graph is None:
             raise RuntimeError("call capture() before replay()")
+        _check_weight_set(self)
         if self._derived_key is not None and self.model._derived_key() != self._derived_key:
             # the reference's graph reads the parameters themselves; this one
             # reads copies made at capture, so a weight update needs a new capture
@@ -139,8 +151,11 @@ class GraphedPrefill:
         except RuntimeError as e:
             self.graph = None
             raise CUDAGraphUnsupported(f"graph capture failed: {e}") from e
+        self._weight_set = _weight_set(self.model)
 
     def replay(self, ids: torch.Tensor) -> torch.Tensor:
+        if self.graph is not None:
+            _check_weight_set(self)
         if tuple(ids.shape) != tuple(self.static_ids.shape):
             raise ValueError(f"ids must be {tuple(self.static_ids.shape)}, got {tuple(ids.shape)}")
         self.static_ids.copy_(ids)

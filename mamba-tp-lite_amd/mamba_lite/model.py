@@ -668,19 +668,24 @@ class MambaLM(nn.Module):
                     lm_head: bool = True) -> "MambaLM":
         """Puts every block's in_proj and out_proj, and with lm_head a copy of the tied embedding for the head, into
         4-bit codes (LinearW4), in place; the embedding itself and the small projections stay as they are.  A model
-        at the mamba-1.4b width keeps about a sixth of its fp32 bytes.  Returns self."""
+        at the mamba-1.4b width keeps about a third of its fp32 bytes.  Graphs captured before refuse to replay.  Returns
+        self."""
         for blk in self.layers:
             for name in ("in_proj", "out_proj"):
                 if type(getattr(blk.mixer, name)) is not nn.Linear:
                     raise TypeError(f"quantize_w4: {name} must be a plain nn.Linear, got "
                                     f"{type(getattr(blk.mixer, name)).__name__}")
-        for blk in self.layers:
-            for name in ("in_proj", "out_proj"):
-                setattr(blk.mixer, name, LinearW4.from_linear(getattr(blk.mixer, name), group, zero_points, scale_dtype))
+        # (all of them before any is put in: a weight that cannot be quantized leaves the model as it was)
+        new = [(blk.mixer, name, LinearW4.from_linear(getattr(blk.mixer, name), group, zero_points, scale_dtype))
+               for blk in self.layers for name in ("in_proj", "out_proj")]
         if lm_head:
-            self.head_w4 = LinearW4(ops.quantize_w4(self.embedding.weight, group, zero_points, scale_dtype))
+            new.append((self, "head_w4", LinearW4(ops.quantize_w4(self.embedding.weight, group, zero_points,
+                                                                  scale_dtype))))
+        for owner, name, mod in new:
+            setattr(owner, name, mod)
         for name in _CALL_PLANS:                 # (they hold the replaced weights' addresses)
             self.__dict__.pop(name, None)
+        self.weight_set = getattr(self, "weight_set", 0) + 1
         return self
 
     def lm_head(self, x: torch.Tensor) -> torch.Tensor:

@@ -15,6 +15,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import math
 import typing
 
 import torch
@@ -1457,7 +1458,7 @@ def token_logprobs(logits, tokens, top=0):
         x = x.contiguous()
     dim = len(shape)
     if dim > 3:
-        x = x.reshape(-1, *shape[-2:])            # (a view where the strides allow it)
+        x = x.reshape(math.prod(shape[:-2]), *shape[-2:])      # (a view where the strides allow it)
     if dim >= 3:
         (outer, inner, _), (so, si, _) = x.shape, x.stride()
     elif dim == 2:

@@ -155,6 +155,8 @@ def test_strides_and_shapes(dtype):
     _check(x[0, 0], c[0, 0], 4)
     _check(x.view(2, 3, 5, 703)[:, 1:, ::2], c.view(2, 3, 5)[:, 1:, ::2], 4)
     _check(x[:1, 0].expand(4, 703), c[:4, 0], 4)
+    e = x.view(2, 3, 5, 703)[:, :, :0]
+    assert ops.token_logprobs(e, c.view(2, 3, 5)[:, :, :0], top=2).top_logprob.shape == (2, 3, 0, 2)
     r = ops.token_logprobs(x[:0], c[:0], top=3)
     assert r.logprob.shape == (0, 5) and r.top_token.shape == (0, 5, 3)
 

@@ -286,3 +286,45 @@ def test_what_keeps_the_step_op_by_op():
         got = q.step(ids, fresh())
         want = copy.deepcopy(q).step(ids, fresh())
         assert torch.equal(got, want)
+
+
+def test_a_graph_of_replaced_weights_is_refused():
+    m = _model()
+    cache = MambaCache.allocate(m.cfg, 1, "cuda", torch.float32)
+    step, pre = GraphedStepper(m, cache, 1, "cuda"), GraphedPrefill(m, cache, 1, 8, "cuda")
+    with torch.no_grad():
+        step.capture()
+        pre.capture()
+        held = [m.layers[0].mixer.in_proj.weight]          # (kept alive here: only the refusal is looked at)
+        ids = torch.zeros(1, 8, dtype=torch.long, device="cuda")
+        pre.replay(ids)
+        step.replay(ids[:, :1])
+        m.quantize_w4()
+        for call in (lambda: pre.replay(ids), lambda: step.replay(ids[:, :1])):
+            with pytest.raises(RuntimeError, match="capture again"):
+                call()
+        step.capture()
+        assert held and bool(torch.isfinite(step.replay(ids[:, :1])).all())
+
+
+def test_a_long_batch_of_prompts():
+    """From 16384 tokens on a plain mixer splits its in_proj; a 4-bit one is called whole."""
+    q = _model(64, 1).quantize_w4()
+    ref = _on_matrices(q)
+    ids = torch.randint(0, 1003, (4, 4100), device="cuda")
+    with torch.no_grad():
+        got, want = q._prefill_hidden(ids)[0], ref._prefill_hidden(ids)[0]
+    assert _rel(got, want) < TOL
+
+
+def test_a_mixer_by_itself():
+    q = _model(256, 1).quantize_w4()
+    mx, ref = q.layers[0].mixer, _on_matrices(q).layers[0].mixer
+    x = torch.randn(2, 9, 256, device="cuda")
+    from mamba_lite.model import LayerCache
+    with torch.no_grad():
+        y, cs, hs = mx.prefill(x)
+        yr, csr, hsr = ref.prefill(x)
+        assert _rel(y, yr) < TOL and _rel(hs, hsr) < TOL
+        a, b = LayerCache(cs, hs), LayerCache(csr, hsr)
+        assert _rel(mx.step(x[:, 0], a), ref.step(x[:, 0], b)) < TOL and _rel(a.ssm_state, b.ssm_state) < TOL

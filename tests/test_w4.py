@@ -203,3 +203,27 @@ def test_the_library_refuses_a_step(change, error):
     lib = _lib.load()
     assert lib.mtl_decode_step_w4(*_step_args(**change)) == 1
     assert error in lib.mtl_last_error()
+
+
+def test_struct_layouts_match_the_header():
+    # six pointers, five int64, four int32; six pointers, five int64, two int32; three pointers, two int32
+    assert ctypes.sizeof(_lib.LinearW4Args) == 6 * 8 + 5 * 8 + 4 * 4 and _lib.LinearW4Args.group.offset == 88
+    assert ctypes.sizeof(_lib.TokenLogprobsArgs) == 6 * 8 + 5 * 8 + 2 * 4 and _lib.TokenLogprobsArgs.top.offset == 88
+    assert ctypes.sizeof(_lib.W4Matrix) == 3 * 8 + 2 * 4
+
+
+def test_a_weight_that_cannot_be_quantized_leaves_the_model_alone():
+    from mamba_lite.model import LinearW4, MambaConfig, MambaLM
+    m = MambaLM(MambaConfig(d_model=64, n_layer=2, vocab_size=40))
+    with torch.no_grad():
+        m.layers[1].mixer.out_proj.weight[3, 5] = float("nan")
+    with pytest.raises(ValueError, match="NaN"):
+        m.quantize_w4()
+    assert all(type(getattr(b.mixer, n)) is torch.nn.Linear for b in m.layers for n in ("in_proj", "out_proj"))
+    with torch.no_grad():
+        m.layers[1].mixer.out_proj.weight[3, 5] = 0.0
+    keys = set(m.state_dict())
+    assert all(type(getattr(b.mixer, n)) is LinearW4 for b in m.quantize_w4().layers for n in ("in_proj", "out_proj"))
+    new = set(m.state_dict()) - keys
+    assert new == {f"layers.{i}.mixer.{n}.scales" for i in range(2) for n in ("in_proj", "out_proj")} | \
+        {"head_w4.weight", "head_w4.scales"}
