@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
     };
     // The first tiles' floor lets about top x tiles / wavefronts keys by where it has the right rank; the looser one a few
     // times that, so it is set once more from all tiles before they are placed.
-    const bool again = waves > 1 && a.top > 8;
+    const bool again = waves > 1 && a.top > 8 && tiles > waves;
     if (wave < tiles) load(wave);
     for (int tile = wave; tile < tiles; tile += waves) {
         float v[kChunks][VEC], most[kChunks];

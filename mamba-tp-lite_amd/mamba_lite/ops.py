@@ -1205,7 +1205,15 @@ class W4:
             raise ValueError(f"zeros must be contiguous uint8 {shape}, got {tuple(zeros.shape)} {zeros.dtype}")
         if any(t is not None and t.device != codes.device for t in (scales, zeros)):
             raise ValueError("codes, scales and zeros must be on one device")
-        self.codes, self.scales, self.zeros, self.n, self.k, self.group = codes, scales, zeros, n, k, group
+        # (calls rely on what was checked here: the parts stay as they are)
+        for name, value in zip(self.__slots__, (codes, scales, zeros, n, k, group)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"a W4's {name} is fixed; make another W4")
+
+    def __reduce__(self):                      # copies and pickles go through the checks again
+        return W4, tuple(getattr(self, name) for name in self.__slots__)
 
 
 def _w4_tiles(t, n, k, per_row):
@@ -1346,9 +1354,9 @@ def linear_w4(x, w4, bias=None, out=None):
             raise ValueError("out must not overlap an operand")
         if out.dim() == 2 and M > 1:
             ldy = out.stride(0)
-    if bias is not None or w4.zeros is not None:
-        _same_device(x, bias, w4.zeros)
-    _same_device(x, out)
+        _same_device(x, out)
+    if bias is not None:
+        _same_device(x, bias)
     a = _lib.LinearW4Args(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(w4.zeros), _ptr(bias), out.data_ptr(),
                           ldx, ldy, M, n, k, w4.group, code, _ACT_DTYPES[scales.dtype])
     with _dev_guard(x):

@@ -164,7 +164,9 @@ def test_refusals_on_the_gpu():
         ops.linear_w4(x.requires_grad_(), w4)
     with torch.no_grad():
         ops.linear_w4(x, w4)
-    half = ops.W4(w4.codes, w4.scales, w4.zeros, 20, 200, 64)
-    half.scales = torch.zeros(2000, device="cuda", dtype=torch.bfloat16)[1:1 + w4.scales.numel()].view_as(w4.scales)
+    odd = torch.zeros(2000, device="cuda", dtype=torch.bfloat16)[1:1 + w4.scales.numel()].view_as(w4.scales)
+    half = ops.W4(w4.codes, odd, w4.zeros, 20, 200, 64)
+    with pytest.raises(AttributeError):
+        half.scales = w4.scales
     with pytest.raises(_lib.MTLError, match="aligned"):
         ops.linear_w4(_x(2, 200, torch.float32, 12), half)

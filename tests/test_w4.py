@@ -1,4 +1,5 @@
 """4-bit weights on the host: the layout word by word, the choice of codes, and what the entry points refuse."""
+import copy
 import ctypes
 
 import pytest
@@ -105,6 +106,14 @@ def test_a_made_up_layout_is_refused():
               (w.codes, w.scales, w.zeros, 0, 200, 64), (w.codes, w.scales.half(), None, 20, 200, 64)):
         with pytest.raises(ValueError):
             ops.W4(*a)
+
+
+def test_a_matrix_is_fixed_and_can_be_copied():
+    w = ops.pack_w4(*_random(20, 200, 64, True), group=64)
+    with pytest.raises(AttributeError):
+        w.zeros = None
+    c = copy.deepcopy(w)
+    assert c.codes is not w.codes and torch.equal(c.codes, w.codes) and torch.equal(c.scales, w.scales) and c.n == 20
 
 
 def test_calls_are_refused_on_the_host():
