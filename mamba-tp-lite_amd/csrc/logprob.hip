@@ -142,7 +142,7 @@ template <typename T, bool TOP>
 __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
     constexpr int VEC = 16 / (int)sizeof(T);
     __shared__ Sums s_sums[16];
-    __shared__ uint64_t s_best[TOP ? 80 : 1], s_own[16];
+    __shared__ uint64_t s_best[TOP ? 80 : 1], s_own[16], s_first;
     __shared__ int s_keys;
     extern __shared__ __align__(16) uint64_t s_key[];      // TOP: [waves][128] waiting, then 8 more; the same again
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
     c.wait = s_key + wave * 128;
     // Each wavefront shows the largest keys of share + 1 of its lanes, `top` or more together (at most top + 15): nothing
     // below the top-th largest of them is wanted.  Past 8, finding that one costs more than it saves: the least of the
-    // wavefronts' last ones is not far below (1 row of 50280, 64 alternatives: 16.6 against 19.6 us).
+    // wavefronts' last ones is not far below (1 row of 50280, 64 alternatives: 17.4 against 18.2 us; 5: 11.6, 10.9).
     const int share = TOP ? (a.top - 1) / waves : 0;
     auto show = [&]() __attribute__((always_inline)) {
         uint64_t k = best;
@@ -202,8 +202,7 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
             }
         }
     };
-    auto row_floor = [&]() __attribute__((always_inline)) {
-        if (waves > 1 && a.top <= 8) return nth_largest(lane < waves * (share + 1) ? s_best[lane] : 0, a.top - 1, lane);
+    auto least_shown = [&]() __attribute__((always_inline)) {
         return ~wave_max64(~s_best[min(lane, waves - 1) * (share + 1) + share]);
     };
     // The first tiles' floor lets about top x tiles / wavefronts keys by where it has the right rank; the looser one a few
@@ -230,14 +229,22 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
         // (fmaxf drops a NaN; e^NaN reaches s all the same)
         rescale(q, m);
         const float base = base_of(m);
+        // (a tile's terms by themselves first: one rounding a tile, not one a term, falls on the running sums, which the
+        // row's few large terms have made large)
+        float s[kChunks], t[kChunks];
 #pragma unroll
-        for (int u = 0; u < kChunks; ++u)
+        for (int u = 0; u < kChunks; ++u) {
+            s[u] = t[u] = 0.f;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const float d = v[u][e] - base, ex = fast_exp(d);
-                q.s += ex;
-                q.t = fmaf(fmaxf(d, -1e30f), ex, q.t);
+                s[u] += ex;
+                t[u] = fmaf(fmaxf(d, -1e30f), ex, t[u]);
             }
+        }
+        static_assert(kChunks == 4, "four partial sums");
+        q.s += (s[0] + s[1]) + (s[2] + s[3]);
+        q.t += (t[0] + t[1]) + (t[2] + t[3]);
         if constexpr (TOP) {
             const int i0 = (int)((int64_t)tile * kTile * VEC - off) + lane * VEC;
             float all = most[0];
@@ -251,7 +258,16 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
                 best = key_of(all, i0 + (v[0][0] == all ? 0 : at));
                 show();
                 lds_barrier();
-                c.raise(row_floor());
+                if (waves > 1 && a.top <= 8) {     // one wavefront finds it for all
+                    if (wave == 0) {
+                        const uint64_t f = nth_largest(lane < waves * (share + 1) ? s_best[lane] : 0, a.top - 1, lane);
+                        if (lane == 0) s_first = f;
+                    }
+                    lds_barrier();
+                    c.raise(lane_read64(s_first, 0));
+                } else {
+                    c.raise(least_shown());
+                }
             }
             if (__any(all >= c.floor_value)) {
 #pragma unroll
@@ -301,7 +317,7 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
     if constexpr (TOP) {
         // What reaches the highest floor is little more than `top` keys.  They are put side by side in any order; a
         // key's place in the answer is how many are larger.
-        const uint64_t f0 = again ? row_floor() : 0, f1 = wave_max64(s_own[min(lane, waves - 1)]);
+        const uint64_t f0 = again ? least_shown() : 0, f1 = wave_max64(s_own[min(lane, waves - 1)]);
         const uint64_t f = f0 > f1 ? f0 : f1;
         uint64_t* keep = s_key + waves * 128 + 8;
         const uint64_t k0 = lane < a.top ? c.list : 0, k1 = lane < c.waiting ? c.wait[lane] : 0;

@@ -325,12 +325,14 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
     }
 }
 
-// One wavefront per tile of 16 rows x 128 columns.  Rows of W on 16-byte boundaries (VEC): a lane's 8 columns leave in
-// 16-byte stores as they are.  Others: through LDS, so that a store writes neighbouring columns of one row.
+// One wavefront per tile of 16 rows x 128 columns, through LDS, so that a store writes neighbouring columns of a row or
+// a few whole rows: with rows of W on 16-byte boundaries (VEC) 16 bytes a lane, else a value.  (Lanes that stored their
+// own 8 columns, 64-byte pieces of 16 rows at a time, took 61 us for 24323 x 3784 bf16, 3.8 TB/s.)
 template <typename T, typename S, int G, bool Z, bool VEC>
 __global__ void __launch_bounds__(256) dequantize_w4_kernel(const W4Args a) {
     constexpr int NG = kBlockK / G;
-    __shared__ T s_row[VEC ? 1 : 4][VEC ? 1 : kTileRows][kBlockK + 4];
+    constexpr int kPer = 16 / (int)sizeof(T), kPitch = kBlockK + kPer;       // (rows start in different banks)
+    __shared__ __align__(16) T s_row[4][kTileRows * kPitch];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, j = lane >> 4;
     const int64_t tile = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + wave, t = tile / a.KB;
     const int kb = (int)(tile - t * a.KB);
@@ -341,7 +343,6 @@ __global__ void __launch_bounds__(256) dequantize_w4_kernel(const W4Args a) {
     const Scales<S, NG> sc = static_cast<const Scales<S, NG>*>(a.scales)[b * kTileRows + r];
     Scales<uint8_t, NG> zr;
     if constexpr (Z) zr = reinterpret_cast<const Scales<uint8_t, NG>*>(a.zeros)[b * kTileRows + r];
-    T* out = static_cast<T*>(a.y) + n0 * a.ldy;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float s = sc.at(i / (G / 32));
@@ -349,33 +350,36 @@ __global__ void __launch_bounds__(256) dequantize_w4_kernel(const W4Args a) {
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = s * (float)((int)code_of(w[i], e) - zero);
-        const int k = 32 * i + 8 * j, k0 = kb * kBlockK + k;
-        if constexpr (!VEC) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) Act<T>::store(&s_row[wave][r][k + e], v[e]);
-        } else if (n0 + r < a.N) {
-            T* to = out + r * a.ldy + k0;
-            if (k0 + 8 <= a.K) {
-                if constexpr (sizeof(T) == 4) {
-                    st4(to, F4v{v[0], v[1], v[2], v[3]});
-                    st4(to + 4, F4v{v[4], v[5], v[6], v[7]});
-                } else {
-                    *reinterpret_cast<U4*>(to) = U4{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]),
-                                                    f32x2_to_bf16x2(v[4], v[5]), f32x2_to_bf16x2(v[6], v[7])};
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (k0 + e < a.K) Act<T>::store(to + e, v[e]);
-            }
+        T* to = &s_row[wave][r * kPitch + 32 * i + 8 * j];
+        if constexpr (sizeof(T) == 4) {
+            st4(to, F4v{v[0], v[1], v[2], v[3]});
+            st4(to + 4, F4v{v[4], v[5], v[6], v[7]});
+        } else {
+            *reinterpret_cast<U4*>(to) = U4{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]),
+                                            f32x2_to_bf16x2(v[4], v[5]), f32x2_to_bf16x2(v[6], v[7])};
         }
     }
-    if constexpr (!VEC) {
-        __builtin_amdgcn_wave_barrier();           // (a wavefront reads what it wrote: LDS is in order within it)
+    __builtin_amdgcn_wave_barrier();               // (a wavefront reads what it wrote: LDS is in order within it)
+    T* out = static_cast<T*>(a.y) + n0 * a.ldy + kb * kBlockK;
+    const int rows = (int)min((int64_t)kTileRows, a.N - n0), cols = min(kBlockK, a.K - kb * kBlockK);
+    if constexpr (VEC) {
+        constexpr int kRuns = kBlockK / kPer;      // 16-byte runs of a row
+#pragma unroll
+        for (int o = lane; o < kTileRows * kRuns; o += 64) {
+            const int row = o / kRuns, k = o % kRuns * kPer;
+            const T* from = &s_row[wave][row * kPitch + k];
+            if (row >= rows) continue;
+            if (k + kPer <= cols) {
+                *reinterpret_cast<U4*>(out + row * a.ldy + k) = *reinterpret_cast<const U4*>(from);
+            } else {
+                for (int e = k; e < cols; ++e) out[row * a.ldy + e] = from[e - k];
+            }
+        }
+    } else {
 #pragma unroll 4
         for (int o = lane; o < kTileRows * kBlockK; o += 64) {
             const int row = o / kBlockK, k = o % kBlockK;
-            if (n0 + row < a.N && kb * kBlockK + k < a.K) out[row * a.ldy + kb * kBlockK + k] = s_row[wave][row][k];
+            if (row < rows && k < cols) out[row * a.ldy + k] = s_row[wave][row * kPitch + k];
         }
     }
 }
