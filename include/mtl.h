@@ -798,8 +798,8 @@ int mtl_decode_step_persist(const mtl_decode_step_args* args, const mtl_decode_l
 /* ------------------------------------------------------------------------
  * Weights in 4-bit codes with group scales: w[n, k] = (code[n, k] -
  * zeros[n, k / group]) scales[n, k / group], codes and zeros in 0..15 (8 where
- * zeros is NULL), group 32, 64 or 128.  No counterpart in the reference,
- * whose projections are nn.Linear (model.py:151-170).
+ * zeros is NULL), scales finite, group 32, 64 or 128.  No counterpart in the
+ * reference, whose projections are nn.Linear (model.py:151-170).
  *
  * Layout, with NT = ceil(N / 16) and KB = ceil(K / 128):
  *   codes   [NT, KB, 64, 16] bytes.  Of rows 16 t .. and columns 128 kb ..,

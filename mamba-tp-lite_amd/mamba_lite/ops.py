@@ -1226,8 +1226,8 @@ def _w4_tiles(t, n, k, per_row):
 
 def pack_w4(codes, scales, zeros=None, group=64):
     """Lays out a 4-bit matrix once: codes [n, k] uint8 in 0..15, scales [n, ceil(k / group)] float32 or bfloat16, zeros
-    the same shape, uint8 in 0..15 (None: 8 everywhere).  Works on any device; one that holds values past 15 raises
-    (which waits for the device)."""
+    the same shape, uint8 in 0..15 (None: 8 everywhere).  Works on any device; codes or zeros past 15 and scales that are
+    not finite raise (which waits for the device)."""
     if codes.dim() != 2 or codes.dtype != torch.uint8:
         raise ValueError(f"codes must be uint8 [n, k], got {tuple(codes.shape)} {codes.dtype}")
     if group not in W4_GROUPS:
@@ -1245,6 +1245,8 @@ def pack_w4(codes, scales, zeros=None, group=64):
     if any(t is not None and int(t.max()) > 15 for t in (codes, zeros)):
         raise ValueError("codes and zeros must be in 0..15")
     scales = scales.detach()
+    if not bool(torch.isfinite(scales).all()):
+        raise ValueError("scales hold infinities or NaN")     # (an infinite scale of a zero difference is no number)
     c = _w4_tiles(codes, n, k, _W4_BLOCK)                                   # [nt, kb, 16 r, 128]
     c = c.view(*c.shape[:3], 4, 4, 8).permute(0, 1, 4, 2, 3, 5)             # [nt, kb, 4 j, 16 r, 4 i, 8 e]
     # nibbles of a word, low to high: codes 0 2 4 6 1 3 5 7

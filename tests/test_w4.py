@@ -86,6 +86,19 @@ def test_pack_refuses(change, error):
         ops.pack_w4(**a)
 
 
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_pack_refuses_scales_that_are_not_finite(bad, dtype):
+    scales = torch.ones(4, 2, dtype=dtype)
+    scales[3, 1] = bad
+    with pytest.raises(ValueError, match="infinities or NaN"):
+        ops.pack_w4(torch.zeros(4, 128, dtype=torch.uint8), scales)
+    # a finite matrix whose float32 form is not
+    if dtype == torch.float32 and bad > 0:
+        with pytest.raises(ValueError, match="infinities or NaN"):
+            ops.quantize_w4(torch.full((2, 64), 1e300, dtype=torch.float64))
+
+
 def test_quantize_refuses():
     for bad in (torch.zeros(3), torch.zeros(3, 4, dtype=torch.int32), torch.zeros(0, 4),
                 torch.tensor([[1.0, float("inf")]]), torch.tensor([[float("nan"), 1.0]])):
