@@ -173,6 +173,13 @@ __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x
 // every store on its way.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// A wavefront's own: what one lane wrote to LDS before it, another reads after it (LDS is in order within a wavefront,
+// so it holds the compiler's order only and costs no wait).
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Fixed-count register blocking: kernels that hold RUNS values per lane are
 // instantiated for these counts; a size needing `need` runs uses the
 // smallest instantiated count >= need (the extra runs are masked).

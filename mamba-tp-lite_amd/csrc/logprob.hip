@@ -117,7 +117,7 @@ struct Candidates {
         if (hit) wait[waiting + __builtin_popcountll(mask & ((uint64_t(1) << lane) - 1))] = key;
         waiting += __builtin_popcountll(mask);
         if (waiting < 64) return;
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_fence();
         uint64_t k = wait[lane];
         bitonic_sort(k, lane);
         // the larger of each and the reversed other list are the 64 largest, in bitonic order
@@ -126,7 +126,7 @@ struct Candidates {
         bitonic_steps<64, 32>(list, lane);
         k = wait[64 + lane];
         waiting -= 64;
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_fence();
         if (lane < waiting) wait[lane] = k;
         raise(lane_read64(list, top - 1));
     }

@@ -310,9 +310,9 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
             }
         };
         if (p.wk == 1) {                                     // a wavefront's own sums: no other waits for it
-            __builtin_amdgcn_wave_barrier();
+            wave_lds_fence();
             for (int m = j; m < M; m += 4) store(t, wave, m);
-            __builtin_amdgcn_wave_barrier();
+            wave_lds_fence();
         } else {
             lds_barrier();
             const int step = threads / (spread ? 64 : 16);
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(256) dequantize_w4_kernel(const W4Args a) {
                                             f32x2_to_bf16x2(v[4], v[5]), f32x2_to_bf16x2(v[6], v[7])};
         }
     }
-    __builtin_amdgcn_wave_barrier();               // (a wavefront reads what it wrote: LDS is in order within it)
+    wave_lds_fence();
     T* out = static_cast<T*>(a.y) + n0 * a.ldy + kb * kBlockK;
     const int rows = (int)min((int64_t)kTileRows, a.N - n0), cols = min(kBlockK, a.K - kb * kBlockK);
     if constexpr (VEC) {
