@@ -21,6 +21,8 @@ struct LpArgs {
     int64_t* top_token;
     int64_t inner, so, si;     // row i: x + (i / inner) so + (i % inner) si
     int V, top;
+    // how a row's floor is found, see launch()
+    int shown, run_log2, share, again;
 };
 
 struct Sums {
@@ -86,14 +88,25 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
     const uint32_t hi = group_umax<64>(uint32_t(v >> 32));
     return uint64_t(hi) << 32 | group_umax<64>(uint32_t(v >> 32) == hi ? uint32_t(v) : 0u);
 }
-// the n-th largest of the lanes' keys (0: the largest); nonzero keys differ
-__device__ __forceinline__ uint64_t nth_largest(uint64_t key, int n, int lane) {
-    if (n >= 8) {
-        bitonic_sort(key, lane);
-        return lane_read64(key, n);
+__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+// place[o] += how many of this wavefront's share of n keys in LDS are larger than keys[o], for every o; zeros follow the
+// keys (kPad of them)
+constexpr int kPad = 8;
+__device__ __forceinline__ void add_places(const uint64_t* keys, int n, int* place, int wave, int waves, int lane) {
+    typedef uint64_t Pair __attribute__((ext_vector_type(2)));
+    for (int o = lane; o < n; o += 64) {
+        const uint64_t k = keys[o];
+        int larger = 0;
+        for (int i = wave * kPad; i < n; i += waves * kPad) {
+            Pair other[kPad / 2];
+#pragma unroll
+            for (int e = 0; e < kPad / 2; ++e) other[e] = *reinterpret_cast<const Pair*>(keys + i + 2 * e);
+#pragma unroll
+            for (int e = 0; e < kPad; ++e) larger += other[e / 2][e % 2] > k;
+        }
+        if (larger) atomicAdd(&place[o], larger);
     }
-    for (; n > 0; --n) key = key == wave_max64(key) ? 0 : key;
-    return wave_max64(key);
 }
 
 // Candidates of one wavefront for the row's `top` largest keys: those that reach the floor, a key that `top` keys of
@@ -101,6 +114,7 @@ __device__ __forceinline__ uint64_t nth_largest(uint64_t key, int n, int lane) {
 // lane, whose last wanted key is a floor too.
 struct Candidates {
     uint64_t* wait;                    // [128]
+    uint64_t* shared;                  // the highest floor a flush of any wavefront has found
     uint64_t list = 0, floor = 1;
     float floor_value = -FLT_MAX;      // (above -inf, which never enters)
     int waiting = 0;
@@ -111,24 +125,32 @@ struct Candidates {
             floor_value = key_value(f);
         }
     }
+    __device__ __forceinline__ void see() {
+        raise(lane_read64(__hip_atomic_load(shared, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP), 0));
+    }
     __device__ __forceinline__ void add(uint64_t key, int lane, int top) {
         const bool hit = key >= floor;
         const uint64_t mask = __ballot(hit);
         if (hit) wait[waiting + __builtin_popcountll(mask & ((uint64_t(1) << lane) - 1))] = key;
         waiting += __builtin_popcountll(mask);
-        if (waiting < 64) return;
+        if (waiting >= 64) flush(lane, top);
+    }
+    __device__ __forceinline__ void flush(int lane, int top) {
         wave_lds_fence();
-        uint64_t k = wait[lane];
+        uint64_t k = lane < waiting ? wait[lane] : 0;
         bitonic_sort(k, lane);
         // the larger of each and the reversed other list are the 64 largest, in bitonic order
         k = uint64_t(uint32_t(__shfl(int(k >> 32), 63 - lane))) << 32 | uint32_t(__shfl(int(k), 63 - lane));
         list = k > list ? k : list;
         bitonic_steps<64, 32>(list, lane);
         k = wait[64 + lane];
-        waiting -= 64;
+        waiting = max(waiting - 64, 0);
         wave_lds_fence();
         if (lane < waiting) wait[lane] = k;
-        raise(lane_read64(list, top - 1));
+        const uint64_t f = lane_read64(list, top - 1);
+        raise(f);
+        if (lane == 0) __hip_atomic_fetch_max(shared, f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        see();
     }
 };
 
@@ -136,18 +158,22 @@ struct Candidates {
 // one is summed.  A tile costs about ten instructions a logit; candidates for the list are looked for only where
 // some lane's largest reaches the list's last value, which after the first tiles is rare.
 constexpr int kChunks = 4, kTile = 64 * kChunks;
+constexpr int kShown = 256;            // 16 of each of 16 wavefronts
+constexpr int kKeptBytes = 2 * sizeof(uint64_t) + sizeof(int);
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
     constexpr int VEC = 16 / (int)sizeof(T);
     __shared__ Sums s_sums[16];
-    __shared__ uint64_t s_best[TOP ? 80 : 1], s_own[16], s_first;
-    __shared__ int s_keys;
-    extern __shared__ __align__(16) uint64_t s_key[];      // TOP: [waves][128] waiting, then 8 more; the same again
+    __shared__ __align__(16) uint64_t s_shown[TOP ? kShown + kPad : 1], s_least[16], s_again[16];
+    __shared__ int s_keys, s_shown_place[TOP ? kShown : 1];
+    __shared__ uint64_t s_floor;
+    extern __shared__ __align__(16) uint64_t s_key[];      // TOP: [waves][128] waiting, [waves][128] kept, their places
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int64_t row = blockIdx.x;
-    const T* x = static_cast<const T*>(a.x) + (row / a.inner) * a.so + (row % a.inner) * a.si;
+    const uint32_t outer = blockIdx.x / (uint32_t)a.inner;     // (fewer than 2^24 rows)
+    const T* x = static_cast<const T*>(a.x) + outer * a.so + (blockIdx.x - outer * (uint32_t)a.inner) * a.si;
     // chunk c holds logits c VEC - off .. + VEC - 1: chunks lie on 16-byte boundaries wherever the row starts
     const int off = int(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
     const int tiles = (int)(((int64_t)a.V + off + kTile * VEC - 1) / (kTile * VEC));
@@ -174,41 +200,30 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
         }
     };
 
+    if (wave < tiles) load(wave);
+    __builtin_amdgcn_sched_barrier(0);
     int64_t token = 0;
     float given = 0.f;                              // the token's logit
     if (threadIdx.x == 0) {
         s_keys = 0;
+        s_floor = 0;
         token = a.tokens[row];
         if (token >= 0 && token < a.V) given = Act<T>::load(x + token);
     }
     Sums q = {-INFINITY, 0.f, 0.f};
     Candidates c;
-    uint64_t best = 0;                              // a lane's largest key, where it has reached the floor
     c.wait = s_key + wave * 128;
-    // Each wavefront shows the largest keys of share + 1 of its lanes, `top` or more together (at most top + 15): nothing
-    // below the top-th largest of them is wanted.  Past 8, finding that one costs more than it saves: the least of the
-    // wavefronts' last ones is not far below (1 row of 50280, 64 alternatives: 17.4 against 18.2 us; 5: 11.6, 10.9).
-    const int share = TOP ? (a.top - 1) / waves : 0;
-    auto show = [&]() __attribute__((always_inline)) {
-        uint64_t k = best;
-        if (share >= 8) {
-            bitonic_sort(k, lane);
-            if (lane <= share) s_best[wave * (share + 1) + lane] = k;
-        } else {
-            for (int n = 0; n <= share; ++n) {
-                const uint64_t most = wave_max64(k);
-                if (lane == 0) s_best[wave * (share + 1) + n] = most;
-                k = k == most ? 0 : k;
-            }
-        }
-    };
-    auto least_shown = [&]() __attribute__((always_inline)) {
-        return ~wave_max64(~s_best[min(lane, waves - 1) * (share + 1) + share]);
-    };
-    // The first tiles' floor lets about top x tiles / wavefronts keys by where it has the right rank; the looser one a few
-    // times that, so it is set once more from all tiles before they are placed.
-    const bool again = waves > 1 && a.top > 8 && tiles > waves;
-    if (wave < tiles) load(wave);
+    c.shared = &s_floor;
+    uint64_t* keep = s_key + waves * 128;
+    int* place = reinterpret_cast<int*>(keep + waves * 128 + kPad);
+    if constexpr (TOP) {
+        typedef uint64_t Pair __attribute__((ext_vector_type(2)));
+        reinterpret_cast<Pair*>(keep)[threadIdx.x] = Pair{0, 0};
+        reinterpret_cast<uint64_t*>(place)[threadIdx.x] = 0;
+        if (threadIdx.x < a.shown) s_shown_place[threadIdx.x] = 0;
+        if (threadIdx.x < kPad) keep[waves * 128 + threadIdx.x] = s_shown[a.shown + threadIdx.x] = 0;
+    }
+    auto least = [&](const uint64_t* of) __attribute__((always_inline)) { return ~wave_max64(~of[min(lane, waves - 1)]); };
     for (int tile = wave; tile < tiles; tile += waves) {
         float v[kChunks][VEC], most[kChunks];
 #pragma unroll
@@ -255,18 +270,30 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
                 int at = 0;                        // the lowest index of the lane's largest
 #pragma unroll
                 for (int n = kChunks * VEC - 1; n > 0; --n) at = v[n / VEC][n % VEC] == all ? n / VEC * 64 * VEC + n % VEC : at;
-                best = key_of(all, i0 + (v[0][0] == all ? 0 : at));
-                show();
-                lds_barrier();
-                if (waves > 1 && a.top <= 8) {     // one wavefront finds it for all
-                    if (wave == 0) {
-                        const uint64_t f = nth_largest(lane < waves * (share + 1) ? s_best[lane] : 0, a.top - 1, lane);
-                        if (lane == 0) s_first = f;
-                    }
+                uint64_t k = key_of(all, i0 + (v[0][0] == all ? 0 : at));
+                if (a.share >= 0) {
+                    bitonic_sort(k, lane);
+                    if (lane == a.share) s_least[wave] = k;
                     lds_barrier();
-                    c.raise(lane_read64(s_first, 0));
+                    c.raise(least(s_least));
                 } else {
-                    c.raise(least_shown());
+                    if (a.run_log2 == 6) {
+                        k = wave_max64(k);
+                    } else {
+                        k = max64(k, dpp_mov64<kDppXor1>(k));
+                        k = max64(k, dpp_mov64<kDppXor2>(k));
+                        if (a.run_log2 > 2) k = max64(k, dpp_mov64<kDppHalfMirror>(k));
+                        if (a.run_log2 > 3) k = max64(k, dpp_mov64<kDppRowMirror>(k));
+                    }
+                    if ((lane & ((1 << a.run_log2) - 1)) == 0) s_shown[(wave * 64 + lane) >> a.run_log2] = k;
+                    lds_barrier();
+                    add_places(s_shown, a.shown, s_shown_place, wave, waves, lane);
+                    lds_barrier();
+                    for (int o0 = 0; o0 < a.shown; o0 += 64) {
+                        const int o = min(o0 + lane, a.shown - 1);
+                        const uint64_t mask = __ballot(s_shown_place[o] == a.top - 1);
+                        if (mask) c.raise(lane_read64(s_shown[o], __builtin_ctzll(mask)));
+                    }
                 }
             }
             if (__any(all >= c.floor_value)) {
@@ -283,7 +310,6 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
 #pragma unroll
                         for (int n = 1; n < VEC; ++n) value = e == n ? v[u][n] : value;
                         const uint64_t k = which ? key_of(value, i0 + u * 64 * VEC + e) : 0;
-                        best = k > best ? k : best;
                         c.add(k, lane, a.top);
                         which &= which - 1;
                     }
@@ -295,11 +321,24 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
     q = group_join<64>(q);
     if (lane == 0) s_sums[wave] = q;
     if constexpr (TOP) {
-        if (again) {
-            lds_barrier();                         // (s_best was read)
-            show();
+        // What reaches the floor is little more than `top` keys.  They are put side by side in any order; a key's place in
+        // the answer is how many are larger.
+        if (a.again >= 0) {
+            if (c.waiting) c.flush(lane, a.top);
+            if (lane == a.again) s_again[wave] = c.list;
+            lds_barrier();
+            c.raise(least(s_again));
         }
-        if (lane == 0) s_own[wave] = c.floor;
+        c.see();
+        const uint64_t k0 = lane < a.top ? c.list : 0, k1 = lane < c.waiting ? c.wait[lane] : 0;
+        const uint64_t mask0 = __ballot(k0 >= c.floor), mask1 = __ballot(k1 >= c.floor);
+        const int n0 = __builtin_popcountll(mask0), n1 = __builtin_popcountll(mask1);
+        int first = 0;
+        if (lane == 0 && n0 + n1) first = atomicAdd(&s_keys, n0 + n1);
+        first = __builtin_amdgcn_readfirstlane(first);
+        const uint64_t below = (uint64_t(1) << lane) - 1;
+        if (mask0 >> lane & 1) keep[first + __builtin_popcountll(mask0 & below)] = k0;
+        if (mask1 >> lane & 1) keep[first + n0 + __builtin_popcountll(mask1 & below)] = k1;
     }
     lds_barrier();
     q = (lane & 15) < waves ? s_sums[lane & 15] : Sums{-INFINITY, 0.f, 0.f};
@@ -315,35 +354,15 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
         a.entropy[row] = bad ? NAN : empty ? 0.f : ls - q.t / q.s;
     }
     if constexpr (TOP) {
-        // What reaches the highest floor is little more than `top` keys.  They are put side by side in any order; a
-        // key's place in the answer is how many are larger.
-        const uint64_t f0 = again ? least_shown() : 0, f1 = wave_max64(s_own[min(lane, waves - 1)]);
-        const uint64_t f = f0 > f1 ? f0 : f1;
-        uint64_t* keep = s_key + waves * 128 + 8;
-        const uint64_t k0 = lane < a.top ? c.list : 0, k1 = lane < c.waiting ? c.wait[lane] : 0;
-        const uint64_t mask0 = __ballot(k0 >= f && !bad), mask1 = __ballot(k1 >= f && !bad);
-        const int n0 = __builtin_popcountll(mask0), n1 = __builtin_popcountll(mask1);
-        int first = 0;
-        if (lane == 0 && n0 + n1) first = atomicAdd(&s_keys, n0 + n1);
-        first = __builtin_amdgcn_readfirstlane(first);
-        const uint64_t below = (uint64_t(1) << lane) - 1;
-        if (mask0 >> lane & 1) keep[first + __builtin_popcountll(mask0 & below)] = k0;
-        if (mask1 >> lane & 1) keep[first + n0 + __builtin_popcountll(mask1 & below)] = k1;
+        const int keys = bad ? 0 : s_keys;
+        add_places(keep, keys, place, wave, waves, lane);
         lds_barrier();
-        const int keys = s_keys;
         for (int o = threadIdx.x; o < keys; o += blockDim.x) {
-            const uint64_t k = keep[o];
-            int place = 0;
-            for (int i = 0; i < keys; i += 8) {
-                uint64_t other[8];
-#pragma unroll
-                for (int n = 0; n < 8; ++n) other[n] = keep[i + n];
-#pragma unroll
-                for (int n = 0; n < 8; ++n) place += i + n < keys && other[n] > k;
-            }
-            if (place < a.top) {
-                a.top_token[row * a.top + place] = (int64_t)(uint32_t)~uint32_t(k);
-                a.top_logprob[row * a.top + place] = (key_value(k) - q.m) - ls;
+            const int at = place[o];
+            if ((uint32_t)at < (uint32_t)a.top) {
+                const uint64_t k = keep[o];
+                a.top_token[row * a.top + at] = (int64_t)(uint32_t)~uint32_t(k);
+                a.top_logprob[row * a.top + at] = (key_value(k) - q.m) - ls;
             }
         }
         if (wave == 0 && lane >= keys && lane < a.top) {         // fewer than `top` tokens are left
@@ -354,13 +373,30 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
 }
 
 template <typename T>
-int launch(const LpArgs& a, int64_t rows, hipStream_t st) {
+int launch(LpArgs a, int64_t rows, hipStream_t st) {
     const int64_t tiles = (a.V + kTile * (16 / (int)sizeof(T)) - 1) / (kTile * (16 / (int)sizeof(T)));
     // Few rows: many wavefronts each; no more than share the tiles evenly, and every one has a first tile (the kernel's
     // barrier after it counts on that).  1022 rows of 50280 bf16 with 5 alternatives: 4 wavefronts 33.7 us, 8 36.3, 16 55.
     const int64_t most = std::clamp<int64_t>(4096 / rows, 4, 16), turns = (tiles + most - 1) / most;
     const int waves = (int)((tiles + turns - 1) / turns);
-    if (a.top) hipLaunchKernelGGL((logprob_kernel<T, true>), dim3((unsigned)rows), dim3(waves * 64), 2 * (waves * 128 + 8) * sizeof(uint64_t), st, a);
+    // The floor from the first tiles: each wavefront shows the largest key of every run of lanes, the longest runs (64, 16, 8
+    // or 4 lanes) that make 2 top of them, and the top-th largest of those is the floor.  Where runs of 4 are too few, the
+    // wavefronts sort their lanes' and the least of their (top / wavefronts)-th is not far below.  Then about
+    // top x tiles / wavefronts keys reach it, and where counting all of those would take longer than a sort in each wavefront,
+    // a second floor comes from the wavefronts' sorted lists.  Measured, us, against floors from the least of the wavefronts'
+    // last shown throughout: 32 rows of 50280 with 20 alternatives 12.3, 15.7; 256 of 6285 with 20 6.9, 14.2; 37 of 10007
+    // with 64 8.6, 11.7; 1 of 50280 with 5 10.0, 10.7; and 300 of 2100 with 64, where they still sort, 20.5, 22.7.
+    const int share = (a.top - 1) / waves;
+    a.run_log2 = 6;
+    while (waves << (6 - a.run_log2) < 2 * a.top && a.run_log2 > 2) a.run_log2 -= a.run_log2 == 6 ? 2 : 1;
+    a.shown = waves << (6 - a.run_log2);
+    a.share = a.shown < 2 * a.top ? share : -1;
+    const int64_t keys = a.top * tiles / waves;
+    a.again = waves > 1 && tiles > waves && keys * keys > 1024 * waves ? share : -1;
+    if (a.top) {
+        const size_t lds = waves * 128 * kKeptBytes + kPad * sizeof(uint64_t);
+        hipLaunchKernelGGL((logprob_kernel<T, true>), dim3((unsigned)rows), dim3(waves * 64), lds, st, a);
+    }
     else hipLaunchKernelGGL((logprob_kernel<T, false>), dim3((unsigned)rows), dim3(waves * 64), 0, st, a);
     return check_launch("token_logprobs");
 }
@@ -382,7 +418,7 @@ extern "C" int mtl_token_logprobs(const mtl_token_logprobs_args* p, mtl_stream_t
     MTL_REQUIRE(p->logits && p->tokens && p->logprob && p->entropy && (p->top == 0 || (p->top_logprob && p->top_token)),
                 "null pointer");
     const LpArgs a{p->logits, p->tokens, p->logprob, p->entropy, p->top_logprob, p->top_token, p->inner, p->stride_outer,
-                   p->stride_inner, (int)p->vocab, p->top};
+                   p->stride_inner, (int)p->vocab, p->top, 0, 0, -1, -1};
     return p->dtype == MTL_F32 ? launch<float>(a, p->outer * p->inner, as_stream(stream))
                                : launch<uint16_t>(a, p->outer * p->inner, as_stream(stream));
 }

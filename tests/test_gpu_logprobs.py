@@ -90,6 +90,25 @@ def test_sorted_rows(rows, dtype):
         _check(x, torch.arange(rows, device="cuda") % v, 33)
 
 
+# one wavefront and several, with one tile each and more, few alternatives a wavefront and many
+@DTYPES
+@pytest.mark.parametrize("rows,v,top", [(1, 64, 8), (1, 1000, 64), (2, 2049, 33), (3, 9000, 64), (40, 5000, 20), (2, 20011, 64),
+                                        (300, 2100, 64), (1100, 20011, 20), (1100, 9000, 64), (1, 131075, 9)])
+def test_the_order_of_alternatives(rows, v, top, dtype):
+    torch.manual_seed(rows + v)
+    x = torch.randn(rows, v, device="cuda") * 3
+    lowest = torch.finfo(dtype).min
+    some = torch.rand(rows, v, device="cuda")
+    for kind in (x, x.sort(-1)[0], x.sort(-1, descending=True)[0], x.round(), torch.full_like(x, 1.5),
+                 torch.where(some < 0.95, lowest, x), torch.where(some < 0.95, -INF, x)):
+        kind = kind.to(dtype)
+        got = ops.token_logprobs(kind, torch.zeros(rows, dtype=torch.int64, device="cuda"), top=top)
+        value, order = torch.sort(kind.float(), dim=-1, descending=True, stable=True)
+        value, order = value[:, :top], order[:, :top]
+        assert torch.equal(got.top_token, torch.where(value == -INF, -1, order))
+        assert bool((got.top_logprob[:, 1:] <= got.top_logprob[:, :-1]).all())
+
+
 @DTYPES
 @pytest.mark.parametrize("rows,v", [(1, 7), (1, 50280), (9, 3001), (4200, 300)])
 def test_masks(rows, v, dtype):
