@@ -49,7 +49,6 @@ struct LinearW4 {
     int rows;                  // rows of x per workgroup (blockIdx.y takes the next ones)
     int kblocks;               // 128-column blocks of x in LDS at a time
     int wk, wk_log2;           // wavefronts that share a tile of W, each on every wk-th block
-    int xvec;                  // rows of x start on 16-byte boundaries
 };
 
 template <typename S, int NG> struct alignas(sizeof(S) * NG) Scales {        // one row's scales of a block
@@ -92,37 +91,29 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
 
     // u / n8 for the fewer than 2^19 runs of x and at most 48 rows: the product is off by less than half of 1 / n8
     auto row_of = [&](int u, float inv) __attribute__((always_inline)) { return (int)((u + 0.5f) * inv); };
-    // x to LDS: a thread takes 8 columns of a row at a time, kUnits of them in flight
-    constexpr int kRaw = 8 * (int)sizeof(T) / 16, kUnits = 4 / kRaw;
+    // x to LDS: a thread takes 8 columns of a row at a time, kUnits of them in flight (8 of bf16 spill beside two operand
+    // tiles).  Whole runs at any alignment: rows of 777 bf16 taken value by value where they start off a 16-byte boundary
+    // cost 1.3 of 6.4 us at 33 rows for 1001 rows of W.
+    constexpr int kRaw = 8 * (int)sizeof(T) / 16, kUnits = P > 1 ? 2 : TM == 1 ? 8 : 4;
     U4 raw[kUnits][kRaw];
     auto fetch = [&](int kb0, int nb, int u0) __attribute__((always_inline)) {
-        const int n8 = nb * 16;
+        const int n8 = nb * 16, runs = a.K < 8 ? 0 : M * n8;
         const float inv = 1.f / n8;
 #pragma unroll
         for (int n = 0; n < kUnits; ++n) {
-            if (__builtin_amdgcn_readfirstlane(u0) + n * threads >= M * n8) break;
-            const int u = min(u0 + n * threads, M * n8 - 1), m = row_of(u, inv), k = kb0 * kBlockK + (u - m * n8) * 8;
-            const T* src = x + m * a.ldx + k;
-            if (p.xvec && k + 8 <= a.K) {
-#pragma unroll
-                for (int q = 0; q < kRaw; ++q) raw[n][q] = reinterpret_cast<const U4*>(src)[q];
-            } else {
-                T v[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = src[min(e, a.K - 1 - k)];      // past the row: its last value again
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = k + e < a.K ? v[e] : T(0);
-                __builtin_memcpy(raw[n], v, sizeof(v));
-            }
+            if (__builtin_amdgcn_readfirstlane(u0) + n * threads >= runs) break;
+            const int u = min(u0 + n * threads, runs - 1), m = row_of(u, inv), k = kb0 * kBlockK + (u - m * n8) * 8;
+            // (the row's last 8 again where fewer are left: put_end shifts them)
+            __builtin_memcpy(raw[n], x + m * a.ldx + min(k, a.K - 8), sizeof(raw[n]));
         }
     };
     auto put = [&](int nb, int u0) __attribute__((always_inline)) {
-        const int n8 = nb * 16;
+        const int n8 = nb * 16, runs = a.K < 8 ? 0 : M * n8;
         const float inv = 1.f / n8;
 #pragma unroll
         for (int n = 0; n < kUnits; ++n) {
             const int u = u0 + n * threads;
-            if (u >= M * n8) break;
+            if (u >= runs) break;
             const int m = row_of(u, inv), k8 = u - m * n8;
             if constexpr (P == 1) {                // bf16 as it is; its largest magnitude two values at a time
                 H2 most = {0, 0};
@@ -151,6 +142,36 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
                     }
                     s_x[(q * M + m) * pitch + k8] = part;
                 }
+            }
+        }
+    };
+
+    // the last block's runs that reach past the row: the row's last 8 values, which are there, shifted down, zeros behind
+    auto put_end = [&](int kb0) __attribute__((always_inline)) {
+        for (int u = threadIdx.x; u < M * 16; u += threads) {
+            const int m = u >> 4, k = (a.KB - 1) * kBlockK + (u & 15) * 8, past = k + 8 - a.K;
+            if (past <= 0) continue;
+            uint16_t* run = reinterpret_cast<uint16_t*>(s_x + m * pitch) + k - kb0 * kBlockK;
+            if (a.K < 8) {                         // (nothing is there)
+#pragma unroll 1
+                for (int e = 0; e < 8; ++e) {
+                    float v = k + e < a.K ? Act<T>::load(x + m * a.ldx + k + e) : 0.f;
+                    if (abs_bits(v) >= kWide) s_wide = 1;
+#pragma unroll
+                    for (int q = 0; q < P; ++q) {
+                        run[q * M * pitch * 8 + e] = __float_as_uint(v) >> 16;
+                        v -= __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+                    }
+                }
+                continue;
+            }
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+                uint16_t v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = run[q * M * pitch * 8 + min(e + past, 7)];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) run[q * M * pitch * 8 + e] = e + past < 8 ? v[e] : 0;
             }
         }
     };
@@ -216,6 +237,8 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
     __builtin_amdgcn_sched_barrier(0);
     if (threadIdx.x == 0) s_wide = 0;
     lds_barrier();
+    put(min(p.kblocks, a.KB), threadIdx.x);                  // (here, not in the loop: its wait then counts W's loads out)
+    int u0 = threadIdx.x + kUnits * threads;                 // the first run of x that is not in LDS yet
     bool staged = false;
     for (int t0 = blockIdx.x * WN; t0 < tiles; t0 += stride, t += stride) {
 #pragma unroll
@@ -227,13 +250,16 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
                 if (staged) {
                     lds_barrier();
                     if (threadIdx.x == 0) s_wide = 0;
-                    fetch(kb0, nb, threadIdx.x);
                     lds_barrier();
+                    u0 = threadIdx.x;
                 }
-                put(nb, threadIdx.x);
-                for (int u = threadIdx.x + kUnits * threads; u < M * nb * 16; u += kUnits * threads) {
-                    fetch(kb0, nb, u);
-                    put(nb, u);
+                for (; u0 < M * nb * 16; u0 += kUnits * threads) {
+                    fetch(kb0, nb, u0);
+                    put(nb, u0);
+                }
+                if (a.K % kBlockK != 0 && kb1 == a.KB) {
+                    lds_barrier();
+                    put_end(kb0);
                 }
                 staged = true;
                 lds_barrier();
@@ -438,15 +464,15 @@ extern "C" int mtl_linear_w4(const mtl_linear_w4_args* p, mtl_stream_t stream) {
     MTL_REQUIRE(reinterpret_cast<uintptr_t>(p->zeros) % 4 == 0, "zeros must be 4-byte aligned");
     const W4Args a{p->x, p->codes, p->scales, p->zeros, p->bias, p->y, p->ldx, p->ldy, (int)p->M, (int)p->N, (int)p->K,
                    (int)((p->K + kBlockK - 1) / kBlockK), p->y_f32 != 0};
-    const int es = dtype == MTL_F32 ? 4 : 2, parts = dtype == MTL_F32 ? 3 : 1;
-    LinearW4 l{a, 0, 0, 1, 0, reinterpret_cast<uintptr_t>(p->x) % 16 == 0 && p->ldx * es % 16 == 0};
+    const int parts = dtype == MTL_F32 ? 3 : 1;
+    LinearW4 l{a, 0, 0, 1, 0};
     const int tiles = (a.N + kTileRows - 1) / kTileRows;
     // Rows of x to a workgroup: one operand tile's (16, of fp32 x 5) while that makes at most 2048 (tile of W, rows of x)
     // pairs, two tiles' where there are more: W is then read half as often.  Wavefronts to a pair: so many that the pairs
     // make about 2048; pairs to a workgroup: so many that it has 8 wavefronts, 16 where its LDS leaves room for one
     // workgroup a CU.  Measured, GPU us (pairs; chosen, its neighbours): 768x1536 1 row bf16 (48) 3.8, 4 / 2 wavefronts
-    // 3.7 / 5.0; 8192x2048 16 rows bf16 (512) 7.2, 8 / 2 9.7 / 8.3; 8192x2048 8 rows fp32 (1024) 6.8, 4 / 1 8.3 / 8.7;
-    // 50280x2048 8 rows fp32 (6286) two tiles 21.4, one 27.7; 2048x4096 64 rows bf16 (512) 10.7, two tiles 22.
+    // 3.7 / 5.0; 8192x2048 16 rows bf16 (512) 6.6, 8 / 2 9.7 / 8.3; 8192x2048 8 rows fp32 (1024) 6.8, 4 / 1 8.3 / 8.7;
+    // 50280x2048 8 rows fp32 (6286) two tiles 21.4, one 27.7; 2048x4096 64 rows bf16 (512) 9.2, two tiles 22.
     const auto chunks_of = [&](int tm) { return (a.M + tm * 16 / parts - 1) / (tm * 16 / parts); };
     int tm = tiles * (int64_t)chunks_of(1) <= 2048 ? 1 : 2;
     const int chunks = chunks_of(tm);

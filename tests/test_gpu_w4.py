@@ -170,3 +170,22 @@ def test_refusals_on_the_gpu():
         half.scales = w4.scales
     with pytest.raises(_lib.MTLError, match="aligned"):
         ops.linear_w4(_x(2, 200, torch.float32, 12), half)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k", [1, 5, 7, 8, 9, 15, 127, 128, 129, 136, 777, 1300, 9001])
+def test_linear_on_rows_at_any_alignment(k, dtype):
+    w4, w = _matrix(40, k, 32, True, torch.float32, k)
+    for m, offset, gap in ((1, 1, 0), (5, 2, 3), (33, 7, 1), (64, 0, 5)):
+        # what lies around the rows is NaN
+        buffer = torch.full((offset + m * (k + gap),), torch.nan, device="cuda", dtype=dtype)
+        x = buffer[offset:].view(m, k + gap)[:, :k]
+        x.copy_(_x(m, k, dtype, k + m))
+        _check(ops.linear_w4(x, w4), x.double() @ w.t().contiguous(), _tol(k, 32, dtype))
+        # an infinity in the row's last column sends that row alone to infinities
+        x[m - 1, k - 1] = torch.inf
+        y = ops.linear_w4(x, w4)
+        ref = x.double()[m - 1] @ w.t().contiguous()
+        assert torch.equal(torch.isnan(y[m - 1]), torch.isnan(ref)) and torch.equal(y[m - 1] == torch.inf, ref == torch.inf)
+        if m > 1:
+            _check(y[:m - 1], x[:m - 1].double() @ w.t().contiguous(), _tol(k, 32, dtype))
