@@ -375,9 +375,11 @@ __global__ void __launch_bounds__(1024) logprob_kernel(const LpArgs a) {
 template <typename T>
 int launch(LpArgs a, int64_t rows, hipStream_t st) {
     const int64_t tiles = (a.V + kTile * (16 / (int)sizeof(T)) - 1) / (kTile * (16 / (int)sizeof(T)));
-    // Few rows: many wavefronts each; no more than share the tiles evenly, and every one has a first tile (the kernel's
-    // barrier after it counts on that).  1022 rows of 50280 bf16 with 5 alternatives: 4 wavefronts 33.7 us, 8 36.3, 16 55.
-    const int64_t most = std::clamp<int64_t>(4096 / rows, 4, 16), turns = (tiles + most - 1) / most;
+    // Few rows: many wavefronts each, past 256 no more than two rows on a CU leave room for; no more than share the tiles
+    // evenly, and every one has a first tile (the kernel's barrier after it counts on that).  Rows of 50280 with 5
+    // alternatives, us: 300 fp32 with 8 wavefronts 17.9, 13 21.7; 513 bf16 with 7 23.6, 5 26.7; 1022 bf16 with 4 31.3,
+    // 8 32.8, 16 44.7.
+    const int64_t most = std::clamp<int64_t>(4096 / rows, 4, rows <= 256 ? 16 : 8), turns = (tiles + most - 1) / most;
     const int waves = (int)((tiles + turns - 1) / turns);
     // The floor from the first tiles: each wavefront shows the largest key of every run of lanes, the longest runs (64, 16, 8
     // or 4 lanes) that make 2 top of them, and the top-th largest of those is the floor.  Where runs of 4 are too few, the
