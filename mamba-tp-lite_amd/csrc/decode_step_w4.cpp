@@ -8,8 +8,8 @@
 //   cores) -> the partials summed in order -> the SSM update in place, y -> out_proj from the codes into floats -> the
 //   residual add and the next RMSNorm.
 // Captured steps at the mamba-1.4b width (48 layers, vocabulary 50280, groups of 128, the head in 4 bits too), against
-// the same model's fp32 or bf16 weights: fp32 1 row 1394 -> 1134 us, 8 rows 1859 -> 1486, 32 rows 2311 -> 2423; bf16
-// 1213 -> 1117, 1443 -> 1447, 1714 -> 1909.  Past a few rows what is left beside the projections bounds it: six
+// the same model's fp32 or bf16 weights: fp32 1 row 1390 -> 1104 us, 8 rows 1858 -> 1492, 32 rows 2304 -> 2420; bf16
+// 1212 -> 1087, 1439 -> 1415, 1713 -> 1814.  Past a few rows what is left beside the projections bounds it: six
 // launches of about 4 us a layer, and matrix work that the wider weights' kernels fuse with the conv step.  Eager 1 row
 // fp32: 3839 op by op, 1278 here.
 #include <hip/hip_runtime.h>
