@@ -23,13 +23,11 @@ DEV = "cuda"
 VOCAB = 50280
 
 
-_PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mamba-tp-lite_amd")
-if _PKG not in sys.path:
-    sys.path.insert(0, _PKG)
-
-
 def _ops():
     """This framework's operators (only where `own` is true)."""
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mamba-tp-lite_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
     from mamba_lite import ops
 
     return ops
