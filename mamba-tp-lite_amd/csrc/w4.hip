@@ -39,6 +39,39 @@ typedef __bf16 B8h __attribute__((ext_vector_type(8)));
 typedef uint16_t H2 __attribute__((ext_vector_type(2)));
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 
+// The weights of a word's 8 codes, in order, as bf16 numbers in units of kUnit: with zeros (z in every byte) q - z through
+// the signed bytes of a register (19 instructions), without them (q - 8) / 16 of the nibbles q ^ 8, two's complements,
+// which one conversion makes (14).
+template <bool Z> constexpr float kUnit = Z ? 1.f : 0.0625f;
+template <bool Z> __device__ __forceinline__ B8h word_weights(uint32_t c, uint32_t zeros) {
+    float f[8];
+    if constexpr (Z) {
+        // q + 128 - z in every byte: no borrow leaves it
+        const uint32_t lo = (((c & 0x0f0f0f0fu) | 0x80808080u) - zeros) ^ 0x80808080u;
+        const uint32_t hi = (((c >> 4 & 0x0f0f0f0fu) | 0x80808080u) - zeros) ^ 0x80808080u;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {              // byte b: codes (b / 2) + 4 (b & 1) and 2 more
+            f[b / 2 + 4 * (b & 1)] = (float)(int8_t)(lo >> (8 * b));
+            f[b / 2 + 4 * (b & 1) + 2] = (float)(int8_t)(hi >> (8 * b));
+        }
+    } else {
+        const uint32_t lo = c ^ 0x88888888u;
+        uint32_t hi = lo >> 4;
+        asm("" : "+v"(hi));                        // (its bytes are operands then, not shifts of lo)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {              // (the conversion reads four bits)
+            f[b / 2 + 4 * (b & 1)] = __builtin_amdgcn_cvt_off_f32_i4(b ? lo >> (8 * b) & 0xffu : lo);
+            f[b / 2 + 4 * (b & 1) + 2] = __builtin_amdgcn_cvt_off_f32_i4(b ? hi >> (8 * b) & 0xffu : hi);
+        }
+    }
+    U4 pairs;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        pairs[i] = __builtin_amdgcn_perm(__float_as_uint(f[2 * i + 1]), __float_as_uint(f[2 * i]), 0x07060302);
+    return __builtin_bit_cast(B8h, pairs);
+}
+
+
 constexpr int kWaves = 16;                 // most wavefronts of a workgroup
 constexpr uint32_t kWide = 0x6f800000u;    // 2^96
 constexpr int kAhead = 4;                  // blocks of W that a wavefront has in flight
@@ -59,18 +92,17 @@ template <typename S, int NG> struct alignas(sizeof(S) * NG) Scales {        // 
     }
 };
 
-// Products on the bf16 matrix cores, exact: a code is the bf16 number 16 + q (its four bits under an exponent), x in
-// float32 the sum of three bf16 numbers of 8 significand bits each, as rows of their own.  A group's sums run in fp32 on
-// v_mfma_f32_16x16x32_bf16, whose second operand is once 16 + q and once -(16 + z), the same for the whole group:
-//   acc += s sum x ((16 + q) - (16 + z))
-// 8 vector instructions unpack the 8 codes of a word; making q - z first, in fp32, would take three times that, and the
-// matrix cores idle meanwhile.
+// Products on the bf16 matrix cores, exact: q - z is a bf16 number, x in float32 the sum of three bf16 numbers of 8
+// significand bits each, as rows of their own.  A group's sums run in fp32 on v_mfma_f32_16x16x32_bf16:
+//   acc += s sum x (q - z)
+// (Products with 16 + q, which the four bits under an exponent give for half the instructions, less x times 16 + z leave
+// the rounding of sums of 31 |x|, on columns of zero weight too.)
 //
 // A workgroup keeps x, as the operand's 16-byte runs, in LDS; each wavefront streams tiles of W into registers, kAhead
 // blocks before their use.  Where there are few tiles, wk wavefronts share one and add their sums in order.
 //
-// |x| >= 2^96, infinities and NaN would spoil the difference: a part of x in which some row holds one takes the products
-// weight by weight instead, as the matrix form would round them.
+// |x| >= 2^96 could overflow before its scale is applied, and infinities and NaN have no three parts: a part of x in which
+// some row holds one takes the products weight by weight instead, as the matrix form would round them.
 template <typename T, typename S, int G, bool Z, int TM>
 __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p) {
     constexpr int NG = kBlockK / G, P = sizeof(T) == 4 ? 3 : 1, R16 = TM * 16;
@@ -192,8 +224,6 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
         if constexpr (Z) zr[u] = reinterpret_cast<const Scales<uint8_t, NG>*>(a.zeros)[b * kTileRows + r];
     };
     F4v acc[TM];
-    uint32_t mask = 0x00780078u, sixteen = 0x41804180u;      // (in registers: an and-or takes no literals)
-    asm("" : "+v"(mask), "+v"(sixteen));
     // acc += the block in slot u times columns 128 kc .. of the part of x in LDS
     auto multiply = [&](int u, int kc) __attribute__((always_inline)) {
         F4v part[TM];
@@ -203,21 +233,20 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
 #pragma unroll
                 for (int q = 0; q < TM; ++q) part[q] = F4v{0.f, 0.f, 0.f, 0.f};
             }
-            const uint32_t c = w[u][i];
-            const U4 b = {(c << 3 & mask) | sixteen, (c >> 1 & mask) | sixteen, (c >> 5 & mask) | sixteen,
-                          (c >> 9 & mask) | sixteen};
-            // - (16 + z) in bf16, for every column
-            uint32_t z = 0xc1c0c1c0u;
-            if constexpr (Z) {
-                z = __float_as_uint(-16.f - (float)zr[u].v[i / (G / 32)]);
-                z |= z >> 16;
-            }
+            // (x on its way while the codes are unpacked: 16 rows by 50280 x 2048 17.5 us, read after it 18.4)
+            B8h xa[TM];
 #pragma unroll
-            for (int q = 0; q < TM; ++q) {
-                const B8h xa = __builtin_bit_cast(B8h, s_x[at_x[q] + kc * 16 + i * 4]);
-                part[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa, __builtin_bit_cast(B8h, b), part[q], 0, 0, 0);
-                part[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa, __builtin_bit_cast(B8h, U4{z, z, z, z}), part[q], 0, 0, 0);
+            for (int q = 0; q < TM; ++q) xa[q] = __builtin_bit_cast(B8h, s_x[at_x[q] + kc * 16 + i * 4]);
+            __builtin_amdgcn_sched_barrier(0);
+            uint32_t zeros = 0;                    // the group's, in every byte
+            if constexpr (Z) {
+                __builtin_memcpy(&zeros, &zr[u], NG);
+                zeros = __builtin_amdgcn_perm(0u, zeros, 0x01010101u * (i / (G / 32)));
             }
+            const B8h weights = word_weights<Z>(w[u][i], zeros);
+#pragma unroll
+            for (int q = 0; q < TM; ++q)
+                part[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[q], weights, part[q], 0, 0, 0);
             if (i % (G / 32) == G / 32 - 1) {
                 const float s = sc[u].at(i / (G / 32));
 #pragma unroll
@@ -306,7 +335,7 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
                     // into row m's accumulator: lanes 4 j .. + 3 of tile m / 16
 #pragma unroll
                     for (int q = 0; q < TM * 4; ++q)
-                        if ((m >> 4) * 4 + (m & 3) == q && ((m >> 2) & 3) == j) acc[q >> 2][q & 3] += v;
+                        if ((m >> 4) * 4 + (m & 3) == q && ((m >> 2) & 3) == j) acc[q >> 2][q & 3] += v * kUnit<Z>;
                 }
             }
         }
@@ -327,6 +356,7 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
                 v += __shfl_xor(v, 16);
                 v += __shfl_xor(v, 32);
             }
+            v *= 1.f / kUnit<Z>;
             const int n = tile * kTileRows + r;
             if ((j == 0 || !spread) && n < a.N) {
                 if (a.bias) v += Act<T>::load(static_cast<const T*>(a.bias) + n);

@@ -189,3 +189,51 @@ def test_linear_on_rows_at_any_alignment(k, dtype):
         assert torch.equal(torch.isnan(y[m - 1]), torch.isnan(ref)) and torch.equal(y[m - 1] == torch.inf, ref == torch.inf)
         if m > 1:
             _check(y[:m - 1], x[:m - 1].double() @ w.t().contiguous(), _tol(k, 32, dtype))
+
+
+def _each(y, x, w, bias=None):
+    """Every value against float64, within what k fp32 products and sums may be off in any order: each of the k + 8
+    operations rounds by 2^-24 of what it makes, or cuts off 2^-23, and what is made never passes sum |x| |w|; then the
+    output's own rounding."""
+    k = x.shape[-1]
+    ref = x.double() @ w.t().contiguous()
+    most = x.double().abs() @ w.abs().t().contiguous()
+    if bias is not None:
+        ref, most = ref + bias.double(), most + bias.double().abs()
+    tol = (k + 8) * 2.0 ** -23 * most + (2.0 ** -8 * ref.abs() if y.dtype == torch.bfloat16 else 0) + 1e-37
+    off = (y.double() - ref).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True), (128, False)])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 256), (6, 100, 777), (17, 33, 1024), (40, 50, 4000)])
+def test_a_large_value_meets_a_weight_of_zero(m, n, k, group, zeros, dtype):
+    """Columns whose code is their zero weigh nothing, whatever x holds there."""
+    g = torch.Generator(device="cuda").manual_seed(n + k)
+    ng = -(-k // group)
+    codes = torch.randint(0, 16, (n, k), device="cuda", generator=g, dtype=torch.uint8)
+    z = torch.randint(0, 16, (n, ng), device="cuda", generator=g, dtype=torch.uint8)
+    z = z if zeros else torch.full_like(z, 8)
+    col = torch.arange(k, device="cuda") // group
+    large = torch.arange(0, k, 29, device="cuda")
+    codes[:, large] = z[:, col[large]]
+    scales = (torch.rand(n, ng, device="cuda", generator=g) + 0.5) * 0.01
+    w4 = ops.pack_w4(codes, scales, z if zeros else None, group)
+    w = (codes.double() - z.double()[:, col]) * scales.double()[:, col]
+    for size in (1e3, 1e10, 1e20, 7e28):
+        x = _x(m, k, dtype, m)
+        x[:, large] = (x[:, large].sign() * size).to(dtype)
+        _each(ops.linear_w4(x, w4), x, w)
+        one = _x(m, k, dtype, m)                              # in a single row: no other row notices
+        one[m // 2, large[1]] = size
+        _each(ops.linear_w4(one, w4), one, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offset", [0.0, 10.0, 1e4])
+def test_rows_about_an_offset(offset, dtype):
+    """x whose values share an offset: sums of x over a group are large, sums of x w are as large as x and w make them."""
+    w4, w = _matrix(100, 2048, 128, True, torch.bfloat16, 21)
+    x = (_x(5, 2048, torch.float32, 22) + offset).to(dtype)
+    _each(ops.linear_w4(x, w4), x, w)
