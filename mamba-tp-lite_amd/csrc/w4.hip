@@ -101,8 +101,9 @@ template <typename S, int NG> struct alignas(sizeof(S) * NG) Scales {        // 
 // A workgroup keeps x, as the operand's 16-byte runs, in LDS; each wavefront streams tiles of W into registers, kAhead
 // blocks before their use.  Where there are few tiles, wk wavefronts share one and add their sums in order.
 //
-// |x| >= 2^96 could overflow before its scale is applied, and infinities and NaN have no three parts: a part of x in which
-// some row holds one takes the products weight by weight instead, as the matrix form would round them.
+// |x| >= 2^96 could overflow before its scale is applied, and infinities and NaN have no three parts: a row that holds one
+// in a part of x is zeros there to the matrix cores, and takes its products weight by weight, as the matrix form would
+// round them.  Other rows stay as they are, to the bit.
 template <typename T, typename S, int G, bool Z, int TM>
 __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p) {
     constexpr int NG = kBlockK / G, P = sizeof(T) == 4 ? 3 : 1, R16 = TM * 16;
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
 #pragma unroll
     for (int q = 0; q < TM; ++q) at_x[q] = min(q * 16 + r, R - 1) * pitch + j;
     float* s_red = reinterpret_cast<float*>(s_x + P * p.rows * pitch);                         // [wave][R16][16]
-    __shared__ int s_wide;
+    __shared__ uint32_t s_wide;                               // bit m: row m of this part of x is such a one
 
     // u / n8 for the fewer than 2^19 runs of x and at most 48 rows: the product is off by less than half of 1 / n8
     auto row_of = [&](int u, float inv) __attribute__((always_inline)) { return (int)((u + 0.5f) * inv); };
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                     most = __builtin_elementwise_max(most, __builtin_bit_cast(H2, raw[n][0][q] & 0x7fff7fffu));
-                if (max(most[0], most[1]) >= (kWide >> 16)) s_wide = 1;
+                if (max(most[0], most[1]) >= (kWide >> 16)) atomicOr(&s_wide, 1u << m);
                 s_x[m * pitch + k8] = raw[n][0];
             } else {
                 float v[8];
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
                     v[e] = __uint_as_float(raw[n][e / 4 % kRaw][e % 4]);
                     most = max(most, abs_bits(v[e]));
                 }
-                if (most >= kWide) s_wide = 1;
+                if (most >= kWide) atomicOr(&s_wide, 1u << m);
 #pragma unroll
                 for (int q = 0; q < P; ++q) {      // the upper 8 significand bits of what is left, three times
                     U4 part;
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
 #pragma unroll 1
                 for (int e = 0; e < 8; ++e) {
                     float v = k + e < a.K ? Act<T>::load(x + m * a.ldx + k + e) : 0.f;
-                    if (abs_bits(v) >= kWide) s_wide = 1;
+                    if (abs_bits(v) >= kWide) atomicOr(&s_wide, 1u << m);
 #pragma unroll
                     for (int q = 0; q < P; ++q) {
                         run[q * M * pitch * 8 + e] = __float_as_uint(v) >> 16;
@@ -292,12 +293,19 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
                 }
                 staged = true;
                 lds_barrier();
+                if (s_wide) {
+                    for (int u = threadIdx.x; u < R * nb * 16; u += threads) {
+                        const int row = u / (nb * 16);
+                        if (s_wide >> row % M & 1) s_x[row * pitch + u - row * nb * 16] = U4{0, 0, 0, 0};
+                    }
+                    lds_barrier();
+                }
             }
-            const bool wide = s_wide;
+            uint32_t wide = __builtin_amdgcn_readfirstlane(s_wide);
             for (int kb = kb0 + wkid; kb < kb1; kb += kAhead * p.wk) {
                 const bool more = kb + kAhead * p.wk < a.KB;
                 const int tn = more ? t : t + stride, kbn = more ? kb + kAhead * p.wk : wkid;
-                const int blocks = wide ? 0 : ((kb1 - 1 - kb) >> p.wk_log2) + 1, kc = kb - kb0;
+                const int blocks = ((kb1 - 1 - kb) >> p.wk_log2) + 1, kc = kb - kb0;
                 if (tn < tiles) {
                     const int64_t b0 = (int64_t)tn * a.KB + kbn;
                     const int last = (a.KB - 1 - kbn) >> p.wk_log2;
@@ -312,31 +320,29 @@ __global__ void __launch_bounds__(kWaves * 64) linear_w4_kernel(const LinearW4 p
                         if (u < blocks) multiply(u, kc + u * p.wk);
                 }
             }
-            if (wide) {
-                const int64_t tb = (int64_t)min(t, tiles - 1) * a.KB;
+            const int64_t tb = (int64_t)min(t, tiles - 1) * a.KB;
+            for (; wide; wide &= wide - 1) {
+                const int m = __builtin_ctz(wide);
+                float v = 0.f;
 #pragma unroll 1
-                for (int m = 0; m < M; ++m) {
-                    float v = 0.f;
+                for (int kb = kb0 + wkid; kb < kb1; kb += p.wk) {
 #pragma unroll 1
-                    for (int kb = kb0 + wkid; kb < kb1; kb += p.wk) {
-#pragma unroll 1
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t c = reinterpret_cast<const uint32_t*>(a.codes)[((tb + kb) * 64 + lane) * 4 + i];
-                            const int64_t at = ((tb + kb) * kTileRows + r) * NG + 32 * i / G;
-                            const float s = scale_at<S>(a.scales, at), z = Z ? (float)a.zeros[at] : 8.f;
-                            const int k = kb * kBlockK + 32 * i + 8 * j;
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t c = reinterpret_cast<const uint32_t*>(a.codes)[((tb + kb) * 64 + lane) * 4 + i];
+                        const int64_t at = ((tb + kb) * kTileRows + r) * NG + 32 * i / G;
+                        const float s = scale_at<S>(a.scales, at), z = Z ? (float)a.zeros[at] : 8.f;
+                        const int k = kb * kBlockK + 32 * i + 8 * j;
 #pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (k + e < a.K) v = fmaf(Act<T>::load(x + m * a.ldx + k + e), s * ((float)code_of(c, e) - z), v);
-                        }
+                        for (int e = 0; e < 8; ++e)
+                            if (k + e < a.K) v = fmaf(Act<T>::load(x + m * a.ldx + k + e), s * ((float)code_of(c, e) - z), v);
                     }
-                    v += __shfl_xor(v, 16);
-                    v += __shfl_xor(v, 32);
-                    // into row m's accumulator: lanes 4 j .. + 3 of tile m / 16
-#pragma unroll
-                    for (int q = 0; q < TM * 4; ++q)
-                        if ((m >> 4) * 4 + (m & 3) == q && ((m >> 2) & 3) == j) acc[q >> 2][q & 3] += v * kUnit<Z>;
                 }
+                v += __shfl_xor(v, 16);
+                v += __shfl_xor(v, 32);
+                // into row m's accumulator: lanes 4 j .. + 3 of tile m / 16
+#pragma unroll
+                for (int q = 0; q < TM * 4; ++q)
+                    if ((m >> 4) * 4 + (m & 3) == q && ((m >> 2) & 3) == j) acc[q >> 2][q & 3] += v * kUnit<Z>;
             }
         }
         // D[i][j]: row 4 (lane / 16) + i of x, row lane % 16 of W

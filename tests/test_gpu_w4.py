@@ -237,3 +237,21 @@ def test_rows_about_an_offset(offset, dtype):
     w4, w = _matrix(100, 2048, 128, True, torch.bfloat16, 21)
     x = (_x(5, 2048, torch.float32, 22) + offset).to(dtype)
     _each(ops.linear_w4(x, w4), x, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("m,n,k", [(2, 20, 5), (7, 70, 400), (16, 300, 1300), (40, 33, 777), (10, 40, 9001), (64, 17000, 300)])
+def test_a_row_that_holds_an_infinity_changes_no_bit_of_another(m, n, k, zeros, dtype):
+    w4, _ = _matrix(n, k, 64, zeros, torch.bfloat16, 31)
+    x = _x(m, k, dtype, 32)
+    clean = ops.linear_w4(x, w4)
+    for bad in (float("inf"), float("nan"), 3e38):
+        for rows in ([0], [m - 1], list(range(0, m, 2))):
+            xb = x.clone()
+            for i, row in enumerate(rows):
+                xb[row, (i * 37 + k - 1) % k] = bad
+            y = ops.linear_w4(xb, w4)
+            rest = [i for i in range(m) if i not in rows]
+            assert torch.equal(y[rest], clean[rest])
+            assert bool((~torch.isfinite(y[rows]) | (y[rows] != clean[rows])).any(1).all())
