@@ -255,3 +255,31 @@ def test_a_row_that_holds_an_infinity_changes_no_bit_of_another(m, n, k, zeros, 
             rest = [i for i in range(m) if i not in rows]
             assert torch.equal(y[rest], clean[rest])
             assert bool((~torch.isfinite(y[rows]) | (y[rows] != clean[rows])).any(1).all())
+
+
+# What few and short rows of W do not reach: two operand tiles, workgroups of 16 wavefronts, several tiles of W to a
+# wavefront (the next one's loads under the last products), x in parts for each of them, a last tile that is partial.
+LARGE = [(1, 50280, 2048), (16, 50280, 2048), (33, 50277, 777), (64, 33000, 520), (10, 20011, 9000), (64, 8192, 2048),
+         (48, 2043, 4096), (33, 8190, 8192), (40, 50277, 6000)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group,zeros,scale_dtype", [(32, True, torch.bfloat16), (64, False, torch.float32)])
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_large_matrices_match_float64(m, n, k, group, zeros, scale_dtype, dtype):
+    w4, w = _matrix(n, k, group, zeros, scale_dtype, n + k)
+    x = _x(m, k, dtype, m)
+    bias = _x(1, n, dtype, 7)[0] if zeros else None
+    y = ops.linear_w4(x, w4, bias)
+    _check(y, x.double() @ w.t().contiguous() + (0 if bias is None else bias.double()), _tol(k, group, dtype))
+    _each(y, x, w, bias)
+    assert torch.equal(y, ops.linear_w4(x, w4, bias))
+    xb = x.clone()
+    at, where = m // 2, k - 3
+    xb[at, where] = torch.inf
+    yb = ops.linear_w4(xb, w4, bias)
+    ref = torch.inf * w[:, where]                          # NaN where the weight is zero
+    assert torch.equal(torch.isnan(yb[at]), torch.isnan(ref))
+    assert torch.equal(yb[at][~torch.isnan(ref)].double(), ref[~torch.isnan(ref)])
+    rest = [i for i in range(m) if i != at]
+    assert torch.equal(yb[rest], y[rest])
