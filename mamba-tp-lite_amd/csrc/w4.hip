@@ -505,10 +505,13 @@ extern "C" int mtl_linear_w4(const mtl_linear_w4_args* p, mtl_stream_t stream) {
     const int tiles = (a.N + kTileRows - 1) / kTileRows;
     // Rows of x to a workgroup: one operand tile's (16, of fp32 x 5) while that makes at most 2048 (tile of W, rows of x)
     // pairs, two tiles' where there are more: W is then read half as often.  Wavefronts to a pair: so many that the pairs
-    // make about 2048; pairs to a workgroup: so many that it has 8 wavefronts, 16 where its LDS leaves room for one
-    // workgroup a CU.  Measured, GPU us (pairs; chosen, its neighbours): 768x1536 1 row bf16 (48) 3.8, 4 / 2 wavefronts
-    // 3.7 / 5.0; 8192x2048 16 rows bf16 (512) 6.6, 8 / 2 9.7 / 8.3; 8192x2048 8 rows fp32 (1024) 6.8, 4 / 1 8.3 / 8.7;
-    // 50280x2048 8 rows fp32 (6286) two tiles 21.4, one 27.7; 2048x4096 64 rows bf16 (512) 9.2, two tiles 22.
+    // make about 2048; pairs to a workgroup: so many that it has 8 wavefronts.  Measured, GPU us (pairs; chosen, its
+    // neighbours): 768x1536 1 row bf16 (48) 3.8, 4 / 2 wavefronts 4.2 / 4.5; 8192x2048 16 rows bf16 (512) 7.0, 8 / 2 8.8 /
+    // 8.4; 8192x2048 8 rows fp32 (1024) 7.5, 4 / 1 8.7 / 9.7; 50280x2048 8 rows fp32 (6286) two tiles 19.4, one 27.3;
+    // 2048x4096 64 rows bf16 (512) 9.8, two tiles 15.1.
+    // A workgroup whose LDS has a CU to itself has 16 wavefronts, unless 8 make no more workgroups than CUs (16 would
+    // leave CUs idle).  fp32, 16 / 8 wavefronts (workgroups of 8): 64 rows of 8192x2048 (448) 18.0 / 20.1, 12 of 20000x2048
+    // (314) 17.8 / 19.1; 32 of 8192x2048 (256) 17.4 / 11.9, 48 of 2048x4096 (160) 24.7 / 16.8.
     const auto chunks_of = [&](int tm) { return (a.M + tm * 16 / parts - 1) / (tm * 16 / parts); };
     int tm = tiles * (int64_t)chunks_of(1) <= 2048 ? 1 : 2;
     const int chunks = chunks_of(tm);
@@ -522,7 +525,7 @@ extern "C" int mtl_linear_w4(const mtl_linear_w4_args* p, mtl_stream_t stream) {
     while (l.wk < 8 && l.wk * 2 * pairs <= 2048 && l.wk * 2 <= a.KB) l.wk *= 2;
     int wn = std::min(8 / l.wk, std::max(2, pairs / 64));
     const bool two = (size_t)l.kblocks * per_block + pad + 8 * tm * 1024 <= kLdsBytes / 2;
-    if (l.wk == 1 && !two) {
+    if (l.wk == 1 && !two && (int64_t)((tiles + 7) / 8) * chunks > 256) {
         wn = 16;
         l.kblocks = blocks_of(16);
     }
