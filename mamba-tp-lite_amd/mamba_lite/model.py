@@ -261,8 +261,10 @@ def _linear_mod(mod, x: torch.Tensor) -> torch.Tensor:
 class LinearW4(nn.Module):
     """nn.Linear with its weight [out_features, in_features] in 4-bit codes and group scales (ops.W4); made from a
     nn.Linear, or by MambaLM.quantize_w4.  A decode step's rows (up to ops.W4_MAX_ROWS) are multiplied from the codes; a
-    prompt's take the matrix made from them, as does a call whose gradient is recorded (with respect to x: the weight
-    has none)."""
+    prompt's take the matrix made from them, as does a call whose gradient is recorded (with respect to x and the bias:
+    the weight has none) or whose x is of a tensor subclass.  Forward-mode derivatives, functorch transforms, tracing
+    and torch's modes see that product and the matrix's making as torch operations.  Autocast changes a prompt's
+    product, as it does nn.Linear's, and not those from the codes, which keep x's type."""
 
     def __init__(self, w4: ops.W4, bias: torch.Tensor | None = None):
         super().__init__()
@@ -285,10 +287,13 @@ class LinearW4(nn.Module):
                f"zero_points={self.zeros is not None}, bias={self.bias is not None}"
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        w4 = self.w4()
-        if x.numel() <= ops.W4_MAX_ROWS * w4.k and not (torch.is_grad_enabled() and x.requires_grad):
-            return ops.linear_w4(x, w4, self.bias)
-        return _linear(x, ops.dequantize_w4(w4, x.dtype), self.bias)
+        w4, bias = self.w4(), self.bias
+        if not ops.no_transform():
+            return F.linear(x, ops.w4_matrix(w4, x.dtype), bias)
+        if x.numel() <= ops.W4_MAX_ROWS * w4.k and type(x) in ops.PLAIN_TENSORS and \
+                not (torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad))):
+            return ops.linear_w4(x, w4, bias)
+        return _linear(x, ops.dequantize_w4(w4, x.dtype), bias)
 
 
 def _skinny_split(K: int, most: int = 16) -> int:

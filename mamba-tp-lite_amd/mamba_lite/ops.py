@@ -950,12 +950,16 @@ def _no_function_mode() -> bool:
                for i in range(torch._C._len_torch_function_stack()))
 
 
-def plain_call() -> bool:
-    """No autocast, functorch or forward-mode transform, tracing, function or dispatch mode that a raw launch would
-    bypass."""
-    return _no_function_mode() and not torch.is_autocast_enabled("cuda") and \
+def no_transform() -> bool:
+    """No functorch or forward-mode transform, tracing, function or dispatch mode that a raw launch would bypass."""
+    return _no_function_mode() and \
         torch.autograd.forward_ad._current_level < 0 and torch._C._functorch.peek_interpreter_stack() is None and torch._C._len_torch_dispatch_stack() == 0 and \
         not torch.jit.is_tracing() and not torch.compiler.is_compiling()
+
+
+def plain_call() -> bool:
+    """no_transform(), and no autocast either."""
+    return not torch.is_autocast_enabled("cuda") and no_transform()
 
 
 def _plain_forward(*ts) -> bool:
@@ -1299,6 +1303,16 @@ def _no_grad_recorded(name, *ts):
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
+def _no_dual(name, *ts):
+    """(where forward-mode differentiation is on)"""
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f"{name} has no forward-mode derivative: call it on the primal")
+
+
+def _not_traced(name):
+    raise RuntimeError(f"{name} launches a kernel, which torch.jit.trace would not record")
+
+
 def _rows_of(t, cols):
     """t [..., cols] as (2-D tensor with unit column stride and rows that do not overlap, row stride)."""
     if t.dim() != 2 or (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
@@ -1331,6 +1345,10 @@ def linear_w4(x, w4, bias=None, out=None):
         raise RuntimeError(f"all operands must be on one device, got x on {x.device}, w4 on {codes.device}")
     if torch.is_grad_enabled():
         _no_grad_recorded("linear_w4", x, bias)
+    if torch.autograd.forward_ad._current_level >= 0:
+        _no_dual("linear_w4", x, bias)
+    if torch._C._is_tracing():
+        _not_traced("linear_w4")
     if x.is_contiguous():
         M, ldx = x.numel() // k, k
     else:
@@ -1410,6 +1428,8 @@ def dequantize_w4(w4, dtype=torch.float32, out=None):
         raise TypeError(f"dequantize_w4: w4 must be a W4 (pack_w4, quantize_w4), got {type(w4).__name__}")
     if dtype not in _ACT_DTYPES:
         raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
+    if torch._C._is_tracing():
+        _not_traced("dequantize_w4")
     if out is None:
         out = w4.codes.new_empty((w4.n, w4.k), dtype=dtype)
     else:
@@ -1426,6 +1446,17 @@ def dequantize_w4(w4, dtype=torch.float32, out=None):
                                                  w4.k, w4.group, _ACT_DTYPES[dtype], _ACT_DTYPES[w4.scales.dtype],
                                                  _stream(out)), "dequantize_w4")
     return out
+
+
+def w4_matrix(w4, dtype=torch.float32):
+    """dequantize_w4 as torch operations, for transforms and tracing: the same values, on any device."""
+    nt, kb = w4.codes.shape[:2]
+    c = w4.codes.view(nt, kb, 4, _W4_TILE, 4, 4)                            # [nt, kb, j, r, i, byte]
+    c = torch.stack((c & 15, c >> 4), -1).view(nt, kb, 4, _W4_TILE, 4, 2, 4)  # a word's nibbles: codes 0 2 4 6, 1 3 5 7
+    c = c.permute(0, 3, 1, 4, 2, 6, 5).reshape(nt, _W4_TILE, kb, -1, w4.group).float()
+    each = lambda t: t.float().transpose(1, 2)[..., None]                   # [nt, r, kb, 128 / group, 1]
+    w = (c - (8.0 if w4.zeros is None else each(w4.zeros))) * each(w4.scales)
+    return w.view(nt * _W4_TILE, kb * _W4_BLOCK)[:w4.n, :w4.k].to(dtype)
 
 
 # --------------------------------------------------------------------------- log probabilities
@@ -1463,6 +1494,10 @@ def token_logprobs(logits, tokens, top=0):
         raise RuntimeError(f"all operands must be on one device, got logits on {logits.device}, tokens on {tokens.device}")
     if torch.is_grad_enabled():
         _no_grad_recorded("token_logprobs", logits)
+    if torch.autograd.forward_ad._current_level >= 0:
+        _no_dual("token_logprobs", logits)
+    if torch._C._is_tracing():
+        _not_traced("token_logprobs")
     x = logits
     if V > 1 and x.stride(-1) != 1:
         x = x.contiguous()

@@ -328,3 +328,43 @@ def test_a_mixer_by_itself():
         assert _rel(y, yr) < TOL and _rel(hs, hsr) < TOL
         a, b = LayerCache(cs, hs), LayerCache(csr, hsr)
         assert _rel(mx.step(x[:, 0], a), ref.step(x[:, 0], b)) < TOL and _rel(a.ssm_state, b.ssm_state) < TOL
+
+
+@pytest.mark.parametrize("zero_points", [False, True])
+def test_linear_w4_module_under_transforms(zero_points):
+    """What torch does around a module it does around this one: few rows (from the codes otherwise) as many."""
+    torch.manual_seed(1)
+    lin = torch.nn.Linear(300, 200).cuda()
+    q = LinearW4.from_linear(lin, 64, zero_points)
+    w = ops.dequantize_w4(q.w4(), torch.float32)
+    assert torch.equal(ops.w4_matrix(q.w4()), w) and torch.equal(ops.w4_matrix(q.w4(), torch.bfloat16), w.bfloat16())
+    for rows in (5, 65):
+        x, v = torch.randn(rows, 300, device="cuda"), torch.randn(rows, 300, device="cuda")
+        with torch.no_grad():
+            want = q(x)
+            # forward mode, plain and through functorch
+            with torch.autograd.forward_ad.dual_level():
+                y, dy = torch.autograd.forward_ad.unpack_dual(q(torch.autograd.forward_ad.make_dual(x, v)))
+            assert dy is not None and _rel(y, want) < TOL and _rel(dy, v.double() @ w.double().t().contiguous()) < TOL
+            y, dy = torch.func.jvp(q, (x,), (v,))
+            assert _rel(y, want) < TOL and _rel(dy, v.double() @ w.double().t().contiguous()) < TOL
+            assert _rel(torch.func.vmap(q)(x), want) < TOL
+            traced = torch.jit.trace(q, (x,), check_trace=False)
+            assert _rel(traced(v), q(v)) < TOL
+            seen = []
+
+            class Mode(torch.overrides.TorchFunctionMode):
+                def __torch_function__(self, func, types, args=(), kwargs=None):
+                    seen.append(func)
+                    return func(*args, **(kwargs or {}))
+
+            with Mode():
+                q(x)
+            assert F.linear in seen
+        g = torch.func.grad(lambda x: q(x).square().sum())(x)
+        assert _rel(g, 2 * want.double() @ w.double()) < TOL
+        bias = q.bias.requires_grad_()                             # a bias that learns
+        q(x).sum().backward()
+        assert torch.equal(bias.grad, torch.full_like(bias, rows))
+        bias.grad = None
+        bias.requires_grad_(False)

@@ -249,3 +249,32 @@ def test_a_weight_that_cannot_be_quantized_leaves_the_model_alone():
     new = set(m.state_dict()) - keys
     assert new == {f"layers.{i}.mixer.{n}.scales" for i in range(2) for n in ("in_proj", "out_proj")} | \
         {"head_w4.weight", "head_w4.scales"}
+
+
+@pytest.mark.parametrize("n,k,group,zeros", [(1, 1, 32, True), (40, 300, 32, True), (33, 256, 128, False), (17, 129, 64, True)])
+def test_the_matrix_as_torch_operations(n, k, group, zeros):
+    codes, scales, z = _random(n, k, group, zeros)
+    col = torch.arange(k) // group
+    w = (codes.double() - (z.double()[:, col] if zeros else 8.0)) * scales.double()[:, col]
+    w4 = ops.pack_w4(codes, scales, z, group)
+    assert torch.equal(ops.w4_matrix(w4), w.float()) and torch.equal(ops.w4_matrix(w4, torch.bfloat16), w.float().bfloat16())
+
+
+def test_forward_mode_and_tracing_are_refused():
+    """A raw launch would come back without its tangent, or with a trace of memory that nothing fills."""
+    w4 = ops.pack_w4(*_random(20, 200, 64, True), group=64)
+    x, tokens = torch.zeros(2, 200), torch.zeros(2, dtype=torch.int64)
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.linear_w4(dual, w4)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.linear_w4(x, w4, torch.autograd.forward_ad.make_dual(torch.zeros(20), torch.ones(20)))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.token_logprobs(dual, tokens)
+        with pytest.raises(RuntimeError, match="GPU"):             # a primal by itself is an ordinary operand
+            ops.linear_w4(x, w4)
+    for call in (lambda x: ops.linear_w4(x, w4), lambda x: ops.token_logprobs(x, tokens).logprob,
+                 lambda x: x @ ops.dequantize_w4(w4).t()):
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(call, (x,), check_trace=False)
