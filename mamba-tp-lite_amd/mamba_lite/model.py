@@ -264,7 +264,8 @@ class LinearW4(nn.Module):
     prompt's take the matrix made from them, as does a call whose gradient is recorded (with respect to x and the bias:
     the weight has none) or whose x is of a tensor subclass.  Forward-mode derivatives, functorch transforms, tracing
     and torch's modes see that product and the matrix's making as torch operations.  Autocast changes a prompt's
-    product, as it does nn.Linear's, and not those from the codes, which keep x's type."""
+    product, as it does nn.Linear's (and casts a bias of another type), and not those from the codes, which keep x's
+    type."""
 
     def __init__(self, w4: ops.W4, bias: torch.Tensor | None = None):
         super().__init__()
@@ -291,7 +292,8 @@ class LinearW4(nn.Module):
         if not ops.no_transform():
             return F.linear(x, ops.w4_matrix(w4, x.dtype), bias)
         if x.numel() <= ops.W4_MAX_ROWS * w4.k and type(x) in ops.PLAIN_TENSORS and \
-                not (torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad))):
+                not (torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad))) and \
+                not (bias is not None and bias.dtype != x.dtype and torch.is_autocast_enabled("cuda")):
             return ops.linear_w4(x, w4, bias)
         return _linear(x, ops.dequantize_w4(w4, x.dtype), bias)
 
@@ -412,6 +414,10 @@ class MambaMixer(nn.Module):
         """prefill(); with parts_ok, out_proj of a short prefill may come back
         as _Parts (split-K partial products for the residual add to sum);
         skinny=False keeps every projection on torch's GEMMs."""
+        if type(self.in_proj) is LinearW4 and torch.is_autocast_enabled("cuda"):
+            # as its steps run: the products from the codes keep x's type, so must the matrices' and x_proj's
+            with torch.autocast("cuda", enabled=False):
+                return self._prefill(x, cache, out, parts_ok, skinny)
         b, l, dm = x.shape
         Dm, N, R, K = self.cfg.d_inner, self.cfg.d_state, self.cfg.dt_rank, self.cfg.d_conv
         bf16 = x.dtype == torch.bfloat16

@@ -368,3 +368,30 @@ def test_linear_w4_module_under_transforms(zero_points):
         assert torch.equal(bias.grad, torch.full_like(bias, rows))
         bias.grad = None
         bias.requires_grad_(False)
+
+
+@pytest.mark.parametrize("l", [20, 100, 700])
+def test_prompts_and_steps_under_autocast(l):
+    """The layers keep the embedding's type, as a step from the codes does."""
+    q = _model(256).quantize_w4()
+    ids = torch.randint(0, 1003, (3, l + 1), device="cuda")
+    clone = lambda c: MambaCache([type(lc)(lc.conv_state.clone(), lc.ssm_state.clone()) for lc in c.layers])
+    with torch.no_grad():
+        want, cache = q.prefill(ids[:, :l])
+        hidden, _ = q._prefill_hidden(ids[:, :l])
+        c1, c2 = clone(cache), clone(cache)
+        step = q.step(ids[:, l:], c1)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            assert torch.equal(q._prefill_hidden(ids[:, :l])[0], hidden)
+            got, c3 = q.prefill(ids[:, :l])
+            assert _rel(got, want) < 2.0 ** -8 * 2                    # the head's operands and logits in bf16
+            assert _rel(q.step(ids[:, l:], c2), step) < TOL
+        for a, b, c in zip(c1.layers, c2.layers, c3.layers):
+            assert _rel(b.ssm_state, a.ssm_state) < TOL and _rel(b.conv_state, a.conv_state) < TOL
+            assert c.conv_state.dtype == torch.float32
+    lin = torch.nn.Linear(128, 40).cuda()
+    m = LinearW4.from_linear(lin)
+    x = torch.randn(5, 128, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):       # a bias of the module's type, x of autocast's
+        ref = x.double() @ ops.dequantize_w4(m.w4()).double().t().contiguous() + lin.bias.double()
+        assert m(x).dtype == torch.bfloat16 and _rel(m(x), ref) < 2.0 ** -7   # x's products and the matrix: a rounding each
