@@ -1063,8 +1063,8 @@ class MambaLM(nn.Module):
         """(ctypes arrays of mtl_decode_layer with this call's cache pointers and of mtl_w4_matrix) for
         mtl_decode_step_w4, or None where it does not apply: sizes, a stack of more than plain modules and LinearW4, a
         weight or cache tensor that is not a contiguous tensor of x's dtype (SSM states: float32) and its shape on x's
-        device.  The weights are checked when their addresses (or x_proj's version, which its transposed copy follows)
-        change; the cache tensors every call."""
+        device.  The weights are checked when their addresses, the projections' form (group, scales' type, sizes) or
+        x_proj's version (which its transposed copy follows) change; the cache tensors every call."""
         cfg, act, dev = self.cfg, x.dtype, x.device
         nl = len(lt)
         D, N, K, R = cfg.d_inner, cfg.d_state, cfg.d_conv, cfg.dt_rank
@@ -1088,7 +1088,8 @@ class MambaLM(nn.Module):
             return None
         ptr = lambda t: 0 if t is None else t.data_ptr()
         sig = (dev, dm, act, tuple(ptr(t) for ts in lt for t in ts),
-               tuple(ptr(p._parameters[n]) for p in proj for n in ("scales", "zeros")),
+               tuple((ptr(s), s.dtype, ptr(p._parameters["zeros"]), p.group, p.out_features, p.in_features)
+                     for p in proj for s in (p._parameters["scales"],)),
                tuple(ts[_LT_XPROJ]._version for ts in lt) if act == torch.float32 else None, self._norm_eps())
         cached = getattr(self, "_w4_tmpl", None)
         if cached is None or cached[0] != sig:

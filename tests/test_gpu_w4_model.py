@@ -395,3 +395,28 @@ def test_prompts_and_steps_under_autocast(l):
     with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):       # a bias of the module's type, x of autocast's
         ref = x.double() @ ops.dequantize_w4(m.w4()).double().t().contiguous() + lin.bias.double()
         assert m(x).dtype == torch.bfloat16 and _rel(m(x), ref) < 2.0 ** -7   # x's products and the matrix: a rounding each
+
+
+def test_a_projection_of_another_form_at_the_same_addresses():
+    """Groups of 64 with bf16 scales and of 128 with fp32 ones take as many bytes: the step after a swap reads the new ones."""
+    m = _model(256)
+    other = copy.deepcopy(m)
+    q = m.quantize_w4(group=64, scale_dtype=torch.bfloat16)
+    other.quantize_w4(group=128, scale_dtype=torch.float32)
+    ids = torch.randint(0, 1003, (2, 1), device="cuda")
+    fresh = lambda: MambaCache.allocate(q.cfg, 2, "cuda", torch.float32)
+    with torch.no_grad():
+        q.step(ids, fresh())                                              # the plan is made
+        for a, b in zip(q.layers, other.layers):
+            for name in ("in_proj", "out_proj"):
+                old, new = getattr(a.mixer, name), getattr(b.mixer, name)
+                # the new module's values in the old one's memory, as an allocator may place them
+                assert old.scales.numel() * 2 == new.scales.numel() * 4
+                old.weight.copy_(new.weight)
+                scales = old.scales.data.view(-1).view(torch.float32).view(new.scales.shape)
+                scales.copy_(new.scales)
+                w4 = ops.W4(old.weight.data, scales, None, new.out_features, new.in_features, 128)
+                assert w4.scales.data_ptr() == old.scales.data_ptr()
+                setattr(a.mixer, name, LinearW4(w4, new.bias))
+        q.head_w4 = other.head_w4
+        assert torch.equal(q.step(ids, fresh()), other.step(ids, fresh()))
