@@ -876,7 +876,8 @@ class MambaLM(nn.Module):
         the library's, the conv-step and SSM-update kernels)."""
         lt = self._layer_tensors()
         w4 = len(lt) > 0 and type(self.layers[0].mixer.in_proj) is LinearW4
-        if not w4 and self._fused_step_ok(input_ids, cache, lt=lt):
+        # (the fused step's head is the embedding)
+        if not w4 and "head_w4" not in self._modules and self._fused_step_ok(input_ids, cache, lt=lt):
             return self._step_fused(input_ids, cache, lt=lt)
         x = self.embedding(input_ids).squeeze(1)
         if w4 and BATCHED_STEP_NATIVE:

@@ -420,3 +420,16 @@ def test_a_projection_of_another_form_at_the_same_addresses():
                 setattr(a.mixer, name, LinearW4(w4, new.bias))
         q.head_w4 = other.head_w4
         assert torch.equal(q.step(ids, fresh()), other.step(ids, fresh()))
+
+
+@pytest.mark.parametrize("b", [1, 3])
+def test_a_4_bit_head_on_plain_projections(b):
+    """Projections put back as matrices, the head left in 4 bits: steps answer through it as prompts do."""
+    q = _model(256).quantize_w4()
+    m = _on_matrices(q)
+    m.head_w4 = q.head_w4
+    ids = torch.randint(0, 1003, (b, 6), device="cuda")
+    with torch.no_grad():
+        _, c1 = q.prefill(ids[:, :5])
+        _, c2 = m.prefill(ids[:, :5])
+        assert _rel(m.step(ids[:, 5:], c2), q.step(ids[:, 5:], c1)) < TOL
