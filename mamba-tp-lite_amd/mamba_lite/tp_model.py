@@ -228,6 +228,8 @@ class LocalTPLM:
     @classmethod
     def from_dense(cls, lm, world_size: int = 2, allreduce_dtype="fp32", naive: bool = False) -> "LocalTPLM":
         """Every rank's shard of a dense MambaLM."""
+        if getattr(lm, "head_w4", None) is not None:
+            raise TypeError("LocalTPLM's lm_head is the embedding: shard the model before quantize_w4")
         blocks = [LocalTPBlock(blk.norm.weight.detach(),
                                LocalTPMixer.from_dense(blk.mixer, world_size, allreduce_dtype, i, naive))
                   for i, blk in enumerate(lm.layers)]

@@ -71,6 +71,8 @@ def shard_mixer_tensors(tensors, d_inner: int, rank: int, world_size: int,
     rank 0 then holds only x rows and rank 1 only z rows."""
     sl = channel_slice(rank, world_size, d_inner)
     t = tensors
+    if any(t[n].dim() != 2 for n in ("in_proj.weight", "out_proj.weight")):
+        raise TypeError("shards are cut from matrices, not from 4-bit codes: shard the model before quantize_w4")
     if naive:
         full = channel_slice(rank, world_size, 2 * d_inner)
         packed = lambda v: v[full]

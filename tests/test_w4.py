@@ -278,3 +278,18 @@ def test_forward_mode_and_tracing_are_refused():
                  lambda x: x @ ops.dequantize_w4(w4).t()):
         with pytest.raises(RuntimeError, match="trace"):
             torch.jit.trace(call, (x,), check_trace=False)
+
+
+@pytest.mark.parametrize("lm_head", [False, True])
+def test_codes_are_not_sharded(lm_head):
+    from mamba_lite import tp_utils
+    from mamba_lite.model import MambaConfig, MambaLM
+    from mamba_lite.tp_model import LocalTPLM
+    m = MambaLM(MambaConfig(d_model=64, n_layer=1, vocab_size=40))
+    LocalTPLM.from_dense(m)
+    m.quantize_w4(lm_head=lm_head)
+    with pytest.raises(TypeError, match="quantize_w4"):
+        LocalTPLM.from_dense(m)
+    for shard in (tp_utils.shard_mixer_params, tp_utils.naive_shard_mixer_params):
+        with pytest.raises(TypeError, match="quantize_w4"):
+            shard(m.layers[0].mixer, 0, 2)
