@@ -765,9 +765,11 @@ class MambaLM(nn.Module):
         """input_ids [b, l] -> ln p of each token but a row's first, given the ones before it (logprob, entropy
         [b, l - 1]), with the `top` most probable tokens at each place (top_logprob, top_token [b, l - 1, top]).  The
         logits are made a part at a time and not kept."""
+        if input_ids.dim() != 2 or input_ids.shape[1] < 1:
+            raise ValueError(f"score: input_ids must be [b, l >= 1], got {tuple(input_ids.shape)}")
         xf, _ = self._prefill_hidden(input_ids)
         b, l = input_ids.shape
-        xf, given = xf[:, :-1].reshape(b * (l - 1), xf.shape[-1]), input_ids[:, 1:].reshape(-1)
+        xf, given = xf[:, :-1].reshape(b * (l - 1), xf.shape[-1]), input_ids[:, 1:].reshape(-1).long()
         step = max(1, self._SCORE_LOGITS // self.embedding.weight.shape[0])
         parts = [ops.token_logprobs(self.lm_head(xf[i:i + step]), given[i:i + step], top=top)
                  for i in range(0, max(len(given), 1), step)]

@@ -433,3 +433,13 @@ def test_a_4_bit_head_on_plain_projections(b):
         _, c1 = q.prefill(ids[:, :5])
         _, c2 = m.prefill(ids[:, :5])
         assert _rel(m.step(ids[:, 5:], c2), q.step(ids[:, 5:], c1)) < TOL
+
+
+def test_score_takes_what_prefill_takes():
+    m = _model()
+    ids = torch.randint(0, 1003, (2, 9), device="cuda")
+    for a, b in zip(m.score(ids.int(), top=2), m.score(ids, top=2)):
+        assert torch.equal(a, b)
+    for bad in (ids[:, :0], ids[0]):
+        with pytest.raises(ValueError, match="input_ids"):
+            m.score(bad)
