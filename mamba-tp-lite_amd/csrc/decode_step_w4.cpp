@@ -8,10 +8,11 @@
 //   cores) -> the partials summed in order -> the SSM update in place, y -> out_proj from the codes into floats -> the
 //   residual add and the next RMSNorm.
 // Captured steps at the mamba-1.4b width (48 layers, vocabulary 50280, groups of 128, the head in 4 bits too), against
-// the same model's fp32 or bf16 weights: fp32 1 row 1390 -> 1104 us, 8 rows 1858 -> 1492, 32 rows 2304 -> 2420; bf16
-// 1212 -> 1087, 1439 -> 1415, 1713 -> 1814.  Past a few rows what is left beside the projections bounds it: six
-// launches of about 4 us a layer, and matrix work that the wider weights' kernels fuse with the conv step.  Eager 1 row
-// fp32: 3839 op by op, 1278 here.
+// the same model's fp32 or bf16 weights: fp32 1 row 1388 -> 1114 us, 8 rows 1851 -> 1510, 32 rows 2318 -> 2195; bf16
+// 1208 -> 1092, 1440 -> 1477, 1712 -> 1831.  At the mamba-130m width (24 layers) all are slower: fp32 321 -> 465, 539 ->
+// 573, 616 -> 658; bf16 393 -> 442, 482 -> 576, 549 -> 623.  What is left beside the projections bounds it: six launches
+// of about 4 us a layer, and matrix work that the wider weights' kernels fuse with the conv step.  Eager 1 row fp32 at
+// the mamba-1.4b width: 3839 op by op, 1275 here.
 #include <hip/hip_runtime.h>
 
 #include <string>

@@ -679,8 +679,11 @@ class MambaLM(nn.Module):
                     lm_head: bool = True) -> "MambaLM":
         """Puts every block's in_proj and out_proj, and with lm_head a copy of the tied embedding for the head, into
         4-bit codes (LinearW4), in place; the embedding itself and the small projections stay as they are.  A model
-        at the mamba-1.4b width keeps about a third of its fp32 bytes.  Graphs captured before refuse to replay.  Returns
-        self."""
+        at the mamba-1.4b width keeps a quarter of its fp32 bytes (5.5 -> 1.3 GB), one at the mamba-130m width half.  A
+        step gets faster only where the weight stream bounds it: mamba-1.4b fp32 (1 row 1388 -> 1114 us, 32 rows 2318 ->
+        2195) and bf16 at a few rows (1 row 1208 -> 1092, 32 rows 1712 -> 1831).  At the mamba-130m width steps take
+        longer (fp32 1 row 321 -> 465 us), and prompts do at both (1024 tokens fp32: 3.0 -> 4.6 ms, 16.2 -> 16.7).
+        Graphs captured before refuse to replay.  Returns self."""
         for blk in self.layers:
             for name in ("in_proj", "out_proj"):
                 if type(getattr(blk.mixer, name)) is not nn.Linear:
