@@ -813,8 +813,9 @@ int mtl_decode_step_persist(const mtl_decode_step_args* args, const mtl_decode_l
  *
  * mtl_linear_w4: y [M, N] = x [M, K] W^T (+ bias [N]) for 0 <= M <= 64 rows;
  *   x, bias and y of type dtype (MTL_F32 or MTL_BF16), rows ldx and ldy
- *   elements apart.  Products and sums are as exact as fp32 ones.  y must
- *   not overlap x.  No row of x changes another row's result.
+ *   elements apart.  Products and sums are as exact as fp32 ones (of float
+ *   x, what lies below 2^-133 is cut off: the last bits of |x| < 2^-110).
+ *   y must not overlap x.  No row of x changes another row's result.
  * mtl_dequantize_w4: W [N, K] (rows ldw elements apart) of type dtype, each
  *   value rounded once from fp32.
  * ---------------------------------------------------------------------- */

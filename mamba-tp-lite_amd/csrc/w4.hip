@@ -93,7 +93,8 @@ template <typename S, int NG> struct alignas(sizeof(S) * NG) Scales {        // 
 };
 
 // Products on the bf16 matrix cores, exact: q - z is a bf16 number, x in float32 the sum of three bf16 numbers of 8
-// significand bits each, as rows of their own.  A group's sums run in fp32 on v_mfma_f32_16x16x32_bf16:
+// significand bits each (down to bf16's least, 2^-133), as rows of their own.  A group's sums run in fp32 on
+// v_mfma_f32_16x16x32_bf16:
 //   acc += s sum x (q - z)
 // (Products with 16 + q, which the four bits under an exponent give for half the instructions, less x times 16 + z leave
 // the rounding of sums of 31 |x|, on columns of zero weight too.)

@@ -283,3 +283,16 @@ def test_large_matrices_match_float64(m, n, k, group, zeros, scale_dtype, dtype)
     assert torch.equal(yb[at][~torch.isnan(ref)].double(), ref[~torch.isnan(ref)])
     rest = [i for i in range(m) if i != at]
     assert torch.equal(yb[rest], y[rest])
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("scale", [1e-33, 1e-36, 1e-39])
+def test_values_near_the_least_ones(scale, zeros):
+    """fp32 x to 2^-133, where bf16's least values end: each of k values by less than that, on top of the sums' rounding."""
+    k = 512
+    w4, w = _matrix(64, k, 64, zeros, torch.float32, 3)
+    x = _x(3, k, torch.float32, 4) * scale
+    ref = x.double() @ w.t().contiguous()
+    most = x.double().abs() @ w.abs().t().contiguous()
+    tol = (k + 8) * 2.0 ** -23 * most + 2.0 ** -133 * w.abs().sum(1) + k * 2.0 ** -149
+    assert bool(((ops.linear_w4(x, w4).double() - ref).abs() <= tol).all())
