@@ -71,7 +71,6 @@ template <bool Z> __device__ __forceinline__ B8h word_weights(uint32_t c, uint32
     return __builtin_bit_cast(B8h, pairs);
 }
 
-
 constexpr int kWaves = 16;                 // most wavefronts of a workgroup
 constexpr uint32_t kWide = 0x6f800000u;    // 2^96
 constexpr int kAhead = 4;                  // blocks of W that a wavefront has in flight
