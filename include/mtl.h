@@ -866,6 +866,62 @@ int mtl_decode_step_w4(const mtl_decode_step_batched_args* args, const mtl_decod
                        const mtl_w4_matrix* matrices, int32_t dtype, mtl_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Rows in 8-bit integers with a scale each: a row t of floats is held as
+ *   a = max |t|,  codes[k] = the whole number nearest to 127 t[k] / a (halves
+ *   to the even one; in -127..127),  scale = a / 127
+ * and stands for codes[k] scale; a row of zeros has codes and scale 0, one
+ * that holds an infinity or NaN codes 0 and scale NaN.  No counterpart in the
+ * reference, whose int8 is that of a payload (tp_utils.py:103-131).
+ *
+ * Layout: codes [M, K rounded up to 128] contiguous, 16-byte aligned, zeros
+ * past K; scales [M] float.  1 <= K < 2^17 (sums of products of codes are
+ * exact in 32 bits), M < 2^31.
+ *
+ * mtl_quantize_int8: rows of x (dtype MTL_F32 or MTL_BF16, ldx elements apart).
+ * mtl_add_rmsnorm_int8: h = x + y (y NULL: x), stored in x_out unless that is
+ *   NULL (it may be x, or a float y), and the row w rmsnorm(h) (model.py:
+ *   130-135 with the residual add of 306/311) in int8: the codes of the float
+ *   row t = h w, and scale = a / 127 / sqrt(mean(h^2) + eps).  x, x_out float,
+ *   y of y_dtype, all [M, K] contiguous, w [K] of w_dtype.
+ * mtl_linear_int8: y [M, N] = x W^T (+ bias [N]) for x [M, K] and W [N, K] in
+ *   this layout, y (rows ldy elements apart) and bias of type dtype: the sum
+ *   exact, then times x's scale and W's, each rounded in fp32.  N <= 2^27.  y
+ *   must not overlap an operand.
+ * mtl_dequantize_int8: the floats that rows stand for (dtype, ldo elements
+ *   apart), rounded once from fp32.
+ * All are deterministic and take no workspace.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    const float* x;
+    const void* y;             /* or NULL */
+    float* x_out;              /* or NULL */
+    const void* w;
+    int8_t* codes;
+    float* scales;
+    int64_t M, K;
+    float eps;
+    int32_t y_dtype, w_dtype, reserved;
+} mtl_add_rmsnorm_int8_args;
+
+typedef struct {
+    const int8_t* x;
+    const float* x_scales;
+    const int8_t* w;
+    const float* w_scales;
+    const void* bias;          /* [N] or NULL */
+    void* y;
+    int64_t ldy, M, N, K;
+    int32_t dtype, reserved;
+} mtl_linear_int8_args;
+
+int mtl_quantize_int8(const void* x, int64_t ldx, int8_t* codes, float* scales, int64_t M, int64_t K, int32_t dtype,
+                      mtl_stream_t stream);
+int mtl_add_rmsnorm_int8(const mtl_add_rmsnorm_int8_args* args, mtl_stream_t stream);
+int mtl_linear_int8(const mtl_linear_int8_args* args, mtl_stream_t stream);
+int mtl_dequantize_int8(const int8_t* codes, const float* scales, void* out, int64_t ldo, int64_t M, int64_t K,
+                        int32_t dtype, mtl_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Log probabilities of given tokens, with entropy and the most probable
  * tokens, of rows of logits (float or bf16, dtype); row i is logits +
  * (i / inner) stride_outer + (i % inner) stride_inner, its vocab values

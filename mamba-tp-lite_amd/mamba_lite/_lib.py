@@ -15,7 +15,7 @@ import os
 import torch  # noqa: F401  (must be loaded first, see module docstring)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmtl.so")
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 MTL_F32 = 0
 MTL_BF16 = 1
@@ -148,6 +148,22 @@ class TokenLogprobsArgs(ctypes.Structure):
     ]
 
 
+class AddRmsnormInt8Args(ctypes.Structure):
+    """mirror of mtl_add_rmsnorm_int8_args"""
+    _fields_ = [
+        ("x", _vp), ("y", _vp), ("x_out", _vp), ("w", _vp), ("codes", _vp), ("scales", _vp), ("M", _i64), ("K", _i64),
+        ("eps", ctypes.c_float), ("y_dtype", _i32), ("w_dtype", _i32), ("reserved", _i32),
+    ]
+
+
+class LinearInt8Args(ctypes.Structure):
+    """mirror of mtl_linear_int8_args"""
+    _fields_ = [
+        ("x", _vp), ("x_scales", _vp), ("w", _vp), ("w_scales", _vp), ("bias", _vp), ("y", _vp),
+        ("ldy", _i64), ("M", _i64), ("N", _i64), ("K", _i64), ("dtype", _i32), ("reserved", _i32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol of include/mtl.h
 SIGNATURES = {
     "mtl_last_error": (ctypes.c_char_p, []),
@@ -207,6 +223,10 @@ SIGNATURES = {
     "mtl_dequantize_w4": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp]),
     "mtl_decode_step_w4": (ctypes.c_int, [ctypes.POINTER(DecodeStepBatchedArgs), ctypes.POINTER(DecodeLayer),
                                           ctypes.POINTER(W4Matrix), _i32, _vp]),
+    "mtl_quantize_int8": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "mtl_add_rmsnorm_int8": (ctypes.c_int, [ctypes.POINTER(AddRmsnormInt8Args), _vp]),
+    "mtl_linear_int8": (ctypes.c_int, [ctypes.POINTER(LinearInt8Args), _vp]),
+    "mtl_dequantize_int8": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
     "mtl_token_logprobs": (ctypes.c_int, [ctypes.POINTER(TokenLogprobsArgs), _vp]),
 }
 

@@ -1461,6 +1461,246 @@ def w4_matrix(w4, dtype=torch.float32):
     return w.view(nt * _W4_TILE, kb * _W4_BLOCK)[:w4.n, :w4.k].to(dtype)
 
 
+# --------------------------------------------------------------------------- rows in 8-bit integers
+INT8_MAX_K = (1 << 17) - 1      # columns whose sums of products of codes are exact in 32 bits
+_INT8_PAD = 128
+
+
+class Int8:
+    """Rows in 8-bit integers, code * scale with one scale per row: values [..., k], codes [..., k rounded up to 128]
+    int8 with zeros past k, scales [...] float32.  dtype (float32 or bfloat16) is the type of the values they stand for:
+    what dequantize_int8 and, of its first operand, linear_int8 return.  quantize_int8, add_rmsnorm_int8 and pack_int8
+    make it."""
+
+    __slots__ = ("codes", "scales", "k", "dtype")
+
+    def __init__(self, codes, scales, k, dtype=torch.float32):
+        if dtype not in _ACT_DTYPES:
+            raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
+        if not 1 <= k <= INT8_MAX_K:
+            raise ValueError(f"int8 rows have 1..{INT8_MAX_K} columns, got {k}")
+        kp = -(-k // _INT8_PAD) * _INT8_PAD
+        if codes.dtype != torch.int8 or codes.dim() < 1 or codes.shape[-1] != kp or not codes.is_contiguous() or \
+                codes.data_ptr() % 16:
+            raise ValueError(f"codes must be contiguous, 16-byte aligned int8 [..., {kp}], got {tuple(codes.shape)} "
+                             f"{codes.dtype}")
+        if scales.dtype != torch.float32 or scales.shape != codes.shape[:-1] or not scales.is_contiguous():
+            raise ValueError(f"scales must be contiguous float32 {tuple(codes.shape[:-1])}, got {tuple(scales.shape)} "
+                             f"{scales.dtype}")
+        if type(codes) not in PLAIN_TENSORS or type(scales) not in PLAIN_TENSORS:
+            raise TypeError("codes and scales must be plain tensors")
+        if scales.device != codes.device:
+            raise ValueError("codes and scales must be on one device")
+        # (calls rely on what was checked here: the parts stay as they are)
+        for name, value in zip(self.__slots__, (codes, scales, k, dtype)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"an Int8's {name} is fixed; make another Int8")
+
+    def __reduce__(self):                      # copies and pickles go through the checks again
+        return Int8, tuple(getattr(self, name) for name in self.__slots__)
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((*self.scales.shape, self.k))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def rows(self, start, stop) -> "Int8":
+        """Rows [start, stop) of a matrix [n, k], sharing its memory."""
+        return Int8(self.codes[start:stop], self.scales[start:stop], self.k, self.dtype)
+
+
+def _new_int8(like, lead, k, dtype):
+    """An Int8 for a kernel to fill, without the constructor's checks."""
+    q = object.__new__(Int8)
+    set_ = object.__setattr__
+    set_(q, "codes", like.new_empty((*lead, -(-k // _INT8_PAD) * _INT8_PAD), dtype=torch.int8))
+    set_(q, "scales", like.new_empty(lead, dtype=torch.float32))
+    set_(q, "k", k)
+    set_(q, "dtype", dtype)
+    return q
+
+
+def _int8_call(name, *ts):
+    """What a raw launch cannot take: subclasses, recorded gradients, forward-mode derivatives, tracing."""
+    for t in ts:
+        if t is not None and type(t) not in PLAIN_TENSORS:
+            raise TypeError(f"{name} takes plain tensors, got {type(t).__name__}")
+    if torch.is_grad_enabled():
+        _no_grad_recorded(name, *ts)
+    if torch.autograd.forward_ad._current_level >= 0:
+        _no_dual(name, *ts)
+    if torch._C._is_tracing():
+        _not_traced(name)
+
+
+def _is_int8(name, what, q):
+    if type(q) is not Int8:
+        raise TypeError(f"{name}: {what} must be an Int8 (quantize_int8, add_rmsnorm_int8, pack_int8), got "
+                        f"{type(q).__name__}")
+
+
+def pack_int8(codes, scales, dtype=torch.float32):
+    """codes [..., k] int8 and scales [...] float32, finite, as an Int8 (a copy).  Works on any device; a scale that is
+    not finite raises (which waits for the device)."""
+    if codes.dtype != torch.int8 or codes.dim() < 1:
+        raise ValueError(f"codes must be int8 [..., k], got {tuple(codes.shape)} {codes.dtype}")
+    if scales.dtype != torch.float32 or scales.shape != codes.shape[:-1]:
+        raise ValueError(f"scales must be float32 {tuple(codes.shape[:-1])}, got {tuple(scales.shape)} {scales.dtype}")
+    k = codes.shape[-1]
+    if not 1 <= k <= INT8_MAX_K:
+        raise ValueError(f"int8 rows have 1..{INT8_MAX_K} columns, got {k}")
+    scales = scales.detach()
+    if not bool(torch.isfinite(scales).all()):
+        raise ValueError("scales hold infinities or NaN")
+    full = codes.new_zeros((*codes.shape[:-1], -(-k // _INT8_PAD) * _INT8_PAD))
+    full[..., :k] = codes
+    return Int8(full, scales.clone(memory_format=torch.contiguous_format), k, dtype)
+
+
+def quantize_int8(x):
+    """Rows of x [..., k] (float32 or bfloat16) as an Int8 of x's type (mtl_quantize_int8): code = the whole number
+    nearest to 127 x / max |x| of the row, halves to the even one.  A row of zeros has scale 0; one with an infinity or
+    NaN has scale NaN, and every product with it is NaN."""
+    dt, shape = x.dtype, x.shape
+    code = _ACT_DTYPES.get(dt)
+    if code is None:
+        raise TypeError(f"x must be float32 or bfloat16, got {dt}")
+    if not shape or not 1 <= shape[-1] <= INT8_MAX_K:
+        raise ValueError(f"x must be [..., 1 <= k <= {INT8_MAX_K}], got {tuple(shape)}")
+    _int8_call("quantize_int8", x)
+    k = shape[-1]
+    if x.is_contiguous():
+        M, ldx = x.numel() // k, k
+    else:
+        x, ldx = _rows_of(x, k)
+        M = x.shape[0]
+    with _dev_guard(x):
+        q = _new_int8(x, shape[:-1], k, dt)
+        rc = _lib.load().mtl_quantize_int8(x.data_ptr(), ldx, q.codes.data_ptr(), q.scales.data_ptr(), M, k, code,
+                                           _stream(x))
+    if rc:
+        _lib.check(rc, "quantize_int8")
+    return q
+
+
+def add_rmsnorm_int8(x, weight, eps, y=None, x_out=None, dtype=torch.float32):
+    """weight * rmsnorm(x + y) over rows [..., k] as an Int8 of `dtype` (mtl_add_rmsnorm_int8); x_out (may be x) receives
+    x + y.  x and x_out contiguous float32, y (may be None) contiguous float32 or bfloat16 of x's shape, weight [k]
+    float32 or bfloat16.  The codes are those of the float32 row (x + y) weight; the norm's factor goes into its scale."""
+    shape = x.shape
+    if x.dtype != torch.float32 or not x.is_contiguous() or not shape:
+        raise ValueError("x must be contiguous float32 [..., k]")
+    k = shape[-1]
+    if not 1 <= k <= INT8_MAX_K:
+        raise ValueError(f"x must be [..., 1 <= k <= {INT8_MAX_K}], got {tuple(shape)}")
+    if dtype not in _ACT_DTYPES:
+        raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
+    w_code = _ACT_DTYPES.get(weight.dtype)
+    if w_code is None or weight.shape != (k,) or not weight.is_contiguous():
+        raise ValueError(f"weight must be contiguous float32 or bfloat16 [{k}], got {tuple(weight.shape)} {weight.dtype}")
+    y_code = _lib.MTL_F32
+    if y is not None:
+        y_code = _ACT_DTYPES.get(y.dtype)
+        if y_code is None or y.shape != shape or not y.is_contiguous():
+            raise ValueError(f"y must be contiguous float32 or bfloat16 {tuple(shape)}, got {tuple(y.shape)} {y.dtype}")
+    if x_out is not None:
+        if x_out.shape != shape or x_out.dtype != torch.float32 or not x_out.is_contiguous():
+            raise ValueError(f"x_out must be contiguous float32 {tuple(shape)}")
+        for t in (x, y, weight):
+            # (x or a float y itself is read before it is written)
+            if t is not None and (t.data_ptr() != x_out.data_ptr() or t.dtype != torch.float32 or t is weight) and \
+                    _overlap(x_out, t):
+                raise ValueError("x_out must be x, a float32 y, or overlap no operand")
+    _int8_call("add_rmsnorm_int8", x, weight, y, x_out)
+    _same_device(x, weight, y, x_out)
+    with _dev_guard(x):
+        q = _new_int8(x, shape[:-1], k, dtype)
+        a = _lib.AddRmsnormInt8Args(x.data_ptr(), _ptr(y), _ptr(x_out), weight.data_ptr(), q.codes.data_ptr(),
+                                    q.scales.data_ptr(), x.numel() // k, k, float(eps), y_code, w_code, 0)
+        rc = _lib.load().mtl_add_rmsnorm_int8(ctypes.byref(a), _stream(x))
+    if rc:
+        _lib.check(rc, "add_rmsnorm_int8")
+    return q
+
+
+def linear_int8(x, w, bias=None, out=None):
+    """x [..., k] W^T (+ bias [n]) of an Int8 x and an Int8 matrix W [n, k] (mtl_linear_int8): [..., n] of x's type.  The
+    sum over k is exact; it is multiplied by the two scales in float32.  bias and out have x's type."""
+    _is_int8("linear_int8", "x", x)
+    _is_int8("linear_int8", "w", w)
+    k, dt, lead = x.k, x.dtype, x.scales.shape
+    if w.k != k or w.scales.dim() != 1:
+        raise ValueError(f"w must be [n, {k}], got {tuple(w.shape)}")
+    n, M = w.scales.shape[0], x.scales.numel()
+    if n < 1:
+        raise ValueError("w has no rows")
+    codes = x.codes
+    if codes.get_device() != w.codes.get_device():
+        raise RuntimeError(f"all operands must be on one device, got x on {x.device}, w on {w.device}")
+    if bias is not None:
+        if bias.dtype != dt:
+            raise TypeError(f"bias must be {dt} like x, got {bias.dtype}")
+        if bias.shape != (n,) or not bias.is_contiguous():
+            raise ValueError(f"bias must be contiguous [{n}], got {tuple(bias.shape)}")
+        _same_device(codes, bias)
+    _int8_call("linear_int8", bias, out)
+    ldy = n
+    if out is not None:
+        if out.dtype != dt:
+            raise TypeError(f"out must be {dt} like x, got {out.dtype}")
+        if tuple(out.shape) != (*lead, n) or not (out.is_contiguous() or (
+                out.dim() == 2 and (n == 1 or out.stride(1) == 1) and out.stride(0) >= n)):
+            raise ValueError(f"out must be {(*lead, n)} with contiguous rows, got {tuple(out.shape)} strides "
+                             f"{out.stride()}")
+        _same_device(codes, out)
+        if any(t is not None and _overlap(out, t) for t in (codes, x.scales, w.codes, w.scales, bias)):
+            raise ValueError("out must not overlap an operand")
+        if out.dim() == 2 and M > 1:
+            ldy = out.stride(0)
+    with _dev_guard(codes):
+        if out is None:
+            out = codes.new_empty((*lead, n), dtype=dt)
+        a = _lib.LinearInt8Args(codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias),
+                                out.data_ptr(), ldy, M, n, k, _ACT_DTYPES[dt], 0)
+        rc = _lib.load().mtl_linear_int8(ctypes.byref(a), _stream(codes))
+    if rc:
+        _lib.check(rc, "linear_int8")
+    return out
+
+
+def dequantize_int8(q, dtype=None, out=None):
+    """The values [..., k] that an Int8 stands for, in its type or `dtype` (mtl_dequantize_int8)."""
+    _is_int8("dequantize_int8", "q", q)
+    dt = q.dtype if dtype is None else dtype
+    if dt not in _ACT_DTYPES:
+        raise TypeError(f"dtype must be float32 or bfloat16, got {dt}")
+    k, lead, codes = q.k, q.scales.shape, q.codes
+    _int8_call("dequantize_int8", out)
+    M, ldo = q.scales.numel(), k
+    if out is not None:
+        if tuple(out.shape) != (*lead, k) or out.dtype != dt or not (out.is_contiguous() or (
+                out.dim() == 2 and (k == 1 or out.stride(1) == 1) and out.stride(0) >= k)):
+            raise ValueError(f"out must be {dt} {(*lead, k)} with contiguous rows, got {tuple(out.shape)} {out.dtype}")
+        _same_device(codes, out)
+        if _overlap(out, codes) or _overlap(out, q.scales):
+            raise ValueError("out must not overlap an operand")
+        if out.dim() == 2 and M > 1:
+            ldo = out.stride(0)
+    with _dev_guard(codes):
+        if out is None:
+            out = codes.new_empty((*lead, k), dtype=dt)
+        rc = _lib.load().mtl_dequantize_int8(codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), ldo, M, k,
+                                             _ACT_DTYPES[dt], _stream(codes))
+    if rc:
+        _lib.check(rc, "dequantize_int8")
+    return out
+
+
 # --------------------------------------------------------------------------- log probabilities
 TOP_MAX = 64              # alternatives per row of token_logprobs
 

@@ -1,0 +1,190 @@
+"""Rows in 8-bit integers on the host: the layout, and what the entry points refuse."""
+import copy
+import ctypes
+import pickle
+
+import pytest
+import torch
+
+from mamba_lite import _lib, ops
+
+
+def _q(*lead, k=40, dtype=torch.float32):
+    g = torch.Generator().manual_seed(0)
+    return ops.pack_int8(torch.randint(-127, 128, (*lead, k), generator=g, dtype=torch.int8),
+                         torch.rand(lead, generator=g) + 0.5, dtype)
+
+
+@pytest.mark.parametrize("lead,k", [((), 1), ((1,), 128), ((3,), 129), ((2, 5), 40), ((0,), 7), ((4,), 777)])
+def test_layout_is_the_documented_one(lead, k):
+    g = torch.Generator().manual_seed(1)
+    codes = torch.randint(-128, 128, (*lead, k), generator=g, dtype=torch.int8)
+    scales = torch.rand(lead, generator=g)
+    q = ops.pack_int8(codes, scales, torch.bfloat16)
+    kp = -(-k // 128) * 128
+    assert tuple(q.codes.shape) == (*lead, kp) and q.codes.is_contiguous()
+    assert torch.equal(q.codes[..., :k], codes) and not bool(q.codes[..., k:].any())
+    assert torch.equal(q.scales, scales) and q.scales.data_ptr() != scales.data_ptr() or scales.numel() == 0
+    assert tuple(q.shape) == (*lead, k) and q.dtype == torch.bfloat16 and q.k == k
+
+
+def test_pack_takes_strided_operands():
+    codes = torch.arange(60, dtype=torch.int8).view(6, 10)
+    scales = torch.arange(12, dtype=torch.float32)
+    q = ops.pack_int8(codes[::2, 1::3], scales[::4])
+    assert torch.equal(q.codes[:, :3], codes[::2, 1::3]) and torch.equal(q.scales, scales[::4])
+
+
+def test_rows_share_memory_and_parts_are_fixed():
+    q = _q(6)
+    r = q.rows(2, 5)
+    assert tuple(r.shape) == (3, 40) and r.codes.data_ptr() == q.codes[2:].data_ptr()
+    for name in ("codes", "scales", "k", "dtype"):
+        with pytest.raises(AttributeError, match="fixed"):
+            setattr(q, name, getattr(q, name))
+    for c in (copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+        assert torch.equal(c.codes, q.codes) and torch.equal(c.scales, q.scales) and c.k == q.k and c.dtype == q.dtype
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(codes=torch.zeros(4, 40)), "int8"),
+    (dict(codes=torch.zeros(4, 40, dtype=torch.uint8)), "int8"),
+    (dict(codes=torch.zeros((), dtype=torch.int8), scales=torch.ones(())), "int8"),
+    (dict(codes=torch.zeros(4, 0, dtype=torch.int8)), "columns"),
+    (dict(codes=torch.zeros(1, 1 << 17, dtype=torch.int8), scales=torch.ones(1)), "columns"),
+    (dict(scales=torch.ones(5)), "scales"),
+    (dict(scales=torch.ones(4, 1)), "scales"),
+    (dict(scales=torch.ones(4, dtype=torch.bfloat16)), "scales"),
+    (dict(scales=torch.tensor([1.0, float("inf"), 1.0, 1.0])), "infinities"),
+    (dict(scales=torch.tensor([1.0, float("nan"), 1.0, 1.0])), "infinities"),
+])
+def test_pack_refuses(change, error):
+    a = dict(codes=torch.zeros(4, 40, dtype=torch.int8), scales=torch.ones(4))
+    a.update(change)
+    with pytest.raises(ValueError, match=error):
+        ops.pack_int8(**a)
+
+
+def test_a_made_up_layout_is_refused():
+    q = _q(6)
+    ops.Int8(q.codes, q.scales, 128)
+    for a in ((q.codes[:5], q.scales, 40), (q.codes, q.scales[:5], 40), (q.codes, q.scales, 129), (q.codes, q.scales, 0),
+              (q.codes.float(), q.scales, 40), (q.codes, q.scales.double(), 40), (q.codes.t(), q.scales, 40),
+              (q.codes[:, :40], q.scales, 40), (torch.zeros(6 * 128 + 1, dtype=torch.int8)[1:].view(6, 128), q.scales, 40)):
+        with pytest.raises(ValueError):
+            ops.Int8(*a)
+    with pytest.raises(TypeError, match="dtype"):
+        ops.Int8(q.codes, q.scales, 40, torch.float16)
+
+
+def test_kernels_need_gpu_tensors():
+    x = torch.zeros(3, 40)
+    for call in (lambda: ops.quantize_int8(x), lambda: ops.add_rmsnorm_int8(x, torch.ones(40), 1e-5),
+                 lambda: ops.linear_int8(_q(3), _q(6)), lambda: ops.dequantize_int8(_q(3))):
+        with pytest.raises(RuntimeError, match="GPU tensors"):
+            call()
+
+
+class _Sub(torch.Tensor):
+    pass
+
+
+def test_quantize_refuses():
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        ops.quantize_int8(torch.zeros(3, 4, dtype=torch.float16))
+    for bad in (torch.zeros(()), torch.zeros(3, 0), torch.zeros(1, 1 << 17)):
+        with pytest.raises(ValueError, match="x must be"):
+            ops.quantize_int8(bad)
+    with pytest.raises(RuntimeError, match="backward"):
+        ops.quantize_int8(torch.zeros(3, 4, requires_grad=True))
+    with pytest.raises(TypeError, match="plain"):
+        ops.quantize_int8(torch.zeros(3, 4).as_subclass(_Sub))
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(x=torch.zeros(3, 8, dtype=torch.bfloat16)), "x must be"),
+    (dict(x=torch.zeros(8, 3).t()), "x must be"),
+    (dict(x=torch.zeros(3, 0), weight=torch.zeros(0)), "x must be"),
+    (dict(weight=torch.ones(7)), "weight"),
+    (dict(weight=torch.ones(8, dtype=torch.float16)), "weight"),
+    (dict(weight=torch.ones(16)[::2]), "weight"),
+    (dict(y=torch.zeros(3, 7)), "y must be"),
+    (dict(y=torch.zeros(3, 8, dtype=torch.float16)), "y must be"),
+    (dict(y=torch.zeros(8, 3).t()), "y must be"),
+    (dict(x_out=torch.zeros(3, 8, dtype=torch.bfloat16)), "x_out"),
+    (dict(x_out=torch.zeros(2, 8)), "x_out"),
+])
+def test_norm_refuses(change, error):
+    a = dict(x=torch.zeros(3, 8), weight=torch.ones(8), eps=1e-5)
+    a.update(change)
+    with pytest.raises(ValueError, match=error):
+        ops.add_rmsnorm_int8(**a)
+
+
+def test_norm_refuses_outputs_over_operands_and_gradients():
+    room = torch.zeros(64)
+    x = room[:24].view(3, 8)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.add_rmsnorm_int8(x, torch.ones(8), 1e-5, x_out=room[8:32].view(3, 8))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.add_rmsnorm_int8(x, room[40:48], 1e-5, x_out=room[40:].view(3, 8))
+    yb = torch.zeros(48, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.add_rmsnorm_int8(x, torch.ones(8), 1e-5, y=yb[:24].view(3, 8), x_out=yb.view(torch.float32).view(3, 8))
+    with pytest.raises(TypeError, match="dtype"):
+        ops.add_rmsnorm_int8(x, torch.ones(8), 1e-5, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="backward"):
+        ops.add_rmsnorm_int8(x, torch.ones(8, requires_grad=True), 1e-5)
+
+
+def test_linear_and_dequantize_refuse():
+    x, w = _q(3), _q(6)
+    for a, kind, error in (
+            ((torch.zeros(3, 40), w), TypeError, "x must be an Int8"), ((x, torch.zeros(6, 40)), TypeError, "w must be"),
+            ((x, _q(6, k=41)), ValueError, r"w must be \[n, 40\]"), ((x, _q(2, 6)), ValueError, "w must be"),
+            ((x, _q(0)), ValueError, "no rows"), ((x, w, torch.zeros(6, dtype=torch.bfloat16)), TypeError, "bias"),
+            ((x, w, torch.zeros(5)), ValueError, "bias"), ((x, w, torch.zeros(12)[::2]), ValueError, "bias"),
+            ((x, w, torch.zeros(6, requires_grad=True)), RuntimeError, "backward"),
+            ((x, w, None, torch.zeros(3, 6, dtype=torch.bfloat16)), TypeError, "out"),
+            ((x, w, None, torch.zeros(3, 5)), ValueError, "out"), ((x, w, None, torch.zeros(6, 3).t()), ValueError, "out"),
+            ((x, w, None, x.scales.expand(6, 3).t()), ValueError, "out")):
+        with pytest.raises(kind, match=error):
+            ops.linear_int8(*a)
+    with pytest.raises(TypeError, match="q must be an Int8"):
+        ops.dequantize_int8(torch.zeros(3, 4))
+    with pytest.raises(TypeError, match="dtype"):
+        ops.dequantize_int8(x, torch.float16)
+    for out in (torch.zeros(3, 41), torch.zeros(3, 40, dtype=torch.bfloat16), torch.zeros(40, 3).t()):
+        with pytest.raises(ValueError, match="out"):
+            ops.dequantize_int8(x, out=out)
+
+
+def test_library_refuses_before_any_launch():
+    lib = _lib.load()
+    some = ctypes.cast(ctypes.create_string_buffer(64), ctypes.c_void_p).value // 16 * 16 + 16
+    refused = lambda rc, text: rc == 1 and text in lib.mtl_last_error()
+    assert refused(lib.mtl_quantize_int8(some, 8, some, some, 1, 0, 0, None), b"K must be")
+    assert refused(lib.mtl_quantize_int8(some, 8, some, some, 1, 1 << 17, 0, None), b"K must be")
+    assert refused(lib.mtl_quantize_int8(some, 8, some, some, -1, 8, 0, None), b"rows must be")
+    assert refused(lib.mtl_quantize_int8(some, 8, some, some, 1, 8, 2, None), b"dtype")
+    assert refused(lib.mtl_quantize_int8(None, 8, some, some, 1, 8, 0, None), b"null")
+    assert refused(lib.mtl_quantize_int8(some, 8, some + 8, some, 1, 8, 0, None), b"aligned")
+    assert refused(lib.mtl_dequantize_int8(some, some, some, 7, 1, 8, 0, None), b"overlap")
+    assert refused(lib.mtl_dequantize_int8(some, None, some, 8, 1, 8, 0, None), b"null")
+    assert lib.mtl_quantize_int8(None, 8, None, None, 0, 8, 0, None) == 0          # no rows: nothing to do
+    assert lib.mtl_dequantize_int8(None, None, None, 8, 0, 8, 0, None) == 0
+    n = _lib.AddRmsnormInt8Args(some, None, None, some, some, some, 1, 8, 1e-5, 0, 0, 0)
+    for name, value, text in (("K", 0, b"K must be"), ("y_dtype", 2, b"y_dtype"), ("w_dtype", 3, b"w_dtype"),
+                              ("w", None, b"null"), ("codes", some + 4, b"aligned"), ("M", 1 << 31, b"rows must be")):
+        bad = _lib.AddRmsnormInt8Args.from_buffer_copy(n)
+        setattr(bad, name, value)
+        assert refused(lib.mtl_add_rmsnorm_int8(ctypes.byref(bad), None), text), name
+    p = _lib.LinearInt8Args(some, some, some, some, None, some, 4, 1, 4, 8, 0, 0)
+    for name, value, text in (("K", 1 << 17, b"K must be"), ("N", 0, b"N must be"), ("N", (1 << 27) + 1, b"N must be"),
+                              ("ldy", 3, b"overlap"), ("dtype", 5, b"dtype"), ("w_scales", None, b"null"),
+                              ("x", some + 8, b"aligned")):
+        bad = _lib.LinearInt8Args.from_buffer_copy(p)
+        setattr(bad, name, value)
+        assert refused(lib.mtl_linear_int8(ctypes.byref(bad), None), text), name
+    for f in (lib.mtl_linear_int8, lib.mtl_add_rmsnorm_int8):
+        assert refused(f(None, None), b"null")
