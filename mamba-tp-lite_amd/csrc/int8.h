@@ -1,0 +1,24 @@
+// The layout of rows in 8-bit integers, shared by int8.hip and int8_linear.hip.
+//
+// A row of K codes takes K rounded up to 128 bytes, zeros past K, so no product needs to know where K ends.  Sums of
+// products of codes are exact in 32 bits: 2^14 K < 2^31 for K < 2^17.
+#pragma once
+
+#include "common.h"
+
+namespace mtl {
+
+constexpr int kInt8Pad = 128;              // bytes that rows are rounded up to
+constexpr int64_t kInt8MaxK = (1 << 17) - 1;
+
+inline int64_t int8_row(int64_t k) { return (k + kInt8Pad - 1) / kInt8Pad * kInt8Pad; }
+inline bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+inline bool act_dtype(int32_t dtype) { return dtype == MTL_F32 || dtype == MTL_BF16; }
+
+#define MTL_INT8_SIZES(M, K)                                                        \
+    MTL_REQUIRE((M) >= 0 && (M) < (int64_t(1) << 31), "rows must be in [0, 2^31)"); \
+    MTL_REQUIRE((K) >= 1 && (K) <= kInt8MaxK, "K must be in [1, 2^17 - 1]")
+
+typedef int I4 __attribute__((ext_vector_type(4)));
+
+}  // namespace mtl

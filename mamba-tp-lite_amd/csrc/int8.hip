@@ -1,26 +1,28 @@
 // Rows in 8-bit integers (gfx950): floats into codes with a scale for each row, the residual add and RMSNorm with such
-// an output, products of two such matrices, and the floats that they stand for.
+// an output, and the floats that they stand for.  int8_linear.hip multiplies them.
 //   a = max_k |t[k]|,  code[k] = the whole number nearest to 127 t[k] / a (halves to the even one),  scale = a / 127
-//   y[m, n] = bias[n] + sx[m] sw[n] sum_k cx[m, k] cw[n, k]
-//
-// Layout: a row of K codes takes K rounded up to 128 bytes, zeros past K, so no product needs to know where K ends.
-// Sums of products are exact in 32 bits: 2^14 K < 2^31 for K < 2^17.
 
-#include "common.h"
+#include "int8.h"
 
 namespace mtl {
 namespace {
 
-constexpr int kPad = 128;                  // bytes that rows are rounded up to
-constexpr int64_t kMaxK = (1 << 17) - 1;
-
-__host__ __device__ inline int64_t padded(int64_t k) { return (k + kPad - 1) / kPad * kPad; }
-
-typedef int I4 __attribute__((ext_vector_type(4)));
-
 // 127 t / a to the nearest whole number: 127 t is exact in 64 bits, and the quotient's rounding there crosses no border
-// (one that is no half is 2^-33 or more from it)
+// (one that is no half is 2^-33 or more from it).
 __device__ __forceinline__ int code_of(float t, float a) { return (int)rint((double)t * 127.0 / (double)a); }
+
+// The same without 64 bits, for a in [kLeast, kMost] and inv = 127 / a rounded: t inv is off by less than 2e-5, so its
+// rounding is the code unless it comes within kNear of a half h = c + 1/2.  There 127 |t| - h a decides, and is exact:
+// 127 |t| = p + pl in two floats; p and h a are whole multiples of half an ulp of a and 2^10 of those apart at most, pl is
+// 2^-8 of that.
+constexpr float kLeast = 0x1p-90f, kMost = 0x1p120f, kNear = 0.5f - 3e-5f;
+__device__ __forceinline__ float near_code(float t, float a, float q) {
+#pragma clang fp contract(off)
+    const float c = floorf(fabsf(q)), u = fabsf(t), p = 127.f * u, pl = fmaf(127.f, u, -p);
+    const float e = fmaf(-(c + 0.5f), a, p) + pl;
+    const float up = e > 0.f || (e == 0.f && ((int)c & 1)) ? c + 1.f : c;
+    return copysignf(up, t);
+}
 
 struct RowsArgs {
     const void* x;             // [M, ldx]
@@ -28,113 +30,304 @@ struct RowsArgs {
     const void* y;             // [M, K] to add to x, or null
     float* x_out;              // [M, K], x + y, or null
     const void* w;             // [K]
-    int8_t* codes;             // [M, padded(K)]
+    int8_t* codes;             // [M, Kp]
     float* scales;             // [M]
+    int64_t M;
     int K, Kp;
     float eps;
+    bool vec;                  // 16-byte aligned rows (x, y, x_out, w) of whole runs of 8
 };
 
-constexpr int kThreads = 256;
+constexpr int kRun = 8;                    // columns a lane takes at a time
 
-template <typename V, typename F> __device__ __forceinline__ V block_reduce(V v, V* s, F f) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (lane == 0) s[wave] = v;
-    __syncthreads();
-    V r = s[0];
+// a run's first n values (all of them, from a 16-byte boundary, with `vec`); zeros behind
+template <typename T> __device__ __forceinline__ void load_run(const T* p, int n, bool vec, float* v) {
+    if (vec) {
+        const F4v lo = ld4(p), hi = ld4(p + 4);
 #pragma unroll
-    for (int i = 1; i < kThreads / 64; ++i) r = f(r, s[i]);
-    return r;
+        for (int j = 0; j < 4; ++j) { v[j] = lo[j]; v[4 + j] = hi[j]; }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) v[j] = j < n ? Act<T>::load(p + j) : 0.f;
+    }
+}
+template <> __device__ __forceinline__ void load_run<uint16_t>(const uint16_t* p, int n, bool vec, float* v) {
+    if (vec) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { v[2 * j] = __uint_as_float(w[j] << 16); v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) v[j] = j < n ? Act<uint16_t>::load(p + j) : 0.f;
+    }
 }
 
-// One workgroup per row.
-template <typename T, typename Y, typename W, bool NORM>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const RowsArgs p) {
+// a row's scale from its largest magnitude's bits (NaN for a row that holds an infinity or NaN) and the norm's factor
+__device__ __forceinline__ float row_scale(uint32_t most, float r) {
+    return most < 0x7f800000u ? __uint_as_float(most) * r / 127.f : __uint_as_float(0x7fc00000u);
+}
+
+// 8 codes of a row of largest magnitude a, as 8 bytes (exact: a is outside [kLeast, kMost])
+__device__ __forceinline__ uint2 run_codes(const float* t, float a, float inv, bool exact) {
+    float c[kRun];
+    if (exact) {
+#pragma unroll 1
+        for (int j = 0; j < kRun; ++j) c[j] = (float)code_of(t[j], a);
+    } else {
+        bool near = false;
+        float q[kRun];
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+            q[j] = t[j] * inv;
+            c[j] = rintf(q[j]);
+            near |= fabsf(q[j] - c[j]) > kNear;
+        }
+        if (near) {
+#pragma unroll
+            for (int j = 0; j < kRun; ++j)
+                if (fabsf(q[j] - c[j]) > kNear) c[j] = near_code(t[j], a, q[j]);
+        }
+    }
+    uint32_t b[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) b[j / 4] |= ((uint32_t)(int)c[j] & 0xffu) << (8 * (j % 4));
+    return uint2{b[0], b[1]};
+}
+
+// Rows held in registers from one pass over memory: G threads to a row, RU runs of 8 columns to a thread (Kp <= 8 G RU).
+// HBM is the bound.
+template <typename T, typename Y, typename W, bool NORM, int G, int RU>
+__global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_kernel(const RowsArgs p) {
 #pragma clang fp contract(off)
-    __shared__ uint32_t s_max[kThreads / 64];
-    __shared__ float s_sum[kThreads / 64];
-    const int64_t row = blockIdx.x;
+    constexpr int NT = G < 256 ? 256 : G, NW = G / 64;
+    __shared__ uint32_t s_max[NT / 64];
+    __shared__ float s_sum[NT / 64];
+    const int64_t row = (int64_t)blockIdx.x * (NT / G) + threadIdx.x / G;
+    const int t = threadIdx.x % G;
+    if (row >= p.M) return;                                   // (whole wavefronts; G > 64: one row)
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    const Y* y = p.y ? static_cast<const Y*>(p.y) + row * p.K : nullptr;
-    auto stored = [&](int k) { return y ? Act<T>::load(x + k) + Act<Y>::load(y + k) : Act<T>::load(x + k); };
-    auto weighted = [&](float h, int k) { return NORM ? h * Act<W>::load(static_cast<const W*>(p.w) + k) : h; };
+    const bool add = NORM && p.y;
+    float v[RU][kRun], wv[RU][kRun];
+#pragma unroll
+    for (int u = 0; u < RU; ++u) {
+        const int k = (u * G + t) * kRun, kc = min(k, (p.K - 1) / kRun * kRun);
+        load_run(x + kc, p.K - kc, p.vec, v[u]);
+        if constexpr (NORM) load_run(static_cast<const W*>(p.w) + kc, p.K - kc, p.vec, wv[u]);
+    }
+    if (add) {
+        const Y* y = static_cast<const Y*>(p.y) + row * p.K;
+        float yv[RU][kRun];
+#pragma unroll
+        for (int u = 0; u < RU; ++u) {
+            const int k = (u * G + t) * kRun, kc = min(k, (p.K - 1) / kRun * kRun);
+            load_run(y + kc, p.K - kc, p.vec, yv[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < RU; ++u)
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) v[u][j] += yv[u][j];
+    }
     uint32_t most = 0;
     float ss = 0.f;
-    for (int k = threadIdx.x; k < p.K; k += kThreads) {
-        const float h = stored(k);
-        ss = fmaf(h, h, ss);
-        most = max(most, abs_bits(weighted(h, k)));
-    }
-    most = block_reduce(group_umax<64>(most), s_max, [](uint32_t u, uint32_t v) { return max(u, v); });
-    float r = 1.f;
-    if constexpr (NORM)
-        r = rsqrtf(block_reduce(group_sum<64>(ss), s_sum, [](float u, float v) { return u + v; }) / (float)p.K + p.eps);
-    const bool finite = most < 0x7f800000u;
-    const float a = __uint_as_float(most);
-    if (threadIdx.x == 0) p.scales[row] = finite ? a * r / 127.f : __uint_as_float(0x7fc00000u);
-    int8_t* codes = p.codes + row * p.Kp;
-    for (int k = threadIdx.x; k < p.Kp; k += kThreads) {
-        int c = 0;
-        if (k < p.K) {
-            const float h = stored(k);
-            if (p.x_out) p.x_out[row * p.K + k] = h;
-            if (finite && most) c = code_of(weighted(h, k), a);
-        }
-        codes[k] = (int8_t)c;
-    }
-}
-
-template <typename T> __global__ void __launch_bounds__(kThreads)
-dequantize_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out, int64_t ld,
-                  int K, int Kp) {
-    const int64_t row = blockIdx.x;
-    const float s = scales[row];
-    for (int k = threadIdx.x; k < K; k += kThreads) Act<T>::store(out + row * ld + k, (float)codes[row * Kp + k] * s);
-}
-
-struct LinearArgs {
-    const int8_t* x; const float* sx;      // [M, Kp], [M]
-    const int8_t* w; const float* sw;      // [N, Kp], [N]
-    const void* bias;                      // [N] or null
-    void* y;
-    int64_t ldy;
-    int M, N, Kp;
-};
-
-template <typename T> __device__ __forceinline__ float scaled(int acc, float sx, float sw, float bias) {
-    return fmaf((float)acc * sx, sw, bias);
-}
-
-// A wavefront takes 16 x 16 outputs: rows of W as the first operand, so a lane holds 4 neighbouring columns of y.
-template <typename T> __global__ void __launch_bounds__(kThreads) linear_tile_kernel(const LinearArgs p) {
-    const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
-    const int tn = (p.N + 63) / 64;
-    const int64_t n0 = ((int64_t)(blockIdx.x % tn) * 4 + (threadIdx.x >> 6)) * 16;
-    const int m0 = blockIdx.x / tn * 16;
-    if (n0 >= p.N) return;
-    const int8_t* x = p.x + (int64_t)min(m0 + r, p.M - 1) * p.Kp + j * 16;
-    const int8_t* w = p.w + min(n0 + r, (int64_t)p.N - 1) * p.Kp + j * 16;
-    I4 acc = {0, 0, 0, 0};
-    for (int k = 0; k < p.Kp; k += 64)
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const I4*>(w + k), *reinterpret_cast<const I4*>(x + k),
-                                                    acc, 0, 0, 0);
-    const int m = m0 + r;
-    if (m >= p.M) return;
-    const float sx = p.sx[m];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int64_t n = n0 + 4 * j + q;
-        if (n >= p.N) return;
-        const float b = p.bias ? Act<T>::load(static_cast<const T*>(p.bias) + n) : 0.f;
-        Act<T>::store(static_cast<T*>(p.y) + m * p.ldy + n, scaled<T>(acc[q], sx, p.sw[n], b));
+    for (int u = 0; u < RU; ++u) {
+        const int k = (u * G + t) * kRun;
+        if (k < p.K) {
+            if constexpr (NORM) {
+                if (p.x_out) {
+                    float* o = p.x_out + row * p.K + k;
+                    if (p.vec) {
+                        st4(o, F4v{v[u][0], v[u][1], v[u][2], v[u][3]});
+                        st4(o + 4, F4v{v[u][4], v[u][5], v[u][6], v[u][7]});
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < kRun; ++j)
+                            if (k + j < p.K) o[j] = v[u][j];
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) {
+                if constexpr (NORM) {
+                    ss = fmaf(v[u][j], v[u][j], ss);
+                    v[u][j] *= wv[u][j];
+                }
+                most = max(most, abs_bits(v[u][j]));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) v[u][j] = 0.f;
+        }
+    }
+    most = group_umax<64>(most);
+    if constexpr (NORM) ss = group_sum<64>(ss);
+    if constexpr (G > 64) {
+        if (t % 64 == 0) {
+            s_max[t / 64] = most;
+            s_sum[t / 64] = ss;
+        }
+        lds_barrier();
+        most = s_max[0];
+        ss = s_sum[0];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) {
+            most = max(most, s_max[i]);
+            ss += s_sum[i];
+        }
+    }
+    const float r = NORM ? rsqrtf(ss / (float)p.K + p.eps) : 1.f;
+    if (t == 0) p.scales[row] = row_scale(most, r);
+    const bool none = most == 0 || most >= 0x7f800000u;
+    const float a = __uint_as_float(most), inv = 127.f / a;
+    const bool exact = a < kLeast || a > kMost;
+#pragma unroll
+    for (int u = 0; u < RU; ++u) {
+        const int k = (u * G + t) * kRun;
+        if (k < p.Kp) {
+            const uint2 c = none ? uint2{0, 0} : run_codes(v[u], a, inv, exact);
+            *reinterpret_cast<uint2*>(p.codes + row * p.Kp + k) = c;
+        }
     }
 }
 
-bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-bool act(int32_t dtype) { return dtype == MTL_F32 || dtype == MTL_BF16; }
+// Longer rows: one workgroup each, read twice.
+constexpr int kLongThreads = 1024;
+template <typename T, typename Y, typename W, bool NORM>
+__global__ void __launch_bounds__(kLongThreads) quantize_long_kernel(const RowsArgs p) {
+#pragma clang fp contract(off)
+    constexpr int NW = kLongThreads / 64;
+    __shared__ uint32_t s_max[NW];
+    __shared__ float s_sum[NW];
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const Y* y = NORM && p.y ? static_cast<const Y*>(p.y) + row * p.K : nullptr;
+    auto load = [&](int k, float* v) {
+        load_run(x + k, p.K - k, p.vec, v);
+        if (y) {
+            float yv[kRun];
+            load_run(y + k, p.K - k, p.vec, yv);
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) v[j] += yv[j];
+        }
+    };
+    auto weigh = [&](int k, float* v) {
+        if constexpr (NORM) {
+            float wv[kRun];
+            load_run(static_cast<const W*>(p.w) + k, p.K - k, p.vec, wv);
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) v[j] *= wv[j];
+        }
+    };
+    uint32_t most = 0;
+    float ss = 0.f, v[kRun];
+    for (int k = threadIdx.x * kRun; k < p.K; k += kLongThreads * kRun) {
+        load(k, v);
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) ss = fmaf(v[j], v[j], ss);
+        weigh(k, v);
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) most = max(most, abs_bits(v[j]));
+    }
+    most = group_umax<64>(most);
+    ss = group_sum<64>(ss);
+    if (threadIdx.x % 64 == 0) {
+        s_max[threadIdx.x / 64] = most;
+        s_sum[threadIdx.x / 64] = ss;
+    }
+    lds_barrier();
+    most = s_max[0];
+    ss = s_sum[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) {
+        most = max(most, s_max[i]);
+        ss += s_sum[i];
+    }
+    const float r = NORM ? rsqrtf(ss / (float)p.K + p.eps) : 1.f;
+    if (threadIdx.x == 0) p.scales[row] = row_scale(most, r);
+    const bool none = most == 0 || most >= 0x7f800000u;
+    const float a = __uint_as_float(most), inv = 127.f / a;
+    const bool exact = a < kLeast || a > kMost;
+    for (int k = threadIdx.x * kRun; k < p.Kp; k += kLongThreads * kRun) {
+        uint2 c{0, 0};
+        if (k < p.K) {
+            load(k, v);
+            if (NORM && p.x_out) {                            // (x and y, which it may be, are read before)
+#pragma unroll
+                for (int j = 0; j < kRun; ++j)
+                    if (k + j < p.K) p.x_out[row * p.K + k + j] = v[j];
+            }
+            weigh(k, v);
+            if (!none) c = run_codes(v, a, inv, exact);
+        }
+        *reinterpret_cast<uint2*>(p.codes + row * p.Kp + k) = c;
+    }
+}
 
-#define MTL_SIZES(M, K)                                                                                    \
-    MTL_REQUIRE((M) >= 0 && (M) < (int64_t(1) << 31), "rows must be in [0, 2^31)");                        \
-    MTL_REQUIRE((K) >= 1 && (K) <= kMaxK, "K must be in [1, 2^17 - 1]")
+template <typename T, typename Y, typename W, bool NORM> int launch_rows(RowsArgs a, hipStream_t st) {
+    const auto aligned = [](const void* p, size_t step) { return al16(p) && step % 16 == 0; };
+    a.vec = a.K % kRun == 0 && aligned(a.x, a.ldx * sizeof(T)) && (!NORM || (al16(a.y) && al16(a.w) && al16(a.x_out)));
+#define MTL_ROWS(G, RU)                                                                                              \
+    hipLaunchKernelGGL((quantize_kernel<T, Y, W, NORM, G, RU>), dim3((unsigned)((a.M + (G < 256 ? 256 / G : 1) - 1) / \
+                                                                                (G < 256 ? 256 / G : 1))),            \
+                       dim3(G < 256 ? 256 : G), 0, st, a)
+    const bool few = a.M < 1024;
+    if (a.Kp <= 512 && !few) MTL_ROWS(64, 1);
+    else if (a.Kp <= 1024 && !few) MTL_ROWS(64, 2);
+    else if (a.Kp <= 2048 && !few) MTL_ROWS(64, 4);
+    else if (a.Kp <= 2048) MTL_ROWS(256, 1);
+    else if (a.Kp <= 4096) MTL_ROWS(256, 2);
+    else if (a.Kp <= 8192) MTL_ROWS(256, 4);
+    else if (a.Kp <= 16384) MTL_ROWS(512, 4);
+    else hipLaunchKernelGGL((quantize_long_kernel<T, Y, W, NORM>), dim3((unsigned)a.M), dim3(kLongThreads), 0, st, a);
+#undef MTL_ROWS
+    return check_launch(NORM ? "add_rmsnorm_int8" : "quantize_int8");
+}
+
+// A wavefront reads runs of R codes of a row and writes 16 bytes a lane.
+template <typename T, bool VEC> __global__ void __launch_bounds__(256)
+dequantize_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out, int64_t ld,
+                  int64_t M, int K, int Kp) {
+    constexpr int R = VEC ? 16 / (int)sizeof(T) : 1, U = VEC ? 4 : 8;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= M) return;
+    const int k0 = (int)blockIdx.y * (64 * R * U) + (threadIdx.x & 63) * R;
+    const float s = scales[row];
+    const int8_t* c = codes + row * Kp;
+    T* o = out + row * ld;
+    if constexpr (VEC) {
+        uint2 q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = min(k0 + u * 64 * R, Kp - R);
+            if constexpr (R == 4) q[u].x = *reinterpret_cast<const uint32_t*>(c + k);
+            else q[u] = *reinterpret_cast<const uint2*>(c + k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u * 64 * R;
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < R; ++j) f[j] = (float)(int8_t)((j < 4 ? q[u].x : q[u].y) >> (8 * (j & 3))) * s;
+            if (k + R <= K) {
+                if constexpr (R == 4) st4(o + k, F4v{f[0], f[1], f[2], f[3]});
+                else *reinterpret_cast<uint4*>(o + k) = uint4{f32x2_to_bf16x2(f[0], f[1]), f32x2_to_bf16x2(f[2], f[3]),
+                                                              f32x2_to_bf16x2(f[4], f[5]), f32x2_to_bf16x2(f[6], f[7])};
+            } else {
+#pragma unroll
+                for (int j = 0; j < R; ++j)
+                    if (k + j < K) Act<T>::store(o + k + j, f[j]);
+            }
+        }
+    } else {
+        int8_t q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = c[min(k0 + u * 64, Kp - 1)];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (k0 + u * 64 < K) Act<T>::store(o + k0 + u * 64, (float)q[u] * s);
+    }
+}
 
 }  // namespace
 }  // namespace mtl
@@ -143,77 +336,56 @@ extern "C" int mtl_quantize_int8(const void* x, int64_t ldx, int8_t* codes, floa
                                  int32_t dtype, mtl_stream_t stream) {
     using namespace mtl;
     clear_error();
-    MTL_SIZES(M, K);
-    MTL_REQUIRE(act(dtype), "dtype must be MTL_F32 or MTL_BF16");
+    MTL_INT8_SIZES(M, K);
+    MTL_REQUIRE(act_dtype(dtype), "dtype must be MTL_F32 or MTL_BF16");
     if (M == 0) return MTL_OK;
     MTL_REQUIRE(x && codes && scales, "null pointer");
     MTL_REQUIRE(ldx >= 0, "ldx must not be negative");
     MTL_REQUIRE(al16(codes), "codes must be 16-byte aligned");
     RowsArgs a{};
-    a.x = x; a.ldx = ldx; a.codes = codes; a.scales = scales; a.K = (int)K; a.Kp = (int)padded(K);
-    const dim3 grid((unsigned)M), nt(kThreads);
-    if (dtype == MTL_F32) hipLaunchKernelGGL((quantize_kernel<float, float, float, false>), grid, nt, 0, as_stream(stream), a);
-    else hipLaunchKernelGGL((quantize_kernel<uint16_t, float, float, false>), grid, nt, 0, as_stream(stream), a);
-    return check_launch("quantize_int8");
+    a.x = x; a.ldx = ldx; a.codes = codes; a.scales = scales; a.M = M; a.K = (int)K; a.Kp = (int)int8_row(K);
+    return dtype == MTL_F32 ? launch_rows<float, float, float, false>(a, as_stream(stream))
+                            : launch_rows<uint16_t, float, float, false>(a, as_stream(stream));
 }
 
 extern "C" int mtl_add_rmsnorm_int8(const mtl_add_rmsnorm_int8_args* p, mtl_stream_t stream) {
     using namespace mtl;
     clear_error();
     MTL_REQUIRE(p, "null pointer");
-    MTL_SIZES(p->M, p->K);
-    MTL_REQUIRE(act(p->y_dtype) && act(p->w_dtype), "y_dtype and w_dtype must be MTL_F32 or MTL_BF16");
+    MTL_INT8_SIZES(p->M, p->K);
+    MTL_REQUIRE(act_dtype(p->y_dtype) && act_dtype(p->w_dtype), "y_dtype and w_dtype must be MTL_F32 or MTL_BF16");
     if (p->M == 0) return MTL_OK;
     MTL_REQUIRE(p->x && p->w && p->codes && p->scales, "null pointer");
     MTL_REQUIRE(al16(p->codes), "codes must be 16-byte aligned");
     RowsArgs a{};
     a.x = p->x; a.ldx = p->K; a.y = p->y; a.x_out = p->x_out; a.w = p->w; a.codes = p->codes; a.scales = p->scales;
-    a.K = (int)p->K; a.Kp = (int)padded(p->K); a.eps = p->eps;
-    const dim3 grid((unsigned)p->M), nt(kThreads);
-    const bool yb = p->y_dtype == MTL_BF16, wb = p->w_dtype == MTL_BF16;
-#define MTL_NORM8(Y, W) hipLaunchKernelGGL((quantize_kernel<float, Y, W, true>), grid, nt, 0, as_stream(stream), a)
-    if (yb) { if (wb) MTL_NORM8(uint16_t, uint16_t); else MTL_NORM8(uint16_t, float); }
-    else { if (wb) MTL_NORM8(float, uint16_t); else MTL_NORM8(float, float); }
-#undef MTL_NORM8
-    return check_launch("add_rmsnorm_int8");
+    a.M = p->M; a.K = (int)p->K; a.Kp = (int)int8_row(p->K); a.eps = p->eps;
+    const hipStream_t st = as_stream(stream);
+    if (p->y_dtype == MTL_BF16)
+        return p->w_dtype == MTL_BF16 ? launch_rows<float, uint16_t, uint16_t, true>(a, st)
+                                      : launch_rows<float, uint16_t, float, true>(a, st);
+    return p->w_dtype == MTL_BF16 ? launch_rows<float, float, uint16_t, true>(a, st)
+                                  : launch_rows<float, float, float, true>(a, st);
 }
 
 extern "C" int mtl_dequantize_int8(const int8_t* codes, const float* scales, void* out, int64_t ldo, int64_t M, int64_t K,
                                    int32_t dtype, mtl_stream_t stream) {
     using namespace mtl;
     clear_error();
-    MTL_SIZES(M, K);
-    MTL_REQUIRE(act(dtype), "dtype must be MTL_F32 or MTL_BF16");
+    MTL_INT8_SIZES(M, K);
+    MTL_REQUIRE(act_dtype(dtype), "dtype must be MTL_F32 or MTL_BF16");
     if (M == 0) return MTL_OK;
     MTL_REQUIRE(codes && scales && out, "null pointer");
     MTL_REQUIRE(al16(codes), "codes must be 16-byte aligned");
     MTL_REQUIRE(ldo >= K, "rows of out must not overlap");
-    const dim3 grid((unsigned)M), nt(kThreads);
-    if (dtype == MTL_F32)
-        hipLaunchKernelGGL((dequantize_kernel<float>), grid, nt, 0, as_stream(stream), codes, scales, static_cast<float*>(out),
-                           ldo, (int)K, (int)padded(K));
-    else
-        hipLaunchKernelGGL((dequantize_kernel<uint16_t>), grid, nt, 0, as_stream(stream), codes, scales,
-                           static_cast<uint16_t*>(out), ldo, (int)K, (int)padded(K));
+    const bool f32 = dtype == MTL_F32, vec = al16(out) && ldo * (f32 ? 4 : 2) % 16 == 0;
+    const int per = vec ? f32 ? 1024 : 2048 : 512;            // columns of a workgroup
+    const dim3 grid((unsigned)((M + 3) / 4), (unsigned)((K + per - 1) / per)), nt(256);
+#define MTL_DEQ(T, VEC)                                                                                               \
+    hipLaunchKernelGGL((dequantize_kernel<T, VEC>), grid, nt, 0, as_stream(stream), codes, scales, static_cast<T*>(out), ldo, \
+                       M, (int)K, (int)int8_row(K))
+    if (f32) { if (vec) MTL_DEQ(float, true); else MTL_DEQ(float, false); }
+    else { if (vec) MTL_DEQ(uint16_t, true); else MTL_DEQ(uint16_t, false); }
+#undef MTL_DEQ
     return check_launch("dequantize_int8");
-}
-
-extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t stream) {
-    using namespace mtl;
-    clear_error();
-    MTL_REQUIRE(p, "null pointer");
-    MTL_SIZES(p->M, p->K);
-    MTL_REQUIRE(p->N >= 1 && p->N <= int64_t(1) << 27, "N must be in [1, 2^27]");
-    MTL_REQUIRE(act(p->dtype), "dtype must be MTL_F32 or MTL_BF16");
-    if (p->M == 0) return MTL_OK;
-    MTL_REQUIRE(p->x && p->x_scales && p->w && p->w_scales && p->y, "null pointer");
-    MTL_REQUIRE(al16(p->x) && al16(p->w), "codes must be 16-byte aligned");
-    MTL_REQUIRE(p->ldy >= p->N, "rows of y must not overlap");
-    const int64_t tiles = ((p->N + 63) / 64) * ((p->M + 15) / 16);
-    MTL_REQUIRE(tiles < (int64_t(1) << 31), "too many output tiles");
-    const LinearArgs a{p->x, p->x_scales, p->w, p->w_scales, p->bias, p->y, p->ldy, (int)p->M, (int)p->N, (int)padded(p->K)};
-    const dim3 grid((unsigned)tiles), nt(kThreads);
-    if (p->dtype == MTL_F32) hipLaunchKernelGGL((linear_tile_kernel<float>), grid, nt, 0, as_stream(stream), a);
-    else hipLaunchKernelGGL((linear_tile_kernel<uint16_t>), grid, nt, 0, as_stream(stream), a);
-    return check_launch("linear_int8");
 }
