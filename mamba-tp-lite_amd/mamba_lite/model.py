@@ -5,7 +5,8 @@ Same public surface as mamba-tp-lite's mamba_lite/model.py:
   (.prefill / .step / .forward), MambaBlock, MambaLM (.prefill / .step /
   .generate / .from_pretrained), load_hf_state_dict.
 Beside it: LinearW4 and MambaLM.quantize_w4 (projections and lm_head from 4-bit
-codes), MambaLM.score and generate's return_logprobs (log probabilities,
+codes), LinearInt8 and MambaLM.quantize_int8 (their products in 8-bit
+integers), MambaLM.score and generate's return_logprobs (log probabilities,
 entropy and the most probable tokens).
 Parameter names and shapes match the reference, so its state dicts (and HF
 `state-spaces/mamba-*-hf` checkpoints through from_pretrained) load as is.
@@ -298,6 +299,63 @@ class LinearW4(nn.Module):
         return _linear(x, ops.dequantize_w4(w4, x.dtype), bias)
 
 
+class LinearInt8(nn.Module):
+    """nn.Linear whose product runs in 8-bit integers: the weight [out_features, in_features] with a scale per row, made once
+    (ops.Int8), and each row of x with its own, made in every call, or an ops.Int8 that add_rmsnorm_int8 left.  Made from a
+    nn.Linear, or by MambaLM.quantize_int8.  The output has x's type, under autocast too.  There is no derivative: x that
+    records a gradient, transforms and tracing are refused (ops.quantize_int8)."""
+
+    def __init__(self, w: ops.Int8, bias: torch.Tensor | None = None):
+        super().__init__()
+        if w.scales.dim() != 1:
+            raise ValueError(f"a matrix expected, got {tuple(w.shape)}")
+        self.out_features, self.in_features = w.shape
+        for name, t in (("weight", w.codes), ("scales", w.scales), ("bias", bias)):
+            self.register_parameter(name, None if t is None else nn.Parameter(t.detach(), requires_grad=False))
+
+    @classmethod
+    def from_linear(cls, lin: nn.Linear) -> "LinearInt8":
+        if type(lin) is not nn.Linear:
+            raise TypeError(f"a plain nn.Linear expected, got {type(lin).__name__}")
+        return cls(_int8_weight(lin.weight), lin.bias)
+
+    def _apply(self, fn, recurse=True):
+        # the scales move with the module and stay float32 where it is cast: its codes belong to them
+        self.scales = nn.Parameter(self.scales.view(torch.int32), requires_grad=False)
+        try:
+            return super()._apply(fn, recurse)
+        finally:
+            self.scales = nn.Parameter(self.scales.view(torch.float32), requires_grad=False)
+
+    def int8(self, start: int = 0, stop: int | None = None) -> ops.Int8:
+        """Rows [start, stop) of the weight."""
+        return ops.Int8(self.weight[start:stop].detach(), self.scales[start:stop].detach(), self.in_features)
+
+    def rows(self, x, start: int, stop: int) -> torch.Tensor:
+        """Outputs [start, stop) of forward(x)."""
+        x = x if type(x) is ops.Int8 else ops.quantize_int8(x)
+        return ops.linear_int8(x, self.int8(start, stop), None if self.bias is None else self.bias[start:stop])
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+    def forward(self, x) -> torch.Tensor:
+        x = x if type(x) is ops.Int8 else ops.quantize_int8(x)
+        return ops.linear_int8(x, ops.Int8(self.weight, self.scales, self.in_features), self.bias)
+
+
+@torch.no_grad()
+def _int8_weight(w: torch.Tensor) -> ops.Int8:
+    q = ops.quantize_int8(w.detach() if w.dtype == torch.bfloat16 else w.detach().float())
+    if not bool(torch.isfinite(q.scales).all()):
+        raise ValueError("the weight holds infinities or NaN")
+    return q
+
+
+# projections that are not nn.Linear: their steps and prompts run op by op, or through a call of their own
+_QUANTIZED = (LinearW4, LinearInt8)
+
+
 def _skinny_split(K: int, most: int = 16) -> int:
     """The largest split of K into ranges of whole 128-column granules, at
     most `most` parts."""
@@ -414,7 +472,7 @@ class MambaMixer(nn.Module):
         """prefill(); with parts_ok, out_proj of a short prefill may come back
         as _Parts (split-K partial products for the residual add to sum);
         skinny=False keeps every projection on torch's GEMMs."""
-        if type(self.in_proj) is LinearW4 and torch.is_autocast_enabled("cuda"):
+        if type(self.in_proj) in _QUANTIZED and torch.is_autocast_enabled("cuda"):
             # as its steps run: the products from the codes keep x's type, so must the matrices' and x_proj's
             with torch.autocast("cuda", enabled=False):
                 return self._prefill(x, cache, out, parts_ok, skinny)
@@ -428,8 +486,10 @@ class MambaMixer(nn.Module):
             if tuple(out.ssm_state.shape) != (b, Dm, N) or out.ssm_state.dtype != torch.float32 or \
                     not out.ssm_state.is_contiguous():
                 raise ValueError(f"out.ssm_state must be contiguous float32 {(b, Dm, N)}")
-        split = b * l >= SPLIT_PROJ_MIN_TOKENS and type(self.in_proj) is not LinearW4
-        x2 = None if split else _skinny_rows(x, self.in_proj.weight, skinny, self.in_proj.bias)
+        int8 = type(self.in_proj) is LinearInt8               # (x may be an ops.Int8 then)
+        split = b * l >= SPLIT_PROJ_MIN_TOKENS and type(self.in_proj) is not LinearW4 and \
+            not (int8 and not (_plain_modules(self.in_proj, (LinearInt8,)) and _no_global_hooks()))
+        x2 = None if split or int8 else _skinny_rows(x, self.in_proj.weight, skinny, self.in_proj.bias)
         # in_proj with the causal conv as its epilogue (<= 64 tokens)
         fused_conv = x2 is not None and ops.in_proj_conv_prefill_ok(x2, self.in_proj.weight, K)
         if fused_conv:
@@ -439,14 +499,17 @@ class MambaMixer(nn.Module):
             # whole contiguous [b, l, D] rows rather than halves of [b, l, 2D] rows
             # (one product that writes the halves apart where ops.linear_f32 takes it)
             w_in, b_in = self.in_proj.weight, self.in_proj.bias
-            if Dm % 32 == 0 and ops.linear_f32_ok(x, w_in, b_in):
+            if int8:
+                x = x if type(x) is ops.Int8 else ops.quantize_int8(x)
+                xs, z = (self.in_proj.rows(x, r, r + Dm).transpose(1, 2) for r in (0, Dm))          # [b, D, l]
+            elif Dm % 32 == 0 and ops.linear_f32_ok(x, w_in, b_in):
                 xs, z = (t.transpose(1, 2) for t in ops.linear_f32(x, w_in, b_in, n_split=Dm))      # [b, D, l]
             else:
                 xs = F.linear(x, w_in[:Dm], b_in[:Dm] if b_in is not None else None).transpose(1, 2)
                 z = F.linear(x, w_in[Dm:], b_in[Dm:] if b_in is not None else None).transpose(1, 2)
         else:
             xz = (ops.linear_skinny(x2, self.in_proj.weight, self.in_proj.bias).view(b, l, 2 * Dm) if x2 is not None
-                  else _linear_mod(self.in_proj, x) if ops.linear_f32_pays(b * l, 2 * Dm, dm)
+                  else _linear_mod(self.in_proj, x) if not int8 and ops.linear_f32_pays(b * l, 2 * Dm, dm)
                   else self.in_proj(x))                          # [b, l, 2D]
             xs = xz[..., :Dm].transpose(1, 2)                    # [b, D, l] view, D-stride 1
             z = xz[..., Dm:].transpose(1, 2)
@@ -541,7 +604,7 @@ class MambaMixer(nn.Module):
         weight cold in HBM, against the library's GEMM: the mamba-130m width
         9.8 -> 6.0 us, 1.4b 17.8-18.7 -> 15.6-15.8 us."""
         w = self.in_proj.weight
-        if ops.linear_skinny_ok(x_t, w, bias=self.in_proj.bias):
+        if type(self.in_proj) is not LinearInt8 and ops.linear_skinny_ok(x_t, w, bias=self.in_proj.bias):
             return ops.linear_skinny(x_t, w, self.in_proj.bias)
         return self.in_proj(x_t)
 
@@ -568,7 +631,7 @@ class MambaMixer(nn.Module):
         J = R + 2 * self.cfg.d_state
         conv_w, conv_b = self._step_conv()
         w_in = self.in_proj.weight
-        if ops.in_proj_conv_xproj_ok(x_t, w_in, cache.conv_state, conv_w.shape[-1], J, self.in_proj.bias, conv_w,
+        if type(self.in_proj) is not LinearInt8 and ops.in_proj_conv_xproj_ok(x_t, w_in, cache.conv_state, conv_w.shape[-1], J, self.in_proj.bias, conv_w,
                                      conv_b):
             # in_proj, the conv step and the x_proj partials of each channel
             # block in one launch (measured at the mamba-1.4b width, 32 tokens:
@@ -684,17 +747,30 @@ class MambaLM(nn.Module):
         2195) and bf16 at a few rows (1 row 1208 -> 1092, 32 rows 1712 -> 1831).  At the mamba-130m width steps take
         longer (fp32 1 row 321 -> 465 us), and prompts do at both (1024 tokens fp32: 3.0 -> 4.6 ms, 16.2 -> 16.7).
         Graphs captured before refuse to replay.  Returns self."""
+        return self._quantize("quantize_w4", lambda lin: LinearW4.from_linear(lin, group, zero_points, scale_dtype),
+                              "head_w4" if lm_head else None,
+                              lambda w: LinearW4(ops.quantize_w4(w, group, zero_points, scale_dtype)))
+
+    @torch.no_grad()
+    def quantize_int8(self, lm_head: bool = True) -> "MambaLM":
+        """Puts every block's in_proj and out_proj, and with lm_head a copy of the tied embedding for the head, into 8-bit
+        integers (LinearInt8), in place; the embedding itself and the small projections stay as they are.  The norm before
+        an in_proj writes its rows in int8, and an out_proj's input is quantized row by row.  Graphs captured before refuse
+        to replay.  Returns self."""
+        return self._quantize("quantize_int8", LinearInt8.from_linear, "head_int8" if lm_head else None,
+                              lambda w: LinearInt8(_int8_weight(w)))
+
+    def _quantize(self, what, from_linear, head, from_weight) -> "MambaLM":
         for blk in self.layers:
             for name in ("in_proj", "out_proj"):
                 if type(getattr(blk.mixer, name)) is not nn.Linear:
-                    raise TypeError(f"quantize_w4: {name} must be a plain nn.Linear, got "
+                    raise TypeError(f"{what}: {name} must be a plain nn.Linear, got "
                                     f"{type(getattr(blk.mixer, name)).__name__}")
         # (all of them before any is put in: a weight that cannot be quantized leaves the model as it was)
-        new = [(blk.mixer, name, LinearW4.from_linear(getattr(blk.mixer, name), group, zero_points, scale_dtype))
-               for blk in self.layers for name in ("in_proj", "out_proj")]
-        if lm_head:
-            new.append((self, "head_w4", LinearW4(ops.quantize_w4(self.embedding.weight, group, zero_points,
-                                                                  scale_dtype))))
+        new = [(blk.mixer, name, from_linear(getattr(blk.mixer, name))) for blk in self.layers
+               for name in ("in_proj", "out_proj")]
+        if head is not None:
+            new.append((self, head, from_weight(self.embedding.weight)))
         for owner, name, mod in new:
             setattr(owner, name, mod)
         for name in _CALL_PLANS:                 # (they hold the replaced weights' addresses)
@@ -703,11 +779,14 @@ class MambaLM(nn.Module):
         return self
 
     def lm_head(self, x: torch.Tensor) -> torch.Tensor:
-        head = self._modules.get("head_w4")
+        head = self._quantized_head()
         if head is not None:
             return head(x)
         w = self.embedding.weight
         return ops.lm_head(x, w) if ops.lm_head_ok(x, w) else _linear(x, w)
+
+    def _quantized_head(self):
+        return self._modules.get("head_w4") or self._modules.get("head_int8")
 
     def _norm_weight(self, i: int) -> torch.Tensor:
         mod = self.layers[i].norm if i < len(self.layers) else self.norm_f
@@ -721,14 +800,29 @@ class MambaLM(nn.Module):
         with each add fused into the following norm."""
         act = x.dtype
         h = x.float().contiguous()
-        normed = ops.add_rmsnorm(h, self._norm_weight(0), self._eps(0))
+        normed = self._add_norm(0, h, None, act)
         for i in range(len(self.layers)):
-            y = per_layer(i, normed.to(act) if act != torch.float32 else normed)
-            if isinstance(y, _Parts):
-                normed = ops.add_rmsnorm(h, self._norm_weight(i + 1), self._eps(i + 1), y_parts=y.parts, x_out=h)
-            else:
-                normed = ops.add_rmsnorm(h, self._norm_weight(i + 1), self._eps(i + 1), y=y.float().contiguous(),
-                                         x_out=h)
+            normed = self._add_norm(i + 1, h, per_layer(i, normed), act)
+        return normed
+
+    def _add_norm(self, i, h, y, act):
+        """h += y (a mixer's output or _Parts, None: nothing) and the norm of it that layer i, or past the last one the
+        lm_head, takes: in `act`, or as an ops.Int8 for a plain LinearInt8."""
+        kw = {} if y is None else dict(x_out=h)
+        if i < len(self.layers):
+            proj = self.layers[i].mixer.in_proj
+            if type(proj) is LinearInt8 and _plain_modules(proj, (LinearInt8,)) and _no_global_hooks():
+                norm = self.layers[i].norm
+                w = norm.weight if norm.weight.dtype == torch.bfloat16 and norm.weight.is_contiguous() else _f32(norm.weight)
+                if isinstance(y, _Parts):
+                    y = ops.sum_parts(y.parts)
+                with torch.no_grad():
+                    return ops.add_rmsnorm_int8(h, w, norm.eps, y=None if y is None else y.contiguous(), dtype=act, **kw)
+        if isinstance(y, _Parts):
+            kw["y_parts"] = y.parts
+        elif y is not None:
+            kw["y"] = y.float().contiguous()
+        normed = ops.add_rmsnorm(h, self._norm_weight(i), self._eps(i), **kw)
         return normed.to(act) if act != torch.float32 else normed
 
     def prefill(self, input_ids: torch.Tensor, cache: MambaCache | None = None,
@@ -881,8 +975,9 @@ class MambaLM(nn.Module):
         the library's, the conv-step and SSM-update kernels)."""
         lt = self._layer_tensors()
         w4 = len(lt) > 0 and type(self.layers[0].mixer.in_proj) is LinearW4
+        plain = not (len(lt) > 0 and type(self.layers[0].mixer.in_proj) in _QUANTIZED)
         # (the fused step's head is the embedding)
-        if not w4 and "head_w4" not in self._modules and self._fused_step_ok(input_ids, cache, lt=lt):
+        if plain and self._quantized_head() is None and self._fused_step_ok(input_ids, cache, lt=lt):
             return self._step_fused(input_ids, cache, lt=lt)
         x = self.embedding(input_ids).squeeze(1)
         if w4 and BATCHED_STEP_NATIVE:
@@ -891,7 +986,7 @@ class MambaLM(nn.Module):
                 h = x if x.dtype == torch.float32 else x.float()
                 normed = ops.decode_step_w4(*got, h, self.norm_f.weight, self.norm_f.eps, self.cfg, dtype=x.dtype)
                 return self.lm_head(normed).unsqueeze(1)
-        if BATCHED_STEP_NATIVE and not w4:
+        if BATCHED_STEP_NATIVE and plain:
             got = self._batched_step_layers(x, cache, lt)
             if got is not None:
                 arr, fold = got

@@ -1534,6 +1534,8 @@ def _int8_call(name, *ts):
         _no_grad_recorded(name, *ts)
     if torch.autograd.forward_ad._current_level >= 0:
         _no_dual(name, *ts)
+    if torch._C._functorch.peek_interpreter_stack() is not None:
+        raise RuntimeError(f"{name} launches a kernel, which a functorch transform would not see")
     if torch._C._is_tracing():
         _not_traced(name)
 

@@ -230,6 +230,8 @@ class LocalTPLM:
         """Every rank's shard of a dense MambaLM."""
         if getattr(lm, "head_w4", None) is not None:
             raise TypeError("LocalTPLM's lm_head is the embedding: shard the model before quantize_w4")
+        if getattr(lm, "head_int8", None) is not None:
+            raise TypeError("LocalTPLM's lm_head is the embedding: shard the model before quantize_int8")
         blocks = [LocalTPBlock(blk.norm.weight.detach(),
                                LocalTPMixer.from_dense(blk.mixer, world_size, allreduce_dtype, i, naive))
                   for i, blk in enumerate(lm.layers)]

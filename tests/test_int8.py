@@ -188,3 +188,36 @@ def test_library_refuses_before_any_launch():
         assert refused(lib.mtl_linear_int8(ctypes.byref(bad), None), text), name
     for f in (lib.mtl_linear_int8, lib.mtl_add_rmsnorm_int8):
         assert refused(f(None, None), b"null")
+
+
+def test_linear_int8_module_on_the_host():
+    from mamba_lite.model import LinearInt8
+
+    q = LinearInt8(_q(6), torch.zeros(6))
+    assert (q.in_features, q.out_features) == (40, 6) and "in_features=40" in repr(q)
+    s = q.scales.detach().clone()
+    for cast in (lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.double(), lambda m: m.to("cpu", torch.float32)):
+        cast(q)
+        assert q.scales.dtype == torch.float32 and torch.equal(q.scales, s) and q.weight.dtype == torch.int8
+        assert isinstance(q.scales, torch.nn.Parameter) and set(q.state_dict()) == {"weight", "scales", "bias"}
+    p = LinearInt8(_q(6), torch.ones(6))
+    p.load_state_dict(q.state_dict())
+    assert torch.equal(p.bias, q.bias)
+    assert torch.equal(q.int8(2, 5).codes, q.weight[2:5]) and tuple(q.int8().shape) == (6, 40)
+    with pytest.raises(ValueError, match="matrix"):
+        LinearInt8(_q(2, 3))
+
+
+def test_shards_of_an_int8_model_are_refused():
+    from mamba_lite import tp_utils
+    from mamba_lite.model import LinearInt8, MambaConfig, MambaLM
+    from mamba_lite.tp_model import LocalTPLM
+
+    m = MambaLM(MambaConfig(d_model=32, n_layer=1, vocab_size=40))
+    mx = m.layers[0].mixer
+    mx.in_proj, mx.out_proj = LinearInt8(_q(128, k=32)), LinearInt8(_q(32, k=64))
+    with pytest.raises(TypeError, match="quantize_int8"):
+        tp_utils.shard_mixer_tensors({k: v.detach() for k, v in mx.state_dict().items()}, 64, 0, 2)
+    m.head_int8 = LinearInt8(_q(40, k=32))
+    with pytest.raises(TypeError, match="quantize_int8"):
+        LocalTPLM.from_dense(m)
