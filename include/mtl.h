@@ -911,7 +911,8 @@ typedef struct {
     const void* bias;          /* [N] or NULL */
     void* y;
     int64_t ldy, M, N, K;
-    int32_t dtype, reserved;
+    int32_t dtype;
+    int32_t y_f32;             /* 1: y holds floats whatever dtype is */
 } mtl_linear_int8_args;
 
 int mtl_quantize_int8(const void* x, int64_t ldx, int8_t* codes, float* scales, int64_t M, int64_t K, int32_t dtype,
@@ -920,6 +921,32 @@ int mtl_add_rmsnorm_int8(const mtl_add_rmsnorm_int8_args* args, mtl_stream_t str
 int mtl_linear_int8(const mtl_linear_int8_args* args, mtl_stream_t stream);
 int mtl_dequantize_int8(const int8_t* codes, const float* scales, void* out, int64_t ldo, int64_t M, int64_t K,
                         int32_t dtype, mtl_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * mtl_decode_step_int8: mtl_decode_step_w4 for a stack whose in_proj and
+ * out_proj are matrices of the layout above.  Per layer: mtl_linear_int8
+ * (in_proj), the conv step, x_proj's partial products and their ordered sum,
+ * the SSM update, mtl_quantize_int8, mtl_linear_int8 (out_proj, in floats),
+ * mtl_add_rmsnorm_int8 (after the last layer norm_f's, in dtype).
+ *   matrices    [2 n_layers]: in_proj [2 d_inner, d_model] and out_proj
+ *               [d_model, d_inner] of each layer
+ *   args        as mtl_decode_step_w4, but inp [b, d_model rounded up to 128]
+ *               and xn [b, d_inner rounded up to 128] bytes, 16-byte aligned,
+ *               and sq [2 b] floats; counters is not read
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    const int8_t* codes;
+    const float* scales;
+} mtl_int8_matrix;
+
+int mtl_decode_step_int8(const mtl_decode_step_batched_args* args, const mtl_decode_layer* layers,
+                         const mtl_int8_matrix* matrices, int32_t dtype, mtl_stream_t stream);
+
+/* mtl_prefill_long with in_proj and out_proj as such matrices: layers without
+ * W_in and W_out, skinny_rows not read, d_model and d_inner >= 64, xn and u
+ * 16-byte aligned (they hold the rows in int8 as well). */
+int mtl_prefill_long_int8(const mtl_prefill_long_args* args, const mtl_prefill_layer* layers,
+                          const mtl_int8_matrix* matrices, mtl_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Log probabilities of given tokens, with entropy and the most probable

@@ -26,6 +26,8 @@ void clear_error();
 // Checks the launch that was just enqueued.
 int check_launch(const char* what);
 
+inline bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
 inline hipStream_t as_stream(mtl_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
 // ---------------------------------------------------------------- device side

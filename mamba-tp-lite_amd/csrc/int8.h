@@ -12,7 +12,6 @@ constexpr int kInt8Pad = 128;              // bytes that rows are rounded up to
 constexpr int64_t kInt8MaxK = (1 << 17) - 1;
 
 inline int64_t int8_row(int64_t k) { return (k + kInt8Pad - 1) / kInt8Pad * kInt8Pad; }
-inline bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 inline bool act_dtype(int32_t dtype) { return dtype == MTL_F32 || dtype == MTL_BF16; }
 
 #define MTL_INT8_SIZES(M, K)                                                        \

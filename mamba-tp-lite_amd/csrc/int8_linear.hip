@@ -16,6 +16,7 @@ struct LinearArgs {
     int M, N, Kp;
     int tm, tn;                            // tiles along M and N
     bool vec;                              // 16-byte aligned rows of y
+    bool bias_bf16;
 };
 
 // the float of a sum, each factor rounded once
@@ -34,7 +35,7 @@ __device__ __forceinline__ void copy_kilobyte(const int8_t* base, uint32_t off, 
 #endif
 }
 
-// T: y and bias.  A workgroup takes BN columns by BM rows of y, a wavefront WN x WM of them as 16 x 16 MFMA tiles with the
+// T: y.  A workgroup takes BN columns by BM rows of y, a wavefront WN x WM of them as 16 x 16 MFMA tiles with the
 // rows of W as the first operand, so that a lane holds 4 neighbouring columns of y.
 template <typename T, int BN, int BM, int WN, int WM, int ST, int OCC>
 __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_kernel(const LinearArgs a) {
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_ker
     for (int n = threadIdx.x; n < BN; n += NT) {
         const int nc = min(n0 + n, a.N - 1);
         s_sw[n] = a.sw[nc];
-        s_b[n] = a.bias ? Act<T>::load(static_cast<const T*>(a.bias) + nc) : 0.f;
+        s_b[n] = a.bias ? load_param(a.bias, nc, a.bias_bf16) : 0.f;
     }
     lds_barrier();
     const int nw = n0 + wn * WN;
@@ -237,7 +238,7 @@ template <typename T, int NW> __global__ void __launch_bounds__(NW * 64) stream_
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const int nc = min(n + q, a.N - 1);
-        v[q] = scaled(acc[q], sx, a.sw[nc], a.bias ? Act<T>::load(static_cast<const T*>(a.bias) + nc) : 0.f);
+        v[q] = scaled(acc[q], sx, a.sw[nc], a.bias ? load_param(a.bias, nc, a.bias_bf16) : 0.f);
     }
     if (a.vec && n + 4 <= a.N) {
         st4(y, v);
@@ -281,9 +282,9 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     MTL_REQUIRE(p->x && p->x_scales && p->w && p->w_scales && p->y, "null pointer");
     MTL_REQUIRE(al16(p->x) && al16(p->w), "codes must be 16-byte aligned");
     MTL_REQUIRE(p->ldy >= p->N, "rows of y must not overlap");
-    const bool f32 = p->dtype == MTL_F32;
+    const bool f32 = p->dtype == MTL_F32 || p->y_f32;
     LinearArgs a{p->x, p->x_scales, p->w, p->w_scales, p->bias, p->y, p->ldy, (int)p->M, (int)p->N, (int)int8_row(p->K),
-                 0, 0, al16(p->y) && p->ldy * (f32 ? 4 : 2) % 16 == 0};
+                 0, 0, al16(p->y) && p->ldy * (f32 ? 4 : 2) % 16 == 0, p->dtype == MTL_BF16};
     const hipStream_t st = as_stream(stream);
     // Few rows: the stream.  us at rows x N x K, bf16: 1x768x1536 3.0, tiles of 32 4.2; 64x768x1536 3.7 / 4.3, 128x768x1536
     // 5.5 / 4.4; 1x8192x2048 5.3 / 5.6, 32x8192x2048 9.7 / 5.9.  Eight wavefronts on long rows: 1x2048x4096 4.8, four 5.1;

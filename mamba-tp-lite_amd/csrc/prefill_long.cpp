@@ -51,6 +51,7 @@
 
 #include "common.h"
 #include "gemm.h"
+#include "int8.h"
 
 namespace {
 
@@ -159,13 +160,11 @@ int32_t rows_per_block_of(int64_t M, int64_t N, int32_t ksplit) {
     return (M > 16 && M <= 32 && (N + 31) / 32 * ksplit >= 256) ? 32 : 16;
 }
 
-}  // namespace
-
-extern "C" int mtl_prefill_long(const mtl_prefill_long_args* a, const mtl_prefill_layer* layers,
-                                mtl_stream_t stream) {
+// `mats`: in_proj and out_proj of each layer in 8-bit integers, in place of W_in and W_out (null: none).  The rows that go
+// into them then stand in xn and u, codes first, which are free where they are written.
+int prefill_long(const mtl_prefill_long_args* a, const mtl_prefill_layer* layers, const mtl_int8_matrix* mats,
+                 mtl_stream_t stream) {
     using namespace mtl;
-    clear_error();
-    MTL_REQUIRE(a && layers, "null args or layers");
     const int64_t b = a->batch, l = a->seqlen, M = a->d_model, D = a->d_inner, N = a->d_state, R = a->dt_rank;
     const int64_t rows = b * l, J = R + 2 * N;
     const int32_t K = a->d_conv;
@@ -184,17 +183,21 @@ extern "C" int mtl_prefill_long(const mtl_prefill_long_args* a, const mtl_prefil
     // nothing half written
     for (int32_t i = 0; i < a->n_layers; ++i) {
         const mtl_prefill_layer& L = layers[i];
-        MTL_REQUIRE(L.norm_w && L.W_in && L.conv_w && L.W_x && L.W_dt && L.A_log && L.W_out && L.h_out &&
+        MTL_REQUIRE(L.norm_w && (mats || (L.W_in && L.W_out)) && L.conv_w && L.W_x && L.W_dt && L.A_log && L.h_out &&
                     (K == 1 || L.conv_state_out), "layer " + std::to_string(i) + ": null required pointer");
         MTL_REQUIRE(K == 1 || L.conv_state_in != L.conv_state_out,
                     "layer " + std::to_string(i) + ": conv_state_out must not alias conv_state_in");
+        for (int j = 0; mats && j < 2; ++j)
+            MTL_REQUIRE(mats[2 * i + j].codes && mats[2 * i + j].scales && al16(mats[2 * i + j].codes),
+                        "layer " + std::to_string(i) + ": codes and scales must be there, codes 16-byte aligned");
     }
+    MTL_REQUIRE(!mats || (M >= 64 && D >= 64 && al16(a->xn) && al16(a->u)),
+                "d_model and d_inner must be >= 64, xn and u 16-byte aligned");
     // the skinny form: sizes and alignments the skinny GEMMs and the fused
     // x_proj sum + dt_proj take, on every layer, and room for the parts
     constexpr int32_t kOutSplit = 4;
     const int32_t xs = split_of(D, 16);
-    auto al16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    bool skinny = a->skinny_rows > 0 && rows <= a->skinny_rows && M % 128 == 0 && D % (128 * kOutSplit) == 0 &&
+    bool skinny = !mats && a->skinny_rows > 0 && rows <= a->skinny_rows && M % 128 == 0 && D % (128 * kOutSplit) == 0 &&
                   J % 4 == 0 && R <= 160 && al16(a->xn) && al16(a->u) && al16(a->y) && al16(a->xz) &&
                   al16(a->blas_ws) && (int64_t)xs * J * rows < (int64_t(1) << 31) &&
                   (int64_t)(xs * J + kOutSplit * M) * rows * (int64_t)sizeof(float) <= a->blas_ws_bytes;
@@ -209,10 +212,10 @@ extern "C" int mtl_prefill_long(const mtl_prefill_long_args* a, const mtl_prefil
     // call may use it between that norm and the in_proj.
     const int64_t xb = (split_bytes(rows, M) + 1023) / 1024 * 1024, in_bytes = xb + split_bytes(2 * D, M);
     const int64_t yb = (split_bytes(rows, D) + 1023) / 1024 * 1024, out_bytes = yb + split_bytes(M, D);
-    const bool split_in = !skinny && split_pays(rows, 2 * D, M) && in_bytes <= a->blas_ws_bytes && al16(a->blas_ws);
+    const bool split_in = !mats && !skinny && split_pays(rows, 2 * D, M) && in_bytes <= a->blas_ws_bytes && al16(a->blas_ws);
     bool norm_splits = split_in && norm_split_ok(a->h, a->out, nullptr, a->xn, M);
     for (int32_t i = 0; norm_splits && i < a->n_layers; ++i) norm_splits = al16(layers[i].norm_w);
-    const bool split_out = !skinny && split_pays(rows, M, D) && out_bytes <= a->blas_ws_bytes && al16(a->blas_ws);
+    const bool split_out = !mats && !skinny && split_pays(rows, M, D) && out_bytes <= a->blas_ws_bytes && al16(a->blas_ws);
     uint8_t* sws = static_cast<uint8_t*>(a->blas_ws);
     float* x_parts = static_cast<float*>(a->blas_ws);                 // [xs, rows, J]
     float* y_parts = x_parts + (int64_t)xs * rows * J;                 // [4, rows, M]
@@ -225,9 +228,21 @@ extern "C" int mtl_prefill_long(const mtl_prefill_long_args* a, const mtl_prefil
     std::lock_guard<std::mutex> lock(g_mu);
     void* ws = a->blas_ws;
     const size_t wsb = (size_t)std::min<int64_t>(a->blas_ws_bytes, kBlasWs);
+    int8_t *xq = reinterpret_cast<int8_t*>(a->xn), *yq = reinterpret_cast<int8_t*>(a->u);
+    float* xq_s = reinterpret_cast<float*>(xq + rows * int8_row(M));
+    float* yq_s = reinterpret_cast<float*>(yq + rows * int8_row(D));
+    auto linear8 = [&](const int8_t* x, const float* s, const mtl_int8_matrix& m, const float* bias, float* y, int64_t n,
+                       int64_t k) {
+        const mtl_linear_int8_args g{x, s, m.codes, m.scales, bias, y, n, rows, n, k, MTL_F32, 1};
+        return mtl_linear_int8(&g, stream);
+    };
     // norm i's output feeds layer i's in_proj
     auto norm = [&](int32_t i, const float* y) {
         const mtl_prefill_layer& L = layers[i];
+        if (mats) {
+            const mtl_add_rmsnorm_int8_args n{a->h, y, y ? a->h : nullptr, L.norm_w, xq, xq_s, rows, M, L.eps, MTL_F32, MTL_F32, 0};
+            return mtl_add_rmsnorm_int8(&n, stream);
+        }
         if (norm_splits)
             return norm_split(a->h, y, y ? a->h : nullptr, L.norm_w, L.eps, a->xn, rows, M, L.W_in, M, 2 * D, sws,
                               sws + xb, st);
@@ -238,7 +253,9 @@ extern "C" int mtl_prefill_long(const mtl_prefill_long_args* a, const mtl_prefil
     if (rc) return rc;
     for (int32_t i = 0; i < a->n_layers; ++i) {
         const mtl_prefill_layer& L = layers[i];
-        if (skinny)
+        if (mats)
+            rc = linear8(xq, xq_s, mats[2 * i], L.b_in, a->xz, 2 * D, M);
+        else if (skinny)
             rc = mtl_linear_skinny(a->xn, M, L.W_in, L.b_in, a->xz, 2 * D, 0, rows, 2 * D, M, 1,
                                    rows_per_block_of(rows, 2 * D, 1), stream);
         else if (split_in) {
@@ -297,7 +314,10 @@ extern "C" int mtl_prefill_long(const mtl_prefill_long_args* a, const mtl_prefil
             if (rc) return rc;
             rc = mtl_add_rmsnorm_parts(a->h, y_parts, kOutSplit, a->h, w_next, normed, rows, M, eps, stream);
         } else {
-            if (split_out) {
+            if (mats) {
+                if ((rc = mtl_quantize_int8(a->y, D, yq, yq_s, rows, D, MTL_F32, stream))) return rc;
+                rc = linear8(yq, yq_s, mats[2 * i + 1], L.b_out, a->out, M, D);
+            } else if (split_out) {
                 SplitGemm g{};
                 g.x = a->y; g.ldx = D; g.w = L.W_out; g.ldw = D; g.bias = L.b_out; g.y0 = a->out; g.ldy0 = M;
                 g.M = rows; g.N = M; g.K = D; g.xbuf = sws; g.wbuf = sws + yb;
@@ -313,4 +333,21 @@ extern "C" int mtl_prefill_long(const mtl_prefill_long_args* a, const mtl_prefil
         if (rc) return rc;
     }
     return MTL_OK;
+}
+
+}  // namespace
+
+extern "C" int mtl_prefill_long(const mtl_prefill_long_args* a, const mtl_prefill_layer* layers, mtl_stream_t stream) {
+    using namespace mtl;
+    clear_error();
+    MTL_REQUIRE(a && layers, "null args or layers");
+    return prefill_long(a, layers, nullptr, stream);
+}
+
+extern "C" int mtl_prefill_long_int8(const mtl_prefill_long_args* a, const mtl_prefill_layer* layers,
+                                     const mtl_int8_matrix* matrices, mtl_stream_t stream) {
+    using namespace mtl;
+    clear_error();
+    MTL_REQUIRE(a && layers && matrices, "null args, layers or matrices");
+    return prefill_long(a, layers, matrices, stream);
 }

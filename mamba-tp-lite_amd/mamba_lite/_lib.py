@@ -160,8 +160,13 @@ class LinearInt8Args(ctypes.Structure):
     """mirror of mtl_linear_int8_args"""
     _fields_ = [
         ("x", _vp), ("x_scales", _vp), ("w", _vp), ("w_scales", _vp), ("bias", _vp), ("y", _vp),
-        ("ldy", _i64), ("M", _i64), ("N", _i64), ("K", _i64), ("dtype", _i32), ("reserved", _i32),
+        ("ldy", _i64), ("M", _i64), ("N", _i64), ("K", _i64), ("dtype", _i32), ("y_f32", _i32),
     ]
+
+
+class Int8Matrix(ctypes.Structure):
+    """mirror of mtl_int8_matrix"""
+    _fields_ = [("codes", _vp), ("scales", _vp)]
 
 
 # name -> (restype, argtypes); every symbol of include/mtl.h
@@ -227,6 +232,10 @@ SIGNATURES = {
     "mtl_add_rmsnorm_int8": (ctypes.c_int, [ctypes.POINTER(AddRmsnormInt8Args), _vp]),
     "mtl_linear_int8": (ctypes.c_int, [ctypes.POINTER(LinearInt8Args), _vp]),
     "mtl_dequantize_int8": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "mtl_decode_step_int8": (ctypes.c_int, [ctypes.POINTER(DecodeStepBatchedArgs), ctypes.POINTER(DecodeLayer),
+                                            ctypes.POINTER(Int8Matrix), _i32, _vp]),
+    "mtl_prefill_long_int8": (ctypes.c_int, [ctypes.POINTER(PrefillLongArgs), ctypes.POINTER(PrefillLayer),
+                                             ctypes.POINTER(Int8Matrix), _vp]),
     "mtl_token_logprobs": (ctypes.c_int, [ctypes.POINTER(TokenLogprobsArgs), _vp]),
 }
 

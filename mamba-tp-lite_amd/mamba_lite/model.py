@@ -712,12 +712,12 @@ class MambaBlock(nn.Module):
         return x_t + self.mixer.step(self.norm(x_t), cache)
 
 
-_CALL_PLANS = frozenset(("_short_plan", "_batched_tmpl", "_w4_tmpl", "_plan", "_step_tmpl", "_fused_memo", "_persist_tab",
+_CALL_PLANS = frozenset(("_short_plan", "_batched_tmpl", "_quant_tmpl", "_plan", "_step_tmpl", "_fused_memo", "_persist_tab",
                          "_persist_ws"))
 
 # what a MambaLM's layers are made of, and nothing else of, where _plain_stack holds
 _STACK_MODULES = frozenset((nn.ModuleList, MambaBlock, MambaMixer, RMSNorm, nn.Linear, nn.Conv1d))
-_W4_STACK_MODULES = _STACK_MODULES | {LinearW4}
+_QUANT_STACK_MODULES = {cls: _STACK_MODULES | {cls} for cls in _QUANTIZED}
 
 
 class MambaLM(nn.Module):
@@ -894,6 +894,38 @@ class MambaLM(nn.Module):
         self._short_plan = (key, arr)
         return arr
 
+    def _int8_prefill_plan(self):
+        """_short_prefill_plan() and the projections' matrices of a stack in 8-bit integers, or (None, None) when a
+        projection is not a LinearInt8 of its shape, or another weight or a bias no contiguous float32 tensor, on the
+        embedding's device."""
+        cfg, dev = self.cfg, self.embedding.weight.device
+        lt = self._layer_tensors()
+        ip, op = _LT_W_IN, _LT_W_OUT
+        proj = [p for blk in self.layers for p in (blk.mixer.in_proj, blk.mixer.out_proj)]
+        ws = [t for ts in lt for i, t in enumerate(ts) if i not in (ip, op)] + [self.norm_f.weight]
+        key = tuple(0 if t is None else t.data_ptr() for ts in lt for t in ts) + self._norm_eps() + \
+            tuple((p.scales.data_ptr(), p.out_features, p.in_features) if type(p) is LinearInt8 else None for p in proj) + \
+            (self.norm_f.weight.data_ptr(),)
+        plan = getattr(self, "_short_plan", None)
+        if plan is not None and plan[0] == key:
+            return plan[1]
+        got = None, None
+        if all(type(p) is LinearInt8 and p.weight.device == dev and (p.out_features, p.in_features) == shape
+               for p, shape in zip(proj, len(lt) * [(2 * cfg.d_inner, cfg.d_model), (cfg.d_model, cfg.d_inner)])) and \
+                all(t is None or (t.device == dev and t.dtype == torch.float32 and t.is_contiguous()) for t in ws):
+            arr, mats = (_lib.PrefillLayer * len(lt))(), (_lib.Int8Matrix * (2 * len(lt)))()
+            for i, L in enumerate(arr):
+                (L.norm_w, L.W_in, L.b_in, L.conv_w, L.conv_b, L.W_x, L.W_dt, L.dt_bias, L.A_log, L.Dv, L.W_out,
+                 L.b_out) = key[12 * i:12 * i + 12]
+                L.W_in = L.W_out = 0
+                L.eps = self.layers[i].norm.eps
+            for p, m in zip(proj, mats):
+                w = p.int8()                                 # (its checks: layout, types, alignment)
+                m.codes, m.scales = w.codes.data_ptr(), w.scales.data_ptr()
+            got = arr, mats
+        self._short_plan = (key, got)
+        return got
+
     def _plain_stack(self) -> bool:
         """Whether the blocks are nothing but their launches: no module of
         another class in them (an adapter, a parametrization), no hooks or
@@ -924,7 +956,15 @@ class MambaLM(nn.Module):
         kind = self._native_prefill_kind(b, l)
         if kind is None or self.embedding.weight.dtype != torch.float32:
             return None
-        if b * l * D > LONG_PREFILL_PLAIN_ELEMS and not self._plain_stack():
+        int8 = len(self.layers) > 0 and type(self.layers[0].mixer.in_proj) is LinearInt8
+        if int8:
+            if not (ops.plain_call() and _no_global_hooks() and min(cfg.d_model, D) >= 64 and
+                    _plain_modules(self.layers, _QUANT_STACK_MODULES[LinearInt8])):
+                return None
+            kind = "long" if LONG_PREFILL_NATIVE and ops.prefill_long_ok(b, l, cfg.d_model, D, N, cfg.dt_rank, K) else None
+            if kind is None:
+                return None
+        elif b * l * D > LONG_PREFILL_PLAIN_ELEMS and not self._plain_stack():
             return None
         for c in (cache, out_cache):
             if c is not None and not all(
@@ -932,7 +972,7 @@ class MambaLM(nn.Module):
                     lc.conv_state.is_contiguous() and tuple(lc.ssm_state.shape) == (b, D, N) and
                     lc.ssm_state.dtype == torch.float32 and lc.ssm_state.is_contiguous() for lc in c.layers):
                 return None
-        tmpl = self._short_prefill_plan()
+        tmpl, mats = self._int8_prefill_plan() if int8 else (self._short_prefill_plan(), None)
         if tmpl is None:
             return None
         # a copy per call: the library reads it while ctypes has released the
@@ -962,7 +1002,7 @@ class MambaLM(nn.Module):
             skinny = LONG_PREFILL_SKINNY_ROWS if cfg.d_model <= LONG_PREFILL_SKINNY_MAX_D_MODEL else 0
             try:
                 normed = ops.prefill_long(h, arr, self.norm_f.weight, self.norm_f.eps, D, N, cfg.dt_rank, K,
-                                          skinny_rows=skinny)
+                                          skinny_rows=skinny, matrices=mats)
             except torch.OutOfMemoryError:      # its workspace, before any launch: op by op takes less at a time
                 return None
         return normed, (out_cache if out_cache is not None else MambaCache(new_layers))
@@ -974,17 +1014,18 @@ class MambaLM(nn.Module):
         layer); others run the per-op path (the matrix-core skinny GEMMs or
         the library's, the conv-step and SSM-update kernels)."""
         lt = self._layer_tensors()
-        w4 = len(lt) > 0 and type(self.layers[0].mixer.in_proj) is LinearW4
-        plain = not (len(lt) > 0 and type(self.layers[0].mixer.in_proj) in _QUANTIZED)
+        kind = type(self.layers[0].mixer.in_proj) if len(lt) > 0 else nn.Linear
+        plain = kind not in _QUANTIZED
         # (the fused step's head is the embedding)
         if plain and self._quantized_head() is None and self._fused_step_ok(input_ids, cache, lt=lt):
             return self._step_fused(input_ids, cache, lt=lt)
         x = self.embedding(input_ids).squeeze(1)
-        if w4 and BATCHED_STEP_NATIVE:
-            got = self._w4_step_layers(x, cache, lt)
+        if not plain and BATCHED_STEP_NATIVE:
+            got = self._quant_step_layers(x, cache, lt, kind)
             if got is not None:
                 h = x if x.dtype == torch.float32 else x.float()
-                normed = ops.decode_step_w4(*got, h, self.norm_f.weight, self.norm_f.eps, self.cfg, dtype=x.dtype)
+                step = ops.decode_step_w4 if kind is LinearW4 else ops.decode_step_int8
+                normed = step(*got, h, self.norm_f.weight, self.norm_f.eps, self.cfg, dtype=x.dtype)
                 return self.lm_head(normed).unsqueeze(1)
         if BATCHED_STEP_NATIVE and plain:
             got = self._batched_step_layers(x, cache, lt)
@@ -1159,12 +1200,15 @@ class MambaLM(nn.Module):
             L.eps = self.layers[i].norm.eps
         return tmpl
 
-    # ---- a 4-bit stack's step in one call ----
+    # ---- a quantized stack's step in one call ----
     def _w4_step_layers(self, x, cache, lt):
-        """(ctypes arrays of mtl_decode_layer with this call's cache pointers and of mtl_w4_matrix) for
-        mtl_decode_step_w4, or None where it does not apply: sizes, a stack of more than plain modules and LinearW4, a
-        weight or cache tensor that is not a contiguous tensor of x's dtype (SSM states: float32) and its shape on x's
-        device.  The weights are checked when their addresses, the projections' form (group, scales' type, sizes) or
+        return self._quant_step_layers(x, cache, lt, LinearW4)
+
+    def _quant_step_layers(self, x, cache, lt, kind):
+        """(ctypes arrays of mtl_decode_layer with this call's cache pointers and of the projections' matrices) for
+        mtl_decode_step_w4 or mtl_decode_step_int8 (kind: LinearW4 or LinearInt8), or None where it does not apply: sizes,
+        a stack of more than plain modules and `kind`, a weight or cache tensor that is not a contiguous tensor of x's
+        dtype (SSM states: float32) and its shape on x's device.  The weights are checked when their addresses, the projections' form (group, scales' type, sizes) or
         x_proj's version (which its transposed copy follows) change; the cache tensors every call."""
         cfg, act, dev = self.cfg, x.dtype, x.device
         nl = len(lt)
@@ -1179,23 +1223,23 @@ class MambaLM(nn.Module):
         nf = self.norm_f.weight
         if nf.dtype != act or nf.device != dev or not nf.is_contiguous() or tuple(nf.shape) != (dm,):
             return None
-        if not (ops.plain_call() and _no_global_hooks() and _plain_modules(self.layers, _W4_STACK_MODULES)):
+        if not (ops.plain_call() and _no_global_hooks() and _plain_modules(self.layers, _QUANT_STACK_MODULES[kind])):
             return None
         if act == torch.float32 and any(ts[_LT_XPROJ].is_inference() for ts in lt):
             return None                  # (no version that the transposed copy could follow)
         proj = [p for blk in self.layers._modules.values() for p in
                 (blk._modules["mixer"]._modules["in_proj"], blk._modules["mixer"]._modules["out_proj"])]
-        if any(type(p) is not LinearW4 for p in proj):
+        if any(type(p) is not kind for p in proj):
             return None
         ptr = lambda t: 0 if t is None else t.data_ptr()
         sig = (dev, dm, act, tuple(ptr(t) for ts in lt for t in ts),
-               tuple((ptr(s), s.dtype, ptr(p._parameters["zeros"]), p.group, p.out_features, p.in_features)
-                     for p in proj for s in (p._parameters["scales"],)),
+               kind, tuple((ptr(s), s.dtype, ptr(p._parameters.get("zeros")), getattr(p, "group", 0), p.out_features,
+                            p.in_features) for p in proj for s in (p._parameters["scales"],)),
                tuple(ts[_LT_XPROJ]._version for ts in lt) if act == torch.float32 else None, self._norm_eps())
-        cached = getattr(self, "_w4_tmpl", None)
+        cached = getattr(self, "_quant_tmpl", None)
         if cached is None or cached[0] != sig:
-            cached = (sig, self._w4_template(lt, proj, dev, dm, act))
-            self._w4_tmpl = cached
+            cached = (sig, self._quant_template(lt, proj, dev, dm, act, kind))
+            self._quant_tmpl = cached
         if cached[1] is None:
             return None
         cs_shape, hs_shape = (b, D, K - 1), (b, D, N)
@@ -1210,16 +1254,23 @@ class MambaLM(nn.Module):
             L.conv_state, L.ssm_state = lc.conv_state.data_ptr(), lc.ssm_state.data_ptr()
         return arr, mats
 
-    def _w4_template(self, lt, proj, dev, dm, act):
-        """The weight half of _w4_step_layers, or None when a weight is not a contiguous `act` tensor of its shape on
+    def _quant_template(self, lt, proj, dev, dm, act, kind):
+        """The weight half of _quant_step_layers, or None when a weight is not a contiguous `act` tensor of its shape on
         dev, or one the library loads in 16-byte runs (codes, scales, a bf16 x_proj) is not aligned."""
         cfg = self.cfg
         D, N, K, R = cfg.d_inner, cfg.d_state, cfg.d_conv, cfg.dt_rank
         ok = lambda t, shape: t.device == dev and t.dtype == act and t.is_contiguous() and tuple(t.shape) == shape
         opt = lambda t, shape: t is None or ok(t, shape)
-        tmpl, mats = (_lib.DecodeLayer * len(lt))(), (_lib.W4Matrix * (2 * len(lt)))()
+        matrix = _lib.W4Matrix if kind is LinearW4 else _lib.Int8Matrix
+        tmpl, mats = (_lib.DecodeLayer * len(lt))(), (matrix * (2 * len(lt)))()
         for i, (ts, L) in enumerate(zip(lt, tmpl)):
             for p, m, shape in ((proj[2 * i], mats[2 * i], (2 * D, dm)), (proj[2 * i + 1], mats[2 * i + 1], (dm, D))):
+                if kind is LinearInt8:
+                    if (p.out_features, p.in_features) != shape or p.weight.device != dev:
+                        return None
+                    w = p.int8()                             # (its checks: layout, types, alignment)
+                    m.codes, m.scales = w.codes.data_ptr(), w.scales.data_ptr()
+                    continue
                 w = p.w4()
                 if (w.n, w.k) != shape or w.codes.device != dev or not ops.aligned16(w.codes, w.scales) or \
                         (w.zeros is not None and w.zeros.data_ptr() % 4):

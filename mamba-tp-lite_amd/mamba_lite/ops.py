@@ -631,17 +631,20 @@ def prefill_long_ok(b, l, d_model, d_inner, d_state, dt_rank, d_conv) -> bool:
             and 1 <= dt_rank <= d_inner and 1 <= d_conv <= 8)
 
 
-def prefill_long(h, layers, norm_f, eps_f, d_inner, d_state, dt_rank, d_conv, skinny_rows=0):
+def prefill_long(h, layers, norm_f, eps_f, d_inner, d_state, dt_rank, d_conv, skinny_rows=0, matrices=None):
     """mtl_prefill_long: a prompt's whole layer stack in one call (any
     length; the projections on hipBLASLt, up to skinny_rows token rows on
     the library's skinny GEMM where the shapes fit it, and from enough rows
     on the in_proj and out_proj on the split-f16 product).  h [b, l, d_model]
     float32 holds the embedded tokens and is overwritten with the final
     residual stream; `layers` is a ctypes array of _lib.PrefillLayer
-    (weights plus this call's cache pointers).  Returns norm_f(h)
-    [b, l, d_model]."""
+    (weights plus this call's cache pointers); with `matrices`, one of
+    _lib.Int8Matrix, in_proj and out_proj run in 8-bit integers
+    (mtl_prefill_long_int8).  Returns norm_f(h) [b, l, d_model]."""
     _f32c(h, "h")
     _f32c(norm_f, "norm_f")
+    if matrices is not None and len(matrices) != 2 * len(layers):
+        raise ValueError("prefill_long: two matrices for each layer expected")
     b, l, M = h.shape
     rows, J = b * l, dt_rank + 2 * d_state
     if norm_f.numel() != M or norm_f.device != h.device:
@@ -650,7 +653,8 @@ def prefill_long(h, layers, norm_f, eps_f, d_inner, d_state, dt_rank, d_conv, sk
     # GEMM library or, where those products are split, their operands
     lib = _lib.load()
     blas_ws = max([PREFILL_LONG_BLAS_WS] + [lib.mtl_linear_f32_ws_bytes(rows, n, k)
-                                            for n, k in ((2 * d_inner, M), (M, d_inner)) if linear_f32_pays(rows, n, k)])
+                                            for n, k in ((2 * d_inner, M), (M, d_inner))
+                                            if matrices is None and linear_f32_pays(rows, n, k)])
     offs, n = [], 0
     for sz in (rows * M, rows * 2 * d_inner, rows * d_inner, rows * J, rows * d_inner, rows * d_inner, rows * M,
                rows * M):
@@ -675,7 +679,10 @@ def prefill_long(h, layers, norm_f, eps_f, d_inner, d_state, dt_rank, d_conv, sk
     a.d_conv, a.n_layers, a.skinny_rows = d_conv, len(layers), int(skinny_rows)
     a.batch, a.seqlen, a.d_model, a.d_inner, a.d_state, a.dt_rank = b, l, M, d_inner, d_state, dt_rank
     with _dev_guard(h):
-        _lib.check(lib.mtl_prefill_long(ctypes.byref(a), layers, _stream(h)), "prefill_long")
+        if matrices is None:
+            _lib.check(lib.mtl_prefill_long(ctypes.byref(a), layers, _stream(h)), "prefill_long")
+        else:
+            _lib.check(lib.mtl_prefill_long_int8(ctypes.byref(a), layers, matrices, _stream(h)), "prefill_long_int8")
     return normed
 
 
@@ -1388,6 +1395,37 @@ def linear_w4(x, w4, bias=None, out=None):
     return out
 
 
+def _quant_step(name, layers, matrices, h, norm_f, eps_f, cfg, dtype, more):
+    """The checks and workspace that the one-call steps of quantized stacks share; `more`: sizes (in floats) beside or in
+    place of the common ones."""
+    _f32c(h, "h")
+    if dtype not in _ACT_DTYPES or norm_f.dtype != dtype or not norm_f.is_contiguous():
+        raise ValueError(f"{name}: norm_f must be contiguous {dtype} (float32 or bfloat16)")
+    if h.dim() != 2 or h.shape[1] != cfg.d_model:
+        raise ValueError(f"{name}: h must be [b, {cfg.d_model}]")
+    b, M = h.shape
+    if norm_f.numel() != M or norm_f.device != h.device:
+        raise ValueError(f"{name}: norm_f must hold {M} values on {h.device}")
+    if len(matrices) != 2 * len(layers):
+        raise ValueError(f"{name}: two matrices for each layer expected")
+    D, J = cfg.d_inner, cfg.dt_rank + 2 * cfg.d_state
+    pad = lambda n: -(-n // 64) * 64                      # 256-byte aligned slices
+    sizes = {"normed_out": b * M, "inp": b * M, "xc": b * D, "z": 2 * b * D, "y": b * D,
+             "xpart": max(-(-D // 32), 16) * b * J, "x_dbl": b * J, "parts": b * M, **more}
+    ws = torch.empty(sum(pad(n) for n in sizes.values()), device=h.device, dtype=torch.float32)
+    a = _lib.DecodeStepBatchedArgs()
+    off = 0
+    for field, n in sizes.items():
+        setattr(a, field, ws.data_ptr() + 4 * off)
+        off += pad(n)
+    a.h, a.norm_f = h.data_ptr(), norm_f.data_ptr()
+    a.eps_f, a.n_layers, a.batch = float(eps_f), len(layers), b
+    a.d_model, a.d_inner, a.d_state, a.dt_rank, a.d_conv = M, D, cfg.d_state, cfg.dt_rank, cfg.d_conv
+    with _dev_guard(h):
+        _lib.check(getattr(_lib.load(), f"mtl_{name}")(ctypes.byref(a), layers, matrices, _ACT_DTYPES[dtype], _stream(h)), name)
+    return ws.view(dtype)[:b * M].view(b, M)     # normed_out: the workspace's first slice
+
+
 def decode_step_w4(layers, matrices, h, norm_f, eps_f, cfg, dtype=torch.float32):
     """mtl_decode_step_w4: a decode step of every layer of a 4-bit stack in one
     call.  `layers` is a ctypes array of _lib.DecodeLayer (this call's cache
@@ -1395,33 +1433,16 @@ def decode_step_w4(layers, matrices, h, norm_f, eps_f, cfg, dtype=torch.float32)
     each layer); h [b, d_model] float32 holds the step's embedding rows and is
     left holding the final residual stream.  Returns norm_f of it [b, d_model]
     in `dtype`, the weights', conv histories' and output's type."""
-    _f32c(h, "h")
-    if dtype not in _ACT_DTYPES or norm_f.dtype != dtype or not norm_f.is_contiguous():
-        raise ValueError(f"decode_step_w4: norm_f must be contiguous {dtype} (float32 or bfloat16)")
-    if h.dim() != 2 or h.shape[1] != cfg.d_model:
-        raise ValueError(f"decode_step_w4: h must be [b, {cfg.d_model}]")
-    b, M = h.shape
-    if norm_f.numel() != M or norm_f.device != h.device:
-        raise ValueError(f"decode_step_w4: norm_f must hold {M} values on {h.device}")
-    if len(matrices) != 2 * len(layers):
-        raise ValueError("decode_step_w4: two matrices for each layer expected")
-    D, J = cfg.d_inner, cfg.dt_rank + 2 * cfg.d_state
-    pad = lambda n: -(-n // 64) * 64                      # 256-byte aligned slices
-    sizes = {"normed_out": b * M, "inp": b * M, "xc": b * D, "z": 2 * b * D, "y": b * D,
-             "xpart": max(-(-D // 32), 16) * b * J, "x_dbl": b * J, "parts": b * M}
-    ws = torch.empty(sum(pad(n) for n in sizes.values()), device=h.device, dtype=torch.float32)
-    a = _lib.DecodeStepBatchedArgs()
-    off = 0
-    for name, n in sizes.items():
-        setattr(a, name, ws.data_ptr() + 4 * off)
-        off += pad(n)
-    a.h, a.norm_f = h.data_ptr(), norm_f.data_ptr()
-    a.eps_f, a.n_layers, a.batch = float(eps_f), len(layers), b
-    a.d_model, a.d_inner, a.d_state, a.dt_rank, a.d_conv = M, D, cfg.d_state, cfg.dt_rank, cfg.d_conv
-    with _dev_guard(h):
-        _lib.check(_lib.load().mtl_decode_step_w4(ctypes.byref(a), layers, matrices, _ACT_DTYPES[dtype], _stream(h)),
-                   "decode_step_w4")
-    return ws.view(dtype)[:b * M].view(b, M)     # normed_out: the workspace's first slice
+    return _quant_step("decode_step_w4", layers, matrices, h, norm_f, eps_f, cfg, dtype, {})
+
+
+def decode_step_int8(layers, matrices, h, norm_f, eps_f, cfg, dtype=torch.float32):
+    """mtl_decode_step_int8: decode_step_w4 for a stack in 8-bit integers; `matrices` a ctypes array of
+    _lib.Int8Matrix."""
+    b = h.shape[0] if h.dim() else 0
+    row = lambda k: -(-k // _INT8_PAD) * _INT8_PAD // 4
+    return _quant_step("decode_step_int8", layers, matrices, h, norm_f, eps_f, cfg, dtype,
+                       {"inp": b * row(cfg.d_model), "xn": b * row(cfg.d_inner), "sq": 2 * b})
 
 
 def dequantize_w4(w4, dtype=torch.float32, out=None):

@@ -277,3 +277,92 @@ def test_casts_keep_the_scales():
     with torch.no_grad():
         got, _ = q.prefill(ids)
     assert got.dtype == torch.bfloat16 and bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 2, 5, 32])
+def test_steps_in_one_call_are_those_op_by_op(rows, dtype, monkeypatch):
+    q = _model(d_model=512, n_layer=3, dtype=dtype, bias=True).quantize_int8()
+    ids = torch.randint(0, 1003, (rows, 12), device="cuda")
+    calls = []
+    real = ops.decode_step_int8
+    monkeypatch.setattr(ops, "decode_step_int8", lambda *a, **k: (calls.append(1), real(*a, **k))[1])
+    with torch.no_grad():
+        _, cache = q.prefill(ids[:, :8])
+        other = copy.deepcopy(cache)
+        got = [q.step(ids[:, i:i + 1], cache) for i in range(8, 12)]
+        assert len(calls) == 4
+        monkeypatch.setattr(mm, "BATCHED_STEP_NATIVE", False)
+        want = [q.step(ids[:, i:i + 1], other) for i in range(8, 12)]
+        assert len(calls) == 4
+    # float32: the same launches with the same arguments, but for the SSM update's parameters (the same values) and the sums
+    # of the residual; bfloat16: op by op rounds each out_proj's output once more
+    for a, r in zip(got, want):
+        assert a.dtype == dtype and a.shape == r.shape
+        assert _rel(a, r) < TOL[dtype]
+    if dtype == torch.float32:
+        assert all(torch.equal(a, r) for a, r in zip(got, want))
+        for a, r in zip(cache.layers, other.layers):
+            assert torch.equal(a.ssm_state, r.ssm_state) and torch.equal(a.conv_state, r.conv_state)
+
+
+def test_the_one_call_step_leaves_other_stacks_alone():
+    q = _model(d_model=512).quantize_int8()
+    cache = MambaCache.allocate(q.cfg, 2, "cuda", torch.float32)
+    x = torch.zeros(2, 512, device="cuda")
+    took = lambda: q._quant_step_layers(x, cache, q._layer_tensors(), LinearInt8) is not None
+    assert took()
+    handle = q.layers[0].mixer.out_proj.register_forward_hook(lambda *a: None)
+    assert not took()
+    handle.remove()
+    assert took()
+    big = MambaCache.allocate(q.cfg, 33, "cuda", torch.float32)
+    assert q._quant_step_layers(torch.zeros(33, 512, device="cuda"), big, q._layer_tensors(), LinearInt8) is None
+    ids = torch.zeros(2, 1, device="cuda", dtype=torch.long)
+    with torch.no_grad():
+        before = q.step(ids, copy.deepcopy(cache))
+        # another projection in its place, of other sizes' addresses: the plan follows
+        lin = torch.nn.Linear(512, 2048, bias=False).cuda()
+        q.layers[0].mixer.in_proj = LinearInt8.from_linear(lin)
+        after = q.step(ids, copy.deepcopy(cache))
+        assert not torch.equal(before, after)
+        q.layers[0].mixer.in_proj = lin                      # (a plain one: op by op)
+        assert not took() and q.step(ids, copy.deepcopy(cache)).shape == before.shape
+
+
+@pytest.mark.parametrize("b,l", [(1, 1), (1, 64), (2, 65), (3, 130)])
+def test_prompts_in_one_call_are_those_op_by_op(b, l, monkeypatch):
+    q = _model(d_model=256, n_layer=3, bias=True).quantize_int8()
+    ids = torch.randint(0, 1003, (b, 2 * l), device="cuda")
+    calls = []
+    real = ops.prefill_long
+    monkeypatch.setattr(ops, "prefill_long", lambda *a, **k: (calls.append(k["matrices"]), real(*a, **k))[1])
+    with torch.no_grad():
+        got, cache = q.prefill(ids[:, :l])
+        got2, _ = q.prefill(ids[:, l:], cache, out_cache=cache)          # the next part of the prompt, in place
+        assert len(calls) == 2 and all(m is not None for m in calls)
+        monkeypatch.setattr(mm, "LONG_PREFILL_NATIVE", False)
+        want, other = q.prefill(ids[:, :l])
+        want2, other = q.prefill(ids[:, l:], other)
+        assert len(calls) == 2
+    # (x_proj's and dt_proj's library products differ in the order of their sums)
+    assert _rel(got, want) < TOL[torch.float32] and _rel(got2, want2) < TOL[torch.float32]
+    for a, r in zip(cache.layers, other.layers):
+        assert _rel(a.ssm_state, r.ssm_state) < TOL[torch.float32] and _rel(a.conv_state, r.conv_state) < TOL[torch.float32]
+
+
+def test_the_one_call_prompt_follows_its_weights():
+    q = _model().quantize_int8()
+    ids = torch.randint(0, 1003, (1, 30), device="cuda")
+    with torch.no_grad():
+        before, _ = q.prefill(ids)
+        q.layers[1].mixer.out_proj = LinearInt8.from_linear(torch.nn.Linear(512, 256, bias=False).cuda())
+        after, _ = q.prefill(ids)
+        assert not torch.equal(before, after)
+        seen = []
+        handle = q.layers[0].mixer.out_proj.register_forward_hook(lambda m, a, o: seen.append(o))
+        q.prefill(ids)
+        handle.remove()
+        assert len(seen) == 1 and seen[0].shape == (1, 30, 256)
+        q.layers[0].mixer.in_proj = torch.nn.Linear(256, 1024, bias=False).cuda()       # a mixed stack: op by op
+        assert q.prefill(ids)[0].shape == before.shape and q.step(ids[:, :1], q.prefill(ids)[1]).shape[0] == 1

@@ -188,6 +188,7 @@ def test_library_refuses_before_any_launch():
         assert refused(lib.mtl_linear_int8(ctypes.byref(bad), None), text), name
     for f in (lib.mtl_linear_int8, lib.mtl_add_rmsnorm_int8):
         assert refused(f(None, None), b"null")
+    assert lib.mtl_quantize_int8(None, 8, None, None, 0, 8, 0, None) == 0 and lib.mtl_last_error() == b""
 
 
 def test_linear_int8_module_on_the_host():
