@@ -22,74 +22,105 @@ struct LinearArgs {
 // the float of a sum, each factor rounded once
 __device__ __forceinline__ float scaled(int acc, float sx, float sw, float bias) { return fmaf((float)acc * sx, sw, bias); }
 
-// 16 bytes per lane from base + off to LDS, at to + 16 lane, asynchronously (vmcnt).  In assembly because the compiler
-// waits for every copy by the builtin before the next read of LDS, whatever slot it reads: one stage of a product then
-// took a whole round trip to memory (256 rows, 2048 x 4096: 21 us).
-__device__ __forceinline__ void copy_kilobyte(const int8_t* base, uint32_t off, uint8_t* to) {
+// Copies to LDS, asynchronous (vmcnt): 16 or 4 bytes per lane from base + off to `to` + 16 or 4 lane.  In assembly because
+// the compiler waits for every copy by the builtin before the next read of LDS, whatever slot it reads: one stage of a
+// product then took a whole round trip to memory (256 rows, 2048 x 4096: 21 us in place of 12).
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    typedef __attribute__((address_space(3))) const uint8_t* Lds;
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(Lds)p);
+}
 #if defined(__HIP_DEVICE_COMPILE__)
-    typedef __attribute__((address_space(3))) uint8_t* Lds;
-    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(Lds)to);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(at) : "m0");
+#define MTL_COPY_TO_LDS(WIDTH, base, off, to)                                                                        \
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_" WIDTH " %0, %1" ::"v"(off), "s"(base),           \
+                 "s"(lds_address(to))                                                                                \
+                 : "m0")
 #else
-    (void)base; (void)off; (void)to;
+#define MTL_COPY_TO_LDS(WIDTH, base, off, to) (void)(base), (void)(off), (void)(to)
 #endif
+
+// a pointer that is the same for the whole wavefront, in SGPRs
+template <typename P> __device__ __forceinline__ const P* uniform(const P* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return reinterpret_cast<const P*>((uint64_t)hi << 32 | lo);
 }
 
-// T: y.  A workgroup takes BN columns by BM rows of y, a wavefront WN x WM of them as 16 x 16 MFMA tiles with the
-// rows of W as the first operand, so that a lane holds 4 neighbouring columns of y.
-template <typename T, int BN, int BM, int WN, int WM, int ST, int OCC>
+// T: y.  A workgroup takes BN columns by BM rows of y, a wavefront WN x WM of them as 16 x 16 MFMA tiles with the rows of W
+// as the first operand, so that a lane holds 4 neighbouring columns of y.  K runs through a ring of ST stages of 128 columns
+// in LDS.
+//
+// CHAIN: a workgroup takes one tile after the other and its copies never pause: while a tile's last stages are multiplied,
+// the next one's first are on their way, and its first fragments are read before the tile is written.  The tiles' own starts
+// and ends took 93 of the 526 us of 32768 x 8192 x 2048.
+template <typename T, int BN, int BM, int WN, int WM, int ST, int OCC, bool CHAIN>
 __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_kernel(const LinearArgs a) {
     constexpr int NWM = BM / WM, NW = BN / WN * NWM, NT = NW * 64;
-    constexpr int TJ = WN / 16, TI = WM / 16, KB = kInt8Pad, KS = KB / 64;     // MFMA tiles of a wavefront; steps of a stage
-    constexpr int SROWS = BN + BM, STAGE = SROWS * KB;
-    constexpr int CR = 1024 / KB, NC = KB / 16, NI = SROWS / CR / NW;   // rows of a 1 KB copy, chunks of a row, copies per wavefront
-    static_assert(SROWS % (CR * NW) == 0 && BN % CR == 0, "copies divide over the wavefronts");
-    constexpr int kPer = 16 / (int)sizeof(T), kOut = 16 * (WN + kPer);  // a wavefront's 16 rows of y in LDS
-    constexpr int kEnd = NW * kOut * (int)sizeof(T) + 8 * BN, kLds = ST * STAGE > kEnd ? ST * STAGE : kEnd;
+    constexpr int TJ = WN / 16, TI = WM / 16, KB = kInt8Pad, KS = 2;      // MFMA tiles of a wavefront; steps of a stage
+    constexpr int SROWS = BN + BM, STAGE = SROWS * KB, NI = SROWS / 8 / NW;         // 1 KB copies per wavefront and stage
+    static_assert(SROWS % (8 * NW) == 0 && BN % 8 == 0, "copies divide over the wavefronts");
+    static_assert(!CHAIN || (ST == 2 && NT == BN + BM && NT % 64 == 0), "a chain's scales are a copy per wavefront");
+    // a wavefront's 16 rows of y on their way out, OW columns at a time; the scales of the tile's columns and rows
+    constexpr int kPer = 16 / (int)sizeof(T), OW = CHAIN ? 128 / (int)sizeof(T) : WN, kOut = 16 * (OW + kPer);
+    constexpr int kRing = ST * STAGE, kEnd = NW * kOut * (int)sizeof(T) + (CHAIN ? 8 : 4) * SROWS + 4 * BN;
+    constexpr int kLds = CHAIN ? kRing + kEnd : kRing > kEnd ? kRing : kEnd;
     __shared__ __align__(1024) uint8_t ring[kLds];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wn = wave / NWM, wm = wave % NWM;
+    T* const out = reinterpret_cast<T*>(ring + (CHAIN ? kRing : 0)) + wave * kOut;
+    float* s_sw = reinterpret_cast<float*>(ring + (CHAIN ? kRing : 0) + NW * kOut * sizeof(T));    // [BN], then [BM]
+    float* s_next = s_sw + SROWS;                              // (a chain's next tile's)
+    float* const s_b = s_sw + (CHAIN ? 2 : 1) * SROWS;         // [BN]
 
-    int t = blockIdx.x;
-    const int total = a.tm * a.tn;
-    {
-        const int per = total / 8, rem = total % 8, x = t % 8, i = t / 8;
-        t = x * per + min(x, rem) + i;
-    }
-    constexpr int GM = 8;
-    const int group = t / (GM * a.tn), g0 = group * GM, gm = min(GM, a.tm - g0);
-    const int in_g = t - group * GM * a.tn;
-    const int m0 = __builtin_amdgcn_readfirstlane((g0 + in_g % gm) * BM);
-    const int n0 = __builtin_amdgcn_readfirstlane(in_g / gm * BN);
+    // XCD-aware tile order (workgroups are dealt to the 8 XCDs round robin): each XCD takes a contiguous range of tiles,
+    // ordered 8 row tiles by all column tiles, rows fastest, so the tiles resident on an XCD at one time share their operand
+    // rows in its L2
+    const int total = a.tm * a.tn, xcd = blockIdx.x % 8, per = total / 8, rem = total % 8;
+    const int first = xcd * per + min(xcd, rem), count = per + (xcd < rem), stride = (gridDim.x + 7 - xcd) / 8;
+    auto place = [&](int j, int& m, int& n) __attribute__((always_inline)) {
+        constexpr int GM = 8;
+        const int t = first + j, group = t / (GM * a.tn), g0 = group * GM, gm = min(GM, a.tm - g0);
+        const int in_g = t - group * GM * a.tn;
+        // (uniform, but the divisions run on the VALU: back to SGPRs)
+        m = __builtin_amdgcn_readfirstlane((g0 + in_g % gm) * BM);
+        n = __builtin_amdgcn_readfirstlane(in_g / gm * BN);
+    };
 
-    // copy g of a stage: its rows CR g ..; lane l puts a 16-byte chunk of row CR g + l / NC at position l % NC.  Chunk c of
-    // a row stands at position c ^ swizzle(row): the 16 rows of a fragment's chunk then lie in different banks.
-    auto swizzle = [](int row) __attribute__((always_inline)) { return row >> 1 & 7; };
-    const int8_t* const wt = a.w + (int64_t)n0 * a.Kp;
-    const int8_t* const xt = a.x + (int64_t)m0 * a.Kp;
-    uint32_t off[NI];
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const int row = CR * (wave * NI + i) + lane / NC;
-        const int rr = row < BN ? min(row, a.N - 1 - n0) : min(row - BN, a.M - 1 - m0);
-        off[i] = (uint32_t)rr * (uint32_t)a.Kp + 16u * (lane % NC ^ swizzle(row));
-    }
+    // copy g of a stage: its rows 8 g ..; lane l puts a 16-byte chunk of row 8 g + l / 8 at position l % 8.  Chunk c of a row
+    // stands at position c ^ (row / 2 % 8): the 16 rows of a fragment's chunk then lie in different banks (counted: no
+    // conflicts; with row % 8 half of the LDS cycles were).
+    const int8_t *wt, *xt;
+    int wlast, xlast;                                          // the tile's last rows of W and x that are there
+    const int row8 = lane >> 3, chunk = 16 * ((lane & 7) ^ (lane >> 4));
+    auto aim = [&](int m, int n) __attribute__((always_inline)) {
+        wt = uniform(a.w + (int64_t)n * a.Kp);
+        xt = uniform(a.x + (int64_t)m * a.Kp);
+        wlast = a.N - 1 - n;
+        xlast = a.M - 1 - m;
+    };
     auto issue1 = [&](int i, int slot, int s) __attribute__((always_inline)) {
-        copy_kilobyte((CR * (wave * NI + i) < BN ? wt : xt) + (uint32_t)s * KB, off[i], ring + slot * STAGE + (wave * NI + i) * 1024);
+        const int g = wave * NI + i;
+        const bool isw = 8 * g < BN;
+        const int8_t* base = (isw ? wt : xt) + (uint32_t)s * KB;
+        const int row = min(row8 + 8 * g - (isw ? 0 : BN), isw ? wlast : xlast);
+        const uint32_t off = __umul24(row, a.Kp) + (chunk ^ (g & 1) << 6);        // (256 rows, Kp <= 2^17)
+        MTL_COPY_TO_LDS("dwordx4", base, off, ring + slot * STAGE + g * 1024);
+    };
+    // the tile's scales, 64 to a wavefront
+    auto issue_scales = [&](int m, int n, float* to) __attribute__((always_inline)) {
+        const bool col = wave * 64 < BN;
+        const int at = threadIdx.x - (col ? 0 : BN);
+        const float* base = uniform(col ? a.sw + n : a.sx + m);
+        const uint32_t off = 4u * (uint32_t)min(at, col ? a.N - 1 - n : a.M - 1 - m);
+        MTL_COPY_TO_LDS("dword", base, off, to + wave * 64);
     };
 
     I4 acc[TJ][TI];
-#pragma unroll
-    for (int j = 0; j < TJ; ++j)
-#pragma unroll
-        for (int i = 0; i < TI; ++i) acc[j][i] = I4{0, 0, 0, 0};
-
     const int r16 = lane & 15, g4 = lane >> 4;
     uint32_t o[KS];
 #pragma unroll
-    for (int k = 0; k < KS; ++k) o[k] = r16 * KB + 16 * ((4 * k + g4) ^ swizzle(r16));
+    for (int k = 0; k < KS; ++k) o[k] = r16 * KB + 16 * ((4 * k + g4) ^ (r16 >> 1));
     struct Frag { I4 w[TJ], x[TI]; };
     constexpr int NR = TI + TJ, MT = TI * TJ;
     auto read1 = [&](Frag& f, int r, int slot, int k) __attribute__((always_inline)) {
@@ -105,8 +136,8 @@ __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_ker
     const int ns = a.Kp / KB;
     int slot = 0;
     // step k of stage s (its fragments in cur): the next step's fragments are read, and at a stage's end the copies of stage
-    // s + ST into its slot issued, between its products
-    auto body = [&](Frag& cur, Frag& nxt, int s, int k) __attribute__((always_inline)) {
+    // s + ST into its slot issued, between its products.  `more`: stages past the last are the next tile's.
+    auto body = [&](Frag& cur, Frag& nxt, int s, int k, bool more) __attribute__((always_inline)) {
         const bool end = k + 1 == KS;
         const int H = end ? MT / 2 : 0, left = MT - H, prev = slot;
         bool load = false;
@@ -114,21 +145,22 @@ __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_ker
         for (int q = 0; q < H; ++q) mma1(cur, q);
         __builtin_amdgcn_sched_barrier(0);
         if (end) {
-            if (s + 1 < ns) {
-                if (s + ST > ns)
+            if (CHAIN || s + 1 < ns) {
+                if (CHAIN || s + ST > ns)
                     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 else
                     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((ST - 2) * NI) : "memory");
             }
-            load = s + ST < ns;
+            load = s + ST < ns || more;
             slot = slot + 1 == ST ? 0 : slot + 1;                        // (after the last stage: read, never used)
         }
+        const int ahead = CHAIN && s + ST >= ns ? s + ST - ns : s + ST;
 #pragma unroll
         for (int q = 0; q < left; ++q) {
             mma1(cur, H + q);
             if (end && load && q < (left + 1) / 2) {
 #pragma unroll
-                for (int i = 2 * q * NI / left; i < min(2 * (q + 1) * NI / left, NI); ++i) issue1(i, prev, s + ST);
+                for (int i = 2 * q * NI / left; i < min(2 * (q + 1) * NI / left, NI); ++i) issue1(i, prev, ahead);
             }
 #pragma unroll
             for (int r = min(q * NR / left, NR); r < min((q + 1) * NR / left, NR); ++r)
@@ -136,6 +168,14 @@ __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_ker
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+
+    int tile = blockIdx.x / 8, m0, n0, m1 = 0, n1 = 0;
+    place(tile, m0, n0);
+    aim(m0, n0);
+    if constexpr (CHAIN) {
+        issue_scales(m0, n0, s_sw);
+        if (threadIdx.x < BN) s_b[threadIdx.x] = 0.f;
+    }
 #pragma unroll
     for (int s = 0; s < ST; ++s)
         if (s < ns) {
@@ -149,53 +189,78 @@ __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_ker
     Frag f0, f1;
 #pragma unroll
     for (int r = 0; r < NR; ++r) read1(f0, r, 0, 0);
-    for (int s = 0; s < ns; ++s) {
-        body(f0, f1, s, 0);
-        body(f1, f0, s, 1);
-    }
 
-    // D[j][i] of a tile: column lane % 16 (a row m of y), row 4 (lane / 16) + q in register q (a column n)
-    lds_barrier();
-    T* const out = reinterpret_cast<T*>(ring) + wave * kOut;
-    float* const s_sw = reinterpret_cast<float*>(ring + NW * kOut * sizeof(T));
-    float* const s_b = s_sw + BN;
-    for (int n = threadIdx.x; n < BN; n += NT) {
-        const int nc = min(n0 + n, a.N - 1);
-        s_sw[n] = a.sw[nc];
-        s_b[n] = a.bias ? load_param(a.bias, nc, a.bias_bf16) : 0.f;
-    }
-    lds_barrier();
-    const int nw = n0 + wn * WN;
+    for (;;) {
+        const bool more = CHAIN && tile + stride < count;
 #pragma unroll
-    for (int i = 0; i < TI; ++i) {
-        const int mt = m0 + wm * WM + 16 * i;
-        const float sx = a.sx[min(mt + r16, a.M - 1)];
+        for (int j = 0; j < TJ; ++j)
 #pragma unroll
-        for (int j = 0; j < TJ; ++j) {
-            const int c = 16 * j + 4 * g4;
-            const F4v sw = ld4(s_sw + wn * WN + c), b = ld4(s_b + wn * WN + c);
-            F4v v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = scaled(acc[j][i][e], sx, sw[e], b[e]);
-            st4(out + r16 * (WN + kPer) + c, v);
-        }
-        wave_lds_fence();
-        if (a.vec && nw + WN <= a.N) {
-            constexpr int RPR = WN / kPer, RP = 64 / RPR;      // 16-byte runs of a row; rows of an instruction
-#pragma unroll
-            for (int r0 = 0; r0 < 16; r0 += RP) {
-                const int r = r0 + lane / RPR, c = lane % RPR * kPer;
-                if (RP > 16 && r >= 16) break;
-                const I4 v = *reinterpret_cast<const I4*>(out + r * (WN + kPer) + c);
-                if (mt + r < a.M) *reinterpret_cast<I4*>(static_cast<T*>(a.y) + (int64_t)(mt + r) * a.ldy + nw + c) = v;
+            for (int i = 0; i < TI; ++i) acc[j][i] = I4{0, 0, 0, 0};
+        for (int s = 0; s < ns; ++s) {
+            if constexpr (CHAIN) {
+                if (more && s + ST == ns) {
+                    place(tile + stride, m1, n1);
+                    aim(m1, n1);
+                    issue_scales(m1, n1, s_next);
+                }
             }
-        } else {
-            for (int e = lane; e < 16 * WN; e += 64) {
-                const int r = e / WN, c = e % WN;
-                if (mt + r < a.M && nw + c < a.N) static_cast<T*>(a.y)[(int64_t)(mt + r) * a.ldy + nw + c] = out[r * (WN + kPer) + c];
+            body(f0, f1, s, 0, more);
+            body(f1, f0, s, 1, more);
+        }
+
+        // D[j][i] of a tile: column lane % 16 (a row m of y), row 4 (lane / 16) + q in register q (a column n)
+        if constexpr (!CHAIN) lds_barrier();
+        if (!CHAIN || a.bias) {
+            for (int e = threadIdx.x; e < SROWS; e += NT) {
+                if constexpr (!CHAIN) s_sw[e] = e < BN ? a.sw[min(n0 + e, a.N - 1)] : a.sx[min(m0 + e - BN, a.M - 1)];
+                if (e < BN) s_b[e] = a.bias ? load_param(a.bias, min(n0 + e, a.N - 1), a.bias_bf16) : 0.f;
+            }
+            lds_barrier();
+        }
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+            const int mt = m0 + wm * WM + 16 * i;
+            const float sx = s_sw[BN + wm * WM + 16 * i + r16];
+#pragma unroll
+            for (int j0 = 0; j0 < TJ; j0 += OW / 16) {
+                const int nw = n0 + wn * WN + 16 * j0;
+#pragma unroll
+                for (int j = 0; j < OW / 16; ++j) {
+                    const int c = 16 * j + 4 * g4;
+                    // (the bias in LDS too: a load that may stand between the stores would wait for them)
+                    const F4v sw = ld4(s_sw + wn * WN + 16 * j0 + c), b = ld4(s_b + wn * WN + 16 * j0 + c);
+                    F4v v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = scaled(acc[j0 + j][i][e], sx, sw[e], b[e]);
+                    st4(out + r16 * (OW + kPer) + c, v);
+                }
+                wave_lds_fence();
+                if (a.vec && nw + OW <= a.N) {
+                    constexpr int RPR = OW / kPer, RP = 64 / RPR;      // 16-byte runs of a row; rows of an instruction
+#pragma unroll
+                    for (int r0 = 0; r0 < 16; r0 += RP) {
+                        const int r = r0 + lane / RPR, c = lane % RPR * kPer;
+                        if (RP > 16 && r >= 16) break;
+                        const I4 v = *reinterpret_cast<const I4*>(out + r * (OW + kPer) + c);
+                        if (mt + r < a.M) *reinterpret_cast<I4*>(static_cast<T*>(a.y) + (int64_t)(mt + r) * a.ldy + nw + c) = v;
+                    }
+                } else {
+                    for (int e = lane; e < 16 * OW; e += 64) {
+                        const int r = e / OW, c = e % OW;
+                        if (mt + r < a.M && nw + c < a.N)
+                            static_cast<T*>(a.y)[(int64_t)(mt + r) * a.ldy + nw + c] = out[r * (OW + kPer) + c];
+                    }
+                }
+                wave_lds_fence();
             }
         }
-        wave_lds_fence();
+        if (!more) break;
+        tile += stride;
+        m0 = m1;
+        n0 = n1;
+        float* const done = s_sw;
+        s_sw = s_next;
+        s_next = done;
     }
 }
 
@@ -256,14 +321,14 @@ template <int NW> int launch_stream(const LinearArgs& a, bool f32, hipStream_t s
     return check_launch("linear_int8");
 }
 
-template <int BN, int BM, int WN, int WM, int ST, int OCC> int launch(LinearArgs a, bool f32, hipStream_t st) {
+template <int BN, int BM, int WN, int WM, int ST, int OCC, bool CHAIN = false> int launch(LinearArgs a, bool f32, hipStream_t st) {
     const int64_t tm = (a.M + (int64_t)BM - 1) / BM, tn = (a.N + (int64_t)BN - 1) / BN;
     MTL_REQUIRE(tm * tn < (int64_t(1) << 31), "too many output tiles");
     a.tm = (int)tm;
     a.tn = (int)tn;
-    const dim3 grid((unsigned)(tm * tn)), nt(BN / WN * (BM / WM) * 64);
-    if (f32) hipLaunchKernelGGL((linear_int8_kernel<float, BN, BM, WN, WM, ST, OCC>), grid, nt, 0, st, a);
-    else hipLaunchKernelGGL((linear_int8_kernel<uint16_t, BN, BM, WN, WM, ST, OCC>), grid, nt, 0, st, a);
+    const dim3 grid((unsigned)(CHAIN ? std::min<int64_t>(tm * tn, 256) : tm * tn)), nt(BN / WN * (BM / WM) * 64);
+    if (f32) hipLaunchKernelGGL((linear_int8_kernel<float, BN, BM, WN, WM, ST, OCC, CHAIN>), grid, nt, 0, st, a);
+    else hipLaunchKernelGGL((linear_int8_kernel<uint16_t, BN, BM, WN, WM, ST, OCC, CHAIN>), grid, nt, 0, st, a);
     return check_launch("linear_int8");
 }
 
@@ -302,10 +367,10 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     //   227; 4096x2048x4096 51.6 37.1 43.4 53.5 93.8; 1024x2048x4096 48.9 30.0 19.6 15.7 26.2; 256x2048x4096 46.5 28.5 18.3
     //   11.4 9.8; 4096x768x1536 25.0 16.6 11.7 12.0 18.6; 512x768x1536 22.1 14.4 9.6 6.5 5.5
     const auto rounds = [&](int bn, int bm) { return (double)((tiles(bn, bm) + 255) / 256); };
-    const double cost[5] = {1.72 * rounds(256, 256), 1.0 * rounds(256, 128), 0.58 * rounds(128, 128),
+    const double cost[5] = {a.Kp > kInt8Pad ? 1.72 * rounds(256, 256) : 1e9, 1.0 * rounds(256, 128), 0.58 * rounds(128, 128),
                             0.15 + 0.14 * rounds(64, 64), 0.12 + 0.07 * rounds(32, 32)};
     switch (std::min_element(cost, cost + 5) - cost) {
-        case 0: return launch<256, 256, 128, 64, 2, 1>(a, f32, st);
+        case 0: return launch<256, 256, 128, 64, 2, 1, true>(a, f32, st);
         case 1: return launch<256, 128, 64, 64, 3, 1>(a, f32, st);
         case 2: return launch<128, 128, 64, 32, 4, 1>(a, f32, st);
         case 3: return launch<64, 64, 32, 32, 3, 3>(a, f32, st);
