@@ -35,31 +35,32 @@ struct RowsArgs {
     int64_t M;
     int K, Kp;
     float eps;
-    bool vec;                  // 16-byte aligned rows (x, y, x_out, w) of whole runs of 8
 };
 
 constexpr int kRun = 8;                    // columns a lane takes at a time
+typedef float F4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t U4u __attribute__((ext_vector_type(4), aligned(2)));
 
-// a run's first n values (all of them, from a 16-byte boundary, with `vec`); zeros behind
-template <typename T> __device__ __forceinline__ void load_run(const T* p, int n, bool vec, float* v) {
-    if (vec) {
-        const F4v lo = ld4(p), hi = ld4(p + 4);
+// a run's first n values, all 8 in whole 16-byte accesses at any alignment; zeros behind n.  (Value by value where rows do not
+// start on 16 bytes, 32768 rows of 777 took three times as long as of 768.)
+__device__ __forceinline__ void load_run(const float* p, int n, float* v) {
+    if (n >= kRun) {
+        const F4u lo = *reinterpret_cast<const F4u*>(p), hi = *reinterpret_cast<const F4u*>(p + 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) { v[j] = lo[j]; v[4 + j] = hi[j]; }
     } else {
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) v[j] = j < n ? Act<T>::load(p + j) : 0.f;
+        for (int j = 0; j < kRun; ++j) v[j] = j < n ? p[j] : 0.f;
     }
 }
-template <> __device__ __forceinline__ void load_run<uint16_t>(const uint16_t* p, int n, bool vec, float* v) {
-    if (vec) {
-        const uint4 x = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+__device__ __forceinline__ void load_run(const uint16_t* p, int n, float* v) {
+    if (n >= kRun) {
+        const U4u x = *reinterpret_cast<const U4u*>(p);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { v[2 * j] = __uint_as_float(w[j] << 16); v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
+        for (int j = 0; j < 4; ++j) { v[2 * j] = __uint_as_float(x[j] << 16); v[2 * j + 1] = __uint_as_float(x[j] & 0xffff0000u); }
     } else {
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) v[j] = j < n ? Act<uint16_t>::load(p + j) : 0.f;
+        for (int j = 0; j < kRun; ++j) v[j] = j < n ? bf16_to_f32(p[j]) : 0.f;
     }
 }
 
@@ -112,8 +113,8 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_kernel(const RowsA
 #pragma unroll
     for (int u = 0; u < RU; ++u) {
         const int k = (u * G + t) * kRun, kc = min(k, (p.K - 1) / kRun * kRun);
-        load_run(x + kc, p.K - kc, p.vec, v[u]);
-        if constexpr (NORM) load_run(static_cast<const W*>(p.w) + kc, p.K - kc, p.vec, wv[u]);
+        load_run(x + kc, p.K - kc, v[u]);
+        if constexpr (NORM) load_run(static_cast<const W*>(p.w) + kc, p.K - kc, wv[u]);
     }
     if (add) {
         const Y* y = static_cast<const Y*>(p.y) + row * p.K;
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_kernel(const RowsA
 #pragma unroll
         for (int u = 0; u < RU; ++u) {
             const int k = (u * G + t) * kRun, kc = min(k, (p.K - 1) / kRun * kRun);
-            load_run(y + kc, p.K - kc, p.vec, yv[u]);
+            load_run(y + kc, p.K - kc, yv[u]);
         }
 #pragma unroll
         for (int u = 0; u < RU; ++u)
@@ -137,9 +138,10 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_kernel(const RowsA
             if constexpr (NORM) {
                 if (p.x_out) {
                     float* o = p.x_out + row * p.K + k;
-                    if (p.vec) {
-                        st4(o, F4v{v[u][0], v[u][1], v[u][2], v[u][3]});
-                        st4(o + 4, F4v{v[u][4], v[u][5], v[u][6], v[u][7]});
+                    if (k + kRun <= p.K) {
+                        // (read again a layer later only: past the caches, 1024 x 2048 7.2 -> 6.5 us)
+                        __builtin_nontemporal_store(F4u{v[u][0], v[u][1], v[u][2], v[u][3]}, reinterpret_cast<F4u*>(o));
+                        __builtin_nontemporal_store(F4u{v[u][4], v[u][5], v[u][6], v[u][7]}, reinterpret_cast<F4u*>(o + 4));
                     } else {
 #pragma unroll
                         for (int j = 0; j < kRun; ++j)
@@ -203,10 +205,10 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_kernel(const RowsA
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     const Y* y = NORM && p.y ? static_cast<const Y*>(p.y) + row * p.K : nullptr;
     auto load = [&](int k, float* v) {
-        load_run(x + k, p.K - k, p.vec, v);
+        load_run(x + k, p.K - k, v);
         if (y) {
             float yv[kRun];
-            load_run(y + k, p.K - k, p.vec, yv);
+            load_run(y + k, p.K - k, yv);
 #pragma unroll
             for (int j = 0; j < kRun; ++j) v[j] += yv[j];
         }
@@ -214,7 +216,7 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_kernel(const RowsA
     auto weigh = [&](int k, float* v) {
         if constexpr (NORM) {
             float wv[kRun];
-            load_run(static_cast<const W*>(p.w) + k, p.K - k, p.vec, wv);
+            load_run(static_cast<const W*>(p.w) + k, p.K - k, wv);
 #pragma unroll
             for (int j = 0; j < kRun; ++j) v[j] *= wv[j];
         }
@@ -264,17 +266,15 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_kernel(const RowsA
     }
 }
 
-template <typename T, typename Y, typename W, bool NORM> int launch_rows(RowsArgs a, hipStream_t st) {
-    const auto aligned = [](const void* p, size_t step) { return al16(p) && step % 16 == 0; };
-    a.vec = a.K % kRun == 0 && aligned(a.x, a.ldx * sizeof(T)) && (!NORM || (al16(a.y) && al16(a.w) && al16(a.x_out)));
+template <typename T, typename Y, typename W, bool NORM> int launch_rows(const RowsArgs& a, hipStream_t st) {
 #define MTL_ROWS(G, RU)                                                                                              \
     hipLaunchKernelGGL((quantize_kernel<T, Y, W, NORM, G, RU>), dim3((unsigned)((a.M + (G < 256 ? 256 / G : 1) - 1) / \
                                                                                 (G < 256 ? 256 / G : 1))),            \
                        dim3(G < 256 ? 256 : G), 0, st, a)
-    const bool few = a.M < 1024;
-    if (a.Kp <= 512 && !few) MTL_ROWS(64, 1);
-    else if (a.Kp <= 1024 && !few) MTL_ROWS(64, 2);
-    else if (a.Kp <= 2048 && !few) MTL_ROWS(64, 4);
+    // A wavefront to a row of up to 1024 columns where there are many; otherwise so many that a lane has one run, or two or
+    // four of long rows.  Norms, us: 32768 x 2048 with bf16 y 148 with a wavefront, 133 with four; 32768 x 768 58, 60.
+    if (a.Kp <= 512 && a.M >= 1024) MTL_ROWS(64, 1);
+    else if (a.Kp <= 1024 && a.M >= 1024) MTL_ROWS(64, 2);
     else if (a.Kp <= 2048) MTL_ROWS(256, 1);
     else if (a.Kp <= 4096) MTL_ROWS(256, 2);
     else if (a.Kp <= 8192) MTL_ROWS(256, 4);
