@@ -51,7 +51,8 @@ template <typename P> __device__ __forceinline__ const P* uniform(const P* p) {
 //
 // CHAIN: a workgroup takes one tile after the other and its copies never pause: while a tile's last stages are multiplied,
 // the next one's first are on their way, and its first fragments are read before the tile is written.  The tiles' own starts
-// and ends took 93 of the 526 us of 32768 x 8192 x 2048.
+// and ends took 93 of the 526 us of 32768 x 8192 x 2048.  Three stages of K at least: the next tile's scales go where the
+// last one's were, and a barrier has to stand between.
 template <typename T, int BN, int BM, int WN, int WM, int ST, int OCC, bool CHAIN>
 __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_kernel(const LinearArgs a) {
     constexpr int NWM = BM / WM, NW = BN / WN * NWM, NT = NW * 64;
@@ -367,7 +368,7 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     //   227; 4096x2048x4096 51.6 37.1 43.4 53.5 93.8; 1024x2048x4096 48.9 30.0 19.6 15.7 26.2; 256x2048x4096 46.5 28.5 18.3
     //   11.4 9.8; 4096x768x1536 25.0 16.6 11.7 12.0 18.6; 512x768x1536 22.1 14.4 9.6 6.5 5.5
     const auto rounds = [&](int bn, int bm) { return (double)((tiles(bn, bm) + 255) / 256); };
-    const double cost[5] = {a.Kp > kInt8Pad ? 1.72 * rounds(256, 256) : 1e9, 1.0 * rounds(256, 128), 0.58 * rounds(128, 128),
+    const double cost[5] = {a.Kp > 2 * kInt8Pad ? 1.72 * rounds(256, 256) : 1e9, 1.0 * rounds(256, 128), 0.58 * rounds(128, 128),
                             0.15 + 0.14 * rounds(64, 64), 0.12 + 0.07 * rounds(32, 32)};
     switch (std::min_element(cost, cost + 5) - cost) {
         case 0: return launch<256, 256, 128, 64, 2, 1, true>(a, f32, st);

@@ -1561,6 +1561,15 @@ def _int8_call(name, *ts):
         _not_traced(name)
 
 
+def _other_device(t) -> bool:
+    """Whether t is on a GPU that is not the current one (a CPU tensor raises).  Calls then run again under that device:
+    cheaper than a context in every call."""
+    dev = t.get_device()
+    if dev < 0:
+        _dev_guard(t)
+    return dev != _current_device()
+
+
 def _is_int8(name, what, q):
     if type(q) is not Int8:
         raise TypeError(f"{name}: {what} must be an Int8 (quantize_int8, add_rmsnorm_int8, pack_int8), got "
@@ -1602,10 +1611,11 @@ def quantize_int8(x):
     else:
         x, ldx = _rows_of(x, k)
         M = x.shape[0]
-    with _dev_guard(x):
-        q = _new_int8(x, shape[:-1], k, dt)
-        rc = _lib.load().mtl_quantize_int8(x.data_ptr(), ldx, q.codes.data_ptr(), q.scales.data_ptr(), M, k, code,
-                                           _stream(x))
+    if _other_device(x):
+        with torch.cuda.device(x.device):
+            return quantize_int8(x.view(shape))
+    q = _new_int8(x, shape[:-1], k, dt)
+    rc = _lib.load().mtl_quantize_int8(x.data_ptr(), ldx, q.codes.data_ptr(), q.scales.data_ptr(), M, k, code, _stream(x))
     if rc:
         _lib.check(rc, "quantize_int8")
     return q
@@ -1641,11 +1651,13 @@ def add_rmsnorm_int8(x, weight, eps, y=None, x_out=None, dtype=torch.float32):
                 raise ValueError("x_out must be x, a float32 y, or overlap no operand")
     _int8_call("add_rmsnorm_int8", x, weight, y, x_out)
     _same_device(x, weight, y, x_out)
-    with _dev_guard(x):
-        q = _new_int8(x, shape[:-1], k, dtype)
-        a = _lib.AddRmsnormInt8Args(x.data_ptr(), _ptr(y), _ptr(x_out), weight.data_ptr(), q.codes.data_ptr(),
-                                    q.scales.data_ptr(), x.numel() // k, k, float(eps), y_code, w_code, 0)
-        rc = _lib.load().mtl_add_rmsnorm_int8(ctypes.byref(a), _stream(x))
+    if _other_device(x):
+        with torch.cuda.device(x.device):
+            return add_rmsnorm_int8(x, weight, eps, y, x_out, dtype)
+    q = _new_int8(x, shape[:-1], k, dtype)
+    a = _lib.AddRmsnormInt8Args(x.data_ptr(), _ptr(y), _ptr(x_out), weight.data_ptr(), q.codes.data_ptr(),
+                                q.scales.data_ptr(), x.numel() // k, k, float(eps), y_code, w_code, 0)
+    rc = _lib.load().mtl_add_rmsnorm_int8(ctypes.byref(a), _stream(x))
     if rc:
         _lib.check(rc, "add_rmsnorm_int8")
     return q
@@ -1654,8 +1666,9 @@ def add_rmsnorm_int8(x, weight, eps, y=None, x_out=None, dtype=torch.float32):
 def linear_int8(x, w, bias=None, out=None):
     """x [..., k] W^T (+ bias [n]) of an Int8 x and an Int8 matrix W [n, k] (mtl_linear_int8): [..., n] of x's type.  The
     sum over k is exact; it is multiplied by the two scales in float32.  bias and out have x's type."""
-    _is_int8("linear_int8", "x", x)
-    _is_int8("linear_int8", "w", w)
+    if type(x) is not Int8 or type(w) is not Int8:
+        _is_int8("linear_int8", "x", x)
+        _is_int8("linear_int8", "w", w)
     k, dt, lead = x.k, x.dtype, x.scales.shape
     if w.k != k or w.scales.dim() != 1:
         raise ValueError(f"w must be [n, {k}], got {tuple(w.shape)}")
@@ -1685,12 +1698,14 @@ def linear_int8(x, w, bias=None, out=None):
             raise ValueError("out must not overlap an operand")
         if out.dim() == 2 and M > 1:
             ldy = out.stride(0)
-    with _dev_guard(codes):
-        if out is None:
-            out = codes.new_empty((*lead, n), dtype=dt)
-        a = _lib.LinearInt8Args(codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias),
-                                out.data_ptr(), ldy, M, n, k, _ACT_DTYPES[dt], 0)
-        rc = _lib.load().mtl_linear_int8(ctypes.byref(a), _stream(codes))
+    if _other_device(codes):
+        with torch.cuda.device(codes.device):
+            return linear_int8(x, w, bias, out)
+    if out is None:
+        out = codes.new_empty((*lead, n), dtype=dt)
+    a = _lib.LinearInt8Args(codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias),
+                            out.data_ptr(), ldy, M, n, k, _ACT_DTYPES[dt], 0)
+    rc = _lib.load().mtl_linear_int8(ctypes.byref(a), _stream(codes))
     if rc:
         _lib.check(rc, "linear_int8")
     return out
@@ -1698,7 +1713,8 @@ def linear_int8(x, w, bias=None, out=None):
 
 def dequantize_int8(q, dtype=None, out=None):
     """The values [..., k] that an Int8 stands for, in its type or `dtype` (mtl_dequantize_int8)."""
-    _is_int8("dequantize_int8", "q", q)
+    if type(q) is not Int8:
+        _is_int8("dequantize_int8", "q", q)
     dt = q.dtype if dtype is None else dtype
     if dt not in _ACT_DTYPES:
         raise TypeError(f"dtype must be float32 or bfloat16, got {dt}")
@@ -1714,11 +1730,13 @@ def dequantize_int8(q, dtype=None, out=None):
             raise ValueError("out must not overlap an operand")
         if out.dim() == 2 and M > 1:
             ldo = out.stride(0)
-    with _dev_guard(codes):
-        if out is None:
-            out = codes.new_empty((*lead, k), dtype=dt)
-        rc = _lib.load().mtl_dequantize_int8(codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), ldo, M, k,
-                                             _ACT_DTYPES[dt], _stream(codes))
+    if _other_device(codes):
+        with torch.cuda.device(codes.device):
+            return dequantize_int8(q, dt, out)
+    if out is None:
+        out = codes.new_empty((*lead, k), dtype=dt)
+    rc = _lib.load().mtl_dequantize_int8(codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), ldo, M, k, _ACT_DTYPES[dt],
+                                         _stream(codes))
     if rc:
         _lib.check(rc, "dequantize_int8")
     return out

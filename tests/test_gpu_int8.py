@@ -200,6 +200,56 @@ def test_linear_matches_float64(m, n, k, dtype):
     assert torch.equal(y, ops.linear_int8(x, w, bias))          # the same bits every time
 
 
+# (one of each form that mtl_linear_int8 chooses, with partial tiles; the last is a chain of tiles over partial ones)
+FORMS = [(40, 70, 200), (5, 100, 4100), (17, 24700, 200), (250, 2001, 300), (250, 8100, 130), (500, 8101, 300),
+         (1000, 8100, 300), (6001, 8203, 300), (6000, 8200, 1025), (33000, 700, 250), (33000, 2100, 129)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("m,n,k", FORMS)
+def test_every_form_matches_float64(m, n, k, bias, dtype):
+    x, xc, xs = _matrix(m, k, m + k, dtype)
+    w, wc, ws = _matrix(n, k, n + k)
+    b = torch.randn(n, device="cuda", generator=_gen(7)).to(dtype) if bias else None
+    for out in (None, torch.full((m, n + 5), 3.0, device="cuda", dtype=dtype)):       # (rows on 16 bytes or not)
+        y = ops.linear_int8(x, w, b, out=None if out is None else out[:, 2:n + 2])
+        if out is not None:
+            assert bool((out[:, :2] == 3.0).all()) and bool((out[:, n + 2:] == 3.0).all())
+        for i in range(0, m, 4096):
+            ref, off = _reference(xc[i:i + 4096], wc, xs[i:i + 4096], ws, b)
+            got = y[i:i + 4096].double()
+            assert bool(((got - ref).abs() <= off + HALF[dtype] * (ref.abs() + off)).all())
+    first = ops.linear_int8(x, w, b)
+    assert all(torch.equal(first, ops.linear_int8(x, w, b)) for _ in range(3))
+
+
+def test_offsets_past_32_bits():
+    # codes of 8.6 GB, and an output of 2.4e9 values
+    n, k = 1 << 20, 8192
+    codes = torch.randint(-127, 128, (n, k), device="cuda", generator=_gen(0), dtype=torch.int8)
+    w = ops.Int8(codes, torch.full((n,), 0.01, device="cuda"), k)
+    for m in (1, 40):
+        x, xc, xs = _matrix(m, k, m)
+        y = ops.linear_int8(x, w)
+        for rows in (slice(0, 100), slice(n - 100, n)):
+            ref, off = _reference(xc, codes[rows].double(), xs, w.scales[rows].double(), None)
+            assert bool(((y[:, rows].double() - ref).abs() <= off + HALF[torch.float32] * ref.abs()).all())
+    back = ops.dequantize_int8(w, torch.bfloat16)
+    for rows in (slice(0, 5), slice(n - 5, n)):
+        assert torch.equal(back[rows], (codes[rows].float() * w.scales[rows, None]).bfloat16())
+    q = ops.quantize_int8(back)
+    for rows in (slice(0, 5), slice(n - 5, n)):
+        assert torch.equal(q.codes[rows].double(), _codes(back[rows].float())[0])
+    del codes, w, back, q
+    x, xc, xs = _matrix(40000, 128, 1)
+    w, wc, ws = _matrix(60000, 128, 2)
+    y = ops.linear_int8(x, w)
+    for rows in (slice(0, 64), slice(39936, 40000)):
+        ref, off = _reference(xc[rows], wc, xs[rows], ws, None)
+        assert bool(((y[rows].double() - ref).abs() <= off + HALF[torch.float32] * ref.abs()).all())
+
+
 def test_sums_are_exact_at_the_largest_codes():
     k = 131071
     for a, b in ((127, 127), (-127, 127), (-128, -128)):
