@@ -30,12 +30,12 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(Lds)p);
 }
 #if defined(__HIP_DEVICE_COMPILE__)
-#define MTL_COPY_TO_LDS(WIDTH, base, off, to)                                                                        \
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_" WIDTH " %0, %1" ::"v"(off), "s"(base),           \
+#define MTL_COPY_TO_LDS(WIDTH, HINT, base, off, to)                                                                  \
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_" WIDTH " %0, %1" HINT ::"v"(off), "s"(base),      \
                  "s"(lds_address(to))                                                                                \
                  : "m0")
 #else
-#define MTL_COPY_TO_LDS(WIDTH, base, off, to) (void)(base), (void)(off), (void)(to)
+#define MTL_COPY_TO_LDS(WIDTH, HINT, base, off, to) (void)(base), (void)(off), (void)(to)
 #endif
 
 // a pointer that is the same for the whole wavefront, in SGPRs
@@ -53,7 +53,9 @@ template <typename P> __device__ __forceinline__ const P* uniform(const P* p) {
 // the next one's first are on their way, and its first fragments are read before the tile is written.  The tiles' own starts
 // and ends took 93 of the 526 us of 32768 x 8192 x 2048.  Three stages of K at least: the next tile's scales go where the
 // last one's were, and a barrier has to stand between.
-template <typename T, int BN, int BM, int WN, int WM, int ST, int OCC, bool CHAIN>
+//
+// ONCE: no other workgroup reads these rows of W, which go past the caches (16 x 50280 x 2048 21.2 -> 18.7 us).
+template <typename T, int BN, int BM, int WN, int WM, int ST, int OCC, bool CHAIN, bool ONCE>
 __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_kernel(const LinearArgs a) {
     constexpr int NWM = BM / WM, NW = BN / WN * NWM, NT = NW * 64;
     constexpr int TJ = WN / 16, TI = WM / 16, KB = kInt8Pad, KS = 2;      // MFMA tiles of a wavefront; steps of a stage
@@ -106,7 +108,8 @@ __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_ker
         const int8_t* base = (isw ? wt : xt) + (uint32_t)s * KB;
         const int row = min(row8 + 8 * g - (isw ? 0 : BN), isw ? wlast : xlast);
         const uint32_t off = __umul24(row, a.Kp) + (chunk ^ (g & 1) << 6);        // (256 rows, Kp <= 2^17)
-        MTL_COPY_TO_LDS("dwordx4", base, off, ring + slot * STAGE + g * 1024);
+        if (ONCE && isw) MTL_COPY_TO_LDS("dwordx4", " nt", base, off, ring + slot * STAGE + g * 1024);
+        else MTL_COPY_TO_LDS("dwordx4", "", base, off, ring + slot * STAGE + g * 1024);
     };
     // the tile's scales, 64 to a wavefront
     auto issue_scales = [&](int m, int n, float* to) __attribute__((always_inline)) {
@@ -114,7 +117,7 @@ __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_ker
         const int at = threadIdx.x - (col ? 0 : BN);
         const float* base = uniform(col ? a.sw + n : a.sx + m);
         const uint32_t off = 4u * (uint32_t)min(at, col ? a.N - 1 - n : a.M - 1 - m);
-        MTL_COPY_TO_LDS("dword", base, off, to + wave * 64);
+        MTL_COPY_TO_LDS("dword", "", base, off, to + wave * 64);
     };
 
     I4 acc[TJ][TI];
@@ -322,14 +325,15 @@ template <int NW> int launch_stream(const LinearArgs& a, bool f32, hipStream_t s
     return check_launch("linear_int8");
 }
 
-template <int BN, int BM, int WN, int WM, int ST, int OCC, bool CHAIN = false> int launch(LinearArgs a, bool f32, hipStream_t st) {
+template <int BN, int BM, int WN, int WM, int ST, int OCC, bool CHAIN = false, bool ONCE = false>
+int launch(LinearArgs a, bool f32, hipStream_t st) {
     const int64_t tm = (a.M + (int64_t)BM - 1) / BM, tn = (a.N + (int64_t)BN - 1) / BN;
     MTL_REQUIRE(tm * tn < (int64_t(1) << 31), "too many output tiles");
     a.tm = (int)tm;
     a.tn = (int)tn;
     const dim3 grid((unsigned)(CHAIN ? std::min<int64_t>(tm * tn, 256) : tm * tn)), nt(BN / WN * (BM / WM) * 64);
-    if (f32) hipLaunchKernelGGL((linear_int8_kernel<float, BN, BM, WN, WM, ST, OCC, CHAIN>), grid, nt, 0, st, a);
-    else hipLaunchKernelGGL((linear_int8_kernel<uint16_t, BN, BM, WN, WM, ST, OCC, CHAIN>), grid, nt, 0, st, a);
+    if (f32) hipLaunchKernelGGL((linear_int8_kernel<float, BN, BM, WN, WM, ST, OCC, CHAIN, ONCE>), grid, nt, 0, st, a);
+    else hipLaunchKernelGGL((linear_int8_kernel<uint16_t, BN, BM, WN, WM, ST, OCC, CHAIN, ONCE>), grid, nt, 0, st, a);
     return check_launch("linear_int8");
 }
 
@@ -358,10 +362,12 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     const int64_t pairs = ((a.N + 15) / 16) * (int64_t)((a.M + 15) / 16);
     if (pairs <= (a.M <= 16 ? 512 : 256))
         return a.Kp > 2048 ? launch_stream<8>(a, f32, st) : launch_stream<4>(a, f32, st);
-    // Up to 64 rows of a wide W, bound by its stream: 16x50280x2048 21.0 (tiles of 64 24.6, of 32 22.1), 64 rows 23.8 (27.1,
-    // 34.1)
+    // Up to 64 rows of a wide W, bound by its stream, in one tile of rows: 16x50280x2048 18.7 (128 x 64 19.2, 64 x 64 23.4, 32 x
+    // 32 19.6), 64 rows 22.0 (64 x 64 26.0, 32 x 32 34.7); 16x24000x1024 6.9 (7.6 with the rule below), 16x8192x2048 9.5 (6.7).
     const auto tiles = [&](int bn, int bm) { return ((a.N + (int64_t)bn - 1) / bn) * ((a.M + (int64_t)bm - 1) / bm); };
-    if (a.M <= 64 && tiles(128, 64) >= 192) return launch<128, 64, 32, 32, 3, 2>(a, f32, st);
+    if (a.M <= 64 && tiles(128, 64) >= 160)
+        return a.M <= 32 ? launch<128, 32, 32, 32, 4, 2, false, true>(a, f32, st)
+                         : launch<128, 64, 32, 32, 3, 2, false, true>(a, f32, st);
     // Others by the time that a tile's rounds over the 256 CUs take, in units of one of 256 x 128 tiles (K 2048: 22.5 us);
     // the small tiles share a CU.  us with 256 x 256, 256 x 128, 128 x 128, 64 x 64, 32 x 32 (N x M):
     //   1024x8192x2048 31.9 22.5 27.7 32.3 53.5; 512x8192x2048 27.8 18.5 13.1 16.7 27.4; 4096x8192x2048 77.9 88.4 124.7 150
