@@ -269,29 +269,37 @@ __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_ker
 }
 
 // Few rows of x, bound by the stream of W and by latency: nothing is shared.  NW wavefronts take 16 columns by 16 rows of y
-// together, each a run of K, straight from memory to registers with 4 steps of 64 columns on their way, and add their sums.
-// (32 columns or rows to a workgroup: 1x768x1536 3.0 us -> 4.0 and 3.3.  W loaded as nontemporal: 3.6, its lines come twice.)
+// together, each a run of K, straight from memory to registers with 2 steps of 128 columns on their way, and add their sums.
+// A lane takes 32 bytes of its row in a step (the order of K is free where both operands have the same): whole 128-byte
+// lines of 16 rows.  us, 16 bytes at a time with 4 steps of 64 columns: 16x8192x2048 7.2 -> 6.6, 64x768x1536 4.1 -> 3.6.
+// (32 columns or rows to a workgroup: 1x768x1536 3.0 -> 4.0 and 3.3.  W past the caches 3.2: its lines are read twice.)
 template <typename T, int NW> __global__ void __launch_bounds__(NW * 64) stream_int8_kernel(const LinearArgs a) {
-    constexpr int U = 4;
+    constexpr int U = 2;
     __shared__ __align__(16) I4 s_acc[NW][64];
     const int lane = threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
-    const int8_t* w = a.w + (int64_t)min(n0 + r16, a.N - 1) * a.Kp + 16 * g4;
-    const int8_t* x = a.x + (int64_t)min(m0 + r16, a.M - 1) * a.Kp + 16 * g4;
-    const int steps = a.Kp / 64, per = (steps + NW - 1) / NW, s0 = wave * per, s1 = min(s0 + per, steps);
-    I4 acc = {0, 0, 0, 0}, fw[U], fx[U];
+    const int8_t* w = a.w + (int64_t)min(n0 + r16, a.N - 1) * a.Kp + 32 * g4;
+    const int8_t* x = a.x + (int64_t)min(m0 + r16, a.M - 1) * a.Kp + 32 * g4;
+    const int steps = a.Kp / 128, per = (steps + NW - 1) / NW, s0 = wave * per, s1 = min(s0 + per, steps);
+    I4 acc = {0, 0, 0, 0}, fw[U][2], fx[U][2];
     auto load = [&](int u, int s) __attribute__((always_inline)) {
-        const int k = min(s, steps - 1) * 64;                   // (past the run: loaded, never used)
-        fw[u] = *reinterpret_cast<const I4*>(w + k);
-        fx[u] = *reinterpret_cast<const I4*>(x + k);
+        const int k = min(s, steps - 1) * 128;                  // (past the run: loaded, never used)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            fw[u][h] = *reinterpret_cast<const I4*>(w + k + 16 * h);
+            fx[u][h] = *reinterpret_cast<const I4*>(x + k + 16 * h);
+        }
     };
 #pragma unroll
     for (int u = 0; u < U; ++u) load(u, s0 + u);
     for (int s = s0; s < s1; s += U) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (s + u < s1) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], fx[u], acc, 0, 0, 0);
+            if (s + u < s1) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u][h], fx[u][h], acc, 0, 0, 0);
+            }
             if (s + U < s1) load(u, s + U + u);
         }
     }
@@ -356,12 +364,12 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     LinearArgs a{p->x, p->x_scales, p->w, p->w_scales, p->bias, p->y, p->ldy, (int)p->M, (int)p->N, (int)int8_row(p->K),
                  0, 0, al16(p->y) && p->ldy * (f32 ? 4 : 2) % 16 == 0, p->dtype == MTL_BF16};
     const hipStream_t st = as_stream(stream);
-    // Few rows: the stream.  us at rows x N x K, bf16: 1x768x1536 3.0, tiles of 32 4.2; 64x768x1536 3.7 / 4.3, 128x768x1536
-    // 5.5 / 4.4; 1x8192x2048 5.3 / 5.6, 32x8192x2048 9.7 / 5.9.  Eight wavefronts on long rows: 1x2048x4096 4.8, four 5.1;
-    // 16x1536x768 3.3, four 2.8.
+    // Few rows: the stream.  us at rows x N x K, bf16, W from HBM: 1x768x1536 3.0, tiles of 32 4.5; 64x768x1536 3.6 / 4.6;
+    // 1x8192x2048 5.4 / 6.3, 16x8192x2048 6.7 / 6.6, 16x2048x4096 6.4 / 8.9; 128x768x1536 5.5 / 4.4, 32x8192x2048 9.7 / 5.9.
+    // Eight wavefronts from 1536 columns on: 1x768x1536 3.4 with four; 1x1536x768 2.9, with eight 3.0; 33x1001x777 3.4 / 3.9.
     const int64_t pairs = ((a.N + 15) / 16) * (int64_t)((a.M + 15) / 16);
     if (pairs <= (a.M <= 16 ? 512 : 256))
-        return a.Kp > 2048 ? launch_stream<8>(a, f32, st) : launch_stream<4>(a, f32, st);
+        return a.Kp >= 1536 ? launch_stream<8>(a, f32, st) : launch_stream<4>(a, f32, st);
     // Up to 64 rows of a wide W, bound by its stream, in one tile of rows: 16x50280x2048 18.7 (128 x 64 19.2, 64 x 64 23.4, 32 x
     // 32 19.6), 64 rows 22.0 (64 x 64 26.0, 32 x 32 34.7); 16x24000x1024 6.9 (7.6 with the rule below), 16x8192x2048 9.5 (6.7).
     const auto tiles = [&](int bn, int bm) { return ((a.N + (int64_t)bn - 1) / bn) * ((a.M + (int64_t)bm - 1) / bm); };
