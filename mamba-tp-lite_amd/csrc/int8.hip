@@ -12,7 +12,7 @@ namespace {
 __device__ __forceinline__ int code_of(float t, float a) { return (int)rint((double)t * 127.0 / (double)a); }
 
 // The same without 64 bits, for a in [kLeast, kMost] and inv = 127 / a rounded: t inv is off by less than 2e-5, so its
-// rounding is the code unless it comes within kNear of a half h = c + 1/2.  There 127 |t| - h a decides, and is exact:
+// rounding is the code unless it comes within 3e-5 of a half h = c + 1/2.  There 127 |t| - h a decides, and is exact:
 // 127 |t| = p + pl in two floats; p and h a are whole multiples of half an ulp of a and 2^10 of those apart at most, pl is
 // 2^-8 of that.
 constexpr float kLeast = 0x1p-90f, kMost = 0x1p120f, kNear = 0.5f - 3e-5f;
@@ -69,44 +69,53 @@ __device__ __forceinline__ float row_scale(uint32_t most, float r) {
     return most < 0x7f800000u ? __uint_as_float(most) * r / 127.f : __uint_as_float(0x7fc00000u);
 }
 
-// 8 codes of a row of largest magnitude a, as 8 bytes (exact: a is outside [kLeast, kMost])
+// 8 codes of a row of largest magnitude a, as 8 bytes (exact: a is outside [kLeast, kMost]).  One fma rounds t inv + 1.5 2^23
+// to a whole number whose low byte is the code.  (t inv rounded, its nearest whole number and that as an integer, with one
+// maximum of magnitudes in place of two of bits: 32768 x 2048 in bf16 41 us; 35 now.)
 __device__ __forceinline__ uint2 run_codes(const float* t, float a, float inv, bool exact) {
+#pragma clang fp contract(off)
+    constexpr float kWhole = 12582912.f;
     float c[kRun];
     if (exact) {
 #pragma unroll 1
-        for (int j = 0; j < kRun; ++j) c[j] = (float)code_of(t[j], a);
+        for (int j = 0; j < kRun; ++j) c[j] = (float)code_of(t[j], a) + kWhole;
     } else {
-        bool near = false;
-        float q[kRun];
+        float off = 0.f;
 #pragma unroll
         for (int j = 0; j < kRun; ++j) {
-            q[j] = t[j] * inv;
-            c[j] = rintf(q[j]);
-            near |= fabsf(q[j] - c[j]) > kNear;
+            c[j] = fmaf(t[j], inv, kWhole);
+            off = fmaxf(off, fabsf(fmaf(t[j], inv, kWhole - c[j])));
         }
-        if (near) {
+        if (off > kNear) {
 #pragma unroll
             for (int j = 0; j < kRun; ++j)
-                if (fabsf(q[j] - c[j]) > kNear) c[j] = near_code(t[j], a, q[j]);
+                if (fabsf(fmaf(t[j], inv, kWhole - c[j])) > kNear) c[j] = near_code(t[j], a, t[j] * inv) + kWhole;
         }
     }
-    uint32_t b[2] = {0, 0};
+    uint32_t b[2];
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) b[j / 4] |= ((uint32_t)(int)c[j] & 0xffu) << (8 * (j % 4));
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(c[4 * h + 1]), __float_as_uint(c[4 * h]), 0x0c0c0400);
+        const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(c[4 * h + 3]), __float_as_uint(c[4 * h + 2]), 0x04000c0c);
+        b[h] = lo | hi;
+    }
     return uint2{b[0], b[1]};
 }
 
-// Rows held in registers from one pass over memory: G threads to a row, RU runs of 8 columns to a thread (Kp <= 8 G RU).
+// Rows held in registers from one pass over memory: as many wavefronts to a row as RU runs of 8 columns a lane need, or ONE.
 // HBM is the bound.
-template <typename T, typename Y, typename W, bool NORM, int G, int RU>
-__global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_kernel(const RowsArgs p) {
+constexpr int kRowThreads = 512;
+template <typename T, typename Y, typename W, bool NORM, bool ONE, int RU>
+__global__ void __launch_bounds__(ONE ? 256 : kRowThreads) quantize_kernel(const RowsArgs p) {
 #pragma clang fp contract(off)
-    constexpr int NT = G < 256 ? 256 : G, NW = G / 64;
-    __shared__ uint32_t s_max[NT / 64];
-    __shared__ float s_sum[NT / 64];
-    const int64_t row = (int64_t)blockIdx.x * (NT / G) + threadIdx.x / G;
-    const int t = threadIdx.x % G;
-    if (row >= p.M) return;                                   // (whole wavefronts; G > 64: one row)
+    constexpr int NW = ONE ? 4 : kRowThreads / 64;
+    const int G = ONE ? 64 : (int)blockDim.x;
+    __shared__ uint32_t s_max[NW];
+    __shared__ float s_sum[NW];
+    __shared__ __align__(16) float s_out[NORM ? NW : 1][64 * kRun];
+    const int64_t row = ONE ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : blockIdx.x;
+    const int t = ONE ? threadIdx.x % 64 : threadIdx.x;
+    if (row >= p.M) return;                                   // (whole wavefronts)
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     const bool add = NORM && p.y;
     float v[RU][kRun], wv[RU][kRun];
@@ -129,42 +138,59 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_kernel(const RowsA
 #pragma unroll
             for (int j = 0; j < kRun; ++j) v[u][j] += yv[u][j];
     }
-    uint32_t most = 0;
+    if constexpr (NORM) {
+        if (p.x_out) {
+            // through LDS, so that an instruction stores whole lines: 32768 x 2048 with bf16 y 135 -> 121 us (6.1 TB/s).  Past the
+            // caches, as it is read again a layer later only: 131 without, 1024 x 2048 7.2 -> 6.5.
+            const int lane = t & 63, k0 = (t - lane) * kRun;
+            float* s = s_out[threadIdx.x / 64];
+#pragma unroll
+            for (int u = 0; u < RU; ++u) {
+                st4(s + lane * kRun, F4v{v[u][0], v[u][1], v[u][2], v[u][3]});
+                st4(s + lane * kRun + 4, F4v{v[u][4], v[u][5], v[u][6], v[u][7]});
+                wave_lds_fence();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int at = 256 * i + 4 * lane, k = u * G * kRun + k0 + at;
+                    const F4v o = ld4(s + at);
+                    float* d = p.x_out + row * p.K + k;
+                    if (k + 4 <= p.K) {
+                        __builtin_nontemporal_store(F4u{o[0], o[1], o[2], o[3]}, reinterpret_cast<F4u*>(d));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (k + j < p.K) d[j] = o[j];
+                    }
+                }
+                wave_lds_fence();
+            }
+        }
+    }
+    int above = 0;                                            // bits of the largest positive value and of the least
+    uint32_t below = 0;                                       // negative one (of the largest, where there is none)
     float ss = 0.f;
 #pragma unroll
     for (int u = 0; u < RU; ++u) {
         const int k = (u * G + t) * kRun;
         if (k < p.K) {
-            if constexpr (NORM) {
-                if (p.x_out) {
-                    float* o = p.x_out + row * p.K + k;
-                    if (k + kRun <= p.K) {
-                        // (read again a layer later only: past the caches, 1024 x 2048 7.2 -> 6.5 us)
-                        __builtin_nontemporal_store(F4u{v[u][0], v[u][1], v[u][2], v[u][3]}, reinterpret_cast<F4u*>(o));
-                        __builtin_nontemporal_store(F4u{v[u][4], v[u][5], v[u][6], v[u][7]}, reinterpret_cast<F4u*>(o + 4));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < kRun; ++j)
-                            if (k + j < p.K) o[j] = v[u][j];
-                    }
-                }
-            }
 #pragma unroll
             for (int j = 0; j < kRun; ++j) {
                 if constexpr (NORM) {
                     ss = fmaf(v[u][j], v[u][j], ss);
                     v[u][j] *= wv[u][j];
                 }
-                most = max(most, abs_bits(v[u][j]));
+                const uint32_t b = __float_as_uint(v[u][j]);
+                above = max(above, (int)b);
+                below = max(below, b);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < kRun; ++j) v[u][j] = 0.f;
         }
     }
-    most = group_umax<64>(most);
+    uint32_t most = group_umax<64>(max((uint32_t)above, below & 0x7fffffffu));
     if constexpr (NORM) ss = group_sum<64>(ss);
-    if constexpr (G > 64) {
+    if constexpr (!ONE) {
         if (t % 64 == 0) {
             s_max[t / 64] = most;
             s_sum[t / 64] = ss;
@@ -174,6 +200,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_kernel(const RowsA
         ss = s_sum[0];
 #pragma unroll
         for (int i = 1; i < NW; ++i) {
+            if (i >= G / 64) break;
             most = max(most, s_max[i]);
             ss += s_sum[i];
         }
@@ -267,18 +294,17 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_kernel(const RowsA
 }
 
 template <typename T, typename Y, typename W, bool NORM> int launch_rows(const RowsArgs& a, hipStream_t st) {
-#define MTL_ROWS(G, RU)                                                                                              \
-    hipLaunchKernelGGL((quantize_kernel<T, Y, W, NORM, G, RU>), dim3((unsigned)((a.M + (G < 256 ? 256 / G : 1) - 1) / \
-                                                                                (G < 256 ? 256 / G : 1))),            \
-                       dim3(G < 256 ? 256 : G), 0, st, a)
+#define MTL_ROWS(ONE, RU)                                                                                              \
+    hipLaunchKernelGGL((quantize_kernel<T, Y, W, NORM, ONE, RU>), dim3((unsigned)(ONE ? (a.M + 3) / 4 : a.M)),           \
+                       dim3(ONE ? 256 : (a.Kp + 512 * RU - 1) / (512 * RU) * 64), 0, st, a)
     // A wavefront to a row of up to 1024 columns where there are many; otherwise so many that a lane has one run, or two or
-    // four of long rows.  Norms, us: 32768 x 2048 with bf16 y 148 with a wavefront, 133 with four; 32768 x 768 58, 60.
-    if (a.Kp <= 512 && a.M >= 1024) MTL_ROWS(64, 1);
-    else if (a.Kp <= 1024 && a.M >= 1024) MTL_ROWS(64, 2);
-    else if (a.Kp <= 2048) MTL_ROWS(256, 1);
-    else if (a.Kp <= 4096) MTL_ROWS(256, 2);
-    else if (a.Kp <= 8192) MTL_ROWS(256, 4);
-    else if (a.Kp <= 16384) MTL_ROWS(512, 4);
+    // four of long rows.  us: norms of 32768 x 2048 with bf16 y 148 with a wavefront, 133 with four; 32768 x 768 58, 60; rows
+    // of 4096 in bf16, 32768 of them 71 with two runs, 83 with one; 8 of them 3.5, 3.1; 8192 x 8192 34 with two, 36 with four.
+    if (a.Kp <= 512 && a.M >= 1024) MTL_ROWS(true, 1);
+    else if (a.Kp <= 1024 && a.M >= 1024) MTL_ROWS(true, 2);
+    else if (a.Kp <= (a.M <= 1024 ? 4096 : 2048)) MTL_ROWS(false, 1);
+    else if (a.Kp <= 8192) MTL_ROWS(false, 2);
+    else if (a.Kp <= 16384) MTL_ROWS(false, 4);
     else hipLaunchKernelGGL((quantize_long_kernel<T, Y, W, NORM>), dim3((unsigned)a.M), dim3(kLongThreads), 0, st, a);
 #undef MTL_ROWS
     return check_launch(NORM ? "add_rmsnorm_int8" : "quantize_int8");

@@ -31,7 +31,8 @@ def _matrix(n, k, seed, dtype=torch.float32):
 
 # ------------------------------------------------------------------ rows into codes
 ROWS = [(1, 1), (1, 768), (3, 5), (2, 127), (4, 128), (5, 129), (7, 777), (33, 1536), (1, 2048), (9, 2049), (8, 4096),
-        (5, 4100), (300, 1000), (3, 8192), (2, 16391), (1, 40000), (1, 131071), (0, 64), (70000, 3)]
+        (5, 4100), (300, 1000), (3, 8192), (2, 16391), (1, 40000), (1, 131071), (0, 64), (70000, 3),
+        (1025, 129), (1026, 1000), (1500, 1801), (1030, 2500), (1025, 4096), (6, 5121), (3, 9001), (2, 16384)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
