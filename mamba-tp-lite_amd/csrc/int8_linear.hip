@@ -376,19 +376,33 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     if (a.M <= 64 && tiles(128, 64) >= 160)
         return a.M <= 32 ? launch<128, 32, 32, 32, 4, 2, false, true>(a, f32, st)
                          : launch<128, 64, 32, 32, 3, 2, false, true>(a, f32, st);
-    // Others by the time that a tile's rounds over the 256 CUs take, in units of one of 256 x 128 tiles (K 2048: 22.5 us);
-    // the small tiles share a CU.  us with 256 x 256, 256 x 128, 128 x 128, 64 x 64, 32 x 32 (N x M):
-    //   1024x8192x2048 31.9 22.5 27.7 32.3 53.5; 512x8192x2048 27.8 18.5 13.1 16.7 27.4; 4096x8192x2048 77.9 88.4 124.7 150
-    //   227; 4096x2048x4096 51.6 37.1 43.4 53.5 93.8; 1024x2048x4096 48.9 30.0 19.6 15.7 26.2; 256x2048x4096 46.5 28.5 18.3
-    //   11.4 9.8; 4096x768x1536 25.0 16.6 11.7 12.0 18.6; 512x768x1536 22.1 14.4 9.6 6.5 5.5
-    const auto rounds = [&](int bn, int bm) { return (double)((tiles(bn, bm) + 255) / 256); };
-    const double cost[5] = {a.Kp > 2 * kInt8Pad ? 1.72 * rounds(256, 256) : 1e9, 1.0 * rounds(256, 128), 0.58 * rounds(128, 128),
-                            0.15 + 0.14 * rounds(64, 64), 0.12 + 0.07 * rounds(32, 32)};
-    switch (std::min_element(cost, cost + 5) - cost) {
+    // Others by the time that their tiles take on the 256 CUs, in us at bf16 and fp32 sizes of up to 32768 rows: each round of a
+    // tile per CU has its start and end (longer where rows of y are not 16-byte aligned, or floats) and its stages of K; two
+    // or more tiles share a CU, and a round of them has the traffic of all.  Measured at 231 sizes with every tile, the choice
+    // takes 1% more than the best of them (a cost by rounds alone took 6% more); us with the tiles in the table's order:
+    //   bf16 1024x8192x2048 - 22.9 26.9 33.8 - 23.2; fp32 8192x768x1536 - 19.6 25.7 25.0 - 18.8; 1179x2304x4480 56.3 33.6 23.5 28.0
+    //   39.7 32.1; 720x1167x3393 54.1 30.8 19.9 14.0 15.7 27.9; fp32 657x576x1280 24.5 14.5 9.6 6.1 5.2 11.0; fp32
+    //   14280x1685x1184 60.4 70.8 72.9 73.0 111.9 58.2; 32768x8192x2048 496 by the first, 580 by the second
+    constexpr struct { int bn, bm, share; double start, round, stage, loose, floats, traffic; } kTiles[6] = {
+        {256, 256, 1, 0.05, 8.59, 1.39, 5.61, 2.35, 0.0}, {256, 128, 1, 1.01, 6.12, 0.79, 2.79, 0.97, 0.0},
+        {128, 128, 1, 1.14, 3.97, 0.49, 1.07, 0.67, 0.0}, {64, 64, 3, 2.58, 0.64, 0.09, 0.16, 0.26, 0.26},
+        {32, 32, 4, 1.98, 0.50, 0.05, 0.04, 0.01, 0.15},  {128, 128, 2, 1.33, 2.11, 0.06, 1.04, 0.71, 0.78}};
+    const int stages = a.Kp / kInt8Pad;
+    int best = 0;
+    double least = 0;
+    for (int i = stages > 2 ? 0 : 1; i < 6; ++i) {
+        const auto& t = kTiles[i];
+        const int64_t count = tiles(t.bn, t.bm), rounds = (count + 255) / 256, full = (count + 256 * t.share - 1) / (256 * t.share);
+        const double us = t.start + rounds * (t.round + t.stage * stages + (a.vec ? 0 : t.loose) + (f32 ? t.floats : 0)) +
+                          full * t.traffic * stages;
+        if (least == 0 || us < least) { least = us; best = i; }
+    }
+    switch (best) {
         case 0: return launch<256, 256, 128, 64, 2, 1, true>(a, f32, st);
         case 1: return launch<256, 128, 64, 64, 3, 1>(a, f32, st);
         case 2: return launch<128, 128, 64, 32, 4, 1>(a, f32, st);
         case 3: return launch<64, 64, 32, 32, 3, 3>(a, f32, st);
-        default: return launch<32, 32, 16, 16, 5, 4>(a, f32, st);
+        case 4: return launch<32, 32, 16, 16, 5, 4>(a, f32, st);
+        default: return launch<128, 128, 32, 64, 2, 2>(a, f32, st);
     }
 }
