@@ -327,6 +327,15 @@ class LinearInt8(nn.Module):
         finally:
             self.scales = nn.Parameter(self.scales.view(torch.float32), requires_grad=False)
 
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        # a matrix of floats may have the codes' shape, and copying it would cut it to whole numbers
+        for name, dtype, what in (("weight", torch.int8, "8-bit codes"), ("scales", torch.float32, "float32")):
+            t = state_dict.get(prefix + name)
+            if t is not None and t.dtype != dtype:
+                error_msgs.append(f"{prefix}{name} must be {what}, got {t.dtype}: load the model before quantize_int8")
+                return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+
     def int8(self, start: int = 0, stop: int | None = None) -> ops.Int8:
         """Rows [start, stop) of the weight."""
         return ops.Int8(self.weight[start:stop].detach(), self.scales[start:stop].detach(), self.in_features)

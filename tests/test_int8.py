@@ -222,3 +222,17 @@ def test_shards_of_an_int8_model_are_refused():
     m.head_int8 = LinearInt8(_q(40, k=32))
     with pytest.raises(TypeError, match="quantize_int8"):
         LocalTPLM.from_dense(m)
+
+
+def test_a_checkpoint_of_floats_does_not_turn_into_codes():
+    from mamba_lite.model import LinearInt8
+
+    codes = torch.ones(6, 128, dtype=torch.int8)                # (as wide as its codes: nothing else would notice)
+    for strict in (True, False):
+        q = LinearInt8(ops.pack_int8(codes, torch.ones(6)), torch.zeros(6))
+        with pytest.raises(RuntimeError, match="8-bit codes"):
+            q.load_state_dict(torch.nn.Linear(128, 6).state_dict(), strict=strict)
+        assert torch.equal(q.weight, codes) and not bool(q.bias.any())
+    with pytest.raises(RuntimeError, match="float32"):
+        q.load_state_dict({k: v.bfloat16() if k == "scales" else v for k, v in q.state_dict().items()})
+    q.load_state_dict({k: v for k, v in q.state_dict().items() if k == "bias"}, strict=False)
