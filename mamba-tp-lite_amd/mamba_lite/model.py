@@ -338,7 +338,7 @@ class LinearInt8(nn.Module):
 
     def int8(self, start: int = 0, stop: int | None = None) -> ops.Int8:
         """Rows [start, stop) of the weight."""
-        return ops.Int8(self.weight[start:stop].detach(), self.scales[start:stop].detach(), self.in_features)
+        return ops.Int8(self.weight[start:stop], self.scales[start:stop], self.in_features)
 
     def rows(self, x, start: int, stop: int) -> torch.Tensor:
         """Outputs [start, stop) of forward(x)."""

@@ -1684,7 +1684,7 @@ def linear_int8(x, w, bias=None, out=None):
         if bias.shape != (n,) or not bias.is_contiguous():
             raise ValueError(f"bias must be contiguous [{n}], got {tuple(bias.shape)}")
         _same_device(codes, bias)
-    _int8_call("linear_int8", bias, out)
+    _int8_call("linear_int8", x.scales, w.scales, bias, out)
     ldy = n
     if out is not None:
         if out.dtype != dt:
@@ -1719,7 +1719,7 @@ def dequantize_int8(q, dtype=None, out=None):
     if dt not in _ACT_DTYPES:
         raise TypeError(f"dtype must be float32 or bfloat16, got {dt}")
     k, lead, codes = q.k, q.scales.shape, q.codes
-    _int8_call("dequantize_int8", out)
+    _int8_call("dequantize_int8", q.scales, out)
     M, ldo = q.scales.numel(), k
     if out is not None:
         if tuple(out.shape) != (*lead, k) or out.dtype != dt or not (out.is_contiguous() or (

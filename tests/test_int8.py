@@ -236,3 +236,19 @@ def test_a_checkpoint_of_floats_does_not_turn_into_codes():
     with pytest.raises(RuntimeError, match="float32"):
         q.load_state_dict({k: v.bfloat16() if k == "scales" else v for k, v in q.state_dict().items()})
     q.load_state_dict({k: v for k, v in q.state_dict().items() if k == "bias"}, strict=False)
+
+
+def test_scales_that_record_a_gradient_are_refused():
+    from mamba_lite.model import LinearInt8
+
+    codes, s = torch.zeros(6, 128, dtype=torch.int8), torch.ones(6, requires_grad=True)
+    w, x = ops.Int8(codes, s, 40), _q(2)
+    for call in (lambda: ops.linear_int8(x, w), lambda: ops.linear_int8(ops.Int8(codes, s, 40), _q(3)),
+                 lambda: ops.dequantize_int8(w)):
+        with pytest.raises(RuntimeError, match="backward"):
+            call()
+    lin = LinearInt8(_q(6))
+    lin.scales.requires_grad_()
+    for call in (lambda: lin(x), lambda: lin.rows(x, 0, 3)):
+        with pytest.raises(RuntimeError, match="backward"):
+            call()
