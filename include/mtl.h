@@ -887,6 +887,11 @@ int mtl_decode_step_w4(const mtl_decode_step_batched_args* args, const mtl_decod
  *   this layout, y (rows ldy elements apart) and bias of type dtype: the sum
  *   exact, then times x's scale and W's, each rounded in fp32.  N <= 2^27.  y
  *   must not overlap an operand.
+ * mtl_row_linear_int8: mtl_linear_int8 of one float row that it puts into
+ *   codes itself, in one launch and to the bit what two give.  norm_w NULL: x
+ *   [K] of dtype, K <= 8192, as mtl_quantize_int8.  Otherwise x, add and x_out
+ *   float [K], norm_w [K] of dtype, K <= 4096, as mtl_add_rmsnorm_int8, but
+ *   x_out must overlap neither x nor add.
  * mtl_dequantize_int8: the floats that rows stand for (dtype, ldo elements
  *   apart), rounded once from fp32.
  * All are deterministic and take no workspace.
@@ -915,10 +920,25 @@ typedef struct {
     int32_t y_f32;             /* 1: y holds floats whatever dtype is */
 } mtl_linear_int8_args;
 
+typedef struct {
+    const void* x;
+    const float* add;          /* or NULL */
+    float* x_out;              /* or NULL */
+    const void* norm_w;        /* [K] or NULL */
+    const int8_t* w;
+    const float* w_scales;
+    const void* bias;          /* [N] or NULL */
+    void* y;
+    int64_t N, K;
+    float eps;
+    int32_t dtype, y_f32, reserved;
+} mtl_row_linear_int8_args;
+
 int mtl_quantize_int8(const void* x, int64_t ldx, int8_t* codes, float* scales, int64_t M, int64_t K, int32_t dtype,
                       mtl_stream_t stream);
 int mtl_add_rmsnorm_int8(const mtl_add_rmsnorm_int8_args* args, mtl_stream_t stream);
 int mtl_linear_int8(const mtl_linear_int8_args* args, mtl_stream_t stream);
+int mtl_row_linear_int8(const mtl_row_linear_int8_args* args, mtl_stream_t stream);
 int mtl_dequantize_int8(const int8_t* codes, const float* scales, void* out, int64_t ldo, int64_t M, int64_t K,
                         int32_t dtype, mtl_stream_t stream);
 
@@ -927,12 +947,14 @@ int mtl_dequantize_int8(const int8_t* codes, const float* scales, void* out, int
  * out_proj are matrices of the layout above.  Per layer: mtl_linear_int8
  * (in_proj), the conv step, x_proj's partial products and their ordered sum,
  * the SSM update, mtl_quantize_int8, mtl_linear_int8 (out_proj, in floats),
- * mtl_add_rmsnorm_int8 (after the last layer norm_f's, in dtype).
+ * mtl_add_rmsnorm_int8 (after the last layer norm_f's, in dtype); at batch 1
+ * the norm with in_proj and out_proj as mtl_row_linear_int8, where they fit it.
  *   matrices    [2 n_layers]: in_proj [2 d_inner, d_model] and out_proj
  *               [d_model, d_inner] of each layer
  *   args        as mtl_decode_step_w4, but inp [b, d_model rounded up to 128]
- *               and xn [b, d_inner rounded up to 128] bytes, 16-byte aligned,
- *               and sq [2 b] floats; counters is not read
+ *               (at batch 1 [4 d_model]) and xn [b, d_inner rounded up to 128]
+ *               bytes, 16-byte aligned, and sq [2 b] floats; counters is not
+ *               read
  * ---------------------------------------------------------------------- */
 typedef struct {
     const int8_t* codes;

@@ -3,10 +3,14 @@
 //
 // Per layer seven or eight launches: in_proj in int8 (mtl_linear_int8) on the rows that the norm before it left -> the conv
 // step, x_proj's parts and their sum, the SSM update (step_between) -> y in int8 (mtl_quantize_int8) -> out_proj into floats
-// -> the residual add and the next RMSNorm in int8 (mtl_add_rmsnorm_int8), norm_f's in `dtype`.
+// -> the residual add and the next RMSNorm in int8 (mtl_add_rmsnorm_int8), norm_f's in `dtype`.  At batch 1 the norm goes with
+// its in_proj and the codes of y with out_proj (mtl_row_linear_int8): two launches fewer, and the same values.
 #include <hip/hip_runtime.h>
 
+#include <utility>
+
 #include "decode_step_quant.h"
+#include "int8.h"
 
 namespace {
 
@@ -32,16 +36,35 @@ int layers_int8(const mtl_decode_step_batched_args* a, const mtl_decode_layer* l
                                           kType, 0};
         return mtl_add_rmsnorm_int8(&n, stream);
     };
-    int rc = norm(nullptr, layers[0]);
+    const bool row_in = b == 1 && row_linear_int8_pays(2 * (int64_t)D, M, true);
+    const bool row_out = b == 1 && row_linear_int8_pays(M, D, false);
+    // (every workgroup of an in_proj that norms reads h, so the sum goes to another buffer)
+    float *h = a->h, *next = a->inp;
+    int rc = row_in ? MTL_OK : norm(nullptr, layers[0]);
     for (int32_t i = 0; i < nl && !rc; ++i) {
         const mtl_decode_layer& L = layers[i];
-        if ((rc = linear(in, in_s, mats[2 * i], L.b_in, xz, 2 * (int64_t)D, M, 0))) return rc;
-        if ((rc = step_between<T>(a, L, xz, xc, y, stream))) return rc;
-        if ((rc = mtl_quantize_int8(y, D, yq, yq_s, b, D, kType, stream))) return rc;
-        if ((rc = linear(yq, yq_s, mats[2 * i + 1], L.b_out, a->parts, M, D, 1))) return rc;
-        rc = i + 1 < nl ? norm(a->parts, layers[i + 1])
-                        : add_rmsnorm<T>(a->h, a->parts, 1, a->h, t(a->norm_f), w(a->normed_out), b, M,
-                                         a->eps_f, stream);
+        if (row_in) {
+            const mtl_row_linear_int8_args r{h, i ? a->parts : nullptr, i ? next : nullptr, L.norm_w, mats[2 * i].codes,
+                                             mats[2 * i].scales, L.b_in, xz, 2 * (int64_t)D, M, L.eps, kType, 0, 0};
+            rc = mtl_row_linear_int8(&r, stream);
+            if (i) std::swap(h, next);
+        } else {
+            rc = linear(in, in_s, mats[2 * i], L.b_in, xz, 2 * (int64_t)D, M, 0);
+        }
+        if (rc || (rc = step_between<T>(a, L, xz, xc, y, stream))) return rc;
+        if (row_out) {
+            const mtl_row_linear_int8_args r{y, nullptr, nullptr, nullptr, mats[2 * i + 1].codes, mats[2 * i + 1].scales,
+                                             L.b_out, a->parts, M, D, 0.f, kType, 1, 0};
+            rc = mtl_row_linear_int8(&r, stream);
+        } else {
+            if ((rc = mtl_quantize_int8(y, D, yq, yq_s, b, D, kType, stream))) return rc;
+            rc = linear(yq, yq_s, mats[2 * i + 1], L.b_out, a->parts, M, D, 1);
+        }
+        if (rc) return rc;
+        if (i + 1 == nl)
+            rc = add_rmsnorm<T>(h, a->parts, 1, a->h, t(a->norm_f), w(a->normed_out), b, M, a->eps_f, stream);
+        else if (!row_in)
+            rc = norm(a->parts, layers[i + 1]);
     }
     return rc;
 }

@@ -19,9 +19,6 @@ struct LinearArgs {
     bool bias_bf16;
 };
 
-// the float of a sum, each factor rounded once
-__device__ __forceinline__ float scaled(int acc, float sx, float sw, float bias) { return fmaf((float)acc * sx, sw, bias); }
-
 // Copies to LDS, asynchronous (vmcnt): 16 or 4 bytes per lane from base + off to `to` + 16 or 4 lane.  In assembly because
 // the compiler waits for every copy by the builtin before the next read of LDS, whatever slot it reads: one stage of a
 // product then took a whole round trip to memory (256 rows, 2048 x 4096: 21 us in place of 12).
@@ -365,10 +362,11 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
                  0, 0, al16(p->y) && p->ldy * (f32 ? 4 : 2) % 16 == 0, p->dtype == MTL_BF16};
     const hipStream_t st = as_stream(stream);
     // Few rows: the stream.  us at rows x N x K, bf16, W from HBM: 1x768x1536 3.0, tiles of 32 4.5; 64x768x1536 3.6 / 4.6;
-    // 1x8192x2048 5.4 / 6.3, 16x8192x2048 6.7 / 6.6, 16x2048x4096 6.4 / 8.9; 128x768x1536 5.5 / 4.4, 32x8192x2048 9.7 / 5.9.
+    // 1x8192x2048 5.4 / 6.3, 16x8192x2048 6.7 / 6.6, 16x2048x4096 6.4 / 8.9; 4x16384x2048
+    // 8.1 / 8.2, 16 rows of it 10.2 / 8.4; 128x768x1536 5.5 / 4.4, 32x8192x2048 9.7 / 5.9.
     // Eight wavefronts from 1536 columns on: 1x768x1536 3.4 with four; 1x1536x768 2.9, with eight 3.0; 33x1001x777 3.4 / 3.9.
     const int64_t pairs = ((a.N + 15) / 16) * (int64_t)((a.M + 15) / 16);
-    if (pairs <= (a.M <= 16 ? 512 : 256))
+    if (pairs <= (a.M <= 4 ? 1024 : a.M <= 16 ? 512 : 256))
         return a.Kp >= 1536 ? launch_stream<8>(a, f32, st) : launch_stream<4>(a, f32, st);
     // Up to 64 rows of a wide W, bound by its stream, in one tile of rows: 16x50280x2048 18.7 (128 x 64 19.2, 64 x 64 23.4, 32 x
     // 32 19.6), 64 rows 22.0 (64 x 64 26.0, 32 x 32 34.7); 16x24000x1024 6.9 (7.6 with the rule below), 16x8192x2048 9.5 (6.7).

@@ -164,6 +164,14 @@ class LinearInt8Args(ctypes.Structure):
     ]
 
 
+class RowLinearInt8Args(ctypes.Structure):
+    """mirror of mtl_row_linear_int8_args"""
+    _fields_ = [
+        ("x", _vp), ("add", _vp), ("x_out", _vp), ("norm_w", _vp), ("w", _vp), ("w_scales", _vp), ("bias", _vp), ("y", _vp),
+        ("N", _i64), ("K", _i64), ("eps", ctypes.c_float), ("dtype", _i32), ("y_f32", _i32), ("reserved", _i32),
+    ]
+
+
 class Int8Matrix(ctypes.Structure):
     """mirror of mtl_int8_matrix"""
     _fields_ = [("codes", _vp), ("scales", _vp)]
@@ -231,6 +239,7 @@ SIGNATURES = {
     "mtl_quantize_int8": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp]),
     "mtl_add_rmsnorm_int8": (ctypes.c_int, [ctypes.POINTER(AddRmsnormInt8Args), _vp]),
     "mtl_linear_int8": (ctypes.c_int, [ctypes.POINTER(LinearInt8Args), _vp]),
+    "mtl_row_linear_int8": (ctypes.c_int, [ctypes.POINTER(RowLinearInt8Args), _vp]),
     "mtl_dequantize_int8": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
     "mtl_decode_step_int8": (ctypes.c_int, [ctypes.POINTER(DecodeStepBatchedArgs), ctypes.POINTER(DecodeLayer),
                                             ctypes.POINTER(Int8Matrix), _i32, _vp]),

@@ -342,14 +342,12 @@ class LinearInt8(nn.Module):
 
     def rows(self, x, start: int, stop: int) -> torch.Tensor:
         """Outputs [start, stop) of forward(x)."""
-        x = x if type(x) is ops.Int8 else ops.quantize_int8(x)
         return ops.linear_int8(x, self.int8(start, stop), None if self.bias is None else self.bias[start:stop])
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
 
     def forward(self, x) -> torch.Tensor:
-        x = x if type(x) is ops.Int8 else ops.quantize_int8(x)
         return ops.linear_int8(x, ops.Int8(self.weight, self.scales, self.in_features), self.bias)
 
 

@@ -1442,7 +1442,7 @@ def decode_step_int8(layers, matrices, h, norm_f, eps_f, cfg, dtype=torch.float3
     b = h.shape[0] if h.dim() else 0
     row = lambda k: -(-k // _INT8_PAD) * _INT8_PAD // 4
     return _quant_step("decode_step_int8", layers, matrices, h, norm_f, eps_f, cfg, dtype,
-                       {"inp": b * row(cfg.d_model), "xn": b * row(cfg.d_inner), "sq": 2 * b})
+                       {"inp": max(b * row(cfg.d_model), cfg.d_model if b == 1 else 0), "xn": b * row(cfg.d_inner), "sq": 2 * b})
 
 
 def dequantize_w4(w4, dtype=torch.float32, out=None):
@@ -1663,19 +1663,37 @@ def add_rmsnorm_int8(x, weight, eps, y=None, x_out=None, dtype=torch.float32):
     return q
 
 
+# one float row is quantized within the product up to here (past 16384 columns of y two launches are faster: 24000 x 768 8.1
+# us for 9.3)
+_ROW_MAX_K, _ROW_MAX_N = 8192, 16384
+
+
 def linear_int8(x, w, bias=None, out=None):
     """x [..., k] W^T (+ bias [n]) of an Int8 x and an Int8 matrix W [n, k] (mtl_linear_int8): [..., n] of x's type.  The
-    sum over k is exact; it is multiplied by the two scales in float32.  bias and out have x's type."""
-    if type(x) is not Int8 or type(w) is not Int8:
-        _is_int8("linear_int8", "x", x)
+    sum over k is exact; it is multiplied by the two scales in float32.  bias and out have x's type.  x may be a float32 or
+    bfloat16 tensor: quantize_int8(x) is multiplied then, a single row in one launch (mtl_row_linear_int8)."""
+    if type(w) is not Int8:
         _is_int8("linear_int8", "w", w)
-    k, dt, lead = x.k, x.dtype, x.scales.shape
+    row = False
+    if type(x) is not Int8:
+        if not isinstance(x, torch.Tensor):
+            _is_int8("linear_int8", "x", x)
+        row = x.dtype in _ACT_DTYPES and x.dim() > 0 and x.numel() == x.shape[-1] == w.k <= _ROW_MAX_K and \
+            w.scales.numel() <= _ROW_MAX_N
+        if not row:
+            x = quantize_int8(x)
+    if row:
+        _int8_call("linear_int8", x)
+        k, dt, lead = w.k, x.dtype, x.shape[:-1]
+        codes, scales = x.contiguous(), None                 # (the row itself)
+    else:
+        k, dt, scales, codes = x.k, x.dtype, x.scales, x.codes
+        lead = scales.shape
     if w.k != k or w.scales.dim() != 1:
         raise ValueError(f"w must be [n, {k}], got {tuple(w.shape)}")
-    n, M = w.scales.shape[0], x.scales.numel()
+    n, M = w.scales.shape[0], 1 if row else scales.numel()
     if n < 1:
         raise ValueError("w has no rows")
-    codes = x.codes
     if codes.get_device() != w.codes.get_device():
         raise RuntimeError(f"all operands must be on one device, got x on {x.device}, w on {w.device}")
     if bias is not None:
@@ -1684,7 +1702,7 @@ def linear_int8(x, w, bias=None, out=None):
         if bias.shape != (n,) or not bias.is_contiguous():
             raise ValueError(f"bias must be contiguous [{n}], got {tuple(bias.shape)}")
         _same_device(codes, bias)
-    _int8_call("linear_int8", x.scales, w.scales, bias, out)
+    _int8_call("linear_int8", scales, w.scales, bias, out)
     ldy = n
     if out is not None:
         if out.dtype != dt:
@@ -1694,7 +1712,7 @@ def linear_int8(x, w, bias=None, out=None):
             raise ValueError(f"out must be {(*lead, n)} with contiguous rows, got {tuple(out.shape)} strides "
                              f"{out.stride()}")
         _same_device(codes, out)
-        if any(t is not None and _overlap(out, t) for t in (codes, x.scales, w.codes, w.scales, bias)):
+        if any(t is not None and _overlap(out, t) for t in (codes, scales, w.codes, w.scales, bias)):
             raise ValueError("out must not overlap an operand")
         if out.dim() == 2 and M > 1:
             ldy = out.stride(0)
@@ -1703,9 +1721,14 @@ def linear_int8(x, w, bias=None, out=None):
             return linear_int8(x, w, bias, out)
     if out is None:
         out = codes.new_empty((*lead, n), dtype=dt)
-    a = _lib.LinearInt8Args(codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias),
-                            out.data_ptr(), ldy, M, n, k, _ACT_DTYPES[dt], 0)
-    rc = _lib.load().mtl_linear_int8(ctypes.byref(a), _stream(codes))
+    if row:
+        a = _lib.RowLinearInt8Args(codes.data_ptr(), None, None, None, w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias),
+                                   out.data_ptr(), n, k, 0.0, _ACT_DTYPES[dt], 0, 0)
+        rc = _lib.load().mtl_row_linear_int8(ctypes.byref(a), _stream(codes))
+    else:
+        a = _lib.LinearInt8Args(codes.data_ptr(), scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias),
+                                out.data_ptr(), ldy, M, n, k, _ACT_DTYPES[dt], 0)
+        rc = _lib.load().mtl_linear_int8(ctypes.byref(a), _stream(codes))
     if rc:
         _lib.check(rc, "linear_int8")
     return out

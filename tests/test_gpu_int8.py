@@ -1,9 +1,11 @@
 """quantize_int8, add_rmsnorm_int8, linear_int8 and dequantize_int8 against float64, at the ends of their ranges and where
 a tile, a run or a row is partial."""
+import ctypes
+
 import pytest
 import torch
 
-from mamba_lite import ops
+from mamba_lite import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -250,6 +252,65 @@ def test_offsets_past_32_bits():
     for rows in (slice(0, 64), slice(39936, 40000)):
         ref, off = _reference(xc[rows], wc, xs[rows], ws, None)
         assert bool(((y[rows].double() - ref).abs() <= off + HALF[torch.float32] * ref.abs()).all())
+
+
+# ------------------------------------------------------------------ one float row
+ROW_SIZES = [(1, 1), (16, 128), (15, 127), (17, 129), (768, 1536), (1001, 777), (2048, 4096), (33, 4097), (100, 5121),
+             (257, 8192), (8192, 2048), (16384, 64), (16385, 64), (40, 8193)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k", ROW_SIZES)
+def test_a_float_row_gives_the_bits_of_its_codes(n, k, dtype):
+    w, _, _ = _matrix(n, k, n + k)
+    bias = torch.randn(n, device="cuda", generator=_gen(7)).to(dtype)
+    x = torch.randn(5, k, device="cuda", generator=_gen(n)).to(dtype)
+    x[1] = 0.0
+    x[2, k // 2], x[3, k - 1] = float("inf"), float("nan")
+    x[4, 0] = 100.0
+    for i in range(5):
+        for b in (None, bias):
+            want = ops.linear_int8(ops.quantize_int8(x[i]), w, b)
+            assert want.shape == (n,) and want.dtype == dtype
+            for row, shape in ((x[i], (n,)), (x[i:i + 1], (1, n)), (x[i].view(1, 1, k), (1, 1, n)),
+                               (torch.stack([x[i], x[0]], 1)[:, 0], (n,))):
+                y = ops.linear_int8(row, w, b)
+                assert y.shape == shape and torch.equal(y.view(-1).isnan(), want.isnan())
+                assert torch.equal(y.view(-1).nan_to_num(7.0), want.nan_to_num(7.0))
+    # rows of x past 16 bytes' alignment, y too, and what lies beside it
+    out = torch.full((n + 5,), 3.0, device="cuda", dtype=dtype)
+    flat = torch.cat([x[4].new_zeros(3), x[4]])
+    ops.linear_int8(flat[3:], w, bias, out=out[2:n + 2])
+    assert torch.equal(out[2:n + 2], want) and bool((out[:2] == 3.0).all()) and bool((out[n + 2:] == 3.0).all())
+    # more rows than one, from floats
+    assert torch.equal(ops.linear_int8(x[3:], w, bias).isnan(), ops.linear_int8(ops.quantize_int8(x[3:]), w, bias).isnan())
+    assert torch.equal(ops.linear_int8(x[3:], w, bias)[1], want)
+
+
+@pytest.mark.parametrize("wt", DTYPES)
+@pytest.mark.parametrize("n,k", [(16, 1), (15, 127), (17, 129), (100, 777), (768, 768), (2049, 2048), (33, 3333), (64, 4096)])
+def test_a_float_row_with_its_norm(n, k, wt):
+    g = _gen(n + k)
+    x, y = (torch.randn(1, k, device="cuda", generator=g) * 3 for _ in range(2))
+    nw = (1 + 0.3 * torch.randn(k, device="cuda", generator=g)).to(wt)
+    w, _, _ = _matrix(n, k, 1)
+    bias = torch.randn(n, device="cuda", generator=g).to(wt)
+    for add in (None, y):
+        h, keep = torch.full((1, k + 2), 7.0, device="cuda"), x.clone()
+        want_h = torch.empty_like(x)
+        q = ops.add_rmsnorm_int8(x, nw, 1e-5, y=add, x_out=want_h, dtype=wt)
+        want = ops.linear_int8(q, w, bias)
+        for f32 in (0, 1):
+            want_y = want if wt == torch.float32 or not f32 else \
+                ops.linear_int8(ops.Int8(q.codes, q.scales, k), w, bias.float())
+            got = torch.full((n + 1,), 5.0, device="cuda", dtype=torch.float32 if f32 else wt)
+            a = _lib.RowLinearInt8Args(x.data_ptr(), None if add is None else add.data_ptr(), h.data_ptr() + 4, nw.data_ptr(),
+                                       w.codes.data_ptr(), w.scales.data_ptr(), bias.data_ptr(), got.data_ptr(), n, k, 1e-5,
+                                       ops._ACT_DTYPES[wt], f32, 0)
+            _lib.check(_lib.load().mtl_row_linear_int8(ctypes.byref(a), ops._stream(x)), "row_linear_int8")
+            assert torch.equal(got[:n], want_y[0]) and float(got[n]) == 5.0
+            assert torch.equal(h[0, 1:k + 1], want_h[0]) and float(h[0, 0]) == float(h[0, -1]) == 7.0
+            assert torch.equal(x, keep)
 
 
 def test_sums_are_exact_at_the_largest_codes():

@@ -140,7 +140,13 @@ def test_norm_refuses_outputs_over_operands_and_gradients():
 def test_linear_and_dequantize_refuse():
     x, w = _q(3), _q(6)
     for a, kind, error in (
-            ((torch.zeros(3, 40), w), TypeError, "x must be an Int8"), ((x, torch.zeros(6, 40)), TypeError, "w must be"),
+            (([1.0], w), TypeError, "x must be an Int8"), ((x, torch.zeros(6, 40)), TypeError, "w must be"),
+            ((torch.zeros(3, 40).half(), w), TypeError, "float32 or bfloat16"),
+            ((torch.zeros(1, 40).half(), w), TypeError, "float32 or bfloat16"),
+            ((torch.zeros(1, 40, requires_grad=True), w), RuntimeError, "backward"),
+            ((torch.zeros(1, 40), w, torch.zeros(6, dtype=torch.bfloat16)), TypeError, "bias"),
+            ((torch.zeros(1, 40), w, None, torch.zeros(6)), ValueError, "out"),
+            ((torch.zeros(1, 40), w), RuntimeError, "GPU"), ((torch.zeros(3, 40), w), RuntimeError, "GPU"),
             ((x, _q(6, k=41)), ValueError, r"w must be \[n, 40\]"), ((x, _q(2, 6)), ValueError, "w must be"),
             ((x, _q(0)), ValueError, "no rows"), ((x, w, torch.zeros(6, dtype=torch.bfloat16)), TypeError, "bias"),
             ((x, w, torch.zeros(5)), ValueError, "bias"), ((x, w, torch.zeros(12)[::2]), ValueError, "bias"),
@@ -186,7 +192,17 @@ def test_library_refuses_before_any_launch():
         bad = _lib.LinearInt8Args.from_buffer_copy(p)
         setattr(bad, name, value)
         assert refused(lib.mtl_linear_int8(ctypes.byref(bad), None), text), name
-    for f in (lib.mtl_linear_int8, lib.mtl_add_rmsnorm_int8):
+    r = _lib.RowLinearInt8Args(some, None, None, None, some, some, None, some, 4, 8, 1e-5, 0, 0, 0)
+    for change, text in (({"K": 0}, b"K must be"), ({"K": 8193}, b"K must be"), ({"K": 4097, "norm_w": some}, b"K must be"),
+                         ({"N": 0}, b"N must be"), ({"dtype": 2}, b"dtype"), ({"x": None}, b"null"), ({"y": None}, b"null"),
+                         ({"add": some}, b"need a norm"), ({"x_out": some}, b"need a norm"), ({"w": some + 8}, b"aligned"),
+                         ({"norm_w": some, "x_out": some}, b"x_out"),
+                         ({"norm_w": some, "add": some + 64, "x_out": some + 64}, b"x_out")):
+        bad = _lib.RowLinearInt8Args.from_buffer_copy(r)
+        for name, value in change.items():
+            setattr(bad, name, value)
+        assert refused(lib.mtl_row_linear_int8(ctypes.byref(bad), None), text), change
+    for f in (lib.mtl_linear_int8, lib.mtl_add_rmsnorm_int8, lib.mtl_row_linear_int8):
         assert refused(f(None, None), b"null")
     assert lib.mtl_quantize_int8(None, 8, None, None, 0, 8, 0, None) == 0 and lib.mtl_last_error() == b""
 
