@@ -765,8 +765,9 @@ class MambaLM(nn.Module):
         an in_proj writes its rows in int8, and an out_proj's input is quantized row by row.  Prompts get faster wherever their
         projections bound them: 32 x 1024 tokens at the mamba-1.4b width fp32 282 -> 117 ms, bf16 103 -> 79, mamba-130m fp32
         29.6 -> 18.4, bf16 15.6 -> 13.1; 1024 tokens 15.6 -> 7.3, 9.2 -> 8.3, 2.9 -> 2.1, 4.4 -> 4.0.  Steps do at mamba-1.4b
-        in fp32 (1 row 1392 -> 1344 us, 32 rows 2324 -> 1802), and take longer in bf16 (1202 -> 1399, 1706 -> 1823) and at the
-        mamba-130m width (fp32 321 -> 493, bf16 396 -> 516), as do its prompts of 64 tokens in fp32 (0.9 -> 1.2 ms).  Graphs
+        in fp32 (1 row 1394 -> 1108 us, 32 rows 2332 -> 1800) and in bf16 at 1 row (1200 -> 1159), and take longer in bf16 at
+        more (32 rows 1707 -> 1824) and at the mamba-130m width (1 row fp32 321 -> 408, bf16 397 -> 434), as do its prompts
+        of 64 tokens in fp32 (0.9 -> 1.2 ms).  Graphs
         captured before refuse to replay.  Returns self."""
         return self._quantize("quantize_int8", LinearInt8.from_linear, "head_int8" if lm_head else None,
                               lambda w: LinearInt8(_int8_weight(w)))
