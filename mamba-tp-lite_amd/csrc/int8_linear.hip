@@ -51,8 +51,8 @@ template <typename P> __device__ __forceinline__ const P* uniform(const P* p) {
 // and ends took 93 of the 526 us of 32768 x 8192 x 2048.  Three stages of K at least: the next tile's scales go where the
 // last one's were, and a barrier has to stand between.
 //
-// ONCE: no other workgroup reads these rows of W, which go past the caches (16 x 50280 x 2048 21.2 -> 18.7 us).
-template <typename T, int BN, int BM, int WN, int WM, int ST, int OCC, bool CHAIN, bool ONCE>
+// ONCE: no other workgroup reads these rows of W, which go past the caches (16 x 50280 x 2048 21.2 -> 18.7 us).  PAST: y does.
+template <typename T, int BN, int BM, int WN, int WM, int ST, int OCC, bool CHAIN, bool ONCE, bool PAST>
 __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_kernel(const LinearArgs a) {
     constexpr int NWM = BM / WM, NW = BN / WN * NWM, NT = NW * 64;
     constexpr int TJ = WN / 16, TI = WM / 16, KB = kInt8Pad, KS = 2;      // MFMA tiles of a wavefront; steps of a stage
@@ -243,7 +243,11 @@ __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_ker
                         const int r = r0 + lane / RPR, c = lane % RPR * kPer;
                         if (RP > 16 && r >= 16) break;
                         const I4 v = *reinterpret_cast<const I4*>(out + r * (OW + kPer) + c);
-                        if (mt + r < a.M) *reinterpret_cast<I4*>(static_cast<T*>(a.y) + (int64_t)(mt + r) * a.ldy + nw + c) = v;
+                        I4* y = reinterpret_cast<I4*>(static_cast<T*>(a.y) + (int64_t)(mt + r) * a.ldy + nw + c);
+                        if (mt + r < a.M) {
+                            if (PAST) __builtin_nontemporal_store(v, y);
+                            else *y = v;
+                        }
                     }
                 } else {
                     for (int e = lane; e < 16 * OW; e += 64) {
@@ -330,15 +334,15 @@ template <int NW> int launch_stream(const LinearArgs& a, bool f32, hipStream_t s
     return check_launch("linear_int8");
 }
 
-template <int BN, int BM, int WN, int WM, int ST, int OCC, bool CHAIN = false, bool ONCE = false>
+template <int BN, int BM, int WN, int WM, int ST, int OCC, bool CHAIN = false, bool ONCE = false, bool PAST = false>
 int launch(LinearArgs a, bool f32, hipStream_t st) {
     const int64_t tm = (a.M + (int64_t)BM - 1) / BM, tn = (a.N + (int64_t)BN - 1) / BN;
     MTL_REQUIRE(tm * tn < (int64_t(1) << 31), "too many output tiles");
     a.tm = (int)tm;
     a.tn = (int)tn;
     const dim3 grid((unsigned)(CHAIN ? std::min<int64_t>(tm * tn, 256) : tm * tn)), nt(BN / WN * (BM / WM) * 64);
-    if (f32) hipLaunchKernelGGL((linear_int8_kernel<float, BN, BM, WN, WM, ST, OCC, CHAIN, ONCE>), grid, nt, 0, st, a);
-    else hipLaunchKernelGGL((linear_int8_kernel<uint16_t, BN, BM, WN, WM, ST, OCC, CHAIN, ONCE>), grid, nt, 0, st, a);
+    if (f32) hipLaunchKernelGGL((linear_int8_kernel<float, BN, BM, WN, WM, ST, OCC, CHAIN, ONCE, PAST>), grid, nt, 0, st, a);
+    else hipLaunchKernelGGL((linear_int8_kernel<uint16_t, BN, BM, WN, WM, ST, OCC, CHAIN, ONCE, PAST>), grid, nt, 0, st, a);
     return check_launch("linear_int8");
 }
 
@@ -385,6 +389,11 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
         {256, 256, 1, 0.05, 8.59, 1.39, 5.61, 2.35, 0.0}, {256, 128, 1, 1.01, 6.12, 0.79, 2.79, 0.97, 0.0},
         {128, 128, 1, 1.14, 3.97, 0.49, 1.07, 0.67, 0.0}, {64, 64, 3, 2.58, 0.64, 0.09, 0.16, 0.26, 0.26},
         {32, 32, 4, 1.98, 0.50, 0.05, 0.04, 0.01, 0.15},  {128, 128, 2, 1.33, 2.11, 0.06, 1.04, 0.71, 0.78}};
+    // Whole lines of a y of up to 40 MB go past the L2s, which hold it otherwise and write it back when the kernel ends: fp32
+    // 512x8192x2048 16.3 -> 15.0, 1024x8192x2048 24.5 -> 23.8 (bf16 22.8 -> 21.0), 4096x1536x768 13.0 -> 12.2.  Larger ones lose
+    // (fp32 32768x1536x768 60.8 -> 65), as do rows that end inside a line (8184x50280x768 690 -> 855).
+    const int64_t row = p->ldy * (f32 ? 4 : 2);
+    const bool past = row % 128 == 0 && reinterpret_cast<uintptr_t>(p->y) % 128 == 0 && p->M * row <= 40 << 20;
     const int stages = a.Kp / kInt8Pad;
     int best = 0;
     double least = 0;
@@ -395,12 +404,14 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
                           full * t.traffic * stages;
         if (least == 0 || us < least) { least = us; best = i; }
     }
+#define MTL_TILE(...) (past ? launch<__VA_ARGS__, false, false, true>(a, f32, st) : launch<__VA_ARGS__>(a, f32, st))
     switch (best) {
         case 0: return launch<256, 256, 128, 64, 2, 1, true>(a, f32, st);
-        case 1: return launch<256, 128, 64, 64, 3, 1>(a, f32, st);
-        case 2: return launch<128, 128, 64, 32, 4, 1>(a, f32, st);
-        case 3: return launch<64, 64, 32, 32, 3, 3>(a, f32, st);
-        case 4: return launch<32, 32, 16, 16, 5, 4>(a, f32, st);
-        default: return launch<128, 128, 32, 64, 2, 2>(a, f32, st);
+        case 1: return MTL_TILE(256, 128, 64, 64, 3, 1);
+        case 2: return MTL_TILE(128, 128, 64, 32, 4, 1);
+        case 3: return MTL_TILE(64, 64, 32, 32, 3, 3);
+        case 4: return MTL_TILE(32, 32, 16, 16, 5, 4);
+        default: return MTL_TILE(128, 128, 32, 64, 2, 2);
     }
+#undef MTL_TILE
 }
