@@ -1546,18 +1546,23 @@ def _new_int8(like, lead, k, dtype):
     return q
 
 
+# (looked up once: a small call is bound by the host)
+_grad_enabled, _forward_ad = torch.is_grad_enabled, torch.autograd.forward_ad
+_functorch_top, _tracing = torch._C._functorch.peek_interpreter_stack, torch._C._is_tracing
+
+
 def _int8_call(name, *ts):
     """What a raw launch cannot take: subclasses, recorded gradients, forward-mode derivatives, tracing."""
     for t in ts:
         if t is not None and type(t) not in PLAIN_TENSORS:
             raise TypeError(f"{name} takes plain tensors, got {type(t).__name__}")
-    if torch.is_grad_enabled():
+    if _grad_enabled():
         _no_grad_recorded(name, *ts)
-    if torch.autograd.forward_ad._current_level >= 0:
+    if _forward_ad._current_level >= 0:
         _no_dual(name, *ts)
-    if torch._C._functorch.peek_interpreter_stack() is not None:
+    if _functorch_top() is not None:
         raise RuntimeError(f"{name} launches a kernel, which a functorch transform would not see")
-    if torch._C._is_tracing():
+    if _tracing():
         _not_traced(name)
 
 
@@ -1683,9 +1688,7 @@ def linear_int8(x, w, bias=None, out=None):
         if not row:
             x = quantize_int8(x)
     if row:
-        _int8_call("linear_int8", x)
-        k, dt, lead = w.k, x.dtype, x.shape[:-1]
-        codes, scales = x.contiguous(), None                 # (the row itself)
+        k, dt, lead, codes, scales = w.k, x.dtype, x.shape[:-1], x, x           # (the row itself)
     else:
         k, dt, scales, codes = x.k, x.dtype, x.scales, x.codes
         lead = scales.shape
@@ -1703,6 +1706,8 @@ def linear_int8(x, w, bias=None, out=None):
             raise ValueError(f"bias must be contiguous [{n}], got {tuple(bias.shape)}")
         _same_device(codes, bias)
     _int8_call("linear_int8", scales, w.scales, bias, out)
+    if row and not x.is_contiguous():
+        codes = x.contiguous()
     ldy = n
     if out is not None:
         if out.dtype != dt:
