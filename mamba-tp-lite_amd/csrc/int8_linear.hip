@@ -384,16 +384,18 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     // takes 1% more than the best of them (a cost by rounds alone took 6% more); us with the tiles in the table's order:
     //   bf16 1024x8192x2048 - 22.9 26.9 33.8 - 23.2; fp32 8192x768x1536 - 19.6 25.7 25.0 - 18.8; 1179x2304x4480 56.3 33.6 23.5 28.0
     //   39.7 32.1; 720x1167x3393 54.1 30.8 19.9 14.0 15.7 27.9; fp32 657x576x1280 24.5 14.5 9.6 6.1 5.2 11.0; fp32
-    //   14280x1685x1184 60.4 70.8 72.9 73.0 111.9 58.2; 32768x8192x2048 496 by the first, 580 by the second
+    //   14280x1685x1184 60.4 70.8 72.9 73.0 111.9 58.2; 32768x8192x2048 496 by the first, 586 by the second
     constexpr struct { int bn, bm, share; double start, round, stage, loose, floats, traffic; } kTiles[6] = {
         {256, 256, 1, 0.05, 8.59, 1.39, 5.61, 2.35, 0.0}, {256, 128, 1, 1.01, 6.12, 0.79, 2.79, 0.97, 0.0},
         {128, 128, 1, 1.14, 3.97, 0.49, 1.07, 0.67, 0.0}, {64, 64, 3, 2.58, 0.64, 0.09, 0.16, 0.26, 0.26},
         {32, 32, 4, 1.98, 0.50, 0.05, 0.04, 0.01, 0.15},  {128, 128, 2, 1.33, 2.11, 0.06, 1.04, 0.71, 0.78}};
     // Whole lines of a y of up to 40 MB go past the L2s, which hold it otherwise and write it back when the kernel ends: fp32
     // 512x8192x2048 16.3 -> 15.0, 1024x8192x2048 24.5 -> 23.8 (bf16 22.8 -> 21.0), 4096x1536x768 13.0 -> 12.2.  Larger ones lose
-    // (fp32 32768x1536x768 60.8 -> 65), as do rows that end inside a line (8184x50280x768 690 -> 855).
+    // (fp32 32768x1536x768 60.8 -> 65), as do rows that end inside a line (8184x50280x768 690 -> 855), but for those of a chain
+    // that no cache holds (32768x8192x2048 515 -> 496, 16384x50304x1024 964 -> 880; 65536x4096x2048 506 -> 511).
     const int64_t row = p->ldy * (f32 ? 4 : 2);
-    const bool past = row % 128 == 0 && reinterpret_cast<uintptr_t>(p->y) % 128 == 0 && p->M * row <= 40 << 20;
+    const bool lines = row % 128 == 0 && reinterpret_cast<uintptr_t>(p->y) % 128 == 0;
+    const bool past = lines && p->M * row <= 40 << 20, large = lines && p->M * row >= 384 << 20;
     const int stages = a.Kp / kInt8Pad;
     int best = 0;
     double least = 0;
@@ -406,7 +408,8 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     }
 #define MTL_TILE(...) (past ? launch<__VA_ARGS__, false, false, true>(a, f32, st) : launch<__VA_ARGS__>(a, f32, st))
     switch (best) {
-        case 0: return launch<256, 256, 128, 64, 2, 1, true>(a, f32, st);
+        case 0: return large ? launch<256, 256, 128, 64, 2, 1, true, false, true>(a, f32, st)
+                             : launch<256, 256, 128, 64, 2, 1, true>(a, f32, st);
         case 1: return MTL_TILE(256, 128, 64, 64, 3, 1);
         case 2: return MTL_TILE(128, 128, 64, 32, 4, 1);
         case 3: return MTL_TILE(64, 64, 32, 32, 3, 3);
