@@ -366,3 +366,27 @@ def test_the_one_call_prompt_follows_its_weights():
         assert len(seen) == 1 and seen[0].shape == (1, 30, 256)
         q.layers[0].mixer.in_proj = torch.nn.Linear(256, 1024, bias=False).cuda()       # a mixed stack: op by op
         assert q.prefill(ids)[0].shape == before.shape and q.step(ids[:, :1], q.prefill(ids)[1]).shape[0] == 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kw", [dict(d_model=4352, expand=1, dt_rank=16), dict(d_model=4096), dict(d_model=4480, dt_rank=32),
+                                dict(d_model=96, expand=3)])
+def test_a_step_of_one_row_in_every_mix_of_launches(kw, dtype, monkeypatch):
+    # (rows past mtl_row_linear_int8's widths before in_proj, none, and before both)
+    if dtype == torch.bfloat16 and kw["d_model"] == 96:
+        kw = dict(kw, expand=4)                              # (channels in 64s)
+    q = _model(n_layer=3, dtype=dtype, **kw).quantize_int8()
+    ids = torch.randint(0, 1003, (1, 8), device="cuda")
+    calls = []
+    real = ops.decode_step_int8
+    monkeypatch.setattr(ops, "decode_step_int8", lambda *a, **k: (calls.append(1), real(*a, **k))[1])
+    with torch.no_grad():
+        _, cache = q.prefill(ids[:, :4])
+        other = copy.deepcopy(cache)
+        got = [q.step(ids[:, i:i + 1], cache) for i in range(4, 8)]
+        # (in bf16 the one call takes dt_rank + 2 d_state in fours)
+        assert len(calls) == (0 if dtype == torch.bfloat16 and (q.cfg.dt_rank + 2 * q.cfg.d_state) % 4 else 4)
+        monkeypatch.setattr(mm, "BATCHED_STEP_NATIVE", False)
+        want = [q.step(ids[:, i:i + 1], other) for i in range(4, 8)]
+    for a, r in zip(got, want):
+        assert torch.equal(a, r) if dtype == torch.float32 else _rel(a, r) < TOL[dtype]
