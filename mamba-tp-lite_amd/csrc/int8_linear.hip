@@ -7,6 +7,8 @@
 namespace mtl {
 namespace {
 
+typedef int I4u __attribute__((ext_vector_type(4), aligned(2)));
+
 struct LinearArgs {
     const int8_t* x; const float* sx;      // [M, Kp], [M]
     const int8_t* w; const float* sw;      // [N, Kp], [N]
@@ -236,24 +238,20 @@ __global__ void __launch_bounds__(BN / WN * (BM / WM) * 64, OCC) linear_int8_ker
                     st4(out + r16 * (OW + kPer) + c, v);
                 }
                 wave_lds_fence();
-                if (a.vec && nw + OW <= a.N) {
-                    constexpr int RPR = OW / kPer, RP = 64 / RPR;      // 16-byte runs of a row; rows of an instruction
+                constexpr int RPR = OW / kPer, RP = 64 / RPR;          // 16-byte runs of a row; rows of an instruction
 #pragma unroll
-                    for (int r0 = 0; r0 < 16; r0 += RP) {
-                        const int r = r0 + lane / RPR, c = lane % RPR * kPer;
-                        if (RP > 16 && r >= 16) break;
-                        const I4 v = *reinterpret_cast<const I4*>(out + r * (OW + kPer) + c);
-                        I4* y = reinterpret_cast<I4*>(static_cast<T*>(a.y) + (int64_t)(mt + r) * a.ldy + nw + c);
-                        if (mt + r < a.M) {
-                            if (PAST) __builtin_nontemporal_store(v, y);
-                            else *y = v;
-                        }
-                    }
-                } else {
-                    for (int e = lane; e < 16 * OW; e += 64) {
-                        const int r = e / OW, c = e % OW;
-                        if (mt + r < a.M && nw + c < a.N)
-                            static_cast<T*>(a.y)[(int64_t)(mt + r) * a.ldy + nw + c] = out[r * (OW + kPer) + c];
+                for (int r0 = 0; r0 < 16; r0 += RP) {
+                    const int r = r0 + lane / RPR, c = lane % RPR * kPer;
+                    if (RP > 16 && r >= 16) break;
+                    const T* from = out + r * (OW + kPer) + c;
+                    T* y = static_cast<T*>(a.y) + (int64_t)(mt + r) * a.ldy + nw + c;
+                    const int n = mt + r < a.M ? a.N - nw - c : 0;     // columns of the run that are there
+                    if (n >= kPer) {
+                        const I4 v = *reinterpret_cast<const I4*>(from);
+                        if (PAST) __builtin_nontemporal_store(v, reinterpret_cast<I4*>(y));
+                        else *reinterpret_cast<I4u*>(y) = v;           // (at any alignment of a row)
+                    } else {
+                        for (int e = 0; e < n; ++e) y[e] = from[e];
                     }
                 }
                 wave_lds_fence();

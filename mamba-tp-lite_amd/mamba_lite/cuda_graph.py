@@ -28,7 +28,8 @@ def _clone_cache(cache):
 
 
 def _weight_set(model) -> int:
-    """How often the model's weights have been replaced by others (MambaLM.quantize_w4): a graph reads the old ones."""
+    """How often the model's weights have been replaced by others (MambaLM.quantize_w4, quantize_int8): a graph reads the
+    old ones."""
     return getattr(model, "weight_set", 0)
 
 
