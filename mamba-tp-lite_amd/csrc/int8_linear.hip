@@ -376,17 +376,6 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     if (a.M <= 64 && tiles(128, 64) >= 160)
         return a.M <= 32 ? launch<128, 32, 32, 32, 4, 2, false, true>(a, f32, st)
                          : launch<128, 64, 32, 32, 3, 2, false, true>(a, f32, st);
-    // Others by the time that their tiles take on the 256 CUs, in us at bf16 and fp32 sizes of up to 32768 rows: each round of a
-    // tile per CU has its start and end (longer where rows of y are not 16-byte aligned, or floats) and its stages of K; two
-    // or more tiles share a CU, and a round of them has the traffic of all.  Measured at 231 sizes with every tile, the choice
-    // takes 1% more than the best of them (a cost by rounds alone took 6% more); us with the tiles in the table's order:
-    //   bf16 1024x8192x2048 - 22.9 26.9 33.8 - 23.2; fp32 8192x768x1536 - 19.6 25.7 25.0 - 18.8; 1179x2304x4480 56.3 33.6 23.5 28.0
-    //   39.7 32.1; 720x1167x3393 54.1 30.8 19.9 14.0 15.7 27.9; fp32 657x576x1280 24.5 14.5 9.6 6.1 5.2 11.0; fp32
-    //   14280x1685x1184 60.4 70.8 72.9 73.0 111.9 58.2; 32768x8192x2048 496 by the first, 586 by the second
-    constexpr struct { int bn, bm, share; double start, round, stage, loose, floats, traffic; } kTiles[6] = {
-        {256, 256, 1, 0.05, 8.59, 1.39, 5.61, 2.35, 0.0}, {256, 128, 1, 1.01, 6.12, 0.79, 2.79, 0.97, 0.0},
-        {128, 128, 1, 1.14, 3.97, 0.49, 1.07, 0.67, 0.0}, {64, 64, 3, 2.58, 0.64, 0.09, 0.16, 0.26, 0.26},
-        {32, 32, 4, 1.98, 0.50, 0.05, 0.04, 0.01, 0.15},  {128, 128, 2, 1.33, 2.11, 0.06, 1.04, 0.71, 0.78}};
     // Whole lines of a y of up to 40 MB go past the L2s, which hold it otherwise and write it back when the kernel ends: fp32
     // 512x8192x2048 16.3 -> 15.0, 1024x8192x2048 24.5 -> 23.8 (bf16 22.8 -> 21.0), 4096x1536x768 13.0 -> 12.2.  Larger ones lose
     // (fp32 32768x1536x768 60.8 -> 65), as do rows that end inside a line (8184x50280x768 690 -> 855), but for those of a chain
@@ -394,13 +383,24 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     const int64_t row = p->ldy * (f32 ? 4 : 2);
     const bool lines = row % 128 == 0 && reinterpret_cast<uintptr_t>(p->y) % 128 == 0;
     const bool past = lines && p->M * row <= 40 << 20, large = lines && p->M * row >= 384 << 20;
+    // Others by the time that their tiles take on the 256 CUs, in us: each round of a tile per CU has its start and end (longer
+    // where rows of y end inside a line, or are floats) and its stages of K; two or more tiles share a CU, and a round of them
+    // has the traffic of all.  Measured at 210 sizes of up to 32768 rows with every tile, the choice takes 1% more than the best
+    // of them (a cost by rounds alone 7% more); us with the tiles in the table's order:
+    //   bf16 1024x8192x2048 - 21 27 34 - 23; fp32 8192x768x1536 - 19.6 25.7 25.0 - 18.8; 1179x2304x4480 56 34 23 28 40 32;
+    //   720x1167x3393 54 31 20 14 16 28; fp32 657x576x1280 24 14 9.6 6.1 5.2 11; fp32 14280x1685x1184 - - - - - 49 (60 of the
+    //   first); 32768x8192x2048 496 by the first, 586 by the second
+    constexpr struct { int bn, bm, share; double start, round, stage, inside, floats, traffic; } kTiles[6] = {
+        {256, 256, 1, 0.00, 3.81, 1.26, 0.81, 3.90, 0.0}, {256, 128, 1, 0.34, 5.63, 0.80, 0.61, 1.39, 0.0},
+        {128, 128, 1, 1.06, 3.09, 0.54, 0.45, 0.90, 0.0}, {64, 64, 3, 2.49, 0.54, 0.11, 0.06, 0.26, 0.26},
+        {32, 32, 4, 2.22, 0.35, 0.06, 0.02, 0.02, 0.14},  {128, 128, 2, 1.47, 1.72, 0.08, 0.10, 0.75, 0.78}};
     const int stages = a.Kp / kInt8Pad;
     int best = 0;
     double least = 0;
     for (int i = stages > 2 ? 0 : 1; i < 6; ++i) {
         const auto& t = kTiles[i];
         const int64_t count = tiles(t.bn, t.bm), rounds = (count + 255) / 256, full = (count + 256 * t.share - 1) / (256 * t.share);
-        const double us = t.start + rounds * (t.round + t.stage * stages + (a.vec ? 0 : t.loose) + (f32 ? t.floats : 0)) +
+        const double us = t.start + rounds * (t.round + t.stage * stages + (lines ? 0 : t.inside) + (f32 ? t.floats : 0)) +
                           full * t.traffic * stages;
         if (least == 0 || us < least) { least = us; best = i; }
     }
