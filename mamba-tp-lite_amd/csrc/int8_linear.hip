@@ -376,13 +376,14 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     if (a.M <= 64 && tiles(128, 64) >= 160)
         return a.M <= 32 ? launch<128, 32, 32, 32, 4, 2, false, true>(a, f32, st)
                          : launch<128, 64, 32, 32, 3, 2, false, true>(a, f32, st);
-    // Whole lines of a y of up to 40 MB go past the L2s, which hold it otherwise and write it back when the kernel ends: fp32
-    // 512x8192x2048 16.3 -> 15.0, 1024x8192x2048 24.5 -> 23.8 (bf16 22.8 -> 21.0), 4096x1536x768 13.0 -> 12.2.  Larger ones lose
-    // (fp32 32768x1536x768 60.8 -> 65), as do rows that end inside a line (8184x50280x768 690 -> 855), but for those of a chain
-    // that no cache holds (32768x8192x2048 515 -> 496, 16384x50304x1024 964 -> 880; 65536x4096x2048 506 -> 511).
+    // Whole lines of a y that the L2s (32 MB) would hold go past them, since what they hold is written back when the kernel
+    // ends: fp32 512x8192x2048 16.3 -> 15.0, 4096x1536x768 13.0 -> 12.2, bf16 1024x8192x2048 22.8 -> 21.0.  Larger ones lose (fp32
+    // 1024x8192x2048 22.0 -> 22.8, 32768x1536x768 60.8 -> 65), as do rows that end inside a line (8184x50280x768 690 -> 855), but
+    // for those of a chain that no cache holds (32768x8192x2048 517 -> 483, 16384x50304x1024 964 -> 880; 65536x4096x2048 506 ->
+    // 511).
     const int64_t row = p->ldy * (f32 ? 4 : 2);
     const bool lines = row % 128 == 0 && reinterpret_cast<uintptr_t>(p->y) % 128 == 0;
-    const bool past = lines && p->M * row <= 40 << 20, large = lines && p->M * row >= 384 << 20;
+    const bool past = lines && p->M * row < 32 << 20, large = lines && p->M * row >= 384 << 20;
     // Others by the time that their tiles take on the 256 CUs, in us: each round of a tile per CU has its start and end (longer
     // where rows of y end inside a line, or are floats) and its stages of K; two or more tiles share a CU, and a round of them
     // has the traffic of all.  Measured at 210 sizes of up to 32768 rows with every tile, the choice takes 1% more than the best

@@ -208,7 +208,8 @@ FORMS = [(40, 70, 200), (5, 100, 4100), (17, 24700, 200), (50, 24701, 270), (250
          (1000, 8100, 300), (6001, 8203, 300), (6000, 8200, 1025), (33000, 700, 250), (33000, 2100, 129),
          (500, 8101, 2500), (1000, 8101, 4100), (600, 2600, 4200), (16300, 4096, 300), (7001, 4100, 1100),
          # (rows of whole lines, which go past the caches)
-         (250, 2048, 300), (250, 8192, 130), (500, 8192, 2500), (1000, 8192, 4100), (500, 8192, 300), (1000, 8192, 300), (136, 10944, 100), (50000, 4096, 300)]
+         (250, 2048, 300), (250, 8192, 130), (500, 8192, 2500), (1000, 8192, 4100), (500, 8192, 300), (1000, 8192, 300), (136, 10944, 100),
+         (50000, 4096, 300)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
