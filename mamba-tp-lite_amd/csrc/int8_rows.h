@@ -10,9 +10,9 @@ namespace mtl {
 __device__ __forceinline__ int code_of(float t, float a) { return (int)rint((double)t * 127.0 / (double)a); }
 
 // The same without 64 bits, for a in [kLeast, kMost] and inv = 127 / a rounded: t inv is off by less than 2e-5, so its
-// rounding is the code unless it comes within 3e-5 of a half h = c + 1/2.  There 127 |t| - h a decides, and is exact:
-// 127 |t| = p + pl in two floats; p and h a are whole multiples of half an ulp of a and 2^10 of those apart at most, pl is
-// 2^-8 of that.
+// rounding is the code unless it comes within 3e-5 of a half h = c + 1/2.  There the sign of 127 |t| - h a decides, and is
+// exact: 127 |t| = p + pl in two floats; p and h a are whole multiples of a quarter of an ulp of a and 2^12 of those apart at
+// most, so their difference is a float, and a rounded sum of two floats has the sign of the sum.
 constexpr float kLeast = 0x1p-90f, kMost = 0x1p120f, kNear = 0.5f - 3e-5f;
 __device__ __forceinline__ float near_code(float t, float a, float q) {
 #pragma clang fp contract(off)
