@@ -4,6 +4,8 @@
 // products of codes are exact in 32 bits: 2^14 K < 2^31 for K < 2^17.
 #pragma once
 
+#include <algorithm>
+
 #include "common.h"
 
 namespace mtl {
@@ -17,6 +19,17 @@ inline bool act_dtype(int32_t dtype) { return dtype == MTL_F32 || dtype == MTL_B
 // Where mtl_row_linear_int8 takes a row and is no slower than two launches (us, fp32: N x K of 16384x768 7.3 for 7.9,
 // 24000x768 9.3 for 8.1, 50280x768 16.4 for 12.0; 24000x2048 11.1 for 13.4).
 inline bool row_linear_int8_pays(int64_t n, int64_t k, bool norm) { return k <= (norm ? 4096 : 8192) && n <= 16384; }
+
+// f(first row, rows, blocks) for each of the launches that M rows take, `per` of them to a block of `threads`: a launch has
+// fewer than 2^32 threads.
+template <typename F> int in_launches(int64_t M, int64_t per, int threads, F&& f) {
+    const int64_t most = ((int64_t(1) << 32) - 1) / threads * per;
+    for (int64_t m = 0; m < M; m += most) {
+        const int64_t rows = std::min(most, M - m);
+        if (const int rc = f(m, rows, (unsigned)((rows + per - 1) / per))) return rc;
+    }
+    return MTL_OK;
+}
 
 #define MTL_INT8_SIZES(M, K)                                                        \
     MTL_REQUIRE((M) >= 0 && (M) < (int64_t(1) << 31), "rows must be in [0, 2^31)"); \

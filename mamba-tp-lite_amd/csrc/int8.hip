@@ -217,20 +217,31 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_kernel(const RowsA
 }
 
 template <typename T, typename Y, typename W, bool NORM> int launch_rows(const RowsArgs& a, hipStream_t st) {
-#define MTL_ROWS(ONE, RU)                                                                                              \
-    hipLaunchKernelGGL((quantize_kernel<T, Y, W, NORM, ONE, RU>), dim3((unsigned)(ONE ? (a.M + 3) / 4 : a.M)),           \
-                       dim3(ONE ? 256 : (a.Kp + 512 * RU - 1) / (512 * RU) * 64), 0, st, a)
+    auto go = [&](void (*kernel)(RowsArgs), int per, int threads) {
+        return in_launches(a.M, per, threads, [&](int64_t m, int64_t rows, unsigned blocks) {
+            RowsArgs c = a;
+            c.x = static_cast<const T*>(a.x) + m * a.ldx;
+            if (a.y) c.y = static_cast<const Y*>(a.y) + m * a.K;
+            if (a.x_out) c.x_out = a.x_out + m * a.K;
+            c.codes = a.codes + m * a.Kp;
+            c.scales = a.scales + m;
+            c.M = rows;
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3((unsigned)threads), 0, st, c);
+            return check_launch(NORM ? "add_rmsnorm_int8" : "quantize_int8");
+        });
+    };
+#define MTL_ROWS(ONE, RU) \
+    go(quantize_kernel<T, Y, W, NORM, ONE, RU>, ONE ? 4 : 1, ONE ? 256 : (a.Kp + 512 * RU - 1) / (512 * RU) * 64)
     // A wavefront to a row of up to 1024 columns where there are many; otherwise so many that a lane has one run, or two or
     // four of long rows.  us: norms of 32768 x 2048 with bf16 y 148 with a wavefront, 133 with four; 32768 x 768 58, 60; rows
     // of 4096 in bf16, 32768 of them 71 with two runs, 83 with one; 8 of them 3.5, 3.1; 8192 x 8192 34 with two, 36 with four.
-    if (a.Kp <= 512 && a.M >= 1024) MTL_ROWS(true, 1);
-    else if (a.Kp <= 1024 && a.M >= 1024) MTL_ROWS(true, 2);
-    else if (a.Kp <= (a.M <= 1024 ? 4096 : 2048)) MTL_ROWS(false, 1);
-    else if (a.Kp <= 8192) MTL_ROWS(false, 2);
-    else if (a.Kp <= 16384) MTL_ROWS(false, 4);
-    else hipLaunchKernelGGL((quantize_long_kernel<T, Y, W, NORM>), dim3((unsigned)a.M), dim3(kLongThreads), 0, st, a);
+    if (a.Kp <= 512 && a.M >= 1024) return MTL_ROWS(true, 1);
+    if (a.Kp <= 1024 && a.M >= 1024) return MTL_ROWS(true, 2);
+    if (a.Kp <= (a.M <= 1024 ? 4096 : 2048)) return MTL_ROWS(false, 1);
+    if (a.Kp <= 8192) return MTL_ROWS(false, 2);
+    if (a.Kp <= 16384) return MTL_ROWS(false, 4);
+    return go(quantize_long_kernel<T, Y, W, NORM>, 1, kLongThreads);
 #undef MTL_ROWS
-    return check_launch(NORM ? "add_rmsnorm_int8" : "quantize_int8");
 }
 
 typedef uint32_t U4v __attribute__((ext_vector_type(4)));
@@ -335,12 +346,14 @@ extern "C" int mtl_dequantize_int8(const int8_t* codes, const float* scales, voi
     MTL_REQUIRE(ldo >= K, "rows of out must not overlap");
     const bool f32 = dtype == MTL_F32, vec = al16(out) && ldo * (f32 ? 4 : 2) % 16 == 0;
     const int per = vec ? f32 ? 1024 : 2048 : 512;            // columns of a workgroup
-    const dim3 grid((unsigned)((M + 3) / 4), (unsigned)((K + per - 1) / per)), nt(256);
-#define MTL_DEQ(T, VEC)                                                                                               \
-    hipLaunchKernelGGL((dequantize_kernel<T, VEC>), grid, nt, 0, as_stream(stream), codes, scales, static_cast<T*>(out), ldo, \
-                       M, (int)K, (int)int8_row(K))
-    if (f32) { if (vec) MTL_DEQ(float, true); else MTL_DEQ(float, false); }
-    else { if (vec) MTL_DEQ(uint16_t, true); else MTL_DEQ(uint16_t, false); }
-#undef MTL_DEQ
-    return check_launch("dequantize_int8");
+    const unsigned parts = (unsigned)((K + per - 1) / per);
+    auto go = [&](auto* kernel, auto* to) {
+        return in_launches(M, 4, 256, [&](int64_t m, int64_t rows, unsigned blocks) {
+            hipLaunchKernelGGL(kernel, dim3(blocks, parts), dim3(256), 0, as_stream(stream), codes + m * int8_row(K),
+                               scales + m, to + m * ldo, ldo, rows, (int)K, (int)int8_row(K));
+            return check_launch("dequantize_int8");
+        });
+    };
+    if (f32) return go(vec ? dequantize_kernel<float, true> : dequantize_kernel<float, false>, static_cast<float*>(out));
+    return go(vec ? dequantize_kernel<uint16_t, true> : dequantize_kernel<uint16_t, false>, static_cast<uint16_t*>(out));
 }

@@ -353,13 +353,24 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     MTL_REQUIRE(p, "null pointer");
     MTL_INT8_SIZES(p->M, p->K);
     MTL_REQUIRE(p->N >= 1 && p->N <= int64_t(1) << 27, "N must be in [1, 2^27]");
-    MTL_REQUIRE(p->M <= int64_t(1) << 30, "M must be in [0, 2^30]");
     MTL_REQUIRE(act_dtype(p->dtype), "dtype must be MTL_F32 or MTL_BF16");
     if (p->M == 0) return MTL_OK;
     MTL_REQUIRE(p->x && p->x_scales && p->w && p->w_scales && p->y, "null pointer");
     MTL_REQUIRE(al16(p->x) && al16(p->w), "codes must be 16-byte aligned");
     MTL_REQUIRE(p->ldy >= p->N, "rows of y must not overlap");
     const bool f32 = p->dtype == MTL_F32 || p->y_f32;
+    constexpr int64_t kMost = int64_t(1) << 29;                // rows whose tiles, of any size, are whole in 32 bits
+    if (p->M > kMost) {
+        mtl_linear_int8_args c = *p;
+        for (int64_t m = 0; m < p->M; m += kMost) {
+            c.x = p->x + m * int8_row(p->K);
+            c.x_scales = p->x_scales + m;
+            c.y = static_cast<uint8_t*>(p->y) + m * p->ldy * (f32 ? 4 : 2);
+            c.M = std::min(kMost, p->M - m);
+            if (const int rc = mtl_linear_int8(&c, stream)) return rc;
+        }
+        return MTL_OK;
+    }
     LinearArgs a{p->x, p->x_scales, p->w, p->w_scales, p->bias, p->y, p->ldy, (int)p->M, (int)p->N, (int)int8_row(p->K),
                  0, 0, al16(p->y) && p->ldy * (f32 ? 4 : 2) % 16 == 0, p->dtype == MTL_BF16};
     const hipStream_t st = as_stream(stream);
@@ -400,11 +411,14 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     double least = 0;
     for (int i = stages > 2 ? 0 : 1; i < 6; ++i) {
         const auto& t = kTiles[i];
-        const int64_t count = tiles(t.bn, t.bm), rounds = (count + 255) / 256, full = (count + 256 * t.share - 1) / (256 * t.share);
+        const int64_t count = tiles(t.bn, t.bm);
+        if (i > 0 && count >= 1 << 23) continue;               // (512 threads each at most, and a launch has fewer than 2^32)
+        const int64_t rounds = (count + 255) / 256, full = (count + 256 * t.share - 1) / (256 * t.share);
         const double us = t.start + rounds * (t.round + t.stage * stages + (lines ? 0 : t.inside) + (f32 ? t.floats : 0)) +
                           full * t.traffic * stages;
         if (least == 0 || us < least) { least = us; best = i; }
     }
+    MTL_REQUIRE(least > 0, "too many output tiles");
 #define MTL_TILE(...) (past ? launch<__VA_ARGS__, false, false, true>(a, f32, st) : launch<__VA_ARGS__>(a, f32, st))
     switch (best) {
         case 0: return large ? launch<256, 256, 128, 64, 2, 1, true, false, true>(a, f32, st)

@@ -152,6 +152,20 @@ __global__ void __launch_bounds__(kThreads) row_linear_int8_kernel(const RowLine
 }
 
 template <typename T, typename X> int launch(const RowLinearArgs& a, hipStream_t st) {
+    constexpr int kMost = 1 << 26;                             // columns of y: a launch has fewer than 2^32 threads
+    if (a.N > kMost) {
+        RowLinearArgs c = a;
+        c.N = kMost;
+        if (const int rc = launch<T, X>(c, st)) return rc;
+        c = a;
+        c.x_out = nullptr;
+        c.w += (int64_t)kMost * a.Kp;
+        c.sw += kMost;
+        if (a.bias) c.bias = static_cast<const uint8_t*>(a.bias) + (int64_t)kMost * (a.bias_bf16 ? 2 : 4);
+        c.y = static_cast<T*>(a.y) + kMost;
+        c.N -= kMost;
+        return launch<T, X>(c, st);
+    }
     const dim3 grid((unsigned)((a.N + 15) / 16)), nt(kThreads);
     if (a.norm_w) hipLaunchKernelGGL((row_linear_int8_kernel<T, float, X, true, 1>), grid, nt, 0, st, a);
     else if (a.K <= 4096) hipLaunchKernelGGL((row_linear_int8_kernel<T, X, X, false, 1>), grid, nt, 0, st, a);

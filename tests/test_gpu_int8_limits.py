@@ -1,0 +1,127 @@
+"""More rows than one launch has threads for: quantize_int8, add_rmsnorm_int8, dequantize_int8, linear_int8 and the product of
+one float row."""
+import ctypes
+
+import pytest
+import torch
+
+from mamba_lite import _lib, ops
+
+pytestmark = pytest.mark.gpu
+
+STEP = 1 << 24                                             # rows checked at a time
+
+
+@pytest.fixture(autouse=True)
+def _memory():
+    torch.cuda.empty_cache()
+    yield
+    torch.cuda.empty_cache()
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _same_codes(q, t):
+    """q's codes are those of the float32 rows that t(slice) gives, by the definition in 64 bits."""
+    m, k = q.scales.numel(), q.k
+    for i in range(0, m, STEP):
+        rows = t(slice(i, min(i + STEP, m))).double()
+        a = rows.abs().amax(-1, keepdim=True)
+        if not torch.equal(q.codes[i:i + STEP, :k].double(), torch.where(a > 0, (rows * 127 / a).round(), 0.0)):
+            return False
+        if bool(q.codes[i:i + STEP, k:].any()):
+            return False
+    return True
+
+
+def test_rows_into_codes_and_back():
+    # 64 threads a row
+    m, k = (1 << 26) + 5, 8
+    x = torch.randn(m, k, device="cuda", generator=_gen(0), dtype=torch.bfloat16)
+    q = ops.quantize_int8(x)
+    assert _same_codes(q, lambda s: x[s].float())
+    for dt in (torch.bfloat16, torch.float32):
+        out = torch.full((m, k), 7.0, device="cuda", dtype=dt)
+        ops.dequantize_int8(q, dt, out=out)
+        room = torch.full((m, k + 1), 7.0, device="cuda", dtype=dt)          # (rows off 16 bytes)
+        ops.dequantize_int8(q, dt, out=room[:, :k])
+        for i in range(0, m, STEP):
+            want = (q.codes[i:i + STEP, :k].float() * q.scales[i:i + STEP, None]).to(dt)
+            assert torch.equal(out[i:i + STEP], want) and torch.equal(room[i:i + STEP, :k], want)
+        assert bool((room[:, k] == 7.0).all())
+
+
+def test_norm():
+    m, k = (1 << 26) + 5, 8
+    x = torch.randn(m, k, device="cuda", generator=_gen(1))
+    y = torch.randn(m, k, device="cuda", generator=_gen(2), dtype=torch.bfloat16)
+    w = 1 + 0.3 * torch.randn(k, device="cuda", generator=_gen(3))
+    h = torch.full_like(x, 7.0)
+    q = ops.add_rmsnorm_int8(x, w, 1e-5, y=y, x_out=h)
+    for i in range(0, m, STEP):
+        assert torch.equal(h[i:i + STEP], x[i:i + STEP] + y[i:i + STEP].float())
+    assert _same_codes(q, lambda s: h[s] * w)
+    for rows in (slice(0, 1000), slice(m - 1000, m)):
+        t = h[rows].double() * w.double()
+        want = t.abs().amax(-1) / 127 * (h[rows].double().pow(2).mean(-1) + 1e-5).rsqrt()
+        # the sum of 8 squares, half of it in its root; the root, its product, the division and the row's own products
+        assert bool(((q.scales[rows].double() - want).abs() <= 12 * 2.0 ** -24 * want).all())
+
+
+def test_wide_rows_into_codes():
+    # 192 threads a row; the rows are one row, which the library takes as rows 0 elements apart
+    k, m = 1025, ((1 << 32) - 1) // 192 + 7
+    x = torch.randn(k, device="cuda", generator=_gen(4))
+    one = ops.quantize_int8(x)
+    codes = torch.zeros(m, one.codes.numel(), device="cuda", dtype=torch.int8)
+    scales = torch.zeros(m, device="cuda")
+    _lib.check(_lib.load().mtl_quantize_int8(x.data_ptr(), 0, codes.data_ptr(), scales.data_ptr(), m, k, 0, ops._stream(x)),
+               "quantize_int8")
+    assert bool((scales == one.scales).all())
+    want = one.codes.view(torch.int64)
+    for i in range(0, m, 1 << 21):
+        assert bool((codes[i:i + (1 << 21)].view(torch.int64) == want).all())
+
+
+def test_product_of_more_rows_than_one_launch_takes():
+    m, n, k = (1 << 29) + 5, 3, 100
+    codes = torch.zeros(m, 128, device="cuda", dtype=torch.int8)
+    some = [slice(0, 300), slice((1 << 29) - 300, (1 << 29) + 5)]
+    for i, rows in enumerate(some):
+        codes[rows, :k] = torch.randint(-127, 128, (rows.stop - rows.start, k), device="cuda", generator=_gen(i), dtype=torch.int8)
+    x = ops.Int8(codes, torch.full((m,), 0.02, device="cuda"), k, torch.bfloat16)
+    wc = torch.randint(-127, 128, (n, k), device="cuda", generator=_gen(9), dtype=torch.int8)
+    w = ops.pack_int8(wc, torch.tensor([0.5, 1.0, 2.0], device="cuda"))
+    out = torch.full((m, n), 7.0, device="cuda", dtype=torch.bfloat16)
+    ops.linear_int8(x, w, out=out)
+    for rows in some:
+        ref = codes[rows, :k].double() @ wc.double().t().contiguous() * float(x.scales[0]) * w.scales.double()
+        # the float of the sum, two products; and the output's rounding
+        assert bool(((out[rows].double() - ref).abs() <= (3.01 * 2.0 ** -24 + 1.01 * 2.0 ** -8) * ref.abs()).all())
+    for i in range(some[0].stop, some[1].start, 1 << 26):
+        assert not bool(out[i:min(i + (1 << 26), some[1].start)].any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_float_row_through_more_columns_than_one_launch_takes(dtype):
+    n, k = 1 << 27, 8
+    codes = torch.zeros(n, 128, device="cuda", dtype=torch.int8)
+    some = [slice(0, 300), slice((1 << 26) - 300, (1 << 26) + 300), slice(n - 300, n)]
+    for i, rows in enumerate(some):
+        codes[rows, :k] = torch.randint(-127, 128, (rows.stop - rows.start, k), device="cuda", generator=_gen(i), dtype=torch.int8)
+    w = ops.Int8(codes, torch.full((n,), 0.02, device="cuda"), k)
+    bias = torch.randn(n, device="cuda", generator=_gen(7)).to(dtype)
+    x, norm = torch.randn(1, k, device="cuda", generator=_gen(8)), torch.ones(k, device="cuda")
+    for with_norm in (False, True):
+        q = ops.add_rmsnorm_int8(x, norm, 1e-5, dtype=dtype) if with_norm else ops.quantize_int8(x.to(dtype))
+        row = x if with_norm else x.to(dtype)
+        nw, h = norm.to(dtype), torch.full_like(x, 7.0)
+        y = torch.full((n,), 7.0, device="cuda", dtype=dtype)
+        a = _lib.RowLinearInt8Args(row.data_ptr(), None, h.data_ptr() if with_norm else None, nw.data_ptr() if with_norm else None,
+                                   w.codes.data_ptr(), w.scales.data_ptr(), bias.data_ptr(), y.data_ptr(), n, k, 1e-5,
+                                   ops._ACT_DTYPES[dtype], 0, 0)
+        _lib.check(_lib.load().mtl_row_linear_int8(ctypes.byref(a), ops._stream(x)), "row_linear_int8")
+        assert torch.equal(y, ops.linear_int8(q, w, bias)[0])
+        assert torch.equal(h, x) or not with_norm

@@ -268,3 +268,12 @@ def test_scales_that_record_a_gradient_are_refused():
     for call in (lambda: lin(x), lambda: lin.rows(x, 0, 3)):
         with pytest.raises(RuntimeError, match="backward"):
             call()
+
+
+def test_linear_takes_as_many_rows_as_the_others():
+    # (a check behind that of the rows)
+    a = _lib.LinearInt8Args(None, None, None, None, None, None, 4, (1 << 31) - 1, 4, 8, 0, 0)
+    lib = _lib.load()
+    assert lib.mtl_linear_int8(ctypes.byref(a), None) == 1 and b"null" in lib.mtl_last_error()
+    a.M = 1 << 31
+    assert lib.mtl_linear_int8(ctypes.byref(a), None) == 1 and b"rows must be" in lib.mtl_last_error()
