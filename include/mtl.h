@@ -891,7 +891,8 @@ int mtl_decode_step_w4(const mtl_decode_step_batched_args* args, const mtl_decod
  *   codes itself, in one launch and to the bit what two give.  norm_w NULL: x
  *   [K] of dtype, K <= 8192, as mtl_quantize_int8.  Otherwise x, add and x_out
  *   float [K], norm_w [K] of dtype, K <= 4096, as mtl_add_rmsnorm_int8, but
- *   x_out must overlap neither x nor add.
+ *   x_out must not be x or add.  x_out and y may overlap neither each other
+ *   nor any part of an operand: such a call is refused.
  * mtl_dequantize_int8: the floats that rows stand for (dtype, ldo elements
  *   apart), rounded once from fp32.
  * All are deterministic and take no workspace.

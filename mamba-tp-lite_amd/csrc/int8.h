@@ -20,6 +20,12 @@ inline bool act_dtype(int32_t dtype) { return dtype == MTL_F32 || dtype == MTL_B
 // 24000x768 9.3 for 8.1, 50280x768 16.4 for 12.0; 24000x2048 11.1 for 13.4).
 inline bool row_linear_int8_pays(int64_t n, int64_t k, bool norm) { return k <= (norm ? 4096 : 8192) && n <= 16384; }
 
+// whether two runs of bytes meet (a null one is empty)
+inline bool meet(const void* a, int64_t na, const void* b, int64_t nb) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+    return p && q && p < q + (uintptr_t)nb && q < p + (uintptr_t)na;
+}
+
 // f(first row, rows, blocks) for each of the launches that M rows take, `per` of them to a block of `threads`: a launch has
 // fewer than 2^32 threads.
 template <typename F> int in_launches(int64_t M, int64_t per, int threads, F&& f) {

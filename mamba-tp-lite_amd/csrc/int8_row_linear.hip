@@ -185,9 +185,16 @@ extern "C" int mtl_row_linear_int8(const mtl_row_linear_int8_args* p, mtl_stream
     MTL_REQUIRE(act_dtype(p->dtype), "dtype must be MTL_F32 or MTL_BF16");
     MTL_REQUIRE(p->x && p->w && p->w_scales && p->y, "null pointer");
     MTL_REQUIRE(p->norm_w || !(p->add || p->x_out), "add and x_out need a norm");
-    MTL_REQUIRE(!p->x_out || (p->x_out != p->x && p->x_out != p->add), "x_out must not be x or add");
     MTL_REQUIRE(al16(p->w), "codes must be 16-byte aligned");
     const bool bf16 = p->dtype == MTL_BF16, f32 = !bf16 || p->y_f32;
+    // (every workgroup reads all of the row, while others write)
+    const int64_t es = bf16 ? 2 : 4, y_bytes = p->N * (f32 ? 4 : 2), out_bytes = 4 * p->K;
+    const struct { const void* at; int64_t bytes; } in[] = {
+        {p->x, p->K * (p->norm_w ? 4 : es)}, {p->add, 4 * p->K}, {p->norm_w, es * p->K}, {p->w, p->N * int8_row(p->K)},
+        {p->w_scales, 4 * p->N}, {p->bias, es * p->N}};
+    for (const auto& i : in) MTL_REQUIRE(!meet(p->x_out, out_bytes, i.at, i.bytes), "x_out must not overlap an operand");
+    for (const auto& i : in) MTL_REQUIRE(!meet(p->y, y_bytes, i.at, i.bytes), "y must not overlap an operand");
+    MTL_REQUIRE(!meet(p->y, y_bytes, p->x_out, out_bytes), "y must not overlap x_out");
     const RowLinearArgs a{p->x, p->add, p->x_out, p->norm_w, p->w, p->w_scales, p->bias, p->y, (int)p->N, (int)p->K,
                           (int)int8_row(p->K), p->eps, al16(p->y), bf16};
     const hipStream_t st = as_stream(stream);

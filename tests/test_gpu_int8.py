@@ -421,3 +421,21 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i, g in enumerate(got):
         assert all(torch.equal(u, v) for u, v in zip(g, want[i % len(jobs)]))
+
+
+@pytest.mark.parametrize("wt", DTYPES)
+def test_a_float_row_takes_buffers_side_by_side(wt):
+    # x, add, x_out and y follow each other without a gap
+    n, k = 100, 300
+    g = _gen(5)
+    w, _, _ = _matrix(n, k, 1)
+    nw = (1 + 0.3 * torch.randn(k, device="cuda", generator=g)).to(wt)
+    room = torch.randn(3 * k + n, device="cuda", generator=g)
+    x, add, h = room[:k].clone()[None], room[k:2 * k].clone()[None], torch.empty(1, k, device="cuda")
+    want = ops.linear_int8(ops.add_rmsnorm_int8(x, nw, 1e-5, y=add, x_out=h, dtype=wt), w)
+    at = lambda i: room.data_ptr() + 4 * i * k
+    a = _lib.RowLinearInt8Args(at(0), at(1), at(2), nw.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), None, at(3), n, k,
+                               1e-5, ops._ACT_DTYPES[wt], 0, 0)
+    _lib.check(_lib.load().mtl_row_linear_int8(ctypes.byref(a), ops._stream(x)), "row_linear_int8")
+    assert torch.equal(room[:k], x[0]) and torch.equal(room[k:2 * k], add[0]) and torch.equal(room[2 * k:3 * k], h[0])
+    assert torch.equal(room[3 * k:].view(wt)[:n], want[0])

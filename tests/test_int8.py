@@ -277,3 +277,25 @@ def test_linear_takes_as_many_rows_as_the_others():
     assert lib.mtl_linear_int8(ctypes.byref(a), None) == 1 and b"null" in lib.mtl_last_error()
     a.M = 1 << 31
     assert lib.mtl_linear_int8(ctypes.byref(a), None) == 1 and b"rows must be" in lib.mtl_last_error()
+
+
+def test_a_float_row_is_refused_outputs_over_what_other_workgroups_read():
+    # (addresses that nothing reads: every call here is refused)
+    lib, at = _lib.load(), lambda i: (1 << 24) + (i << 16)
+    n, k = 100, 300
+    for dtype, f32 in ((0, 0), (1, 0), (1, 1)):
+        es, ys = 2 if dtype else 4, 2 if dtype and not f32 else 4
+        size = dict(x=4 * k, add=4 * k, norm_w=es * k, w=384 * n, w_scales=4 * n, bias=es * n, x_out=4 * k, y=ys * n)
+        a = dict(x=at(0), add=at(1), x_out=at(2), norm_w=at(3), w=at(4), w_scales=at(5), bias=at(6), y=at(7))
+        for out in ("x_out", "y"):
+            for over in set(a) - {out}:
+                # (the codes are moved in whole 16 bytes)
+                for d in {0, 4, 16, size[over] - 4, 4 - size[out]} if over != "w" else {0, 16, size[over] - 4}:
+                    p = _lib.RowLinearInt8Args(N=n, K=k, eps=1e-5, dtype=dtype, y_f32=f32, **dict(a, **{out: a[over] + d}))
+                    assert lib.mtl_row_linear_int8(ctypes.byref(p), None) == 1, (out, over, d)
+                    assert b"overlap" in lib.mtl_last_error(), (out, over, d)
+        # without a norm the row is of dtype
+        b = dict(a, add=None, x_out=None, norm_w=None)
+        for d in (0, es * k - 2, 2 - ys * n):
+            p = _lib.RowLinearInt8Args(N=n, K=k, dtype=dtype, y_f32=f32, **dict(b, y=a["x"] + d))
+            assert lib.mtl_row_linear_int8(ctypes.byref(p), None) == 1 and b"overlap" in lib.mtl_last_error()
