@@ -879,10 +879,11 @@ int mtl_decode_step_w4(const mtl_decode_step_batched_args* args, const mtl_decod
  *
  * mtl_quantize_int8: rows of x (dtype MTL_F32 or MTL_BF16, ldx elements apart).
  * mtl_add_rmsnorm_int8: h = x + y (y NULL: x), stored in x_out unless that is
- *   NULL (it may be x, or a float y), and the row w rmsnorm(h) (model.py:
- *   130-135 with the residual add of 306/311) in int8: the codes of the float
- *   row t = h w, and scale = a / 127 / sqrt(mean(h^2) + eps).  x, x_out float,
- *   y of y_dtype, all [M, K] contiguous, w [K] of w_dtype.
+ *   NULL (it may be x, or a float y; over any other part of an operand it is
+ *   refused), and the row w rmsnorm(h) (model.py:130-135 with the residual add
+ *   of 306/311) in int8: the codes of the float row t = h w, and scale = a /
+ *   127 / sqrt(mean(h^2) + eps).  x, x_out float, y of y_dtype, all [M, K]
+ *   contiguous, w [K] of w_dtype.
  * mtl_linear_int8: y [M, N] = x W^T (+ bias [N]) for x [M, K] and W [N, K] in
  *   this layout, y (rows ldy elements apart) and bias of type dtype: the sum
  *   exact, then times x's scale and W's, each rounded in fp32.  N <= 2^27.  y

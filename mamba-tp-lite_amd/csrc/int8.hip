@@ -323,6 +323,15 @@ extern "C" int mtl_add_rmsnorm_int8(const mtl_add_rmsnorm_int8_args* p, mtl_stre
     if (p->M == 0) return MTL_OK;
     MTL_REQUIRE(p->x && p->w && p->codes && p->scales, "null pointer");
     MTL_REQUIRE(al16(p->codes), "codes must be 16-byte aligned");
+    if (p->x_out) {
+        // (a value's own place is read before it is written; another's may not be)
+        const int64_t bytes = 4 * p->M * p->K;
+        const bool bf16 = p->y_dtype == MTL_BF16;
+        MTL_REQUIRE((p->x_out == p->x || !meet(p->x_out, bytes, p->x, bytes)) &&
+                    ((!bf16 && p->x_out == p->y) || !meet(p->x_out, bytes, p->y, bf16 ? bytes / 2 : bytes)) &&
+                    !meet(p->x_out, bytes, p->w, (p->w_dtype == MTL_BF16 ? 2 : 4) * p->K),
+                    "x_out must be x, a float y, or overlap no operand");
+    }
     RowsArgs a{};
     a.x = p->x; a.ldx = p->K; a.y = p->y; a.x_out = p->x_out; a.w = p->w; a.codes = p->codes; a.scales = p->scales;
     a.M = p->M; a.K = (int)p->K; a.Kp = (int)int8_row(p->K); a.eps = p->eps;

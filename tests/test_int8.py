@@ -299,3 +299,19 @@ def test_a_float_row_is_refused_outputs_over_what_other_workgroups_read():
         for d in (0, es * k - 2, 2 - ys * n):
             p = _lib.RowLinearInt8Args(N=n, K=k, dtype=dtype, y_f32=f32, **dict(b, y=a["x"] + d))
             assert lib.mtl_row_linear_int8(ctypes.byref(p), None) == 1 and b"overlap" in lib.mtl_last_error()
+
+
+def test_the_norms_sum_is_refused_over_another_place_of_its_operands():
+    # (addresses that nothing reads: every call here is refused)
+    lib, at = _lib.load(), lambda i: (1 << 24) + (i << 16)
+    m, k = 5, 300
+    for y_dtype, w_dtype in ((0, 0), (1, 0), (0, 1), (1, 1)):
+        size = dict(x=4 * m * k, y=(2 if y_dtype else 4) * m * k, w=(2 if w_dtype else 4) * k)
+        a = dict(x=at(0), y=at(1), x_out=at(2), w=at(3), codes=at(4), scales=at(5))
+        for over in size:
+            for d in {0, 4, 4 * k, size[over] - 4, 4 - 4 * m * k, -4}:
+                if d == 0 and (over == "x" or (over == "y" and not y_dtype)):
+                    continue                                     # (in place)
+                p = _lib.AddRmsnormInt8Args(M=m, K=k, eps=1e-5, y_dtype=y_dtype, w_dtype=w_dtype, **dict(a, x_out=a[over] + d))
+                assert lib.mtl_add_rmsnorm_int8(ctypes.byref(p), None) == 1, (over, d)
+                assert b"x_out" in lib.mtl_last_error(), (over, d)
