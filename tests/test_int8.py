@@ -309,7 +309,7 @@ def test_the_norms_sum_is_refused_over_another_place_of_its_operands():
         size = dict(x=4 * m * k, y=(2 if y_dtype else 4) * m * k, w=(2 if w_dtype else 4) * k)
         a = dict(x=at(0), y=at(1), x_out=at(2), w=at(3), codes=at(4), scales=at(5))
         for over in size:
-            for d in {0, 4, 4 * k, size[over] - 4, 4 - 4 * m * k, -4}:
+            for d in {0, 4, k, size[over] - 4, 4 - 4 * m * k, -4}:
                 if d == 0 and (over == "x" or (over == "y" and not y_dtype)):
                     continue                                     # (in place)
                 p = _lib.AddRmsnormInt8Args(M=m, K=k, eps=1e-5, y_dtype=y_dtype, w_dtype=w_dtype, **dict(a, x_out=a[over] + d))
