@@ -828,6 +828,8 @@ class MambaLM(nn.Module):
                 w = norm.weight if norm.weight.dtype == torch.bfloat16 and norm.weight.is_contiguous() else _f32(norm.weight)
                 if isinstance(y, _Parts):
                     y = ops.sum_parts(y.parts)
+                elif y is not None and y.dtype not in (torch.float32, torch.bfloat16):
+                    y = y.float()                            # (a hook's or another projection's type)
                 with torch.no_grad():
                     return ops.add_rmsnorm_int8(h, w, norm.eps, y=None if y is None else y.contiguous(), dtype=act, **kw)
         if isinstance(y, _Parts):

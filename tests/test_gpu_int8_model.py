@@ -390,3 +390,22 @@ def test_a_step_of_one_row_in_every_mix_of_launches(kw, dtype, monkeypatch):
         want = [q.step(ids[:, i:i + 1], other) for i in range(4, 8)]
     for a, r in zip(got, want):
         assert torch.equal(a, r) if dtype == torch.float32 else _rel(a, r) < TOL[dtype]
+
+
+@pytest.mark.parametrize("kind", [torch.float16, torch.float64])
+def test_a_mixers_output_of_another_float_type_is_added(kind):
+    q = _model(n_layer=3).quantize_int8()
+    ids = torch.randint(0, 1003, (2, 9), device="cuda")
+
+    def run(hook):
+        handle = q.layers[0].mixer.out_proj.register_forward_hook(hook)
+        logits, cache = q.prefill(ids)
+        step = q.step(ids[:, :1], cache)
+        handle.remove()
+        return logits, step
+
+    with torch.no_grad():
+        # (the value is converted to float32 where the float norm converts it)
+        want = run(lambda m, a, o: o.to(kind).float())
+        got = run(lambda m, a, o: o.to(kind))
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
