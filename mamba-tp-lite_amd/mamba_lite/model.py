@@ -1035,7 +1035,7 @@ class MambaLM(nn.Module):
             return self._step_fused(input_ids, cache, lt=lt)
         x = self.embedding(input_ids).squeeze(1)
         if not plain and BATCHED_STEP_NATIVE:
-            got = self._quant_step_layers(x, cache, lt, kind)
+            got = self._w4_step_layers(x, cache, lt) if kind is LinearW4 else self._quant_step_layers(x, cache, lt, kind)
             if got is not None:
                 h = x if x.dtype == torch.float32 else x.float()
                 step = ops.decode_step_w4 if kind is LinearW4 else ops.decode_step_int8
@@ -1222,8 +1222,9 @@ class MambaLM(nn.Module):
         """(ctypes arrays of mtl_decode_layer with this call's cache pointers and of the projections' matrices) for
         mtl_decode_step_w4 or mtl_decode_step_int8 (kind: LinearW4 or LinearInt8), or None where it does not apply: sizes,
         a stack of more than plain modules and `kind`, a weight or cache tensor that is not a contiguous tensor of x's
-        dtype (SSM states: float32) and its shape on x's device.  The weights are checked when their addresses, the projections' form (group, scales' type, sizes) or
-        x_proj's version (which its transposed copy follows) change; the cache tensors every call."""
+        dtype (SSM states: float32) and its shape on x's device.  The weights are checked when their addresses, the
+        projections' form (group, scales' type, sizes) or x_proj's version (which its transposed copy follows) change;
+        the cache tensors every call."""
         cfg, act, dev = self.cfg, x.dtype, x.device
         nl = len(lt)
         D, N, K, R = cfg.d_inner, cfg.d_state, cfg.d_conv, cfg.dt_rank
