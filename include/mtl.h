@@ -941,6 +941,9 @@ int mtl_quantize_int8(const void* x, int64_t ldx, int8_t* codes, float* scales, 
 int mtl_add_rmsnorm_int8(const mtl_add_rmsnorm_int8_args* args, mtl_stream_t stream);
 int mtl_linear_int8(const mtl_linear_int8_args* args, mtl_stream_t stream);
 int mtl_row_linear_int8(const mtl_row_linear_int8_args* args, mtl_stream_t stream);
+/* 1 where mtl_row_linear_int8 takes a row of K floats through [N, K], after a
+ * norm or without, and is no slower than the two launches in its place. */
+int mtl_row_linear_int8_pays(int64_t N, int64_t K, int32_t norm);
 int mtl_dequantize_int8(const int8_t* codes, const float* scales, void* out, int64_t ldo, int64_t M, int64_t K,
                         int32_t dtype, mtl_stream_t stream);
 

@@ -176,6 +176,10 @@ template <typename T, typename X> int launch(const RowLinearArgs& a, hipStream_t
 }  // namespace
 }  // namespace mtl
 
+extern "C" int mtl_row_linear_int8_pays(int64_t N, int64_t K, int32_t norm) {
+    return mtl::row_linear_int8_pays(N, K, norm != 0) ? 1 : 0;
+}
+
 extern "C" int mtl_row_linear_int8(const mtl_row_linear_int8_args* p, mtl_stream_t stream) {
     using namespace mtl;
     clear_error();

@@ -15,7 +15,7 @@ import os
 import torch  # noqa: F401  (must be loaded first, see module docstring)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmtl.so")
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 MTL_F32 = 0
 MTL_BF16 = 1
@@ -240,6 +240,7 @@ SIGNATURES = {
     "mtl_add_rmsnorm_int8": (ctypes.c_int, [ctypes.POINTER(AddRmsnormInt8Args), _vp]),
     "mtl_linear_int8": (ctypes.c_int, [ctypes.POINTER(LinearInt8Args), _vp]),
     "mtl_row_linear_int8": (ctypes.c_int, [ctypes.POINTER(RowLinearInt8Args), _vp]),
+    "mtl_row_linear_int8_pays": (ctypes.c_int, [_i64, _i64, _i32]),
     "mtl_dequantize_int8": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
     "mtl_decode_step_int8": (ctypes.c_int, [ctypes.POINTER(DecodeStepBatchedArgs), ctypes.POINTER(DecodeLayer),
                                             ctypes.POINTER(Int8Matrix), _i32, _vp]),

@@ -1668,23 +1668,25 @@ def add_rmsnorm_int8(x, weight, eps, y=None, x_out=None, dtype=torch.float32):
     return q
 
 
-# one float row is quantized within the product up to here (past 16384 columns of y two launches are faster: 24000 x 768 8.1
-# us for 9.3)
-_ROW_MAX_K, _ROW_MAX_N = 8192, 16384
+@functools.lru_cache(maxsize=4096)
+def row_linear_int8_pays(n: int, k: int) -> bool:
+    """Where one float row is put into codes within its product [n, k] (mtl_row_linear_int8): it is faster than two launches."""
+    return bool(_lib.load().mtl_row_linear_int8_pays(n, k, 0))
 
 
 def linear_int8(x, w, bias=None, out=None):
     """x [..., k] W^T (+ bias [n]) of an Int8 x and an Int8 matrix W [n, k] (mtl_linear_int8): [..., n] of x's type.  The
     sum over k is exact; it is multiplied by the two scales in float32.  bias and out have x's type.  x may be a float32 or
-    bfloat16 tensor: quantize_int8(x) is multiplied then, a single row in one launch (mtl_row_linear_int8)."""
+    bfloat16 tensor: quantize_int8(x) is multiplied then, a single row in one launch where that pays
+    (mtl_row_linear_int8)."""
     if type(w) is not Int8:
         _is_int8("linear_int8", "w", w)
     row = False
     if type(x) is not Int8:
         if not isinstance(x, torch.Tensor):
             _is_int8("linear_int8", "x", x)
-        row = x.dtype in _ACT_DTYPES and x.dim() > 0 and x.numel() == x.shape[-1] == w.k <= _ROW_MAX_K and \
-            w.scales.numel() <= _ROW_MAX_N
+        row = x.dtype in _ACT_DTYPES and x.dim() > 0 and x.numel() == x.shape[-1] == w.k and \
+            row_linear_int8_pays(w.scales.numel(), w.k)
         if not row:
             x = quantize_int8(x)
     if row:

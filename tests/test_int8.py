@@ -315,3 +315,19 @@ def test_the_norms_sum_is_refused_over_another_place_of_its_operands():
                 p = _lib.AddRmsnormInt8Args(M=m, K=k, eps=1e-5, y_dtype=y_dtype, w_dtype=w_dtype, **dict(a, x_out=a[over] + d))
                 assert lib.mtl_add_rmsnorm_int8(ctypes.byref(p), None) == 1, (over, d)
                 assert b"x_out" in lib.mtl_last_error(), (over, d)
+
+
+def test_one_rule_says_where_a_float_row_is_put_into_codes_within_its_product():
+    pays = _lib.load().mtl_row_linear_int8_pays
+    # (n, k, norm): one launch measured faster, two
+    for n, k, norm in ((768, 1536, 0), (8192, 64, 0), (12288, 512, 0), (24576, 1024, 0), (24576, 2048, 0), (50280, 2048, 0),
+                       (65536, 4096, 0), (16384, 2560, 0), (16384, 7168, 0), (8192, 256, 1), (8192, 2048, 1), (16384, 4096, 1)):
+        assert pays(n, k, norm) == 1, (n, k, norm)
+    for n, k, norm in ((16384, 64, 0), (20480, 512, 0), (24576, 768, 0), (50280, 768, 0), (32768, 1024, 0), (24576, 2560, 0),
+                       (20480, 7168, 0), (12288, 256, 1), (16384, 768, 1), (24576, 2560, 1), (50280, 2048, 1)):
+        assert pays(n, k, norm) == 0, (n, k, norm)
+    # what the launch does not take
+    for n, k, norm in ((16, 8193, 0), (16, 4097, 1), (0, 64, 0), (16, 0, 0), (1 << 40, 2048, 0)):
+        assert pays(n, k, norm) == 0, (n, k, norm)
+    for n, k in ((768, 1536), (50280, 2048), (50280, 768), (16, 8193)):
+        assert ops.row_linear_int8_pays(n, k) == bool(pays(n, k, 0))
