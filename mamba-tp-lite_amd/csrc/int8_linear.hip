@@ -387,18 +387,22 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
     if (a.M <= 64 && tiles(128, 64) >= 160)
         return a.M <= 32 ? launch<128, 32, 32, 32, 4, 2, false, true>(a, f32, st)
                          : launch<128, 64, 32, 32, 3, 2, false, true>(a, f32, st);
-    // Whole lines of a y that the L2s (32 MB) would hold go past them, since what they hold is written back when the kernel
-    // ends: fp32 512x8192x2048 16.3 -> 15.0, 4096x1536x768 13.0 -> 12.2, bf16 1024x8192x2048 22.8 -> 21.0.  Larger ones lose (fp32
-    // 1024x8192x2048 22.0 -> 22.8, 32768x1536x768 60.8 -> 65), as do rows that end inside a line (8184x50280x768 690 -> 855), but
-    // for those of a chain that no cache holds (32768x8192x2048 517 -> 483, 16384x50304x1024 964 -> 880; 65536x4096x2048 506 ->
-    // 511).
-    const int64_t row = p->ldy * (f32 ? 4 : 2);
+    // Whole lines of y go past the L2s (32 MB) where those would hold them, since what they hold is written back when the kernel
+    // ends, and where not even the MALL (256 MB) does.  us of the product / of it with the quantize_int8 that reads y next, kept
+    // and past, at 200 sizes: fp32 512x8192x2048 (16 MB) 16.5 and 15.0 / 23.3 and 22.5, bf16 16384x768x1536 (24 MB) 25.2 and 23.2 /
+    // 34.8 and 34.2.  From 28 MB on the reader gives back more than the product gains (fp32 896x8192x2048 22.6 and 21.7 / 30.3 and
+    // 30.5; 32 MB 23.5 and 24.2 / 31.5 and 32.7; 64 MB 38.3 and 40.9 / 51.3 and 56.0); at 256 MB three of ten sizes lose 6%, from 320
+    // on none (fp32 20480x4096x2048 173 and 175 / 252 and 240, bf16 32768x8192x2048 519 and 503 / 676 and 651, fp32 87381x1536x768
+    // 197 and 151 / 320 and 289).  Rows that end inside a line lose at any size (8184x50277x768 690 and 855).
+    const int64_t row = p->ldy * (f32 ? 4 : 2), y_bytes = p->M * row;
     const bool lines = row % 128 == 0 && reinterpret_cast<uintptr_t>(p->y) % 128 == 0;
-    const bool past = lines && p->M * row < 32 << 20, large = lines && p->M * row >= 384 << 20;
+    const bool past = lines && y_bytes <= 24 << 20, large = lines && y_bytes >= 320 << 20;
     // Others by the time that their tiles take on the 256 CUs, in us: each round of a tile per CU has its start and end (longer
     // where rows of y end inside a line, or are floats) and its stages of K; two or more tiles share a CU, and a round of them
-    // has the traffic of all.  Measured at 210 sizes of up to 32768 rows with every tile, the choice takes 1% more than the best
-    // of them (a cost by rounds alone 7% more); us with the tiles in the table's order:
+    // has the traffic of all.  Measured at 210 sizes of up to 32768 rows with every tile, the choice takes 1% more than the best of
+    // them on average (a cost by rounds alone 7% more), 5-20% more at ten of them, most of those with one to three stages of K:
+    // 80x19686x76 5.5 by the last one for 4.6, 692x5440x384 7.8 for 6.6, fp32 5694x478x170 7.3 for 6.3.  us with the tiles in the
+    // table's order:
     //   bf16 1024x8192x2048 - 21 27 34 - 23; fp32 8192x768x1536 - 19.6 25.7 25.0 - 18.8; 1179x2304x4480 56 34 23 28 40 32;
     //   720x1167x3393 54 31 20 14 16 28; fp32 657x576x1280 24 14 9.6 6.1 5.2 11; fp32 14280x1685x1184 - - - - - 49 (60 of the
     //   first); 32768x8192x2048 496 by the first, 586 by the second

@@ -1,5 +1,5 @@
-"""More rows than one launch has threads for: quantize_int8, add_rmsnorm_int8, dequantize_int8, linear_int8 and the product of
-one float row."""
+"""More rows than one launch has threads for, and the products whose stores or tiles depend on the size of y: quantize_int8,
+add_rmsnorm_int8, dequantize_int8, linear_int8 and the product of one float row."""
 import ctypes
 
 import pytest
@@ -125,3 +125,29 @@ def test_a_float_row_through_more_columns_than_one_launch_takes(dtype):
         _lib.check(_lib.load().mtl_row_linear_int8(ctypes.byref(a), ops._stream(x)), "row_linear_int8")
         assert torch.equal(y, ops.linear_int8(q, w, bias)[0])
         assert torch.equal(h, x) or not with_norm
+
+
+# ------------------------------------------------------------------ the size of y
+def _int8(rows, k, seed, dtype=torch.float32):
+    g = _gen(seed)
+    codes = torch.randint(-127, 128, (rows, k), device="cuda", generator=g, dtype=torch.int8)
+    return ops.pack_int8(codes, (torch.rand(rows, device="cuda", generator=g) + 0.5) * 0.01, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+# (rows of whole lines: 24 MB in fp32 and in bf16, a row more, and 320 MB of a chain)
+@pytest.mark.parametrize("m,n,k", [(740, 8192, 4100), (768, 8192, 4100), (769, 8192, 4100), (1536, 8192, 2048), (1537, 8192, 2048),
+                                   (40959, 2048, 390), (40960, 2048, 390), (40960, 4096, 390)])
+def test_product_at_the_sizes_of_y_where_its_stores_change(m, n, k, dtype):
+    x, w = _int8(m, k, m, dtype), _int8(n, k, n)
+    bias = torch.randn(n, device="cuda", generator=_gen(1)).to(dtype)
+    out = torch.full((m, n), 7.0, device="cuda", dtype=dtype)
+    ops.linear_int8(x, w, bias, out=out)
+    half = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
+    wc = w.codes[:, :k].double().t().contiguous()
+    for i in range(0, m, 4096):
+        p = x.codes[i:i + 4096, :k].double() @ wc * x.scales[i:i + 4096, None].double() * w.scales.double()
+        ref = p + bias.double()
+        # the sum as a float, times one scale, times the other and with the bias; the output's rounding
+        off = 3.01 * 2.0 ** -24 * p.abs() + 2.0 ** -24 * ref.abs()
+        assert bool(((out[i:i + 4096].double() - ref).abs() <= off + half * (ref.abs() + off)).all())
