@@ -127,7 +127,7 @@ def test_a_float_row_through_more_columns_than_one_launch_takes(dtype):
         assert torch.equal(h, x) or not with_norm
 
 
-# ------------------------------------------------------------------ the size of y
+# ------------------------------------------------------------------ the size of y, and chains of tiles
 def _int8(rows, k, seed, dtype=torch.float32):
     g = _gen(seed)
     codes = torch.randint(-127, 128, (rows, k), device="cuda", generator=g, dtype=torch.int8)
@@ -151,3 +151,52 @@ def test_product_at_the_sizes_of_y_where_its_stores_change(m, n, k, dtype):
         # the sum as a float, times one scale, times the other and with the bias; the output's rounding
         off = 3.01 * 2.0 ** -24 * p.abs() + 2.0 ** -24 * ref.abs()
         assert bool(((out[i:i + 4096].double() - ref).abs() <= off + half * (ref.abs() + off)).all())
+
+
+# (chains of tiles: partial ones and with a bias; whole lines past the caches; the smallest K)
+CHAINS = [(3000, 8200, 400, True), (24000, 4096, 390, False), (6001, 8203, 1025, True)]
+
+
+def _product(x, w, bias, out):
+    return ops.linear_int8(x, w, bias, out=out)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k,bias", CHAINS)
+def test_chains_replay_what_they_compute_eagerly(m, n, k, bias, dtype):
+    x, w = _int8(m, k, 1, dtype), _int8(n, k, 2)
+    b = torch.randn(n, device="cuda", generator=_gen(3)).to(dtype) if bias else None
+    out = torch.empty(m, n, device="cuda", dtype=dtype)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        _product(x, w, b, out)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _product(x, w, b, out)
+    for i in range(3):
+        x.codes[:, :k].copy_(torch.randint(-127, 128, (m, k), device="cuda", generator=_gen(10 + i), dtype=torch.int8))
+        want = ops.linear_int8(x, w, b)
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_chains_on_streams_side_by_side(dtype):
+    jobs = []
+    for i, (m, n, k, bias) in enumerate(CHAINS + [(300, 640, 640, True)]):
+        b = torch.randn(n, device="cuda", generator=_gen(i)).to(dtype) if bias else None
+        jobs.append((_int8(m, k, i, dtype), _int8(n, k, 20 + i), b))
+    want = [ops.linear_int8(*a) for a in jobs]
+    outs = [[torch.full_like(t, 7.0) for t in want] for _ in range(3)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for row in outs:
+        for s, a, out in zip(streams, jobs, row):
+            with torch.cuda.stream(s):
+                _product(*a, out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, w) for row in outs for t, w in zip(row, want))
