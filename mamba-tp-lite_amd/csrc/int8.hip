@@ -20,8 +20,6 @@ struct RowsArgs {
     float eps;
 };
 
-typedef uint32_t U2v __attribute__((ext_vector_type(2)));
-
 // Rows held in registers from one pass over memory: as many wavefronts to a row as RU runs of 8 columns a lane need, or ONE.
 // HBM is the bound.
 constexpr int kRowThreads = 512;
@@ -135,10 +133,10 @@ __global__ void __launch_bounds__(ONE ? 256 : kRowThreads) quantize_kernel(const
         const int k = (u * G + t) * kRun;
         if (k < p.Kp) {
             const uint2 c = none ? uint2{0, 0} : run_codes(v[u], a, inv, exact);
-            // (past the caches: fp32 32768 x 2048 57.7 -> 46.2 us, 8192 x 2048 15.9 -> 14.3; beside the norm's other stores
-            // 36.7 -> 38.3)
-            if constexpr (NORM) *reinterpret_cast<uint2*>(p.codes + row * p.Kp + k) = c;
-            else __builtin_nontemporal_store(U2v{c.x, c.y}, reinterpret_cast<U2v*>(p.codes + row * p.Kp + k));
+            // (kept in the caches for the product that reads them next: past them a call alone is up to a sixth faster, fp32
+            // 32768 x 2048 56 -> 47 us, but with its reader slower, 16384 x 1536 through [768, 1536] 46.4 -> 48.7 and 1024 rows 10.8
+            // -> 11.5; with their values 38.7 -> 42.8)
+            *reinterpret_cast<uint2*>(p.codes + row * p.Kp + k) = c;
         }
     }
 }
