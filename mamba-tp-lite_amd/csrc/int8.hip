@@ -59,7 +59,8 @@ __global__ void __launch_bounds__(ONE ? 256 : kRowThreads) quantize_kernel(const
     if constexpr (NORM) {
         if (p.x_out) {
             // through LDS, so that an instruction stores whole lines: 32768 x 2048 with bf16 y 135 -> 121 us (6.1 TB/s).  Past the
-            // caches, as it is read again a layer later only: 131 without, 1024 x 2048 7.2 -> 6.5.
+            // caches, as it is read again a layer later only: into another buffer 131 without; in place 129, 128 with it, and with
+            // the product behind it level from 32 rows to 32768.
             const int lane = t & 63, k0 = (t - lane) * kRun;
             float* s = s_out[threadIdx.x / 64];
 #pragma unroll
@@ -244,8 +245,8 @@ template <typename T, typename Y, typename W, bool NORM> int launch_rows(const R
 
 typedef uint32_t U4v __attribute__((ext_vector_type(4)));
 
-// A wavefront reads runs of R codes of a row and writes 16 bytes a lane.
-template <typename T, bool VEC> __global__ void __launch_bounds__(256)
+// A wavefront reads runs of R codes of a row and writes 16 bytes a lane; PAST: past the L2s.
+template <typename T, bool VEC, bool PAST = false> __global__ void __launch_bounds__(256)
 dequantize_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out, int64_t ld,
                   int64_t M, int K, int Kp) {
     constexpr int R = VEC ? 16 / (int)sizeof(T) : 1, U = VEC ? 4 : 8;
@@ -274,9 +275,8 @@ dequantize_kernel(const int8_t* __restrict__ codes, const float* __restrict__ sc
                 if constexpr (R == 4) v = U4v{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
                 else v = U4v{f32x2_to_bf16x2(f[0], f[1]), f32x2_to_bf16x2(f[2], f[3]), f32x2_to_bf16x2(f[4], f[5]),
                              f32x2_to_bf16x2(f[6], f[7])};
-                // (past the L2s, which write what they hold back when the kernel ends: 8192 x 2048 bf16 8.8 -> 6.5 us,
-                // 32768 x 2048 fp32 59.8 -> 49.1)
-                __builtin_nontemporal_store(v, reinterpret_cast<U4v*>(o + k));
+                if (PAST) __builtin_nontemporal_store(v, reinterpret_cast<U4v*>(o + k));
+                else *reinterpret_cast<U4v*>(o + k) = v;
             } else {
 #pragma unroll
                 for (int j = 0; j < R; ++j)
@@ -361,6 +361,14 @@ extern "C" int mtl_dequantize_int8(const int8_t* codes, const float* scales, voi
             return check_launch("dequantize_int8");
         });
     };
-    if (f32) return go(vec ? dequantize_kernel<float, true> : dequantize_kernel<float, false>, static_cast<float*>(out));
-    return go(vec ? dequantize_kernel<uint16_t, true> : dequantize_kernel<uint16_t, false>, static_cast<uint16_t*>(out));
+    // Past the L2s between 4 and 16 MB: what they hold is written back when the kernel ends, but a reader of more than they keep
+    // waits for the MALL either way.  us, kept and past, alone / with a reader behind: fp32 256x2048 (2 MB) 2.5, 2.5 / 5.4, 5.7;
+    // bf16 4096x2048 (16 MB) 6.1, 5.0 / 17.6, 17.1; fp32 3072x2048 (24 MB) 6.6, 6.4 / 19.7, 20.6; 32768x1536 39.5, 45.5 / 75.8, 86.5.
+    const int64_t bytes = M * ldo * (f32 ? 4 : 2);
+    const bool past = bytes >= 4 << 20 && bytes <= 16 << 20;
+    if (f32)
+        return go(vec ? past ? dequantize_kernel<float, true, true> : dequantize_kernel<float, true>
+                      : dequantize_kernel<float, false>, static_cast<float*>(out));
+    return go(vec ? past ? dequantize_kernel<uint16_t, true, true> : dequantize_kernel<uint16_t, true>
+                  : dequantize_kernel<uint16_t, false>, static_cast<uint16_t*>(out));
 }

@@ -153,6 +153,15 @@ def test_product_at_the_sizes_of_y_where_its_stores_change(m, n, k, dtype):
         assert bool(((out[i:i + 4096].double() - ref).abs() <= off + half * (ref.abs() + off)).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k", [(1023, 1024), (1024, 1024), (2048, 1024), (4096, 1020), (4096, 1024), (4097, 1024), (8192, 1024), (8193, 1024)])
+def test_values_at_the_sizes_where_their_stores_change(m, k, dtype):
+    q = _int8(m, k, m, dtype)
+    out = torch.full((m + 1, k), 7.0, device="cuda", dtype=dtype)
+    ops.dequantize_int8(q, out=out[:m])
+    assert torch.equal(out[:m], (q.codes[:, :k].float() * q.scales[:, None]).to(dtype)) and bool((out[m] == 7.0).all())
+
+
 # (chains of tiles: partial ones and with a bias; whole lines past the caches; the smallest K)
 CHAINS = [(3000, 8200, 400, True), (24000, 4096, 390, False), (6001, 8203, 1025, True)]
 
