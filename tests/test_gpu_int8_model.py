@@ -409,3 +409,78 @@ def test_a_mixers_output_of_another_float_type_is_added(kind):
         want = run(lambda m, a, o: o.to(kind).float())
         got = run(lambda m, a, o: o.to(kind))
     assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+def _row_rel(a, b):
+    """The largest relative distance of a row (equal rows, of zeros too: 0)."""
+    a, b = (t.double().reshape(-1, t.shape[-1]) for t in (a, b))
+    off = (a - b).norm(dim=-1)
+    return float(torch.where(off == 0, 0.0, off / b.norm(dim=-1)).max())
+
+
+# As TOL, which counts one value of each row and product on the other side of a border, for seven products (three layers and a
+# head): 7 * 4 / 127 / 16 = 1.4e-2, and as much again for what earlier tokens' states bring.
+ROW_TOL = 2 * 7 * 4 / 127 / 16
+
+
+@pytest.mark.parametrize("b,l", [(1, 1), (1, 64), (2, 65), (3, 130), (1, 700)])
+def test_prompts_in_one_call_are_those_op_by_op_row_by_row(b, l, monkeypatch):
+    q = _model(d_model=256, n_layer=3, bias=True).quantize_int8()
+    ids = torch.randint(0, 1003, (b, 2 * l), device="cuda")
+    calls = []
+    real = ops.prefill_long
+    monkeypatch.setattr(ops, "prefill_long", lambda *a, **k: (calls.append(k["matrices"]), real(*a, **k))[1])
+    runs = []
+    with torch.no_grad():
+        for native in (True, False):
+            monkeypatch.setattr(mm, "LONG_PREFILL_NATIVE", native)
+            first, cache = q.prefill(ids[:, :l])
+            kept = copy.deepcopy(cache)
+            second, cache = q.prefill(ids[:, l:], cache)
+            runs.append((first, second, kept, cache))
+    assert len(calls) == 2 and all(m is not None for m in calls)
+    (a0, a1, ka, ca), (r0, r1, kr, cr) = runs
+    assert _row_rel(a0, r0) < ROW_TOL and _row_rel(a1, r1) < ROW_TOL
+    for mine, theirs in ((ka, kr), (ca, cr)):
+        # the first layer's history is what the norm and in_proj give: no library product before it
+        assert torch.equal(mine.layers[0].conv_state, theirs.layers[0].conv_state)
+        for u, v in zip(mine.layers, theirs.layers):
+            # (rows of a state: all channels of a place)
+            assert _row_rel(u.conv_state.transpose(1, 2), v.conv_state.transpose(1, 2)) < ROW_TOL
+            assert _row_rel(u.ssm_state.transpose(1, 2), v.ssm_state.transpose(1, 2)) < ROW_TOL
+
+
+def _by_definition_of(q):
+    """_by_definition() of a stack in which some projections are plain."""
+    m = copy.deepcopy(q)
+    for blk, of in zip(m.layers, q.layers):
+        for name in ("in_proj", "out_proj"):
+            p = getattr(of.mixer, name)
+            if type(p) is LinearInt8:
+                setattr(blk.mixer, name, _Plain(p))
+    if "head_int8" in m._modules:
+        m._modules.pop("head_int8")
+        m._modules["head_w4"] = _Plain(q.head_int8)
+    return m
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,l", [(1, 9), (2, 70)])
+@pytest.mark.parametrize("which", ["no head", "plain in_proj first", "plain in_proj last", "plain out_proj first"])
+def test_stacks_of_both_kinds_are_those_of_the_definition(which, b, l, dtype):
+    m = _model(n_layer=3, dtype=dtype)
+    q = copy.deepcopy(m).quantize_int8(lm_head=which != "no head")
+    if which != "no head":
+        i, name = (2 if "last" in which else 0), "out_proj" if "out" in which else "in_proj"
+        setattr(q.layers[i].mixer, name, getattr(m.layers[i].mixer, name))
+    ref = _by_definition_of(q)
+    ids = torch.randint(0, 1003, (b, l + 3), device="cuda")
+    # as ROW_TOL, with seven roundings of each value to bf16
+    tol = ROW_TOL + (7 * 2.0 ** -8 if dtype == torch.bfloat16 else 0.0)
+    with torch.no_grad():
+        got, cache = q.prefill(ids[:, :l])
+        want, ref_cache = ref.prefill(ids[:, :l])
+        assert got.dtype == dtype and _row_rel(got, want) < tol
+        for i in range(l, l + 3):
+            got, want = q.step(ids[:, i:i + 1], cache), ref.step(ids[:, i:i + 1], ref_cache)
+            assert got.dtype == dtype and got.shape == (b, 1, q.cfg.vocab_size) and _row_rel(got, want) < 2 * tol
