@@ -134,9 +134,9 @@ __global__ void __launch_bounds__(ONE ? 256 : kRowThreads) quantize_kernel(const
         const int k = (u * G + t) * kRun;
         if (k < p.Kp) {
             const uint2 c = none ? uint2{0, 0} : run_codes(v[u], a, inv, exact);
-            // (kept in the caches for the product that reads them next: past them a call alone is up to a sixth faster, fp32
-            // 32768 x 2048 56 -> 47 us, but with its reader slower, 16384 x 1536 through [768, 1536] 46.4 -> 48.7 and 1024 rows 10.8
-            // -> 11.5; with their values 38.7 -> 42.8)
+            // (kept in the caches for the product that reads them next.  Past them a call alone over the same floats is up to a
+            // sixth faster, fp32 32768 x 2048 56 -> 47 us, but slower from HBM, 32768 x 1536 43.3 -> 45.5, and with its reader, 16384
+            // x 1536 through [768, 1536] 46.4 -> 48.7, 1024 rows 10.8 -> 11.5, with the values 42.0 -> 45.1)
             *reinterpret_cast<uint2*>(p.codes + row * p.Kp + k) = c;
         }
     }
@@ -361,11 +361,14 @@ extern "C" int mtl_dequantize_int8(const int8_t* codes, const float* scales, voi
             return check_launch("dequantize_int8");
         });
     };
-    // Past the L2s between 4 and 16 MB: what they hold is written back when the kernel ends, but a reader of more than they keep
-    // waits for the MALL either way.  us, kept and past, alone / with a reader behind: fp32 256x2048 (2 MB) 2.5, 2.5 / 5.4, 5.7;
-    // bf16 4096x2048 (16 MB) 6.1, 5.0 / 17.6, 17.1; fp32 3072x2048 (24 MB) 6.6, 6.4 / 19.7, 20.6; 32768x1536 39.5, 45.5 / 75.8, 86.5.
+    // Past the L2s from 4 to 16 MB, since what they hold is written back when the kernel ends, and from 128 MB on, where the rows'
+    // floats and these do not fit the MALL (256 MB) together.  us, kept and past, alone / with a reader behind / after
+    // quantize_int8 of floats in HBM: fp32 256x2048 (2 MB) 2.5, 2.5 / 5.4, 5.7; bf16 4096x2048 (16 MB) 6.1, 5.0 / 17.6, 17.1; fp32
+    // 4096x2048 (32 MB) 8.0, 7.9 / 21.0, 22.1 / 18.0, 18.0; bf16 24576x2048 (96 MB) 25.5, 26.8 / 50.9, 56.1 / 54.9, 54.8; 128 MB 32.4,
+    // 35.0 / 64.8, 72.0 / 74.1, 71.7; fp32 24576x2048 (192 MB) 41.9, 47.5 / 76.4, 85.7 / 93.5, 81.1, that and a reader 129, 124;
+    // 512 MB 121, 127 / 253, 232 / 241, 230.
     const int64_t bytes = M * ldo * (f32 ? 4 : 2);
-    const bool past = bytes >= 4 << 20 && bytes <= 16 << 20;
+    const bool past = (bytes >= 4 << 20 && bytes <= 16 << 20) || bytes >= 128 << 20;
     if (f32)
         return go(vec ? past ? dequantize_kernel<float, true, true> : dequantize_kernel<float, true>
                       : dequantize_kernel<float, false>, static_cast<float*>(out));

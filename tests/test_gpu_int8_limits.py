@@ -154,7 +154,8 @@ def test_product_at_the_sizes_of_y_where_its_stores_change(m, n, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("m,k", [(1023, 1024), (1024, 1024), (2048, 1024), (4096, 1020), (4096, 1024), (4097, 1024), (8192, 1024), (8193, 1024)])
+@pytest.mark.parametrize("m,k", [(1023, 1024), (1024, 1024), (2048, 1024), (4096, 1020), (4096, 1024), (4097, 1024), (8192, 1024), (8193, 1024),
+                                 (32767, 1024), (32768, 1024), (65535, 1024), (65536, 1024), (65536, 1020)])
 def test_values_at_the_sizes_where_their_stores_change(m, k, dtype):
     q = _int8(m, k, m, dtype)
     out = torch.full((m + 1, k), 7.0, device="cuda", dtype=dtype)
