@@ -18,7 +18,7 @@ inline bool act_dtype(int32_t dtype) { return dtype == MTL_F32 || dtype == MTL_B
 
 // Where mtl_row_linear_int8 takes a row and is no slower than two launches.  Its workgroups of 16 columns of y each put the
 // row into codes again, which pays while there are few or their rows of W long; two launches read a wide W at 5.5 TB/s, but at
-// 4.3-4.9 where its rows are a power of two apart, and one at 5.1.  us of one / of two, fp32, W from HBM, out of 150 sizes:
+// 4.3-4.9 where its rows are a power of two apart, and one at 5.1.  us of one / of two, fp32, W from HBM, out of 160 sizes:
 // 8192x64 4.4 / 4.5, 9216x64 5.6 / 4.6; 12288x512 6.1 / 6.6, 20480x512 8.0 / 7.3; 16384x768 7.1 / 7.0, 24576x768 9.1 / 8.8;
 // 24576x1024 9.1 / 9.6, 32768x1024 11.3 / 10.7; 50280x2048 19.4 / 21.6, 65536x4096 48.7 / 55.0; 16384x2560 11.5 / 13.6, 24576x2560
 // 16.0 / 15.7; 16384x7168 25.4 / 26.9, 20480x7168 33.2 / 30.0.  With a norm: 8192x256 5.2 / 5.3, 12288x256 6.8 / 6.2; 12288x768 6.9 /

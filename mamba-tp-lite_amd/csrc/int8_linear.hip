@@ -389,7 +389,7 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
                          : launch<128, 64, 32, 32, 3, 2, false, true>(a, f32, st);
     // Whole lines of y go past the L2s (32 MB) where those would hold them, since what they hold is written back when the kernel
     // ends, and where not even the MALL (256 MB) does.  us of the product / of it with the quantize_int8 that reads y next, kept
-    // and past, at 200 sizes: fp32 512x8192x2048 (16 MB) 16.5 and 15.0 / 23.3 and 22.5, bf16 16384x768x1536 (24 MB) 25.2 and 23.2 /
+    // and past, at 190 sizes: fp32 512x8192x2048 (16 MB) 16.5 and 15.0 / 23.3 and 22.5, bf16 16384x768x1536 (24 MB) 25.2 and 23.2 /
     // 34.8 and 34.2.  From 28 MB on the reader gives back more than the product gains (fp32 896x8192x2048 22.6 and 21.7 / 30.3 and
     // 30.5; 32 MB 23.5 and 24.2 / 31.5 and 32.7; 64 MB 38.3 and 40.9 / 51.3 and 56.0); at 256 MB three of ten sizes lose 6%, from 320
     // on none (fp32 20480x4096x2048 173 and 175 / 252 and 240, bf16 32768x8192x2048 519 and 503 / 676 and 651, fp32 87381x1536x768
