@@ -767,8 +767,8 @@ class MambaLM(nn.Module):
         29.6 -> 18.4, bf16 15.6 -> 13.1; 1024 tokens 15.6 -> 7.3, 9.2 -> 8.3, 2.9 -> 2.1, 4.4 -> 4.0.  Steps do at mamba-1.4b
         in fp32 (1 row 1394 -> 1108 us, 32 rows 2332 -> 1800) and in bf16 at 1 row (1200 -> 1159), and take longer in bf16 at
         more (32 rows 1707 -> 1824) and at the mamba-130m width (1 row fp32 321 -> 408, bf16 397 -> 434), as do its prompts
-        of 64 tokens in fp32 (0.9 -> 1.2 ms).  Prompts and steps return logits without a graph, inside no_grad and outside,
-        as the unquantized model's do.  Graphs captured before refuse to replay.  Returns self."""
+        of 64 tokens in fp32 (0.9 -> 1.2 ms).  Prompts and steps outside no_grad record nothing of the layers, as an unquantized
+        model's, and of the lm_head only where that stays.  Graphs captured before refuse to replay.  Returns self."""
         return self._quantize("quantize_int8", LinearInt8.from_linear, "head_int8" if lm_head else None,
                               lambda w: LinearInt8(_int8_weight(w)))
 

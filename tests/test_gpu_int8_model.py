@@ -484,3 +484,19 @@ def test_stacks_of_both_kinds_are_those_of_the_definition(which, b, l, dtype):
         for i in range(l, l + 3):
             got, want = q.step(ids[:, i:i + 1], cache), ref.step(ids[:, i:i + 1], ref_cache)
             assert got.dtype == dtype and got.shape == (b, 1, q.cfg.vocab_size) and _row_rel(got, want) < 2 * tol
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_what_a_model_records_outside_no_grad(dtype):
+    m = _model(dtype=dtype)
+    ids = torch.randint(0, 1003, (1, 9), device="cuda")
+    for lm_head in (True, False):
+        q = copy.deepcopy(m).quantize_int8(lm_head=lm_head)
+        logits, cache = q.prefill(ids)
+        # the layers nothing; an lm_head that stays its own product, as in an unquantized model
+        assert logits.requires_grad == (not lm_head)
+        if not lm_head:
+            logits.float().sum().backward()
+            assert q.embedding.weight.grad is not None
+        assert all(p.grad is None for name, p in q.named_parameters() if name != "embedding.weight")
+        assert not any(t.requires_grad for c in cache.layers for t in (c.conv_state, c.ssm_state))
