@@ -331,3 +331,14 @@ def test_one_rule_says_where_a_float_row_is_put_into_codes_within_its_product():
         assert pays(n, k, norm) == 0, (n, k, norm)
     for n, k in ((768, 1536), (50280, 2048), (50280, 768), (16, 8193)):
         assert ops.row_linear_int8_pays(n, k) == bool(pays(n, k, 0))
+
+
+@pytest.mark.parametrize("shape", [(40,), (1, 40), (1, 1, 40), (5, 40)])
+def test_a_trace_is_refused_by_name_for_any_number_of_rows(shape):
+    from mamba_lite.model import LinearInt8
+
+    q = LinearInt8(_q(6))
+    with pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(q, torch.zeros(shape))
+    with pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(lambda x: ops.linear_int8(x, _q(6)), torch.zeros(shape))
