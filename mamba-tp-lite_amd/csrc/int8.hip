@@ -361,14 +361,13 @@ extern "C" int mtl_dequantize_int8(const int8_t* codes, const float* scales, voi
             return check_launch("dequantize_int8");
         });
     };
-    // Past the L2s from 4 to 16 MB, since what they hold is written back when the kernel ends, and from 128 MB on, where the rows'
-    // floats and these do not fit the MALL (256 MB) together.  us, kept and past, alone / with a reader behind / after
-    // quantize_int8 of floats in HBM: fp32 256x2048 (2 MB) 2.5, 2.5 / 5.4, 5.7; bf16 4096x2048 (16 MB) 6.1, 5.0 / 17.6, 17.1; fp32
-    // 4096x2048 (32 MB) 8.0, 7.9 / 21.0, 22.1 / 18.0, 18.0; bf16 24576x2048 (96 MB) 25.5, 26.8 / 50.9, 56.1 / 54.9, 54.8; 128 MB 32.4,
-    // 35.0 / 64.8, 72.0 / 74.1, 71.7; fp32 24576x2048 (192 MB) 41.9, 47.5 / 76.4, 85.7 / 93.5, 81.1, that and a reader 129, 124;
-    // 512 MB 121, 127 / 253, 232 / 241, 230.
-    const int64_t bytes = M * ldo * (f32 ? 4 : 2);
-    const bool past = (bytes >= 4 << 20 && bytes <= 16 << 20) || bytes >= 128 << 20;
+    // Past the L2s from 4 MB on: what they hold is written back when the kernel ends, and from 16 MB on rows read before and values
+    // leave each other more of the MALL.  us, kept and past, inputs from HBM and two outputs in turn, these alone / after a norm of
+    // the rows / with a reader behind that: fp32 256x2048 (2 MB) 2.5, 2.5 / 6.6, 6.6 / 10.1, 10.2; 2048x2048 (16 MB) 5.6, 4.6 / 17.6,
+    // 16.5 / 23.1, 22.3; 4096x2048 8.2, 8.1 / 28.3, 28.2 / 36.8, 37.7; 8192x2048 16.2, 17.4 / 55.7, 51.4 / 67.5, 67.3; 24576x2048 (192 MB)
+    // 45.7, 46.5 / 168, 151 / 202, 194.  Over one output again and again, with nothing between, kept ones are up to 15% faster from
+    // 48 to 224 MB.
+    const bool past = M * ldo * (f32 ? 4 : 2) >= 4 << 20;
     if (f32)
         return go(vec ? past ? dequantize_kernel<float, true, true> : dequantize_kernel<float, true>
                       : dequantize_kernel<float, false>, static_cast<float*>(out));
