@@ -389,14 +389,15 @@ extern "C" int mtl_linear_int8(const mtl_linear_int8_args* p, mtl_stream_t strea
                          : launch<128, 64, 32, 32, 3, 2, false, true>(a, f32, st);
     // Whole lines of y go past the L2s (32 MB) where those would hold them, since what they hold is written back when the kernel
     // ends, and where not even the MALL (256 MB) does.  us of the product / of it with the quantize_int8 that reads y next, kept
-    // and past, at 190 sizes: fp32 512x8192x2048 (16 MB) 16.5 and 15.0 / 23.3 and 22.5, bf16 16384x768x1536 (24 MB) 25.2 and 23.2 /
-    // 34.8 and 34.2.  From 28 MB on the reader gives back more than the product gains (fp32 896x8192x2048 22.6 and 21.7 / 30.3 and
-    // 30.5; 32 MB 23.5 and 24.2 / 31.5 and 32.7; 64 MB 38.3 and 40.9 / 51.3 and 56.0); at 256 MB three of ten sizes lose 6%, from 320
-    // on none (fp32 20480x4096x2048 173 and 175 / 252 and 240, bf16 32768x8192x2048 519 and 503 / 676 and 651, fp32 87381x1536x768
-    // 197 and 151 / 320 and 289).  Rows that end inside a line lose at any size (8184x50277x768 690 and 855).
+    // and past, at 280 sizes, over one y and over two in turn: fp32 512x8192x2048 (16 MB) 16.1 and 14.8 / 21.9 and 21.0, bf16
+    // 16384x768x1536 (24 MB) 27.6 and 25.8 / 38.3 and 37.5.  At 28 MB the product gains 4% and the two lose 1% on average, at 30 MB 2%
+    // and 2% (fp32 5120x1536x768 12.2 and 11.9 / 19.9 and 20.8); fp32 2048x8192x2048 (64 MB) 37.8 and 39.8 / 51.6 and 55.1.  At 256 MB
+    // three of ten sizes lose 6%, at 320 one 5% (fp32 10240x8192x2048 173 and 182 / 245 and 253), from 384 on the two none (12288 rows of
+    // it 212 and 218 / 309 and 303, bf16 32768x8192x2048 519 and 503 / 676 and 651, fp32 87381x1536x768 197 and 151 / 320 and 289).
+    // Rows that end inside a line lose at any size (8184x50277x768 690 and 855).
     const int64_t row = p->ldy * (f32 ? 4 : 2), y_bytes = p->M * row;
     const bool lines = row % 128 == 0 && reinterpret_cast<uintptr_t>(p->y) % 128 == 0;
-    const bool past = lines && y_bytes <= 24 << 20, large = lines && y_bytes >= 320 << 20;
+    const bool past = lines && y_bytes <= 28 << 20, large = lines && y_bytes >= 384 << 20;
     // Others by the time that their tiles take on the 256 CUs, in us: each round of a tile per CU has its start and end (longer
     // where rows of y end inside a line, or are floats) and its stages of K; two or more tiles share a CU, and a round of them
     // has the traffic of all.  Measured at 210 sizes of up to 32768 rows with every tile, the choice takes 1% more than the best of

@@ -135,9 +135,10 @@ def _int8(rows, k, seed, dtype=torch.float32):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-# (rows of whole lines: 24 MB in fp32 and in bf16, a row more, and 320 MB of a chain)
+# (rows of whole lines: up to 28 MB in fp32 and in bf16, a row more, and a chain's around 384 MB)
 @pytest.mark.parametrize("m,n,k", [(740, 8192, 4100), (768, 8192, 4100), (769, 8192, 4100), (1536, 8192, 2048), (1537, 8192, 2048),
-                                   (40959, 2048, 390), (40960, 2048, 390), (40960, 4096, 390)])
+                                   (40959, 2048, 390), (40960, 2048, 390), (40960, 4096, 390), (896, 8192, 4100), (897, 8192, 4100),
+                                   (1792, 8192, 300), (1793, 8192, 300), (49151, 2048, 390), (49152, 2048, 390), (49152, 4096, 390)])
 def test_product_at_the_sizes_of_y_where_its_stores_change(m, n, k, dtype):
     x, w = _int8(m, k, m, dtype), _int8(n, k, n)
     bias = torch.randn(n, device="cuda", generator=_gen(1)).to(dtype)
